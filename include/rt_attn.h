@@ -434,6 +434,119 @@ int rt_gqa_decode_batched_bf16_noalloc(void *stream, const void *q, const void *
 size_t rt_gqa_decode_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim,
                                      int32_t max_seq);
 
+/* ---- caches that are kept small: 4-bit rows, and rows taken out ---------------------------------- */
+
+/* No counterparts in the reference, whose caches are f32 or bf16 and keep every row.
+ *
+ * A 4-bit cache of one of K and V, [batch, n_kv, max_seq, head_dim] with head_dim 64, 128 or 256, is two device buffers:
+ *   codes  bytes [batch, n_kv, max_seq, head_dim / 2], 16-byte aligned
+ *   pairs  uint32 [batch, n_kv, head_dim / 64, max_seq]: for 64 dims of a row a bf16 scale s (low half) and middle z
+ * and a value is z + s (c - 8), c its code of 0 .. 15.  For the largest and the smallest of the 64, hi and lo:
+ *   z = bf16((hi + lo) / 2 + (hi - lo) / 32)    s = max((hi - z) / 7.5, (z - lo) / 8.5), up to the next bf16
+ *   c = 8 + clamp(nearest((x - z) / s), -8, 7)  (ties to even; 8 where s is 0)
+ * in f32, so that a value is off by s / 2 at most.  64 dims that hold a NaN or an infinity, or spread over more than f32
+ * can tell, read as NaN.  With n = head_dim / 32, byte i n + p of a row holds the dims 32 c + 2 i (low bits) and 32 c + 2 i + 1,
+ * c being p with its two lowest bits exchanged (c = p for n = 2).  4.5 bits a value.
+ *
+ * A cache that rows are taken out of keeps, beside K and V, two device arrays [batch, n_kv, max_seq]:
+ *   slots    int32: the position of the token that a row holds
+ *   weights  f32: the sum of the attention weights that its key has drawn
+ * A row's number there is not its position any more: new rows are appended behind the last (`rows` below), keys having their
+ * position in them by the rotation.  Rows behind a sequence's last are never written but by an append.
+ *
+ * All are asynchronous on `stream`, allocate nothing and may be recorded into a HIP graph.  What a call needs besides its
+ * tensors is the caller's `workspace` (device memory, 16-byte aligned), which it works in alone and keeps nothing in: calls that
+ * may overlap (other streams, graphs replayed side by side) have workspaces of their own. */
+
+/* rt_qk_norm_rope_kv_append_bf16 into a 4-bit cache, with the same arithmetic up to the rounding (K rows are rounded to 4 bits
+ * from f32, V rows from bf16).  q [batch, n_heads, seq, head_dim] goes rotated to q_out, which is q itself or shares no memory
+ * with it.  Token s of sequence b sits at position p_b + s (positions, device int32[batch], or `pos` for all) and goes to cache
+ * row r_b + s, r_b = rows[b] (device int32[batch]) or, with rows == NULL, p_b.  slots and weights, where given, take the token's
+ * position and 0 for each new row.  A sequence whose positions or rows would leave the tables or the cache is left untouched;
+ * a host `pos` is checked (RT_ERR_ROPE_POSITION_OVERFLOW, then RT_ERR_KV_OVERFLOW where the rows are the positions).  q, k_in, v_in and
+ * the caches 16-byte aligned; head_dim 64, 128 or 256 (RT_ERR_UNSUPPORTED otherwise). */
+int rt_qk_norm_rope_kv_append_q4(void *stream, const void *q, void *q_out, const void *k_in, const void *v_in,
+                                 void *k_codes, uint32_t *k_pairs, void *v_codes, uint32_t *v_pairs,
+                                 const int32_t *positions, int32_t pos, const int32_t *rows, int32_t *slots,
+                                 float *weights, const float *q_gamma, const float *k_gamma, float eps,
+                                 const float *cos_table, const float *sin_table, int32_t table_rows, int32_t batch,
+                                 int32_t seq, int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t max_seq,
+                                 rt_err_detail *err);
+
+/* The same into a bf16 cache whose rows are not the positions: with rows == NULL the rows written are, bit for bit, those of
+ * rt_qk_norm_rope_kv_append_bf16. */
+int rt_qk_norm_rope_kv_append_rows_bf16(void *stream, const void *q, void *q_out, const void *k_in, const void *v_in,
+                                        void *k_cache, void *v_cache, const int32_t *positions, int32_t pos,
+                                        const int32_t *rows, int32_t *slots, float *weights, const float *q_gamma,
+                                        const float *k_gamma, float eps, const float *cos_table,
+                                        const float *sin_table, int32_t table_rows, int32_t batch, int32_t seq,
+                                        int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t max_seq,
+                                        rt_err_detail *err);
+
+/* rt_kv_cache_append_dev into a 4-bit cache: bf16 new_k / new_v [batch, n_heads, seq_added, head_dim] as they are, the same
+ * checks in the same order. */
+int rt_kv_cache_append_q4_dev(void *stream, void *k_codes, uint32_t *k_pairs, void *v_codes, uint32_t *v_pairs,
+                              const void *new_k, size_t new_k_len, const void *new_v, size_t new_v_len, size_t batch,
+                              size_t n_heads, size_t max_seq, size_t head_dim, size_t current_len, size_t seq_added,
+                              rt_err_detail *err);
+
+/* Rows r_b .. r_b + n_rows - 1 of a 4-bit cache (one of K and V) as bf16, out [batch, n_kv, n_rows, head_dim]: r_b = rows[b]
+ * (device int32[batch]) or, with rows == NULL, `row` (RT_ERR_KV_OVERFLOW where they would leave the cache; a sequence whose
+ * device row would leave it leaves its part of `out` as it is). */
+int rt_kv_cache_read_q4(void *stream, const void *codes, const uint32_t *pairs, void *out, const int32_t *rows,
+                        int32_t row, int32_t n_rows, int32_t batch, int32_t n_kv, int32_t head_dim, int32_t max_seq,
+                        rt_err_detail *err);
+
+/* rt_gqa_decode_chunk_bf16 over a 4-bit cache: q/out bf16 [batch, seq_new, n_heads, head_dim], seq_new = 1 for a decode step;
+ * kv_lens device int32[batch] = keys in the cache including the new ones (counts above max_seq are max_seq, below 0 are 0), or
+ * NULL: every sequence has `kv_len`.  Position s of sequence b sees keys [0, kv_lens[b] - seq_new + s]; one that sees none gives
+ * +0.0.  kv head = h / (n_heads / n_kv), any number of heads a group.  f32 accumulation and softmax, weights of 16 bits, one rounding to
+ * bf16 at the end.  The last bits of a sequence may depend on what else is in the batch (how its keys are cut into spans); the
+ * same call gives the same bits every time.  workspace: rt_gqa_decode_q4_workspace_bytes(...) bytes (RT_ERR_WORKSPACE_TOO_SMALL). */
+size_t rt_gqa_decode_q4_workspace_bytes(int32_t batch, int32_t seq_new, int32_t n_heads, int32_t n_kv,
+                                        int32_t head_dim, int32_t max_seq);
+int rt_gqa_decode_q4(void *stream, const void *q, const void *k_codes, const uint32_t *k_pairs, const void *v_codes,
+                     const uint32_t *v_pairs, void *out, const int32_t *kv_lens, int32_t kv_len, int32_t batch,
+                     int32_t seq_new, int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t max_seq,
+                     void *workspace, size_t workspace_bytes, rt_err_detail *err);
+
+/* Decode attention of one new token per sequence (q/out bf16 [batch, n_heads, head_dim], kv_lens device int32[batch], as
+ * rt_gqa_decode_batched_bf16) that also sums what each key draws:
+ *   weights_out[b, kvh, j] = weights_in[b, kvh, j] + sum over the query heads h of kvh of softmax weight (h, j)     for j < kv_lens[b]
+ * f32 [batch, n_kv, max_seq]; weights_in == NULL counts as zeros, and is weights_out itself or shares no memory with it; entries
+ * j >= kv_lens[b] of weights_out stay as they are.  Over a bf16 cache [batch, n_kv, max_seq, head_dim] or a 4-bit one.  workspace:
+ * rt_gqa_decode_weights_workspace_bytes(...) bytes (it holds the scores: batch * n_heads * max_seq floats, among others). */
+size_t rt_gqa_decode_weights_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim,
+                                             int32_t max_seq);
+int rt_gqa_decode_weights_bf16(void *stream, const void *q, const void *k_cache, const void *v_cache, void *out,
+                               const float *weights_in, float *weights_out, const int32_t *kv_lens, int32_t batch,
+                               int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t max_seq, void *workspace,
+                               size_t workspace_bytes, rt_err_detail *err);
+int rt_gqa_decode_weights_q4(void *stream, const void *q, const void *k_codes, const uint32_t *k_pairs,
+                             const void *v_codes, const uint32_t *v_pairs, void *out, const float *weights_in,
+                             float *weights_out, const int32_t *kv_lens, int32_t batch, int32_t n_heads, int32_t n_kv,
+                             int32_t head_dim, int32_t max_seq, void *workspace, size_t workspace_bytes,
+                             rt_err_detail *err);
+
+/* Cuts every sequence with more than `budget` rows to that many, each kv head by its own sums: the `recent` newest tokens stay
+ * (positions above the head's newest - recent; recent <= budget), and of the others those with the largest weights, of equal sums the lower
+ * row first (NaN counts as -infinity, an infinite sum as much as a newest token).  Kept rows at or behind `budget` move, in order, to the
+ * rows below it that are freed, in order; all other rows of K and V stay as they are, those behind the new length among them.
+ * weights_out and slots_out take the new rows' sums and positions (rows below the new length; the others stay as they are); each is
+ * its input or shares no memory with any.  kv_lens (device int32[batch]) is read; new_lens, if not NULL, takes min(kv_lens[b], budget) and may
+ * be kv_lens itself: the layers of a model, which share kv_lens, are all cut before it changes.
+ * workspace: rt_kv_evict_workspace_bytes(...) bytes. */
+size_t rt_kv_evict_workspace_bytes(int32_t batch, int32_t n_kv, int32_t max_seq, int32_t budget);
+int rt_kv_evict_bf16(void *stream, void *k_cache, void *v_cache, const float *weights_in, const int32_t *slots_in,
+                     float *weights_out, int32_t *slots_out, const int32_t *kv_lens, int32_t *new_lens, int32_t batch,
+                     int32_t n_kv, int32_t head_dim, int32_t max_seq, int32_t budget, int32_t recent, void *workspace,
+                     size_t workspace_bytes, rt_err_detail *err);
+int rt_kv_evict_q4(void *stream, void *k_codes, uint32_t *k_pairs, void *v_codes, uint32_t *v_pairs,
+                   const float *weights_in, const int32_t *slots_in, float *weights_out, int32_t *slots_out,
+                   const int32_t *kv_lens, int32_t *new_lens, int32_t batch, int32_t n_kv, int32_t head_dim,
+                   int32_t max_seq, int32_t budget, int32_t recent, void *workspace, size_t workspace_bytes,
+                   rt_err_detail *err);
+
 /* ---- device buffers (the slot of Storage::Cuda, crates/rustorch-core/src/tensor/storage.rs:776-817) */
 void *rt_buf_alloc(size_t bytes, rt_err_detail *err);
 int rt_buf_free(void *ptr, rt_err_detail *err);

@@ -26,6 +26,9 @@ SYMBOLS = (
     "rt_buf_alloc", "rt_buf_free", "rt_buf_zero", "rt_memcpy_h2d", "rt_memcpy_d2h", "rt_stream_synchronize",
     "rt_stream_create", "rt_stream_destroy", "rt_i32_add_dev", "rt_debug_force_bf16_prefill_kernel", "rt_debug_f32_split_products", "rt_debug_f32_wide_gradients", "rt_set_strict_non_finite_v",
     "rt_flash_forward_window_bf16_dev", "rt_flash_forward_window_bnhd_bf16_dev",
+    "rt_qk_norm_rope_kv_append_q4", "rt_qk_norm_rope_kv_append_rows_bf16", "rt_kv_cache_append_q4_dev", "rt_kv_cache_read_q4",
+    "rt_gqa_decode_q4", "rt_gqa_decode_q4_workspace_bytes", "rt_gqa_decode_weights_bf16", "rt_gqa_decode_weights_q4",
+    "rt_gqa_decode_weights_workspace_bytes", "rt_kv_evict_bf16", "rt_kv_evict_q4", "rt_kv_evict_workspace_bytes",
 )
 
 RT_OK = 0
@@ -115,6 +118,19 @@ def lib():
     L.rt_gqa_decode_batched_bf16_noalloc.argtypes = [vp, vp, vp, vp, vp, i32p, i32, i32, i32, i32, i32, errp]
     L.rt_gqa_decode_workspace_bytes.argtypes = [i32, i32, i32, i32, i32]
     L.rt_gqa_decode_workspace_bytes.restype = sz
+    f32 = C.c_float
+    L.rt_qk_norm_rope_kv_append_q4.argtypes = [vp] * 10 + [i32, vp, vp, vp, vp, vp, f32, vp, vp] + [i32] * 7 + [errp]
+    L.rt_qk_norm_rope_kv_append_rows_bf16.argtypes = [vp] * 8 + [i32, vp, vp, vp, vp, vp, f32, vp, vp] + [i32] * 7 + [errp]
+    L.rt_kv_cache_append_q4_dev.argtypes = [vp, vp, vp, vp, vp, vp, sz, vp, sz, sz, sz, sz, sz, sz, sz, errp]
+    L.rt_kv_cache_read_q4.argtypes = [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, errp]
+    L.rt_gqa_decode_q4.argtypes = [vp] * 8 + [i32] * 7 + [vp, sz, errp]
+    L.rt_gqa_decode_weights_bf16.argtypes = [vp] * 8 + [i32] * 5 + [vp, sz, errp]
+    L.rt_gqa_decode_weights_q4.argtypes = [vp] * 10 + [i32] * 5 + [vp, sz, errp]
+    L.rt_kv_evict_bf16.argtypes = [vp] * 9 + [i32] * 6 + [vp, sz, errp]
+    L.rt_kv_evict_q4.argtypes = [vp] * 11 + [i32] * 6 + [vp, sz, errp]
+    for name, n in (("rt_gqa_decode_q4_workspace_bytes", 6), ("rt_gqa_decode_weights_workspace_bytes", 5), ("rt_kv_evict_workspace_bytes", 4)):
+        getattr(L, name).argtypes = [i32] * n
+        getattr(L, name).restype = sz
     L.rt_buf_alloc.argtypes = [sz, errp]
     L.rt_buf_alloc.restype = vp
     L.rt_buf_free.argtypes = [vp, errp]

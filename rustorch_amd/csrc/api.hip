@@ -21,54 +21,14 @@
 #include <vector>
 
 #include "../../include/rt_attn.h"
+#include "rt_host.hpp"
 #include "rt_kernels.hpp"
-
-#define RT_API extern "C" __attribute__((visibility("default")))
 
 namespace {
 
-void clear_err(rt_err_detail* e) {
-    if (e) {
-        e->which = -1;
-        e->expected = e->got = e->got2 = 0;
-        e->hip_error = 0;
-        e->message[0] = 0;
-    }
-}
-
-int fail(rt_err_detail* e, int status, int which, uint64_t expected, uint64_t got, const char* msg, uint64_t got2 = 0) {
-    if (e) {
-        e->which = which;
-        e->expected = expected;
-        e->got = got;
-        e->got2 = got2;
-        e->hip_error = 0;
-        snprintf(e->message, sizeof(e->message), "%s", msg ? msg : "");
-    }
-    return status;
-}
-
-int fail_hip(rt_err_detail* e, hipError_t code, const char* where) {
-    if (e) {
-        e->which = -1;
-        e->expected = e->got = e->got2 = 0;
-        e->hip_error = (int32_t)code;
-        snprintf(e->message, sizeof(e->message), "%s: %s", where, hipGetErrorString(code));
-    }
-    return RT_ERR_HIP;
-}
-
-#define HIP_TRY(expr, where)                                  \
-    do {                                                      \
-        hipError_t _e = (expr);                               \
-        if (_e != hipSuccess) return fail_hip(err, _e, where); \
-    } while (0)
-
-// Behind the body of an entry that may allocate on the host: no exception passes a C entry.
-#define RT_NO_THROW                                               \
-    catch (const std::exception& e) {                             \
-        return fail_hip(err, hipErrorOutOfMemory, e.what());      \
-    }
+using rt::clear_err;
+using rt::fail;
+using rt::fail_hip;
 
 int g_num_cus = 0;
 int g_decode_waves = 0;  // one-wave workgroups one launch of the decode kernel keeps resident
@@ -784,6 +744,11 @@ private:
 };
 
 }  // namespace
+
+namespace rt {
+int ensure_device(rt_err_detail* err) { return ::ensure_device(err, -1); }
+int device_cus() { return g_num_cus; }
+}  // namespace rt
 
 RT_API const char* rt_version(void) { return "rt_attn_hip 0.1 (gfx950)"; }
 

@@ -188,6 +188,15 @@ PyMethodDef methods[] = {
     RT_BIND(rt_gqa_decode_batched_bf16_noalloc),
     RT_BIND(rt_gqa_decode_chunk_bf16),
     RT_BIND(rt_i32_add_dev),
+    RT_BIND(rt_qk_norm_rope_kv_append_q4),
+    RT_BIND(rt_qk_norm_rope_kv_append_rows_bf16),
+    RT_BIND(rt_kv_cache_append_q4_dev),
+    RT_BIND(rt_kv_cache_read_q4),
+    RT_BIND(rt_gqa_decode_q4),
+    RT_BIND(rt_gqa_decode_weights_bf16),
+    RT_BIND(rt_gqa_decode_weights_q4),
+    RT_BIND(rt_kv_evict_bf16),
+    RT_BIND(rt_kv_evict_q4),
     RT_BIND_HOST(rt_flash_forward_masked_f32),
     RT_BIND_HOST(rt_flash_backward_f32),
     RT_BIND_HOST(rt_gqa_forward_f32),

@@ -747,7 +747,7 @@ private:
 
 namespace rt {
 int ensure_device(rt_err_detail* err) { return ::ensure_device(err, -1); }
-int device_cus() { return g_num_cus; }
+uint64_t next_launch_id() { return ::next_launch_id(); }
 }  // namespace rt
 
 RT_API const char* rt_version(void) { return "rt_attn_hip 0.1 (gfx950)"; }

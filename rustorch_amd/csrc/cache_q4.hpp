@@ -68,11 +68,13 @@ struct CacheAttendParams {
     int group;    // heads / kv_heads
     int rows;     // seq_new * group query rows of a kv head
     int n_tiles;  // of 16 of them
-    int n_waves;  // waves launched
-    int span_min; // a wave takes at least this many steps of 32 keys
+    int n_groups;  // workgroups launched
+    int span_min;  // one takes at least this many steps of 32 keys
     float scale_log2e;
-    float* part;    // partials: (n_waves + segments) slots of part_rows * (dim + 2) floats
+    float* part;    // partials: (n_groups + segments) slots of part_rows * (dim + 2) floats, the rows and behind them their (m, l)
     int part_rows;  // min(16, rows)
+    unsigned char* words;  // a line a segment, see SegmentWord
+    uint64_t launch_id;    // its low 16 bits zero
     // the weights' sums (seq_new = 1), or null
     float* scores;             // [batch, heads, max_seq]: unscaled scores
     float* stats;              // [batch, heads, 2]: the row's maximum (unscaled), 1 / sum

@@ -2,7 +2,7 @@
 //
 //   out = softmax(q K^T / sqrt(dim)) V        weights_out[j] = weights_in[j] + sum over the heads of the group of their softmax weight of key j
 //
-// One wave walks steps of 32 keys of one kv head for up to 16 query rows (heads of the group x new positions) by the matrix cores,
+// A wave walks steps of 32 keys of one kv head for up to 16 query rows (heads of the group x new positions) by the matrix cores,
 // both products transposed: scores^T = K q^T leaves a lane with the scores of ONE query row for eight keys, which is the operand
 // that out^T = V^T P^T takes, so that nothing of a step crosses lanes but the running maximum.
 //
@@ -13,9 +13,11 @@
 // The weights p s are two bf16 terms (16 bits), as are those of a bf16 cache: with one the output's error is half as large again
 // as its own rounding's.
 //
-// The keys of all (sequence, kv head, 16 query rows) segments form one list of steps that is cut into equal spans, one a wave; a wave that
-// does not have a segment to itself leaves an unnormalised partial, which a second kernel folds.
+// The steps of all (sequence, kv head, 16 query rows) segments form one list that is cut into equal spans, one a workgroup of four
+// waves, which deal the steps of a segment among themselves and fold what they have through LDS.  A segment that lies in one span
+// is written at once; of the others every workgroup leaves an unnormalised partial, and the one that finishes last folds them.
 #include <algorithm>
+#include <type_traits>
 
 #include "cache_q4.hpp"
 #include "rt_common.hpp"
@@ -27,7 +29,9 @@ namespace rt {
 namespace {
 
 constexpr int kStep = 32;       // keys a step
-constexpr int kMaxWaves = 2048; // eight a CU
+constexpr int kWaves = 4;        // a workgroup
+constexpr int kCus = 256;
+constexpr int kMaxPieces = 256;  // partials of a segment
 constexpr float kNoMax = -1.0e30f;
 
 __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
@@ -37,424 +41,741 @@ __device__ __forceinline__ int len_of(const CacheAttendParams& p, int b) {
     return p.kv_lens ? min(max(p.kv_lens[b], 0), p.max_seq) : p.kv_len;
 }
 __device__ __forceinline__ int steps_of(int len) { return (len + kStep - 1) / kStep; }
-__device__ __forceinline__ int wave_sum_int(int x) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
-    return x;
-}
-
-// Where a flat step lies: its sequence, and the first step of that sequence; `total`: steps of all.
-struct Place {
-    int total, b, first;
+// What a workgroup's span of the list is, and where it begins.
+struct Span {
+    int total, size, b, first;  // steps of all; of a span; the sequence that holds the span's first step, and that sequence's first
 };
-// Sum of the steps before sequence `upto` (all of them: batch).  Called by a whole wave.
-__device__ __forceinline__ int steps_before(const CacheAttendParams& p, int upto, int lane) {
-    int sum = 0;
-    for (int b = lane; b < upto; b += 64) sum += steps_of(len_of(p, b));
-    return wave_sum_int(sum) * (p.kv_heads * p.n_tiles);
-}
-// The sequence that holds flat step `at`, and its first step.
-__device__ __forceinline__ void find_sequence(const CacheAttendParams& p, int at, int lane, int* seq, int* first) {
+// Lengths 64 at a time, the first of them once for both walks.
+__device__ __forceinline__ Span span_of(const CacheAttendParams& p, int group, int lane) {
     const int per = p.kv_heads * p.n_tiles;
+    auto steps = [&](int b0) { return b0 + lane < p.batch ? steps_of(len_of(p, b0 + lane)) : 0; };
+    const int head = steps(0);
+    int sum = head, most = head;
+    for (int b0 = 64; b0 < p.batch; b0 += 64) {
+        const int x = steps(b0);
+        sum += x;
+        most = max(most, x);
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        sum += __shfl_xor(sum, o, 64);
+        most = max(most, __shfl_xor(most, o, 64));
+    }
+    Span s;
+    s.total = __builtin_amdgcn_readfirstlane(sum) * per;
+    most = __builtin_amdgcn_readfirstlane(most);
+    // (a segment of `most` steps touches at most most / size + 2 spans)
+    s.size = max(max(p.span_min, (s.total + p.n_groups - 1) / p.n_groups), max(min((most + 31) / 32, 64), (most + kMaxPieces - 3) / (kMaxPieces - 2)));
+    s.b = 0;
+    s.first = 0;
+    const long long at = (long long)group * s.size;
+    if (at >= s.total) return s;
     int before = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += 64) {
-        const int mine = b0 + lane < p.batch ? steps_of(len_of(p, b0 + lane)) * per : 0;
+    for (int b0 = 0;; b0 += 64) {
+        const int mine = (b0 ? steps(b0) : head) * per;
         int end = mine;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int y = __shfl_up(end, o, 64);
             if (lane >= o) end += y;
         }
-        const uint64_t past = __ballot(before + end > at);
-        if (past) {
+        const uint64_t past = __ballot(before + end > (int)at);
+        if (past) {  // (it is for one of them: `at` is below the total)
             const int l = __ffsll((unsigned long long)past) - 1;
-            *seq = b0 + l;
-            *first = before + __shfl(end - mine, l, 64);
-            return;
+            s.b = __builtin_amdgcn_readfirstlane(b0 + l);
+            s.first = __builtin_amdgcn_readfirstlane(before + __shfl(end - mine, l, 64));
+            return s;
         }
         before += __shfl(end, 63, 64);
     }
-    *seq = p.batch;
-    *first = before;
 }
-__device__ __forceinline__ int span_of(const CacheAttendParams& p, int total) { return max(p.span_min, (total + p.n_waves - 1) / p.n_waves); }
+
+// ---- partials that another workgroup of the launch reads: device scope both ways, as in decode.hip --------------------------
+constexpr int kScopeDevice = 16;  // sc1
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, kBufferFlags);
+}
+__device__ __forceinline__ void put4(__amdgpu_buffer_rsrc_t rs, uint32_t byte, f32x4_t v) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), rs, byte, 0, kScopeDevice);
+}
+__device__ __forceinline__ void put2(__amdgpu_buffer_rsrc_t rs, uint32_t byte, float a, float b) {
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(a), __float_as_uint(b)}, rs, byte, 0, kScopeDevice);
+}
+__device__ __forceinline__ f32x4_t get4(__amdgpu_buffer_rsrc_t rs, uint32_t byte) {
+    return __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, byte, 0, kScopeDevice));
+}
+__device__ __forceinline__ u32x2_t get2(__amdgpu_buffer_rsrc_t rs, uint32_t byte) { return __builtin_amdgcn_raw_buffer_load_b64(rs, byte, 0, kScopeDevice); }
+
+// The word through which a segment's workgroups learn which of them is the last: (launch id | count).  It lies in the caller's
+// workspace, which holds anything: every workgroup makes sure, ahead of its own count, that the word carries this launch's id.
+// The last one leaves 0 there, so that a recorded launch, which brings its id along on every replay, finds none of its own counts.
+typedef unsigned long long word_t;
+constexpr int kWordPitch = 128;  // bytes: atomics on one line wait for each other
+constexpr word_t kCountMask = 0xffff;
+struct SegmentWord {
+    word_t* at;
+    word_t id;
+    __device__ __forceinline__ bool ours(word_t x) const { return ((x ^ id) & ~kCountMask) == 0; }
+    __device__ __forceinline__ void claim() {
+        word_t seen = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        while (!ours(seen) && !__hip_atomic_compare_exchange_strong(at, &seen, id, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) {
+        }  // (fails only if another workgroup was first, whose id is this one)
+    }
+    // counts one finished partial of `n`; true for the one that completes the set
+    __device__ __forceinline__ bool count(int n) {
+        const word_t old = __hip_atomic_fetch_add(at, (word_t)1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool last = (int)(old & kCountMask) + 1 == n;
+        if (last) __hip_atomic_store(at, (word_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return last;
+    }
+};
 
 // ---- what a lane holds of 32 keys ----------------------------------------------------------------------------------
 // As an operand of scores^T, keys are rows: lane (n, quad) has key n of either 16, and a quarter of each row.  As an operand of
 // out^T, dims are rows and keys the products' inner index: lane (n, quad) has dims by n of the eight keys 4 quad + {0..3}, 16 + those, in the order
 // in which scores^T leaves their weights.
-template <int D, bool Q4>
+//
+// Up to four or eight query rows leave most of the sixteen columns of a product idle, and what is done a (row, key) -- scales, exponentials,
+// the weights' terms -- would be done for all sixteen.  There a row has C = 4 or 2 columns, n, n + 16 / C, ..., and each of them takes a
+// C-th of a lane's eight keys: the others' weights are zeros in its operand, and its part of the row has a maximum and a sum of its own,
+// folded with the waves' at the end.  (Scores of all eight are there anyway: selecting them costs less than finishing them.)
+template <int D, bool Q4, int C>
 struct Keys {
-    static constexpr int kKw = Q4 ? D / 32 : D / 8, kVw = Q4 ? (D + 127) / 128 : D / 32, kG = Q4 ? D / 64 : 1;
+    static constexpr int kKw = Q4 ? D / 32 : D / 8, kVw = Q4 ? (D + 127) / 128 : D / 32, kG = Q4 ? D / 64 : 1, kE = 8 / C;
     uint32_t k[2][kKw], v[8][kVw];
-    uint32_t ks[2][kG][4], vs[2][kG][4];  // pairs of keys 4 quad + i of either 16
+    uint32_t ks[kG][kE], vs[kG][kE];  // pairs of the lane's keys
 };
 
-template <int D, bool Q4>
-__device__ __forceinline__ void load_keys(Keys<D, Q4>& t, const uint8_t* k, const uint8_t* v, const uint32_t* kp, const uint32_t* vp, int max_seq, int key0, int len, int n, int quad) {
-    using T = Keys<D, Q4>;
-    constexpr int kRow = Q4 ? D / 2 : 2 * D;
-    const int last = len - 1;
+// bf16 rows come through registers, K's of the next step as soon as this step's scores are there and V's as soon as its products are.
+template <int D, int C>
+__device__ __forceinline__ void load_k(Keys<D, false, C>& t, const uint8_t* k, int key0, int len, int n, int quad) {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        const uint8_t* row = k + (size_t)min(key0 + 16 * h + n, last) * kRow;
-        if constexpr (Q4) {
+        const uint8_t* row = k + (size_t)min(key0 + 16 * h + n, len - 1) * (2 * D);
 #pragma unroll
-            for (int i = 0; i < T::kKw; i++) t.k[h][i] = ((const uint32_t*)(row + quad * (D / 8)))[i];
-        } else {
-#pragma unroll
-            for (int c = 0; c < D / 32; c++) *(u32x4_t*)(t.k[h] + 4 * c) = *(const u32x4_t*)(row + 64 * c + 16 * quad);
-        }
+        for (int c = 0; c < D / 32; c++) *(u32x4_t*)(t.k[h] + 4 * c) = *(const u32x4_t*)(row + 64 * c + 16 * quad);
     }
+}
+template <int D, int C>
+__device__ __forceinline__ void load_v(Keys<D, false, C>& t, const uint8_t* v, int key0, int len, int n, int quad) {
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        const uint8_t* row = v + (size_t)min(key0 + 16 * (e / 4) + 4 * quad + e % 4, last) * kRow;
-        if constexpr (Q4 && D == 64) t.v[e][0] = *(const uint16_t*)(row + 2 * n);
-        else
+        const uint8_t* row = v + (size_t)min(key0 + 16 * (e / 4) + 4 * quad + e % 4, len - 1) * (2 * D);
 #pragma unroll
-            for (int i = 0; i < T::kVw; i++) t.v[e][i] = ((const uint32_t*)(row + (kRow / 16) * n))[i];
+        for (int i = 0; i < D / 32; i++) t.v[e][i] = ((const uint32_t*)(row + (D / 8) * n))[i];
     }
+}
+
+// 4-bit rows go straight to LDS, kStages steps of a wave under way, and their pairs with them: in registers the pairs alone, of which
+// sixteen lanes need each, were 32 a lane and step.  Rows lie there so that a wave's reads meet no bank twice: K's 16-byte pieces exchanged
+// by the row (16 lanes read a piece each of 16 rows), V's rows 0, 4, 8, 12, 1, ... (four quads read rows 4 apart at once).
+template <int D>
+struct Ring {
+    static constexpr int kRow = D / 2, kStages = 2, kG = D / 64;
+    static constexpr int kRows = 32 * kRow, kPairs = D == 256 ? 512 : 256;  // bytes of K or V, of their pairs
+    static constexpr int kStage = 2 * kRows + 2 * kPairs;
+    static constexpr int kLoads = 2 * (kRows / 1024) + 2 * (kPairs / 256);  // requests a stage
+    // the source of what lands at byte `at` of 16 rows
+    static __device__ __forceinline__ uint32_t k_source(uint32_t at) {
+        const uint32_t r = at / kRow, c = at % kRow / 16;
+        return r * kRow + 16 * (D == 64 ? c : D == 128 ? c ^ (r >> 2 & 3) : c ^ (r >> 1 & 7));
+    }
+    static __device__ __forceinline__ uint32_t v_source(uint32_t at) {
+        const uint32_t slot = at / kRow;
+        return (((slot & 3) << 2) + (slot >> 2)) * kRow + at % kRow;
+    }
+};
+
+template <int D>
+struct RingLanes {  // byte offsets of a lane's requests
+    uint32_t k[D == 64 ? 1 : D == 128 ? 2 : 4], v[D == 64 ? 1 : D == 128 ? 2 : 4], pair;
+    __device__ __forceinline__ RingLanes(int lane, int max_seq) {
+        using R = Ring<D>;
+#pragma unroll
+        for (int i = 0; i < R::kRows / 1024; i++) {
+            const uint32_t at = 1024u * i + 16u * lane, half = at / (16 * R::kRow);
+            k[i] = half * (16 * R::kRow) + R::k_source(at % (16 * R::kRow));
+            v[i] = half * (16 * R::kRow) + R::v_source(at % (16 * R::kRow));
+        }
+        pair = 4u * (uint32_t)(lane & 31) + (lane >= 32 ? 4u * (uint32_t)max_seq : 0u);  // (two groups a request)
+    }
+};
+
+// The requests of one step: keys [key0, key0 + 32) of a slab of `len` keys.  What lies behind the last key lands as zeros, but for pairs
+// of another group's first keys, which no visible key's place takes.  key0 >= len: all zeros, nothing is read.
+template <int D>
+__device__ __forceinline__ void ring_load(const RingLanes<D>& at, uint32_t lds, const uint8_t* k, const uint8_t* v, const uint32_t* kp, const uint32_t* vp, int max_seq, int key0, int len) {
+    using R = Ring<D>;
+    const int keys = max(0, min(kStep, len - key0));
+    const size_t from = keys ? (size_t)key0 : 0;
+    const uint32_t bytes = (uint32_t)keys * R::kRow;
+    const u32x4_t krs = make_rsrc(k + from * R::kRow, bytes), vrs = make_rsrc(v + from * R::kRow, bytes);
+#pragma unroll
+    for (int i = 0; i < R::kRows / 1024; i++) {
+        buffer_to_lds(krs, at.k[i], 0u, lds + 1024u * i);
+        buffer_to_lds(vrs, at.v[i], 0u, lds + R::kRows + 1024u * i);
+    }
+    const uint32_t pair_bytes = keys ? 4u * (uint32_t)keys + (D > 64 ? 4u * (uint32_t)max_seq : 0u) : 0u;
+#pragma unroll
+    for (int i = 0; i < R::kPairs / 256; i++) {
+        buffer_to_lds_b32(make_rsrc(kp + from + (size_t)(2 * i) * max_seq, pair_bytes), at.pair, 0u, lds + 2 * R::kRows + 256u * i);
+        buffer_to_lds_b32(make_rsrc(vp + from + (size_t)(2 * i) * max_seq, pair_bytes), at.pair, 0u, lds + 2 * R::kRows + R::kPairs + 256u * i);
+    }
+}
+// pairs of the lane's keys: of both sixteens, of one, or two of them
+template <int D, int C>
+__device__ __forceinline__ void ring_pairs(uint32_t (&to)[D / 64][8 / C], const unsigned char* pairs, int cls, int quad) {
+#pragma unroll
+    for (int g = 0; g < D / 64; g++) {
+        const unsigned char* at = pairs + 128 * g + 16 * quad;
+        if constexpr (C == 1) {
+            *(u32x4_t*)to[g] = *(const u32x4_t*)at;
+            *(u32x4_t*)(to[g] + 4) = *(const u32x4_t*)(at + 64);
+        } else if constexpr (C == 2) {
+            *(u32x4_t*)to[g] = *(const u32x4_t*)(at + 64 * cls);
+        } else {
+            *(u32x2_t*)to[g] = *(const u32x2_t*)(at + 64 * (cls >> 1) + 8 * (cls & 1));
+        }
+    }
+}
+template <int D, int C>
+__device__ __forceinline__ void ring_k(Keys<D, true, C>& t, const unsigned char* stage, int n, int cls, int quad) {
+    using R = Ring<D>;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const unsigned char* row = stage + (16 * h + n) * R::kRow;
+        if constexpr (D == 64) {
+            *(u32x2_t*)t.k[h] = *(const u32x2_t*)(row + 8 * quad);
+        } else {
+#pragma unroll
+            for (int i = 0; i < D / 128; i++) {
+                const int c = quad * (D / 128) + i;
+                *(u32x4_t*)(t.k[h] + 4 * i) = *(const u32x4_t*)(row + 16 * (D == 128 ? c ^ (n >> 2 & 3) : c ^ (n >> 1 & 7)));
+            }
+        }
+    }
+    ring_pairs<D, C>(t.ks, stage + 2 * R::kRows, cls, quad);
+}
+template <int D, int C>
+__device__ __forceinline__ void ring_v(Keys<D, true, C>& t, const unsigned char* stage, int n, int cls, int quad) {
+    using R = Ring<D>;
+    ring_pairs<D, C>(t.vs, stage + 2 * R::kRows + R::kPairs, cls, quad);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const unsigned char* row = stage + R::kRows + (16 * (e / 4) + 4 * (e % 4) + quad) * R::kRow + (D / 32) * n;
+        if constexpr (D == 64) t.v[e][0] = *(const uint16_t*)row;
+        else if constexpr (D == 128) t.v[e][0] = *(const uint32_t*)row;
+        else *(u32x2_t*)t.v[e] = *(const u32x2_t*)row;
+    }
+}
+
+// The codes at bits 4 nib of every second byte as two bf16 numbers 16 + c.  The constants stand in registers: one and-or takes no two
+// literals, and the compiler, which sees through constants, makes two instructions of it.
+struct Codes {
+    uint32_t mask, sixteen;
+    __device__ __forceinline__ Codes() {
+        asm volatile("s_mov_b32 %0, 0x780078" : "=s"(mask));
+        asm volatile("v_mov_b32 %0, 0x41804180" : "=v"(sixteen));
+    }
+    template <int kNib>
+    __device__ __forceinline__ uint32_t of(uint32_t w) const {
+        return ((kNib == 0 ? w << 3 : w >> (4 * kNib - 3)) & mask) | sixteen;
+    }
+};
+
+// The largest of the four lanes of a query row (rows of 16 lanes swapped, then halves of the wave).
+__device__ __forceinline__ float quad_max(float x) {
+    const u32x2_t a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const float y = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const u32x2_t c = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+    return fmaxf(__uint_as_float(c[0]), __uint_as_float(c[1]));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+    const u32x2_t a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const float y = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const u32x2_t c = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+    return __uint_as_float(c[0]) + __uint_as_float(c[1]);
+}
+
+// The hi and lo terms of two weights: hi by truncation, what it leaves by truncation too (16 bits in all).  Returns the sum of the terms:
+// what is taken off for the codes' offsets has to be what went in, or the truncation's bias comes back 24 times.
+__device__ __forceinline__ float two_terms(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const float ha = __uint_as_float(__float_as_uint(a) & 0xffff0000u), hb = __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+    hi = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+    const float la = a - ha, lb = b - hb;
+    lo = __builtin_amdgcn_perm(__float_as_uint(lb), __float_as_uint(la), 0x07060302u);
+    return (ha + __uint_as_float(__float_as_uint(la) & 0xffff0000u)) + (hb + __uint_as_float(__float_as_uint(lb) & 0xffff0000u));
+}
+
+// Waves that an SIMD holds.
+template <int D, bool Q4>
+constexpr int per_simd() { return D == 64 ? 4 : D == 128 ? (Q4 ? 4 : 2) : Q4 ? 2 : 1; }
+
+// What a lane has of its query row over the keys it has walked.
+template <int D, bool Q4>
+struct State {
+    static constexpr int kG = Q4 ? D / 64 : 1;
+    float m, l, ps[kG], pz[kG];  // ps: the sum of the weights as they enter the products
+    f32x4_t o[D / 16];
+    __device__ __forceinline__ void reset() {
+        m = kNoMax;
+        l = 0.0f;
+#pragma unroll
+        for (int g = 0; g < kG; g++) {
+            ps[g] = pz[g] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) o[i] = f32x4_t{0, 0, 0, 0};
+    }
+};
+
+// One step.  kCut: not every row sees all of its keys.  scores: the lane's row from key0 + 4 quad on, or null.  k_done is called
+// behind the last use of K, v_due ahead of V's first.
+template <int D, bool Q4, int C, bool kCut, bool kWeigh, typename KDone, typename VDue>
+__device__ __forceinline__ void step(State<D, Q4>& st, const Keys<D, Q4, C>& x, KDone k_done, VDue v_due, const Codes& codes, const u32x4_t (&q)[D / 32], const float (&q_sum)[Q4 ? D / 64 : 1],
+                                     int cls, int first_key, int seen, float scale_log2e, float* scores) {
+    constexpr int kG = Keys<D, Q4, C>::kG, kO = D / 16, kE = 8 / C;
+    float y[kE];
+    // of both sixteens' scores, a column's
+    auto own = [&](const f32x4_t (&a)[2], float (&to)[kE]) __attribute__((always_inline)) {
+        if constexpr (C == 1) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) to[e] = a[e / 4][e % 4];
+        } else if constexpr (C == 2) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) to[e] = cls ? a[1][e] : a[0][e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const float a0 = cls & 1 ? a[0][2 + e] : a[0][e], a1 = cls & 1 ? a[1][2 + e] : a[1][e];
+                to[e] = cls & 2 ? a1 : a0;
+            }
+        }
+    };
     if constexpr (Q4) {
 #pragma unroll
-        for (int g = 0; g < T::kG; g++)
+        for (int g = 0; g < kG; g++) {
+            const float c0 = -24.0f * q_sum[g];
+            f32x4_t a[2];
 #pragma unroll
-            for (int h = 0; h < 2; h++)
+            for (int h = 0; h < 2; h++) {
+                a[h] = f32x4_t{c0, c0, c0, c0};
+                u32x4_t lo, hi;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const size_t at = (size_t)g * max_seq + (size_t)min(key0 + 16 * h + 4 * quad + i, last);
-                    t.ks[h][g][i] = kp[at];
-                    t.vs[h][g][i] = vp[at];
+                    // dim 64: word i / 2, chunk i % 2; above: word i of (dim 128 pairs) g / 2, its group g % 2
+                    const uint32_t w = D == 64 ? x.k[h][i / 2] : x.k[h][i * (D / 128) + g / 2];
+                    const bool upper = D == 64 ? i & 1 : g & 1;
+                    lo[i] = upper ? codes.of<2>(w) : codes.of<0>(w);
+                    hi[i] = upper ? codes.of<3>(w) : codes.of<1>(w);
                 }
+                a[h] = mfma(lo, q[2 * g], a[h]);
+                a[h] = mfma(hi, q[2 * g + 1], a[h]);
+            }
+            float f[kE];
+            own(a, f);
+#pragma unroll
+            for (int e = 0; e < kE; e++) {
+                const float z = bf16_hi(x.ks[g][e]) * q_sum[g];
+                y[e] = fmaf(bf16_lo(x.ks[g][e]), f[e], g == 0 ? z : y[e] + z);
+            }
+            if (D > 64) __builtin_amdgcn_sched_barrier(0);  // (one group's words at a time in registers)
+        }
+    } else {
+        f32x4_t a[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            a[h] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) a[h] = mfma(*(const u32x4_t*)(x.k[h] + 4 * c), q[c], a[h]);
+        }
+        own(a, y);
+    }
+    k_done();
+    // the lane's keys: first_key + place(e), of its eight slots
+    auto place = [&](int e) __attribute__((always_inline)) { return C == 1 ? 16 * (e / 4) + e % 4 : C == 2 ? 16 * cls + e : 16 * (cls >> 1) + 2 * (cls & 1) + e; };
+    bool hid[kE];
+#pragma unroll
+    for (int e = 0; e < kE; e++) {
+        hid[e] = kCut && first_key + place(e) >= seen;
+        if (hid[e]) y[e] = neg_inf();
+    }
+    if constexpr (kWeigh) {
+        if (scores) {
+#pragma unroll
+            for (int e = 0; e < kE; e++)
+                if (!hid[e]) scores[place(e)] = y[e];
+        }
+    }
+    // The running maximum, common to the four lanes of a column.  It follows the scores only where they have risen by 8 in the exponent
+    // of two: up to there the weights, all of them f32 or two bf16 terms, are as exact, and sums are scaled once or twice a span.
+    float top = y[0];
+#pragma unroll
+    for (int e = 1; e < kE; e++) top = fmaxf(top, y[e]);
+    top = quad_max(top);
+    if (__any((top - st.m) * scale_log2e > 8.0f)) {
+        const float m_new = fmaxf(st.m, top), alpha = __builtin_amdgcn_exp2f((st.m - m_new) * scale_log2e);
+        st.m = m_new;
+        st.l *= alpha;
+#pragma unroll
+        for (int g = 0; g < kG; g++) {
+            st.ps[g] *= alpha;
+            st.pz[g] *= alpha;
+        }
+#pragma unroll
+        for (int i = 0; i < kO; i++) st.o[i] *= alpha;
+    }
+    float w[kE];
+#pragma unroll
+    for (int e = 0; e < kE; e++) {
+        w[e] = __builtin_amdgcn_exp2f((y[e] - st.m) * scale_log2e);
+        st.l += w[e];
+    }
+    // pairs of weights as the operand's words, zeros in the other columns' places
+    auto operand = [&](const float (&f)[kE], u32x4_t& hi, u32x4_t& lo) __attribute__((always_inline)) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kE / 2; i++) {
+            uint32_t a, c;
+            sum += two_terms(f[2 * i], f[2 * i + 1], a, c);
+            if constexpr (C == 1) {
+                hi[i] = a;
+                lo[i] = c;
+            } else {
+#pragma unroll
+                for (int j = 0; j < C; j++) {
+                    hi[j * (kE / 2) + i] = cls == j ? a : 0u;
+                    lo[j * (kE / 2) + i] = cls == j ? c : 0u;
+                }
+            }
+        }
+        return sum;
+    };
+    // out^T
+    v_due();
+    if constexpr (Q4) {
+#pragma unroll
+        for (int g = 0; g < kG; g++) {
+            u32x4_t p_hi, p_lo;
+            float s[kE];
+#pragma unroll
+            for (int e = 0; e < kE; e++) {
+                s[e] = hid[e] ? 0.0f : w[e] * bf16_lo(x.vs[g][e]);  // (what a hidden row holds stays out, were it NaN)
+                if (kCut) st.pz[g] += hid[e] ? 0.0f : w[e] * bf16_hi(x.vs[g][e]);
+                else st.pz[g] = fmaf(w[e], bf16_hi(x.vs[g][e]), st.pz[g]);
+            }
+            st.ps[g] += operand(s, p_hi, p_lo);
+            // the bytes whose chunks are of this group
+#pragma unroll
+            for (int f = 0; f < 2; f++) {
+                const int byte = D == 64 ? f : (g & 1) + 2 * f, word = D == 64 ? 0 : g / 2;
+                u32x4_t lo, hi;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t z = __builtin_amdgcn_perm(x.v[2 * i + 1][word], x.v[2 * i][word], 0x0c000c00u | (uint32_t)(4 + byte) << 16 | (uint32_t)byte);
+                    lo[i] = codes.of<0>(z);
+                    hi[i] = codes.of<1>(z);
+                }
+                const int at_o = 8 * word + 2 * byte;
+                st.o[at_o] = mfma(lo, p_lo, mfma(lo, p_hi, st.o[at_o]));
+                st.o[at_o + 1] = mfma(hi, p_lo, mfma(hi, p_hi, st.o[at_o + 1]));
+                if (D > 64) __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    } else {
+        u32x4_t p_hi, p_lo;
+        operand(w, p_hi, p_lo);
+#pragma unroll
+        for (int d = 0; d < kO; d++) {  // dim n * (D / 16) + d
+            u32x4_t a;
+#pragma unroll
+            for (int i = 0; i < 4; i++) a[i] = __builtin_amdgcn_perm(x.v[2 * i + 1][d / 2], x.v[2 * i][d / 2], d & 1 ? 0x07060302u : 0x05040100u);
+            st.o[d] = mfma(a, p_lo, mfma(a, p_hi, st.o[d]));
+        }
     }
 }
 
-constexpr uint32_t kCode = 0x00780078u, kSixteen = 0x41804180u;
-// the codes at bits 4 nib of every second byte pair as two bf16 numbers 16 + c
-template <int kNib>
-__device__ __forceinline__ uint32_t codes_of(uint32_t w) {
-    return ((kNib == 0 ? w << 3 : w >> (4 * kNib - 3)) & kCode) | kSixteen;
-}
+template <int D, bool Q4, int C, bool kWeigh>
+__global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4>())) void cache_attend_kernel(CacheAttendParams p) {
+    constexpr int kG = Keys<D, Q4, C>::kG, NT = 64 * kWaves, kPitch = D + 4, kR = 16 / C;  // kR query rows
+    constexpr int kRingBytes = Q4 ? kWaves * Ring<D>::kStages * Ring<D>::kStage : 0, kFold = kWaves * 16 * kPitch * 4, kFolds = kMaxPieces * 16 * 8 + NT * 16;
+    constexpr int kLds = std::max(std::max(kRingBytes, kFold), kFolds);
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[kLds];
+    __shared__ float red_m[kWaves][16], red_l[kWaves][16], inv_l[16];
+    __shared__ int is_last;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, quad = lane >> 4, cls = n / kR, group = blockIdx.x;
+    const int per = p.kv_heads * p.n_tiles;
 
-// The hi and lo terms of two weights: hi by truncation, what it leaves by truncation too (16 bits in all).
-__device__ __forceinline__ void two_terms(float a, float b, uint32_t& hi, uint32_t& lo) {
-    const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
-    hi = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
-    const float la = a - __uint_as_float(ua & 0xffff0000u), lb = b - __uint_as_float(ub & 0xffff0000u);
-    lo = __builtin_amdgcn_perm(__float_as_uint(lb), __float_as_uint(la), 0x07060302u);
-}
-
-template <int D, bool Q4, bool kWeigh>
-__global__ __launch_bounds__(64) void cache_attend_kernel(CacheAttendParams p) {
-    using T = Keys<D, Q4>;
-    constexpr int kG = T::kG, kO = D / 16;
-    const int lane = threadIdx.x, n = lane & 15, quad = lane >> 4;
-    const int total = steps_before(p, p.batch, lane), span = span_of(p, total);
-    const long long begin = (long long)blockIdx.x * span;
-    if (begin >= total) return;
-    int at = (int)begin;
-    const int end = (int)min((long long)total, begin + span);
-    int b, first;
-    find_sequence(p, at, lane, &b, &first);
+    const Span span = span_of(p, group, lane);
+    // sequences without keys, dealt to the workgroups: rows of zeros
+    if (p.kv_lens)
+        for (int b = group; b < p.batch; b += (int)gridDim.x)
+            if (len_of(p, b) == 0)
+                for (int i = tid; i < p.seq_new * p.heads * (D / 8); i += NT) *(u32x4_t*)(p.out + (size_t)b * p.seq_new * p.heads * D + 8 * i) = u32x4_t{0, 0, 0, 0};
+    const long long begin = (long long)group * span.size;
+    if (begin >= span.total) return;
+    int at = (int)begin, b = span.b, first = span.first;
+    const int end = (int)min((long long)span.total, begin + span.size);
 
     while (at < end) {
         // the piece of a segment from here
-        const int len = len_of(p, b), st = steps_of(len);
-        if (st == 0 || at >= first + st * p.kv_heads * p.n_tiles) {  // the next sequence
-            first += st * p.kv_heads * p.n_tiles;
+        const int len = len_of(p, b), steps = steps_of(len);
+        if (at >= first + steps * per) {  // the next sequence
+            first += steps * per;
             b++;
             continue;
         }
-        const int seg = (at - first) / st, t0 = (at - first) - seg * st, t1 = min(st, t0 + (end - at));
+        const int seg = (at - first) / steps, seg_first = first + seg * steps, t0 = at - seg_first, t1 = min(steps, t0 + (end - at));
         const int kvh = seg / p.n_tiles, tile = seg - kvh * p.n_tiles;
+        const int w0 = seg_first / span.size, pieces = (seg_first + steps - 1) / span.size - w0 + 1;  // workgroups that have some of it
+        const size_t segment = (size_t)b * per + seg;
         at += t1 - t0;
 
-        const int r = tile * 16 + n;  // the query row: position * group + head of the group
+        const int r = tile * kR + n % kR;  // the query row: position * group + head of the group
         const bool there = r < p.rows;
         const int s_new = there ? r / p.group : 0, head = kvh * p.group + (there ? r - s_new * p.group : 0);
         const int seen = len - p.seq_new + s_new + 1;  // keys that it sees
-        const size_t q_at = (((size_t)b * p.seq_new + s_new) * p.heads + head) * D;
+        const size_t slab = ((size_t)b * p.kv_heads + kvh) * (size_t)p.max_seq;
 
         // q as the operand that the keys' words pair with
         u32x4_t q[D / 32];
-        float q_sum[kG];
-        {
-            u32x4_t nat[D / 32];
+        float q_sum[kG] = {};
+        u32x4_t nat[D / 32];
 #pragma unroll
-            for (int c = 0; c < D / 32; c++) {
-                nat[c] = u32x4_t{0, 0, 0, 0};
-                if (there) nat[c] = *(const u32x4_t*)(p.q + q_at + 32 * c + 8 * quad);
-            }
-            if constexpr (!Q4) {
-#pragma unroll
-                for (int c = 0; c < D / 32; c++) q[c] = nat[c];
-            } else {
-#pragma unroll
-                for (int g = 0; g < kG; g++) {
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int c = 2 * g; c < 2 * g + 2; c++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) sum += bf16_lo(nat[c][i]) + bf16_hi(nat[c][i]);
-                    sum += __shfl_xor(sum, 16, 64);
-                    sum += __shfl_xor(sum, 32, 64);
-                    q_sum[g] = sum;
-#pragma unroll
-                    for (int par = 0; par < 2; par++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            // dim 64: word (u, c) pairs i's of one chunk; above: chunks 2 g and 2 g + 1 at one i
-                            const uint32_t a = D == 64 ? nat[i & 1][i & 2] : nat[2 * g][i], o = D == 64 ? nat[i & 1][(i & 2) + 1] : nat[2 * g + 1][i];
-                            q[2 * g + par][i] = __builtin_amdgcn_perm(o, a, par ? 0x07060302u : 0x05040100u);
-                        }
-                }
-            }
+        for (int c = 0; c < D / 32; c++) {
+            nat[c] = u32x4_t{0, 0, 0, 0};
+            if (there) nat[c] = *(const u32x4_t*)(p.q + (((size_t)b * p.seq_new + s_new) * p.heads + head) * D + 32 * c + 8 * quad);
         }
-        const size_t slab = ((size_t)b * p.kv_heads + kvh) * (size_t)p.max_seq;
+        const RingLanes<D> lanes(lane, p.max_seq);
         constexpr int kRow = Q4 ? D / 2 : 2 * D;
         const uint8_t* k = (const uint8_t*)p.k + slab * kRow;
         const uint8_t* v = (const uint8_t*)p.v + slab * kRow;
         const uint32_t* kp = Q4 ? p.k_pairs + slab * kG : nullptr;
         const uint32_t* vp = Q4 ? p.v_pairs + slab * kG : nullptr;
-        const int all_see = len - p.seq_new + 1;  // keys that every row sees
-
-        float m = kNoMax, l = 0.0f, pz[kG] = {};
-        f32x4_t o[kO], ps[kG] = {};  // ps: the sums of the weights as they enter the products, by a row of ones
+        const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds + (uint32_t)wave * (Q4 ? Ring<D>::kStages * Ring<D>::kStage : 0);
+        const unsigned char* const ring_at = lds + wave * (Q4 ? Ring<D>::kStages * Ring<D>::kStage : 0);
+        Keys<D, Q4, C> x;
+        if constexpr (Q4) {
 #pragma unroll
-        for (int i = 0; i < kO; i++) o[i] = f32x4_t{0, 0, 0, 0};
-
-        for (int t = t0; t < t1; t++) {
-            const int key0 = t * kStep;
-            T x;
-            load_keys<D, Q4>(x, k, v, kp, vp, p.max_seq, key0, len, n, quad);
-            // scores^T
-            float y[8];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                if constexpr (Q4) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) y[4 * h + i] = 0.0f;
-#pragma unroll
-                    for (int g = 0; g < kG; g++) {
-                        const float c0 = -24.0f * q_sum[g];
-                        f32x4_t a = {c0, c0, c0, c0};
-                        u32x4_t lo, hi;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            // dim 64: word i / 2, chunk i % 2; above: word i of (dim 128 pairs) g / 2, its group g % 2
-                            const uint32_t w = D == 64 ? x.k[h][i / 2] : x.k[h][i * (D / 128) + g / 2];
-                            const bool upper = D == 64 ? i & 1 : g & 1;
-                            lo[i] = upper ? codes_of<2>(w) : codes_of<0>(w);
-                            hi[i] = upper ? codes_of<3>(w) : codes_of<1>(w);
-                        }
-                        a = mfma(lo, q[2 * g], a);
-                        a = mfma(hi, q[2 * g + 1], a);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) y[4 * h + i] += bf16_lo(x.ks[h][g][i]) * a[i] + bf16_hi(x.ks[h][g][i]) * q_sum[g];
-                    }
-                } else {
-                    f32x4_t a = {0, 0, 0, 0};
-#pragma unroll
-                    for (int c = 0; c < D / 32; c++) a = mfma(*(const u32x4_t*)(x.k[h] + 4 * c), q[c], a);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) y[4 * h + i] = a[i];
-                }
-            }
-            const bool cut = key0 + kStep > all_see;  // some row does not see all of them
-            bool hid[8] = {};
-            if (cut) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    hid[e] = key0 + 16 * (e / 4) + 4 * quad + e % 4 >= seen;
-                    if (hid[e]) y[e] = neg_inf();
-                }
-            }
-            if constexpr (kWeigh) {
-                if (there) {
-                    float* dst = p.scores + ((size_t)b * p.heads + head) * (size_t)p.max_seq + key0 + 4 * quad;
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (!hid[e]) dst[16 * (e / 4) + e % 4] = y[e];
-                }
-            }
-            // the running maximum, common to the four lanes of a query row
-            float top = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            if (__any(top > m)) {
-                const float m_new = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f((m - m_new) * p.scale_log2e);
-                m = m_new;
-                l *= alpha;
-#pragma unroll
-                for (int g = 0; g < kG; g++) {
-                    ps[g] *= alpha;  // (rows alike: one would do)
-                    pz[g] *= alpha;
-                }
-#pragma unroll
-                for (int i = 0; i < kO; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) o[i][e] *= alpha;
-            }
-            float w[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                w[e] = __builtin_amdgcn_exp2f((y[e] - m) * p.scale_log2e);
-                l += w[e];
-            }
-            // out^T
-#pragma unroll
-            for (int g = 0; g < kG; g++) {
-                u32x4_t p_hi, p_lo;
-                if constexpr (Q4) {
-                    float s[8];
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const uint32_t pr = x.vs[e / 4][g][e % 4];
-                        s[e] = hid[e] ? 0.0f : w[e] * bf16_lo(pr);  // (what a hidden row holds stays out, were it NaN)
-                        pz[g] += hid[e] ? 0.0f : w[e] * bf16_hi(pr);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        uint32_t a, c;
-                        two_terms(s[2 * i], s[2 * i + 1], a, c);
-                        p_hi[i] = a;
-                        p_lo[i] = c;
-                    }
-                    constexpr u32x4_t kOnes = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-                    ps[g] = mfma(kOnes, p_lo, mfma(kOnes, p_hi, ps[g]));
-                    // the bytes whose chunks are of this group
-#pragma unroll
-                    for (int f = 0; f < 2; f++) {
-                        const int byte = D == 64 ? f : (g & 1) + 2 * f, word = D == 64 ? 0 : g / 2;
-                        u32x4_t lo, hi;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const uint32_t z = __builtin_amdgcn_perm(x.v[2 * i + 1][word], x.v[2 * i][word], 0x0c000c00u | (uint32_t)(4 + byte) << 16 | (uint32_t)byte);
-                            lo[i] = codes_of<0>(z);
-                            hi[i] = codes_of<1>(z);
-                        }
-                        const int at_o = 8 * word + 2 * byte;
-                        o[at_o] = mfma(lo, p_lo, mfma(lo, p_hi, o[at_o]));
-                        o[at_o + 1] = mfma(hi, p_lo, mfma(hi, p_hi, o[at_o + 1]));
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        uint32_t a, c;
-                        two_terms(w[2 * i], w[2 * i + 1], a, c);
-                        p_hi[i] = a;
-                        p_lo[i] = c;
-                    }
-#pragma unroll
-                    for (int d = 0; d < kO; d++) {  // dim n * (D / 16) + d
-                        u32x4_t a;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) a[i] = __builtin_amdgcn_perm(x.v[2 * i + 1][d / 2], x.v[2 * i][d / 2], d & 1 ? 0x07060302u : 0x05040100u);
-                        o[d] = mfma(a, p_lo, mfma(a, p_hi, o[d]));
-                    }
-                }
+            for (int s = 0; s < Ring<D>::kStages; s++) ring_load<D>(lanes, ring + s * Ring<D>::kStage, k, v, kp, vp, p.max_seq, (t0 + wave + s * kWaves) * kStep, t0 + wave + s * kWaves < t1 ? len : 0);
+        } else {
+            if (t0 + wave < t1) {
+                load_k<D, C>(x, k, (t0 + wave) * kStep, len, n, quad);
+                load_v<D, C>(x, v, (t0 + wave) * kStep, len, n, quad);
             }
         }
+        SegmentWord word{(word_t*)(p.words + segment * kWordPitch), p.launch_id};
+        if (pieces > 1 && tid == 0) word.claim();
+        if constexpr (!Q4) {
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) q[c] = nat[c];
+        } else {
+#pragma unroll
+            for (int g = 0; g < kG; g++) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int c = 2 * g; c < 2 * g + 2; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sum += bf16_lo(nat[c][i]) + bf16_hi(nat[c][i]);
+                q_sum[g] = quad_sum(sum);
+#pragma unroll
+                for (int par = 0; par < 2; par++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        // dim 64: word (u, c) pairs i's of one chunk; above: chunks 2 g and 2 g + 1 at one i
+                        const uint32_t a = D == 64 ? nat[i & 1][i & 2] : nat[2 * g][i], o = D == 64 ? nat[i & 1][(i & 2) + 1] : nat[2 * g + 1][i];
+                        q[2 * g + par][i] = __builtin_amdgcn_perm(o, a, par ? 0x07060302u : 0x05040100u);
+                    }
+            }
+        }
+        const int all_see = len - p.seq_new + 1;  // keys that every row sees
+        float* const scores = kWeigh && there ? p.scores + ((size_t)b * p.heads + head) * (size_t)p.max_seq + 4 * quad : nullptr;
 
-        // sums over the four lanes of a query row
-        auto row_sum = [](float f) {
-            f += __shfl_xor(f, 16, 64);
-            return f + __shfl_xor(f, 32, 64);
+        const Codes codes;
+        State<D, Q4> st;
+        st.reset();
+        // Steps that every row sees whole, then the others, in loops of their own: as two branches of one loop they would have the sums in
+        // two sets of registers.
+        const int t_whole = min(t1, max(all_see, 0) / kStep);
+        int t = t0 + wave, stage = 0;
+        auto take = [&](auto cut) __attribute__((always_inline)) {
+            constexpr bool kCut = decltype(cut)::value;
+            const int key0 = t * kStep;
+            float* const to = kWeigh && there ? scores + key0 : nullptr;
+            if constexpr (Q4) {
+                // (all but the newest kStages - 1 steps' requests are there)
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Ring<D>::kLoads * (Ring<D>::kStages - 1)) : "memory");
+                const unsigned char* const rows = ring_at + stage * Ring<D>::kStage;
+                ring_k<D, C>(x, rows, n, cls, quad);
+                step<D, Q4, C, kCut, kWeigh>(st, x, [] {}, [&]() __attribute__((always_inline)) { ring_v<D, C>(x, rows, n, cls, quad); }, codes, q, q_sum, cls, key0 + 4 * quad, seen, p.scale_log2e, to);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read before it is written again)
+                const int next = t + Ring<D>::kStages * kWaves;
+                ring_load<D>(lanes, ring + stage * Ring<D>::kStage, k, v, kp, vp, p.max_seq, next * kStep, next < t1 ? len : 0);
+                stage = stage + 1 == Ring<D>::kStages ? 0 : stage + 1;
+            } else {
+                const int next = t + kWaves;
+                step<D, Q4, C, kCut, kWeigh>(st, x, [&]() __attribute__((always_inline)) { if (next < t1) load_k<D, C>(x, k, next * kStep, len, n, quad); }, [] {}, codes, q, q_sum, cls, key0 + 4 * quad, seen,
+                                             p.scale_log2e, to);
+                if (next < t1) load_v<D, C>(x, v, next * kStep, len, n, quad);
+            }
+            t += kWaves;
         };
-        l = row_sum(l);
+        while (t < t_whole) take(std::false_type{});
+        while (t < t1) take(std::true_type{});
+        if constexpr (Q4) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (what is still under way lands in memory of the fold)
+
+        // ---- fold the four waves, and the columns of a row.  (The thread's number anew: what follows from it would be worked out
+        // ahead of the steps otherwise, and take their registers.)
+        int ft = threadIdx.x;
+        asm volatile("" : "+v"(ft));
+        const int tid = ft, lane = ft & 63, n = ft & 15, quad = lane >> 4;
+        const float l = quad_sum(st.l);
         if constexpr (Q4) {
 #pragma unroll
             for (int g = 0; g < kG; g++) {
-                const float off = row_sum(pz[g]) - 24.0f * ps[g][0];
+                const float off = quad_sum(st.pz[g]) - 24.0f * quad_sum(st.ps[g]);
 #pragma unroll
                 for (int f = 0; f < 4; f++) {
-                    const int byte = D == 64 ? f / 2 : (g & 1) + 2 * (f / 2), i = 8 * (D == 64 ? 0 : g / 2) + 2 * byte + f % 2;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) o[i][e] += off;
+                    const int byte = D == 64 ? f / 2 : (g & 1) + 2 * (f / 2);
+                    st.o[8 * (D == 64 ? 0 : g / 2) + 2 * byte + f % 2] += off;
                 }
             }
         }
-        // a lane's eight dims in a row: of chunk c (dims 32 c + 8 quad on), or of lane row 4 quad + i
-        const bool alone = t0 == 0 && t1 == st;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        if (there) {
-            auto dims = [&](int c, float (&f)[8]) {
+        if (quad == 0) {
+            red_m[wave][n] = st.m;
+            red_l[wave][n] = l;
+        }
+        __syncthreads();  // also: every wave is done with the ring
+        float m_wg = kNoMax, l_wg = 0.0f;  // of row n % kR
+#pragma unroll
+        for (int w = 0; w < kWaves; w++)
+#pragma unroll
+            for (int c = 0; c < C; c++) m_wg = fmaxf(m_wg, red_m[w][n % kR + c * kR]);
+#pragma unroll
+        for (int w = 0; w < kWaves; w++)
+#pragma unroll
+            for (int c = 0; c < C; c++) l_wg += red_l[w][n % kR + c * kR] * __builtin_amdgcn_exp2f((red_m[w][n % kR + c * kR] - m_wg) * p.scale_log2e);
+        float* const red = (float*)lds;
+        {
+            const float f = __builtin_amdgcn_exp2f((st.m - m_wg) * p.scale_log2e);
+            float* row = red + (wave * 16 + n) * kPitch;
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) {  // eight dims in a row
+                float y[8];
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     if constexpr (Q4) {
                         const int byte = D == 64 ? c : (c & ~3) | (c & 1) << 1 | (c >> 1 & 1);
-                        f[e] = o[2 * byte + e % 2][e / 2];
-                    } else {  // dims (4 quad + i) * (D / 16) + d: 8 c on of the lane's D / 4
-                        f[e] = o[(8 * c + e) % (D / 16)][(8 * c + e) / (D / 16)];
+                        y[e] = st.o[2 * byte + e % 2][e / 2] * f;
+                    } else {
+                        y[e] = st.o[(8 * c + e) % (D / 16)][(8 * c + e) / (D / 16)] * f;
                     }
                 }
-            };
-            auto dim_of = [&](int c) { return Q4 ? 32 * c + 8 * quad : quad * (D / 4) + 8 * c; };
-            if (alone) {
+                float* dst = row + (Q4 ? 32 * c + 8 * quad : quad * (D / 4) + 8 * c);
+                *(f32x4_t*)dst = f32x4_t{y[0], y[1], y[2], y[3]};
+                *(f32x4_t*)(dst + 4) = f32x4_t{y[4], y[5], y[6], y[7]};
+            }
+        }
+        if (wave == 0 && quad == 0 && n < kR) inv_l[n] = l_wg == 0.0f ? 0.0f : 1.0f / l_wg;
+        __syncthreads();
+        const int rows = min(kR, p.rows - tile * kR);
+        const uint32_t slot_bytes = (uint32_t)p.part_rows * (D + 2) * 4;
+        float* const slot = p.part + ((size_t)w0 + segment) * (slot_bytes / 4);  // of the segment's first piece; the others follow
+        const uint32_t mine = (uint32_t)(group - w0) * slot_bytes;
+        const __amdgpu_buffer_rsrc_t rs = rsrc_of(slot, (uint32_t)pieces * slot_bytes);
+        auto out_row = [&](int row) {  // of the tile
+            const int rr = tile * kR + row, s = rr / p.group;
+            return (((size_t)b * p.seq_new + s) * p.heads + kvh * p.group + (rr - s * p.group)) * D;
+        };
+        for (int i = tid; i < rows * (D / 4); i += NT) {
+            const int row = i / (D / 4), d = 4 * (i % (D / 4));
+            f32x4_t o = {0, 0, 0, 0};
 #pragma unroll
-                for (int c = 0; c < D / 32; c++) {
-                    float f[8];
-                    dims(c, f);
-                    *(u32x4_t*)(p.out + q_at + dim_of(c)) = u32x4_t{pack_bf16x2(f[0] * inv, f[1] * inv), pack_bf16x2(f[2] * inv, f[3] * inv), pack_bf16x2(f[4] * inv, f[5] * inv),
-                                                                  pack_bf16x2(f[6] * inv, f[7] * inv)};
-                }
-                if (kWeigh && quad == 0) {
-                    float* st_at = p.stats + ((size_t)b * p.heads + head) * 2;
-                    st_at[0] = m;
-                    st_at[1] = inv;
-                }
+            for (int w = 0; w < kWaves * C; w++) o += *(const f32x4_t*)(red + (w * kR + row) * kPitch + d);
+            if (pieces == 1) {
+                o *= inv_l[row];
+                *(u32x2_t*)(p.out + out_row(row) + d) = u32x2_t{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
             } else {
-                const size_t segment = ((size_t)b * p.kv_heads + kvh) * p.n_tiles + tile;
-                float* slot = p.part + ((size_t)blockIdx.x + segment) * p.part_rows * (D + 2);
+                put4(rs, mine + 4u * (uint32_t)(row * D + d), o);
+            }
+        }
+        if (pieces == 1) {
+            if (kWeigh && tid < rows) {
+                float* to = p.stats + ((size_t)b * p.heads + kvh * p.group + tile * kR + tid) * 2;  // (one position: rows are heads)
+                to[0] = m_wg;
+                to[1] = inv_l[tid];
+            }
+            __syncthreads();  // (the next piece's requests land where the fold was)
+            continue;
+        }
+        if (tid < rows) put2(rs, mine + 4u * (uint32_t)(p.part_rows * D + 2 * tid), m_wg, l_wg);  // (tid < kR: n is tid)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (tid == 0) is_last = word.count(pieces) ? 1 : 0;
+        __syncthreads();
+        if (is_last) {
+            // ---- the last workgroup of the segment: the weighted sum of its partials, the weights first
+            float* const wgt = (float*)lds;  // [pieces][16] (m, then the factor), l behind
+            float* const wl = wgt + kMaxPieces * 16;
+            f32x4_t* const part = (f32x4_t*)(wl + kMaxPieces * 16);
+            for (int i = tid; i < pieces * rows; i += NT) {
+                const int piece = i / rows, row = i - piece * rows;
+                const u32x2_t ml = get2(rs, (uint32_t)piece * slot_bytes + 4u * (uint32_t)(p.part_rows * D + 2 * row));
+                wgt[piece * 16 + row] = __uint_as_float(ml[0]);
+                wl[piece * 16 + row] = __uint_as_float(ml[1]);
+            }
+            __syncthreads();
+            for (int row = wave; row < rows; row += kWaves) {
+                float m = kNoMax, sum = 0.0f;
+                for (int i = lane; i < pieces; i += 64) m = fmaxf(m, wgt[i * 16 + row]);
 #pragma unroll
-                for (int c = 0; c < D / 32; c++) {
-                    float f[8];
-                    dims(c, f);
-                    float* dst = slot + n * D + dim_of(c);
-                    *(f32x4_t*)dst = f32x4_t{f[0], f[1], f[2], f[3]};
-                    *(f32x4_t*)(dst + 4) = f32x4_t{f[4], f[5], f[6], f[7]};
+                for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+                for (int i = lane; i < pieces; i += 64) {
+                    const float f = __builtin_amdgcn_exp2f((wgt[i * 16 + row] - m) * p.scale_log2e);
+                    wgt[i * 16 + row] = f;
+                    sum += wl[i * 16 + row] * f;
                 }
-                if (quad == 0) {
-                    slot[p.part_rows * D + n] = m;
-                    slot[p.part_rows * (D + 1) + n] = l;
+#pragma unroll
+                for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+                if (lane == 0) {
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    inv_l[row] = inv;
+                    if (kWeigh) {
+                        float* to = p.stats + ((size_t)b * p.heads + kvh * p.group + tile * kR + row) * 2;
+                        to[0] = m;
+                        to[1] = inv;
+                    }
+                }
+            }
+            __syncthreads();
+            // items of four elements; where there are fewer than threads, several threads an item, each with every sub-th piece
+            const int items = rows * (D / 4), sub_n = items >= NT ? 1 : NT / items;
+            for (int i0 = 0; i0 < items; i0 += NT) {
+                const int i = i0 + (sub_n == 1 ? tid : tid % items), sub = sub_n == 1 ? 0 : tid / items;
+                const bool on = i < items && sub < sub_n;
+                const int row = on ? i / (D / 4) : 0, d = on ? 4 * (i % (D / 4)) : 0;
+                f32x4_t o = {0, 0, 0, 0};
+                for (int k0 = sub; on && k0 < pieces; k0 += 8 * sub_n) {  // eight loads at a time
+                    f32x4_t a[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) a[e] = get4(rs, (uint32_t)min(k0 + e * sub_n, pieces - 1) * slot_bytes + 4u * (uint32_t)(row * D + d));
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (k0 + e * sub_n < pieces) o += a[e] * wgt[(k0 + e * sub_n) * 16 + row];
+                }
+                if (sub_n > 1) {
+                    part[tid] = o;
+                    __syncthreads();
+                    if (on && sub == 0)
+                        for (int e = 1; e < sub_n; e++) o += part[e * items + tid];
+                }
+                if (on && sub == 0) {
+                    o *= inv_l[row];
+                    *(u32x2_t*)(p.out + out_row(row) + d) = u32x2_t{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
                 }
             }
         }
-    }
-}
-
-// Folds the partials of a segment that more than one wave walked; rows without keys are zeros.  Grid (rows of a kv head, kv heads,
-// batch), a thread a dim.
-template <int D, bool kWeigh>
-__global__ __launch_bounds__(D) void cache_merge_kernel(CacheAttendParams p) {
-    const int d = threadIdx.x, lane = d & 63, r = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
-    const int total = steps_before(p, p.batch, lane), first = steps_before(p, b, lane), span = span_of(p, total);
-    const int st = steps_of(len_of(p, b)), tile = r / 16, n = r % 16;
-    const int s_new = r / p.group, head = kvh * p.group + r - s_new * p.group;
-    const int seg = kvh * p.n_tiles + tile, at = first + seg * st;
-    const size_t out_at = (((size_t)b * p.seq_new + s_new) * p.heads + head) * D + d;
-    float* stats = kWeigh ? p.stats + ((size_t)b * p.heads + head) * 2 : nullptr;
-    if (st == 0) {
-        p.out[out_at] = 0;
-        return;
-    }
-    const int w0 = at / span, w1 = (at + st - 1) / span;
-    if (w0 == w1) return;  // the one wave has written it
-    const size_t segment = (size_t)b * p.kv_heads * p.n_tiles + seg, slot_size = (size_t)p.part_rows * (D + 2);
-    const float* slot = p.part + (w0 + segment) * slot_size;
-    float m = kNoMax;
-    for (int w = 0; w <= w1 - w0; w++) m = fmaxf(m, slot[w * slot_size + p.part_rows * D + n]);
-    float o = 0.0f, l = 0.0f;
-    for (int w = 0; w <= w1 - w0; w++) {
-        const float* s = slot + w * slot_size;
-        const float f = __builtin_amdgcn_exp2f((s[p.part_rows * D + n] - m) * p.scale_log2e);
-        o += s[n * D + d] * f;
-        l += s[p.part_rows * (D + 1) + n] * f;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    p.out[out_at] = f32_to_bf16_bits(o * inv);
-    if (kWeigh && d == 0) {
-        stats[0] = m;
-        stats[1] = inv;
+        __syncthreads();
     }
 }
 
@@ -474,34 +795,44 @@ __global__ __launch_bounds__(256) void cache_weigh_kernel(CacheAttendParams p) {
 
 template <int D, bool Q4, bool kWeigh>
 hipError_t launch_attend_as(hipStream_t stream, const CacheAttendParams& p) {
-    hipLaunchKernelGGL((cache_attend_kernel<D, Q4, kWeigh>), dim3(p.n_waves), dim3(64), 0, stream, p);
-    hipLaunchKernelGGL((cache_merge_kernel<D, kWeigh>), dim3(p.rows, p.kv_heads, p.batch), dim3(D), 0, stream, p);
+    const dim3 grid(p.n_groups), block(64 * kWaves);
+    if (p.rows <= 4) hipLaunchKernelGGL((cache_attend_kernel<D, Q4, 4, kWeigh>), grid, block, 0, stream, p);
+    else if (p.rows <= 8) hipLaunchKernelGGL((cache_attend_kernel<D, Q4, 2, kWeigh>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((cache_attend_kernel<D, Q4, 1, kWeigh>), grid, block, 0, stream, p);
     if (kWeigh && p.max_seq > 0)
         hipLaunchKernelGGL(cache_weigh_kernel, dim3((p.max_seq + 1023) / 1024, p.kv_heads, p.batch), dim3(256), 0, stream, p);
     return hipGetLastError();
 }
-
 template <bool Q4, bool kWeigh>
 hipError_t launch_attend(hipStream_t stream, const CacheAttendParams& p, int dim) {
     return dim == 64 ? launch_attend_as<64, Q4, kWeigh>(stream, p) : dim == 128 ? launch_attend_as<128, Q4, kWeigh>(stream, p) : launch_attend_as<256, Q4, kWeigh>(stream, p);
 }
 
-// Segments, steps and waves of a call at its longest.
+// Segments, steps and workgroups of a call at its longest, and what its workspace holds.
 struct AttendPlan {
     int64_t rows, n_tiles, segments, steps;
-    int waves, part_rows;
-    size_t part_bytes, score_bytes, stat_bytes;
+    int groups, part_rows;
+    size_t part_bytes, word_bytes, score_bytes, stat_bytes;
+    size_t bytes() const { return part_bytes + word_bytes + score_bytes + stat_bytes; }
 };
-AttendPlan plan_attend(int64_t batch, int64_t seq_new, int64_t heads, int64_t kv_heads, int64_t dim, int64_t max_seq, bool weigh) {
+// workgroups that the chip holds at once (a wave of each on every SIMD)
+int groups_at_once(int64_t dim, bool q4) {
+    if (dim == 64) return kCus * per_simd<64, true>();
+    if (dim == 128) return kCus * (q4 ? per_simd<128, true>() : per_simd<128, false>());
+    return kCus * (q4 ? per_simd<256, true>() : per_simd<256, false>());
+}
+// (q4: the same workspace serves either kind of cache, so it is sized for the one with more workgroups)
+AttendPlan plan_attend(int64_t batch, int64_t seq_new, int64_t heads, int64_t kv_heads, int64_t dim, int64_t max_seq, bool weigh, bool q4 = true) {
     AttendPlan a{};
     a.rows = seq_new * (heads / kv_heads);
     a.n_tiles = (a.rows + 15) / 16;
     a.segments = batch * kv_heads * a.n_tiles;
     a.steps = a.segments * ((max_seq + kStep - 1) / kStep);
-    a.waves = (int)std::min<int64_t>(kMaxWaves, std::max<int64_t>(a.steps, 1));
+    a.groups = (int)std::min<int64_t>(groups_at_once(dim, q4), std::max<int64_t>((a.steps + kWaves - 1) / kWaves, 1));
     a.part_rows = (int)std::min<int64_t>(16, a.rows);
     auto round = [](size_t x) { return (x + 255) / 256 * 256; };
-    a.part_bytes = round(((size_t)a.waves + (size_t)a.segments) * (size_t)a.part_rows * (size_t)(dim + 2) * 4);
+    a.part_bytes = round(((size_t)a.groups + (size_t)a.segments) * (size_t)a.part_rows * (size_t)(dim + 2) * 4);
+    a.word_bytes = (size_t)a.segments * kWordPitch;
     if (weigh) {
         a.score_bytes = round((size_t)batch * (size_t)heads * (size_t)max_seq * 4);
         a.stat_bytes = round((size_t)batch * (size_t)heads * 8);
@@ -521,14 +852,15 @@ int attend_common(void* stream, CacheAttendParams& p, int head_dim, bool q4, boo
         return fail(err, RT_ERR_KV_OVERFLOW, -1, (uint64_t)p.max_seq, (uint64_t)(int64_t)p.kv_len, "kv_len must cover the new positions and fit the cache");
     if (p.batch == 0 || p.heads == 0 || p.seq_new == 0) return RT_OK;
     const AttendPlan a = plan_attend(p.batch, p.seq_new, p.heads, p.kv_heads, head_dim, p.max_seq, weigh);
-    if (a.steps + a.segments > 0x7fffffffll - kMaxWaves || a.rows > 0x7fffffffll) return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "shape too large for the launch grid");
+    const int groups = plan_attend(p.batch, p.seq_new, p.heads, p.kv_heads, head_dim, p.max_seq, weigh, q4).groups;
+    if (a.steps + a.segments > 0x7fffffffll - 65536 || p.max_seq > (1 << 29) || (int64_t)p.seq_new * p.heads * head_dim > 0x7fffffffll) return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "shape too large for the launch grid");
     if (!p.q || !p.out || (weigh && (!p.weights_out || !p.kv_lens)) || (p.max_seq > 0 && (!p.k || !p.v || (q4 && (!p.k_pairs || !p.v_pairs)))))
         return fail(err, RT_ERR_NULL_POINTER, -1, 0, 0, "NULL buffer");
     if (((uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.out) & 15) return fail(err, RT_ERR_UNSUPPORTED, -1, 16, 0, "q, out and the caches must be 16-byte aligned");
     const size_t sum_bytes = (size_t)p.batch * p.kv_heads * p.max_seq * 4;
     if (weigh && p.weights_in != p.weights_out && overlap(p.weights_in, p.weights_in ? sum_bytes : 0, p.weights_out, sum_bytes))
         return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "weights_out must be weights_in or share no memory with it");
-    const size_t need = a.part_bytes + a.score_bytes + a.stat_bytes;
+    const size_t need = a.bytes();
     if (!workspace || workspace_bytes < need)
         return fail(err, RT_ERR_WORKSPACE_TOO_SMALL, -1, need, workspace ? workspace_bytes : 0, "workspace too small");
     if ((uintptr_t)workspace & 15) return fail(err, RT_ERR_WORKSPACE_TOO_SMALL, -1, 16, (uint64_t)((uintptr_t)workspace & 15), "workspace must be 16-byte aligned");
@@ -537,13 +869,15 @@ int attend_common(void* stream, CacheAttendParams& p, int head_dim, bool q4, boo
     p.group = p.heads / p.kv_heads;
     p.rows = (int)a.rows;
     p.n_tiles = (int)a.n_tiles;
-    p.n_waves = a.waves;
-    p.span_min = 4;
+    p.n_groups = groups;
+    p.span_min = kWaves;
     p.scale_log2e = (1.0f / sqrtf((float)head_dim)) * kLog2eHost;
     p.part = (float*)workspace;
     p.part_rows = a.part_rows;
-    p.scores = (float*)((char*)workspace + a.part_bytes);
-    p.stats = (float*)((char*)workspace + a.part_bytes + a.score_bytes);
+    p.words = (unsigned char*)workspace + a.part_bytes;
+    p.launch_id = next_launch_id() << 8;
+    p.scores = (float*)(p.words + a.word_bytes);
+    p.stats = (float*)(p.words + a.word_bytes + a.score_bytes);
     const hipStream_t s = (hipStream_t)stream;
     const hipError_t e = !q4 ? launch_attend<false, true>(s, p, head_dim) : weigh ? launch_attend<true, true>(s, p, head_dim) : launch_attend<true, false>(s, p, head_dim);
     HIP_TRY(e, "cache_attend launch");
@@ -553,7 +887,7 @@ int attend_common(void* stream, CacheAttendParams& p, int head_dim, bool q4, boo
 size_t attend_bytes(int32_t batch, int32_t seq_new, int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t max_seq, bool weigh) {
     if (batch <= 0 || seq_new <= 0 || n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || !cache_q4_dim(head_dim) || max_seq < 0) return 0;
     const AttendPlan a = plan_attend(batch, seq_new, n_heads, n_kv, head_dim, max_seq, weigh);
-    return a.part_bytes + a.score_bytes + a.stat_bytes;
+    return a.bytes();
 }
 
 }  // namespace

@@ -45,7 +45,7 @@ inline int fail_hip(rt_err_detail* e, hipError_t code, const char* where) {
 
 // Finds the gfx950 device on the first call (api.hip); every compute entry calls it behind its own checks.
 int ensure_device(rt_err_detail* err);
-int device_cus();  // its compute units, after ensure_device
+uint64_t next_launch_id();  // a number no other launch of the process has, its low 8 bits zero
 
 // Does [a, a + n) share a byte with [b, b + m)?
 inline bool overlap(const void* a, size_t n, const void* b, size_t m) {

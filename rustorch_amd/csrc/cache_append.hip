@@ -34,12 +34,14 @@ __device__ __forceinline__ uint32_t code_of(float x, Pair p) {
     return p.s > 0.0f ? (uint32_t)((int)fminf(fmaxf(t, -8.0f), 7.0f) + 8) : 8u;
 }
 
-// dim / 8 lanes a row; lane j has the dims 4 j .. 4 j + 3 and their partners dim / 2 on, which the rotation mixes.
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // 16 bytes from any word
+
+// dim / 16 lanes a row; lane j has the dims 8 j .. 8 j + 7 and their partners dim / 2 on, which the rotation mixes: 16 bytes a request.
 // Grid (rows of 256 / lanes, batch): the rows of a sequence are (head, token) pairs of q, then k, then v, tokens fastest.
 template <int D, bool Q4>
 __global__ __launch_bounds__(256) void cache_append_kernel(CacheAppendParams p) {
-    constexpr int kLanes = D / 8, kRows = 256 / kLanes, kPitch = D + 4, kGroups = D / 64;
-    __shared__ alignas(16) float squares[kRows * kPitch];
+    constexpr int kLanes = D / 16, kRows = 256 / kLanes, kPitch = D + 4, kGroups = D / 64, kHalf = D / 2;
+    extern __shared__ __attribute__((aligned(16))) float squares[];  // kRows * kPitch, where there is a norm
     const int tid = threadIdx.x, j = tid % kLanes, r = tid / kLanes, b = blockIdx.y, S = p.seq;
     const int all = (p.n_heads + 2 * p.n_kv) * S, idx = (int)blockIdx.x * kRows + r;
     const int pos0 = p.positions ? p.positions[b] : p.pos;
@@ -47,30 +49,46 @@ __global__ __launch_bounds__(256) void cache_append_kernel(CacheAppendParams p) 
     // a sequence whose rows would leave the tables or the cache is left as it is
     const bool fits = row0 >= 0 && row0 <= p.max_seq - S && (!p.cos_table || (pos0 >= 0 && pos0 <= p.table_rows - S));
     const bool on = idx < all && fits;
-    const int hh = on ? idx / S : 0, tok = on ? idx - hh * S : 0;
+    const int hh = S == 1 ? min(idx, all - 1) : min(idx, all - 1) / S, tok = min(idx, all - 1) - hh * S;
     const bool is_q = hh < p.n_heads, is_v = hh >= p.n_heads + p.n_kv;
     const int h = is_q ? hh : is_v ? hh - p.n_heads - p.n_kv : hh - p.n_heads;
     const bool turn = !is_v && p.cos_table;
     const float* gamma = !turn ? nullptr : is_q ? p.q_gamma : p.k_gamma;
 
-    float x[8] = {};  // [0, 4): dims 4 j on, [4, 8): D / 2 + 4 j on
-    uint2 raw[2] = {};
-    if (on) {
-        const uint16_t* src = (is_q ? p.q : is_v ? p.v_in : p.k_in) + (((size_t)b * (is_q ? p.n_heads : p.n_kv) + h) * S + tok) * D + 4 * j;
-        raw[0] = *(const uint2*)src;
-        raw[1] = *(const uint2*)(src + D / 2);
+    float x[2][8];  // the lane's dims, and their partners
+    u32x4_t raw[2];
+    {
+        const uint16_t* src = (is_q ? p.q : is_v ? p.v_in : p.k_in) + (((size_t)b * (is_q ? p.n_heads : p.n_kv) + h) * S + tok) * D + 8 * j;
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            x[4 * e] = bf16_lo(raw[e].x);
-            x[4 * e + 1] = bf16_hi(raw[e].x);
-            x[4 * e + 2] = bf16_lo(raw[e].y);
-            x[4 * e + 3] = bf16_hi(raw[e].y);
+        for (int e = 0; e < 2; e++) raw[e] = *(const u32x4_t*)(src + e * kHalf);
+    }
+    float cs[8], sn[8];
+    if (turn && on) {
+        const size_t at = (size_t)(pos0 + tok) * kHalf + 8 * j;
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            const f32x4_t c = *(const f32x4_any*)(p.cos_table + at + e), s = *(const f32x4_any*)(p.sin_table + at + e);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                cs[e + i] = c[i];
+                sn[e + i] = s[i];
+            }
         }
     }
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x[e][2 * i] = bf16_lo(raw[e][i]);
+            x[e][2 * i + 1] = bf16_hi(raw[e][i]);
+        }
     if (p.q_gamma || p.k_gamma) {  // (the same for every thread of the launch)
         float* mine = squares + r * kPitch;
 #pragma unroll
-        for (int e = 0; e < 2; e++) *(f32x4_t*)(mine + e * (D / 2) + 4 * j) = f32x4_t{x[4 * e] * x[4 * e], x[4 * e + 1] * x[4 * e + 1], x[4 * e + 2] * x[4 * e + 2], x[4 * e + 3] * x[4 * e + 3]};
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int i = 0; i < 8; i += 4)
+                *(f32x4_t*)(mine + e * kHalf + 8 * j + i) = f32x4_t{x[e][i] * x[e][i], x[e][i + 1] * x[e][i + 1], x[e][i + 2] * x[e][i + 2], x[e][i + 3] * x[e][i + 3]};
         __syncthreads();
         if (gamma) {
             float sum = 0.0f;
@@ -83,26 +101,38 @@ __global__ __launch_bounds__(256) void cache_append_kernel(CacheAppendParams p) 
             const float inv_d = 1.0f / (float)D;
             const float inv_rms = 1.0f / sqrtf(sum * inv_d + p.eps);
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = x[e] * inv_rms * gamma[(e / 4) * (D / 2) + 4 * j + e % 4];
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int i = 0; i < 8; i += 4) {
+                    const f32x4_t g = *(const f32x4_any*)(gamma + e * kHalf + 8 * j + i);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) x[e][i + k] = x[e][i + k] * inv_rms * g[k];
+                }
         }
     }
     if (!on) return;
     if (turn) {
-        const size_t at = (size_t)(pos0 + tok) * (D / 2) + 4 * j;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const float c = p.cos_table[at + e], s = p.sin_table[at + e], x0 = x[e], x1 = x[e + 4];
-            x[e] = x0 * c - x1 * s;
-            x[e + 4] = x1 * c + x0 * s;
+        for (int e = 0; e < 8; e++) {
+            const float x0 = x[0][e], x1 = x[1][e];
+            x[0][e] = x0 * cs[e] - x1 * sn[e];
+            x[1][e] = x1 * cs[e] + x0 * sn[e];
         }
     }
     if (is_q || !Q4) {
         uint16_t* dst = is_q ? p.q_out + (((size_t)b * p.n_heads + h) * S + tok) * D
                              : (uint16_t*)(is_v ? p.v : p.k) + (((size_t)b * p.n_kv + h) * (size_t)p.max_seq + (size_t)(row0 + tok)) * D;
 #pragma unroll
-        for (int e = 0; e < 2; e++)
-            *(uint2*)(dst + e * (D / 2) + 4 * j) = turn ? uint2{pack_bf16x2(x[4 * e], x[4 * e + 1]), pack_bf16x2(x[4 * e + 2], x[4 * e + 3])} : raw[e];
-        if (is_q) return;
+        for (int e = 0; e < 2; e++) {
+            u32x4_t o = raw[e];
+            if (turn)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[i] = pack_bf16x2(x[e][2 * i], x[e][2 * i + 1]);
+            *(u32x4_t*)(dst + e * kHalf + 8 * j) = o;
+        }
+        if (is_q) {
+            return;
+        }
     }
     const size_t head = (size_t)b * p.n_kv + h;
     if (!is_v && j == 0) {
@@ -110,33 +140,36 @@ __global__ __launch_bounds__(256) void cache_append_kernel(CacheAppendParams p) 
         if (p.weights) p.weights[head * p.max_seq + (size_t)(row0 + tok)] = 0.0f;
     }
     if constexpr (Q4) {
-        // extremes over the lanes of a group: 8 lanes with both halves at dim 64, 16 lanes a half above
+        // extremes over the lanes of a group: 4 lanes with both halves at dim 64, 8 lanes a half above
         float hi[2], lo[2];
-        bool bad[2] = {false, false};
+        int bad[2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            hi[e] = fmaxf(fmaxf(x[4 * e], x[4 * e + 1]), fmaxf(x[4 * e + 2], x[4 * e + 3]));
-            lo[e] = fminf(fminf(x[4 * e], x[4 * e + 1]), fminf(x[4 * e + 2], x[4 * e + 3]));
+            hi[e] = lo[e] = x[e][0];
+            bad[e] = !(fabsf(x[e][0]) < __builtin_inff());
 #pragma unroll
-            for (int i = 0; i < 4; i++) bad[e] |= !(fabsf(x[4 * e + i]) < __builtin_inff());
+            for (int i = 1; i < 8; i++) {
+                hi[e] = fmaxf(hi[e], x[e][i]);
+                lo[e] = fminf(lo[e], x[e][i]);
+                bad[e] |= !(fabsf(x[e][i]) < __builtin_inff());
+            }
         }
         if (D == 64) {
-            hi[0] = hi[1] = fmaxf(hi[0], hi[1]);
-            lo[0] = lo[1] = fminf(lo[0], lo[1]);
-            bad[0] = bad[1] = bad[0] || bad[1];
+            hi[0] = fmaxf(hi[0], hi[1]);
+            lo[0] = fminf(lo[0], lo[1]);
+            bad[0] |= bad[1];
         }
-        constexpr int kSpan = D == 64 ? 8 : 16;
+        constexpr int kSpan = D == 64 ? 4 : 8;
         Pair pr[2];
 #pragma unroll
         for (int e = 0; e < (D == 64 ? 1 : 2); e++) {
-            int any = bad[e];
 #pragma unroll
             for (int o = 1; o < kSpan; o *= 2) {
                 hi[e] = fmaxf(hi[e], __shfl_xor(hi[e], o, 64));
                 lo[e] = fminf(lo[e], __shfl_xor(lo[e], o, 64));
-                any |= __shfl_xor(any, o, 64);
+                bad[e] |= __shfl_xor(bad[e], o, 64);
             }
-            pr[e] = pair_of(hi[e], lo[e], any != 0);
+            pr[e] = pair_of(hi[e], lo[e], bad[e] != 0);
         }
         if (D == 64) pr[1] = pr[0];
         const size_t row = (size_t)(row0 + tok);
@@ -145,27 +178,40 @@ __global__ __launch_bounds__(256) void cache_append_kernel(CacheAppendParams p) 
             pairs[(size_t)(j / kSpan) * p.max_seq] = word_of(pr[0]);
             if (D > 64) pairs[(size_t)(kGroups / 2 + j / kSpan) * p.max_seq] = word_of(pr[1]);
         }
-        // bytes of dims (4 j, 4 j + 1), (4 j + 2, 4 j + 3), and of their partners
-        uint32_t t = 0;
+        uint32_t t[2];  // a byte a pair of dims: i = 4 (j % 4) .. + 3 of the lane's chunk, j / 4, and of its partner's
 #pragma unroll
-        for (int e = 0; e < 4; e++) t |= (code_of(x[2 * e], pr[e / 2]) | code_of(x[2 * e + 1], pr[e / 2]) << 4) << (8 * e);
+        for (int e = 0; e < 2; e++) {
+            t[e] = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) t[e] |= (code_of(x[e][2 * i], pr[e]) | code_of(x[e][2 * i + 1], pr[e]) << 4) << (8 * i);
+        }
+        // bytes (a.0, b.0, a.1, b.1) and (a.2, b.2, a.3, b.3)
+        auto low = [](uint32_t a, uint32_t c) { return __builtin_amdgcn_perm(c, a, 0x05010400u); };
+        auto high = [](uint32_t a, uint32_t c) { return __builtin_amdgcn_perm(c, a, 0x07030602u); };
         uint32_t* codes = (uint32_t*)(is_v ? p.v : p.k) + (head * (size_t)p.max_seq + row) * (D / 8);
-        if constexpr (D == 64) {  // two bytes an i: chunks 0 and 1
-            codes[j] = (t & 0xffu) | (t >> 8 & 0xff00u) | (t & 0xff00u) << 8 | (t & 0xff000000u);
-        } else if constexpr (D == 128) {  // a word an i: chunks 0, 2 from lane j % 8, 1, 3 from the one 8 on
-            const uint32_t o = __shfl_xor(t, 8, 64);
-            const bool odd = j & 8;
-            const uint32_t a = odd ? o >> 8 : t, c = odd ? t >> 8 : o;
-            codes[2 * (j & 7) + (odd ? 1 : 0)] = (a & 0xffu) | (a >> 8 & 0xff00u) | (c & 0xffu) << 16 | (c >> 16 & 0xffu) << 24;
-        } else {  // two words an i, each from four lanes
-            const int k = j >> 3;
-            uint32_t w = 0;
+        if constexpr (D == 64) {  // two bytes an i: chunks 0 and 1, the lane's two
+            *(uint2*)(codes + 2 * j) = uint2{low(t[0], t[1]), high(t[0], t[1])};
+        } else {
+            // a word an i and 128 dims: chunks 0, 2, 1, 3.  At dim 128 lane j % 8 < 4 has 0 and 2, the one 4 on 1 and 3, and each keeps two of
+            // the four i; at dim 256 lanes 0-3, 4-7, 8-11, 12-15 have chunks 0, 1, 2, 3 of one 128 dims (t[0]) and of the other (t[1]).
+            if constexpr (D == 128) {
+                const bool second = j & 4;
+                const uint32_t give = second ? low(t[0], t[1]) : high(t[0], t[1]), keep = second ? high(t[0], t[1]) : low(t[0], t[1]);
+                const uint32_t got = __shfl_xor(give, 4, 64);
+                const uint32_t a = second ? got : keep, c = second ? keep : got;  // of chunks 0 and 2, of 1 and 3: two i's bytes each
+                *(uint2*)(codes + 4 * (j & 3) + (second ? 2 : 0)) = uint2{(a & 0xffffu) | c << 16, a >> 16 | (c & 0xffff0000u)};
+            } else {
+                // lane k (of the four with one j % 4) takes the i-th word k of both: byte k of every lane's
+                const int k = j >> 2;
+                uint2 o = {0u, 0u};
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const uint32_t o = __shfl(t, (tid & 32) + (j & 7) + 8 * c, 64);
-                w |= (o >> (8 * k) & 0xffu) << (8 * ((c & 1) << 1 | c >> 1));
+                for (int c = 0; c < 4; c++) {
+                    const int src = (int)(threadIdx.x & 48) + (j & 3) + 4 * c, to = 8 * ((c & 1) << 1 | c >> 1);
+                    o.x |= (__shfl(t[0], src, 64) >> (8 * k) & 0xffu) << to;
+                    o.y |= (__shfl(t[1], src, 64) >> (8 * k) & 0xffu) << to;
+                }
+                *(uint2*)(codes + 2 * (4 * (j & 3) + k)) = o;
             }
-            codes[2 * (2 * (j & 7) + (k & 1)) + (k >> 1)] = w;
         }
     }
 }
@@ -200,9 +246,11 @@ hipError_t launch_append(hipStream_t stream, const CacheAppendParams& p, int dim
     const dim3 block(256);
     const long long all = ((long long)p.n_heads + 2ll * p.n_kv) * p.seq;
     auto grid = [&](int rows) { return dim3((unsigned)((all + rows - 1) / rows), (unsigned)p.batch); };
-    if (dim == 64) hipLaunchKernelGGL((cache_append_kernel<64, Q4>), grid(32), block, 0, stream, p);
-    else if (dim == 128) hipLaunchKernelGGL((cache_append_kernel<128, Q4>), grid(16), block, 0, stream, p);
-    else hipLaunchKernelGGL((cache_append_kernel<256, Q4>), grid(8), block, 0, stream, p);
+    const int rows = 4096 / dim;  // a workgroup
+    const unsigned lds = p.q_gamma || p.k_gamma ? (unsigned)(rows * (dim + 4) * 4) : 0u;
+    if (dim == 64) hipLaunchKernelGGL((cache_append_kernel<64, Q4>), grid(rows), block, lds, stream, p);
+    else if (dim == 128) hipLaunchKernelGGL((cache_append_kernel<128, Q4>), grid(rows), block, lds, stream, p);
+    else hipLaunchKernelGGL((cache_append_kernel<256, Q4>), grid(rows), block, lds, stream, p);
     return hipGetLastError();
 }
 

@@ -6,8 +6,8 @@
 // after a cut to a quarter three of four kept rows, in a loop that evicts one row a token a single one, where rows moved
 // together in order would all have to move -- and no row that is read lies where one is written, so a copy needs no order either.
 //
-//   cache_select_kernel  one workgroup a (sequence, kv head): the budget-th largest sum by its bytes from the top (four counts of
-//                        256), then one pass in slot order that numbers the freed slots and the rows that move
+//   cache_select_kernel  one workgroup a (sequence, kv head): the budget-th largest sum by counts, then one pass in slot order that
+//                        numbers the freed slots and the rows that move
 //   cache_move_kernel    copies them
 #include <algorithm>
 
@@ -19,46 +19,72 @@ namespace rt {
 
 namespace {
 
-constexpr int kSelect = 1024, kSelectWaves = kSelect / 64;
+constexpr int kSelect = 1024, kSelectWaves = kSelect / 64, kPer = 8, kTile = kSelect * kPer;  // a thread's neighbouring slots; slots of a tile
+constexpr int kBins = 2048;
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // 16 bytes from any word
 
 // The order of the sums as that of whole numbers: NaN counts as -infinity, -0 as 0, the newest tokens' as +infinity.
+constexpr uint32_t kNewest = 0xff800000u;
 __device__ __forceinline__ uint32_t key_of(float w, int pos, long long newest_out) {
-    if ((long long)pos > newest_out) return 0xff800000u;
+    if ((long long)pos > newest_out) return kNewest;
     if (w != w) return 0x007fffffu;
     const uint32_t u = __float_as_uint(w == 0.0f ? 0.0f : w);
     return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-// Exclusive sums over the workgroup's threads, in thread order, of a truth value; `all`: how many there are.  `room`: kSelectWaves ints.
-__device__ __forceinline__ int count_before(bool x, int* room, int* all) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint64_t mine = __ballot(x);
-    __syncthreads();  // (the room may still be read)
-    if (lane == 0) room[wave] = __popcll(mine);
-    __syncthreads();
-    int before = 0, sum = 0;
+// A workgroup's reductions and sums: in a wave, then over the waves' results in `room` (kSelectWaves words), one barrier ahead of
+// their writing and one behind it.
+template <typename T, typename F>
+__device__ __forceinline__ T all_of(T x, F f, T* room) {
 #pragma unroll
-    for (int w = 0; w < kSelectWaves; w++) {
-        const int c = room[w];
-        before += w < wave ? c : 0;
-        sum += c;
+    for (int o = 32; o >= 1; o >>= 1) x = f(x, __shfl_xor(x, o, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = x;
+    __syncthreads();
+    T y = room[threadIdx.x & (kSelectWaves - 1)];
+#pragma unroll
+    for (int o = kSelectWaves / 2; o >= 1; o >>= 1) y = f(y, __shfl_xor(y, o, 64));
+    return y;
+}
+// The sum over the threads before this one; `all`: over all.
+__device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t* room, uint32_t* all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t end = x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t y = __shfl_up(end, o, 64);
+        if (lane >= o) end += y;
     }
-    *all = sum;
-    return before + __popcll(mine & ((1ull << lane) - 1ull));
+    __syncthreads();
+    if (lane == 63) room[wave] = end;
+    __syncthreads();
+    uint32_t y = room[lane & (kSelectWaves - 1)];
+#pragma unroll
+    for (int o = 1; o < kSelectWaves; o <<= 1) {
+        const uint32_t z = __shfl_up(y, o, kSelectWaves);
+        if ((lane & (kSelectWaves - 1)) >= o) y += z;
+    }
+    *all = __shfl(y, kSelectWaves - 1, 64);
+    return end - x + (wave ? __shfl(y, wave - 1, 64) : 0u);
 }
 
-// Grid (kv heads, batch).
+// One workgroup a (sequence, kv head), grid (kv heads, batch).  Thread t has the slots 8 t .. 8 t + 7 of a tile of 8192; up to there the keys are
+// read once and stay in registers (kOne), longer heads are walked tile by tile again for every question.
+// The budget-th largest key is found by counts: the range that the keys in question span is cut into 2048 bins, and the bin it falls in is
+// the next range -- three times at most, since 2048^3 > 2^32, and twice as a rule, since bins that follow the keys' own range hold few of them.
+// (By fixed bytes from the top most sums share a bin, and a wave's counts in one word wait for each other: 8192 keys 30 us.)
+template <bool kOne>
 __global__ __launch_bounds__(kSelect) void cache_select_kernel(CacheEvictParams p) {
-    __shared__ int bins[256], room[kSelectWaves], chosen[2];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.y, head = b * p.n_kv + (int)blockIdx.x;
+    __shared__ uint32_t bins[kBins], room[kSelectWaves], chosen[2];
+    const int tid = threadIdx.x, b = blockIdx.y, head = b * p.n_kv + (int)blockIdx.x;
     const int len = min(max(p.kv_lens[b], 0), p.max_seq);
     const float* w_in = p.weights_in + (size_t)head * p.max_seq;
     const int32_t* s_in = p.slots_in + (size_t)head * p.max_seq;
     float* w_out = p.weights_out + (size_t)head * p.max_seq;
     int32_t* s_out = p.slots_out + (size_t)head * p.max_seq;
     const bool copy_w = w_in != w_out, copy_s = s_in != s_out;
-    if (len <= p.budget) {  // all of it stays
-        for (int j = tid; j < len; j += kSelect) {
+    if (len <= p.budget || p.budget == 0) {  // all of it stays, or nothing
+        for (int j = tid; j < min(len, p.budget); j += kSelect) {
             if (copy_w) w_out[j] = w_in[j];
             if (copy_s) s_out[j] = s_in[j];
         }
@@ -68,81 +94,130 @@ __global__ __launch_bounds__(kSelect) void cache_select_kernel(CacheEvictParams 
         }
         return;
     }
+    const int tiles = kOne ? 1 : (len + kTile - 1) / kTile;
+    float w[kPer];
+    int32_t s[kPer];
+    auto load = [&](int tile) __attribute__((always_inline)) {  // (slots behind the last: what its key is made of does not count)
+        const int j0 = tile * kTile + tid * kPer;
+        if (j0 + kPer <= len) {
+#pragma unroll
+            for (int e = 0; e < kPer; e += 4) {
+                const u32x4_any a = *(const u32x4_any*)(w_in + j0 + e), c = *(const u32x4_any*)(s_in + j0 + e);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    w[e + i] = __uint_as_float(a[i]);
+                    s[e + i] = (int32_t)c[i];
+                }
+            }
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < kPer; e++) {
+            w[e] = j0 + e < len ? w_in[j0 + e] : 0.0f;
+            s[e] = j0 + e < len ? s_in[j0 + e] : INT32_MIN;
+        }
+    };
     // the newest token
     int newest = INT32_MIN;
-    for (int j = tid; j < len; j += kSelect) newest = max(newest, s_in[j]);
+    for (int t = 0; t < tiles; t++) {
+        load(t);
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) newest = max(newest, __shfl_xor(newest, o, 64));
-    if (lane == 0) room[wave] = newest;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kSelectWaves; w++) newest = max(newest, room[w]);
+        for (int e = 0; e < kPer; e++) newest = max(newest, s[e]);
+    }
+    newest = all_of(newest, [](int x, int y) { return max(x, y); }, (int*)room);
     const long long out_from = (long long)newest - p.recent;
-
-    // the budget-th largest key: its bytes from the top, each by a count of the keys that share those above it
-    uint32_t prefix = 0;
-    int left = p.budget;  // of the keys that share the prefix, the left-th largest is it
-    for (int shift = 24; shift >= 0 && p.budget > 0; shift -= 8) {
-        for (int i = tid; i < 256; i += kSelect) bins[i] = 0;
-        __syncthreads();
-        for (int j = tid; j < len; j += kSelect) {
-            const uint32_t k = key_of(w_in[j], s_in[j], out_from);
-            if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&bins[k >> shift & 255u], 1);
-        }
-        __syncthreads();
-        if (wave == 0) {  // lane i has the bins 4 i .. 4 i + 3; those above count first
-            const int c[4] = {bins[4 * lane], bins[4 * lane + 1], bins[4 * lane + 2], bins[4 * lane + 3]};
-            int up = c[0] + c[1] + c[2] + c[3];
-            const int own = up;
+    uint32_t key[kPer];
+    auto keys = [&](int tile) __attribute__((always_inline)) {
+        if (!kOne) load(tile);
 #pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int y = __shfl_down(up, o, 64);
-                if (lane + o < 64) up += y;
-            }
-            int above = up - own;
+        for (int e = 0; e < kPer; e++) key[e] = key_of(w[e], s[e], out_from);
+    };
+    auto in = [&](int tile, int e) __attribute__((always_inline)) { return tile * kTile + tid * kPer + e < len; };
+    // the newest tokens' keys, which are the largest, apart: they would stretch the range of the others
+    uint32_t low = ~0u, high = 0, at_top = 0;
+    for (int t = 0; t < tiles; t++) {
+        keys(t);
 #pragma unroll
-            for (int e = 3; e >= 0; e--) {
-                if (above < left && left <= above + c[e]) {
-                    chosen[0] = 4 * lane + e;
-                    chosen[1] = left - above;
+        for (int e = 0; e < kPer; e++)
+            if (in(t, e)) {
+                at_top += key[e] == kNewest;
+                if (key[e] != kNewest) {
+                    low = min(low, key[e]);
+                    high = max(high, key[e]);
                 }
-                above += c[e];
             }
+    }
+    low = all_of(low, [](uint32_t x, uint32_t y) { return min(x, y); }, room);
+    high = all_of(high, [](uint32_t x, uint32_t y) { return max(x, y); }, room);
+    at_top = all_of(at_top, [](uint32_t x, uint32_t y) { return x + y; }, room);
+    uint32_t left = (uint32_t)p.budget;  // of the keys in [low, high], the left-th largest is the threshold
+    if (left <= at_top) low = high = kNewest;
+    else left -= at_top;
+    while (low < high) {
+        const int shift = max(0, 32 - __builtin_clz(high - low) - 11);  // (high - low) >> shift < 2048
+        bins[tid] = bins[tid + kSelect] = 0;
+        __syncthreads();
+        for (int t = 0; t < tiles; t++) {
+            if (!kOne) keys(t);
+#pragma unroll
+            for (int e = 0; e < kPer; e++)
+                if (in(t, e) && key[e] >= low && key[e] <= high) atomicAdd(&bins[(key[e] - low) >> shift], 1u);
         }
         __syncthreads();
-        prefix |= (uint32_t)chosen[0] << shift;
+        // thread t has the bins 2047 - 2 t and 2046 - 2 t: those above it are those before it
+        const uint32_t c0 = bins[kBins - 1 - 2 * tid], c1 = bins[kBins - 2 - 2 * tid];
+        uint32_t all;
+        const uint32_t above = sum_before(c0 + c1, room, &all);
+        if (above < left && left <= above + c0 + c1) {
+            const bool second = left > above + c0;
+            chosen[0] = (uint32_t)(kBins - 1 - 2 * tid) - (second ? 1u : 0u);
+            chosen[1] = left - above - (second ? c0 : 0u);
+        }
+        __syncthreads();
+        const uint32_t bin = chosen[0];
         left = chosen[1];
+        high = min(high, low + ((bin + 1) << shift) - 1);  // (no further than the range: low + 2^32 does not come up)
+        low += bin << shift;
     }
     // in slot order: keys above it stay, and the first `left` that equal it
-    int equal = 0, freed = 0, moved = 0;
+    uint32_t equal = 0, freed = 0, moved = 0;
     int32_t* from = p.from + (size_t)head * p.most;
     int32_t* to = p.to + (size_t)head * p.most;
-    for (int j0 = 0; j0 < len; j0 += kSelect) {
-        const int j = j0 + tid;
-        const bool in = j < len && p.budget > 0;
-        const float w = in ? w_in[j] : 0.0f;
-        const int s = in ? s_in[j] : 0;
-        const uint32_t k = in ? key_of(w, s, out_from) : 0u;
-        int all;
-        const bool eq = in && k == prefix;
-        const int rank = equal + count_before(eq, room, &all);
+    for (int t = 0; t < tiles; t++) {
+        if (!kOne) keys(t);
+        const int j0 = t * kTile + tid * kPer;
+        uint32_t mine = 0, all;
+#pragma unroll
+        for (int e = 0; e < kPer; e++) mine += in(t, e) && key[e] == low;
+        uint32_t rank = equal + sum_before(mine, room, &all);
         equal += all;
-        const bool keep = in && (k > prefix || (eq && rank < left));
-        const bool hole = in && j < p.budget && !keep, mover = keep && j >= p.budget;
-        const int at_hole = freed + count_before(hole, room, &all);
-        freed += all;
-        const int at_mover = moved + count_before(mover, room, &all);
-        moved += all;
-        if (hole) to[at_hole] = j;
-        if (mover) from[at_mover] = j;
-        if (keep && j < p.budget) {
-            if (copy_w) w_out[j] = w;
-            if (copy_s) s_out[j] = s;
+        uint32_t keep = 0, count = 0;  // count: freed slots in the low half, rows that move in the high one (8192 each at most)
+#pragma unroll
+        for (int e = 0; e < kPer; e++) {
+            const bool eq = key[e] == low, stays = in(t, e) && (key[e] > low || (eq && rank < left));
+            rank += in(t, e) && eq;
+            keep |= (stays ? 1u : 0u) << e;
+            count += in(t, e) && !stays && j0 + e < p.budget ? 1u : 0u;
+            count += stays && j0 + e >= p.budget ? 1u << 16 : 0u;
+        }
+        const uint32_t before = sum_before(count, room, &all);
+        uint32_t at_hole = freed + (before & 0xffffu), at_mover = moved + (before >> 16);
+        freed += all & 0xffffu;
+        moved += all >> 16;
+#pragma unroll
+        for (int e = 0; e < kPer; e++) {
+            const bool stays = keep >> e & 1u, below = j0 + e < p.budget;
+            if (in(t, e) && !stays && below) to[at_hole++] = j0 + e;
+            if (stays && !below) from[at_mover++] = j0 + e;
+            if (stays && below) {
+                if (copy_w) w_out[j0 + e] = w[e];
+                if (copy_s) s_out[j0 + e] = s[e];
+            }
         }
     }
     if (tid == 0) {
         p.header[2 * head] = len;
-        p.header[2 * head + 1] = moved;
+        p.header[2 * head + 1] = (int32_t)moved;
     }
 }
 
@@ -228,7 +303,8 @@ int evict_common(void* stream, CacheEvictParams& p, int head_dim, bool q4, void*
     p.row_bytes = q4 ? head_dim / 2 : 2 * head_dim;
     p.groups = q4 ? head_dim / 64 : 0;
     const hipStream_t s = (hipStream_t)stream;
-    hipLaunchKernelGGL(cache_select_kernel, dim3(p.n_kv, p.batch), dim3(kSelect), 0, s, p);
+    if (p.max_seq <= kTile) hipLaunchKernelGGL(cache_select_kernel<true>, dim3(p.n_kv, p.batch), dim3(kSelect), 0, s, p);
+    else hipLaunchKernelGGL(cache_select_kernel<false>, dim3(p.n_kv, p.batch), dim3(kSelect), 0, s, p);
     HIP_TRY(hipGetLastError(), "cache_select launch");
     hipLaunchKernelGGL(cache_move_kernel, dim3(std::max(1, (a.most + kMoveRows - 1) / kMoveRows), p.n_kv, p.batch), dim3(256), 0, s, p);
     HIP_TRY(hipGetLastError(), "cache_move launch");

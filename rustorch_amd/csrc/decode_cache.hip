@@ -33,6 +33,8 @@ constexpr int kWaves = 4;        // a workgroup
 constexpr int kCus = 256;
 constexpr int kMaxPieces = 256;  // partials of a segment
 constexpr float kNoMax = -1.0e30f;
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // 16 bytes from any word
+typedef float f32x2_any __attribute__((ext_vector_type(2), aligned(4)));
 
 __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
@@ -41,52 +43,85 @@ __device__ __forceinline__ int len_of(const CacheAttendParams& p, int b) {
     return p.kv_lens ? min(max(p.kv_lens[b], 0), p.max_seq) : p.kv_len;
 }
 __device__ __forceinline__ int steps_of(int len) { return (len + kStep - 1) / kStep; }
-// What a workgroup's span of the list is, and where it begins.
+// x / d for 0 <= x < 2^31, 0 < d, by a reciprocal in f32 and what it is off by (nothing or one where the quotient is small).
+__device__ __forceinline__ int quotient(int x, int d) {
+    int q = (int)((float)x * __builtin_amdgcn_rcpf((float)d));
+    int r = x - q * d;
+    while (r < 0) {
+        q--;
+        r += d;
+    }
+    while (r >= d) {
+        q++;
+        r -= d;
+    }
+    return __builtin_amdgcn_readfirstlane(q);
+}
+// Sums over the lanes up to this one, and the largest of all, within registers.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int moved(int x) { return __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xf, false); }
+__device__ __forceinline__ int lane_sums(int x) {
+    x += moved<0x111, 0xf>(x);  // from 1, 2, 4, 8 lanes down a row of 16
+    x += moved<0x112, 0xf>(x);
+    x += moved<0x114, 0xf>(x);
+    x += moved<0x118, 0xf>(x);
+    x += moved<0x142, 0xa>(x);  // a row's last lane to the next row; the second row's to the upper half
+    x += moved<0x143, 0xc>(x);
+    return x;
+}
+__device__ __forceinline__ int lane_max(int x) {  // x >= 0
+    x = max(x, moved<0x111, 0xf>(x));
+    x = max(x, moved<0x112, 0xf>(x));
+    x = max(x, moved<0x114, 0xf>(x));
+    x = max(x, moved<0x118, 0xf>(x));
+    x = max(x, moved<0x142, 0xa>(x));
+    x = max(x, moved<0x143, 0xc>(x));
+    return __builtin_amdgcn_readlane(x, 63);
+}
+
+// The list that the workgroups share: of every segment `kStart` places and its steps.  The places stand for what a segment costs
+// besides its steps, so that a span of short sequences is no longer a walk than one of a long one.
+constexpr int kStart = 4;
+__device__ __forceinline__ int places_of(int len) { return len ? kStart + steps_of(len) : 0; }
 struct Span {
-    int total, size, b, first;  // steps of all; of a span; the sequence that holds the span's first step, and that sequence's first
+    int total, size;    // places of all; of a span
+    int b, first, len;  // the sequence that holds the span's first place, the first place of that sequence, its length
+    uint64_t empty;     // of the first 64 sequences, those without keys
 };
 // Lengths 64 at a time, the first of them once for both walks.
 __device__ __forceinline__ Span span_of(const CacheAttendParams& p, int group, int lane) {
     const int per = p.kv_heads * p.n_tiles;
-    auto steps = [&](int b0) { return b0 + lane < p.batch ? steps_of(len_of(p, b0 + lane)) : 0; };
-    const int head = steps(0);
-    int sum = head, most = head;
-    for (int b0 = 64; b0 < p.batch; b0 += 64) {
-        const int x = steps(b0);
-        sum += x;
-        most = max(most, x);
-    }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-        sum += __shfl_xor(sum, o, 64);
-        most = max(most, __shfl_xor(most, o, 64));
-    }
+    auto len_at = [&](int b0) { return b0 + lane < p.batch ? len_of(p, b0 + lane) : 0; };
+    const int len0 = len_at(0), ends0 = lane_sums(places_of(len0));
     Span s;
-    s.total = __builtin_amdgcn_readfirstlane(sum) * per;
-    most = __builtin_amdgcn_readfirstlane(most);
-    // (a segment of `most` steps touches at most most / size + 2 spans)
-    s.size = max(max(p.span_min, (s.total + p.n_groups - 1) / p.n_groups), max(min((most + 31) / 32, 64), (most + kMaxPieces - 3) / (kMaxPieces - 2)));
-    s.b = 0;
-    s.first = 0;
+    s.empty = __ballot(len0 == 0);
+    int sum = __builtin_amdgcn_readlane(ends0, 63), most = lane_max(len0);
+    for (int b0 = 64; b0 < p.batch; b0 += 64) {
+        const int len = len_at(b0);
+        sum += __builtin_amdgcn_readlane(lane_sums(places_of(len)), 63);
+        most = max(most, lane_max(len));
+    }
+    most = steps_of(most);
+    s.total = sum * per;
+    // (the steps of a segment touch at most steps / size + 2 spans)
+    s.size = max(max(p.span_min, quotient(s.total + p.n_groups - 1, p.n_groups)), max(min((most + 31) / 32, 64), (most + kMaxPieces - 3) / (kMaxPieces - 2)));
+    s.b = s.first = s.len = 0;
     const long long at = (long long)group * s.size;
     if (at >= s.total) return s;
-    int before = 0;
-    for (int b0 = 0;; b0 += 64) {
-        const int mine = (b0 ? steps(b0) : head) * per;
-        int end = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(end, o, 64);
-            if (lane >= o) end += y;
-        }
-        const uint64_t past = __ballot(before + end > (int)at);
+    int before = 0, len = len0, ends = ends0;
+    for (int b0 = 0;;) {
+        const uint64_t past = __ballot((long long)before + (long long)ends * per > at);
         if (past) {  // (it is for one of them: `at` is below the total)
             const int l = __ffsll((unsigned long long)past) - 1;
-            s.b = __builtin_amdgcn_readfirstlane(b0 + l);
-            s.first = __builtin_amdgcn_readfirstlane(before + __shfl(end - mine, l, 64));
+            s.b = b0 + l;
+            s.len = __builtin_amdgcn_readlane(len, l);
+            s.first = before + (__builtin_amdgcn_readlane(ends, l) - places_of(s.len)) * per;
             return s;
         }
-        before += __shfl(end, 63, 64);
+        before += __builtin_amdgcn_readlane(ends, 63) * per;
+        b0 += 64;
+        len = len_at(b0);
+        ends = lane_sums(places_of(len));
     }
 }
 
@@ -114,12 +149,24 @@ constexpr int kWordPitch = 128;  // bytes: atomics on one line wait for each oth
 constexpr word_t kCountMask = 0xffff;
 struct SegmentWord {
     word_t* at;
-    word_t id;
+    word_t id, seen, got;
     __device__ __forceinline__ bool ours(word_t x) const { return ((x ^ id) & ~kCountMask) == 0; }
-    __device__ __forceinline__ void claim() {
-        word_t seen = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        while (!ours(seen) && !__hip_atomic_compare_exchange_strong(at, &seen, id, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) {
-        }  // (fails only if another workgroup was first, whose id is this one)
+    // what is there, asked for ahead of the rows; it is replaced behind their requests, and whether that has held is looked at ahead
+    // of the count: neither is waited for by itself
+    __device__ __forceinline__ void request(void* word, word_t launch_id) {
+        at = (word_t*)word;
+        id = launch_id;
+        seen = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __device__ __forceinline__ void replace() {
+        got = seen;
+        __hip_atomic_compare_exchange_strong(at, &got, ours(seen) ? seen : id, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __device__ __forceinline__ void settle() {
+        while (got != seen && !ours(got)) {  // (fails only if another workgroup was first, whose id is this one, or with another launch's word)
+            seen = got;
+            replace();
+        }
     }
     // counts one finished partial of `n`; true for the one that completes the set
     __device__ __forceinline__ bool count(int n) {
@@ -402,9 +449,16 @@ __device__ __forceinline__ void step(State<D, Q4>& st, const Keys<D, Q4, C>& x, 
     }
     if constexpr (kWeigh) {
         if (scores) {
+            if constexpr (kCut) {
 #pragma unroll
-            for (int e = 0; e < kE; e++)
-                if (!hid[e]) scores[place(e)] = y[e];
+                for (int e = 0; e < kE; e++)
+                    if (!hid[e]) scores[place(e)] = y[e];
+            } else if constexpr (C == 4) {
+                *(f32x2_any*)(scores + place(0)) = f32x2_any{y[0], y[1]};
+            } else {
+#pragma unroll
+                for (int e = 0; e < kE; e += 4) *(f32x4_any*)(scores + place(e)) = f32x4_any{y[e], y[e + 1], y[e + 2], y[e + 3]};
+            }
         }
     }
     // The running maximum, common to the four lanes of a column.  It follows the scores only where they have risen by 8 in the exponent
@@ -508,28 +562,30 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4>())) void cache_attend
 
     const Span span = span_of(p, group, lane);
     // sequences without keys, dealt to the workgroups: rows of zeros
-    if (p.kv_lens)
-        for (int b = group; b < p.batch; b += (int)gridDim.x)
-            if (len_of(p, b) == 0)
-                for (int i = tid; i < p.seq_new * p.heads * (D / 8); i += NT) *(u32x4_t*)(p.out + (size_t)b * p.seq_new * p.heads * D + 8 * i) = u32x4_t{0, 0, 0, 0};
+    for (int b = group; b < p.batch; b += (int)gridDim.x)
+        if (b < 64 ? (span.empty >> b & 1) != 0 : len_of(p, b) == 0)
+            for (int i = tid; i < p.seq_new * p.heads * (D / 8); i += NT) *(u32x4_t*)(p.out + (size_t)b * p.seq_new * p.heads * D + 8 * i) = u32x4_t{0, 0, 0, 0};
     const long long begin = (long long)group * span.size;
     if (begin >= span.total) return;
-    int at = (int)begin, b = span.b, first = span.first;
+    int at = (int)begin, b = span.b, first = span.first, len = span.len;
     const int end = (int)min((long long)span.total, begin + span.size);
 
     while (at < end) {
         // the piece of a segment from here
-        const int len = len_of(p, b), steps = steps_of(len);
-        if (at >= first + steps * per) {  // the next sequence
-            first += steps * per;
+        const int places = places_of(len);
+        if (at >= first + places * per) {  // the next sequence
+            first += places * per;
             b++;
+            len = len_of(p, b);
             continue;
         }
-        const int seg = (at - first) / steps, seg_first = first + seg * steps, t0 = at - seg_first, t1 = min(steps, t0 + (end - at));
-        const int kvh = seg / p.n_tiles, tile = seg - kvh * p.n_tiles;
-        const int w0 = seg_first / span.size, pieces = (seg_first + steps - 1) / span.size - w0 + 1;  // workgroups that have some of it
+        const int seg = quotient(at - first, places), seg_first = first + seg * places;
+        const int t0 = max(at - seg_first - kStart, 0), t1 = min(places, end - seg_first) - kStart;
+        at = min(seg_first + places, end);
+        if (t1 <= 0) continue;  // (places alone)
+        const int kvh = p.n_tiles == 1 ? seg : quotient(seg, p.n_tiles), tile = seg - kvh * p.n_tiles;
+        const int w0 = quotient(seg_first + kStart, span.size), pieces = quotient(seg_first + places - 1, span.size) - w0 + 1;  // workgroups that have some of its steps
         const size_t segment = (size_t)b * per + seg;
-        at += t1 - t0;
 
         const int r = tile * kR + n % kR;  // the query row: position * group + head of the group
         const bool there = r < p.rows;
@@ -537,6 +593,8 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4>())) void cache_attend
         const int seen = len - p.seq_new + s_new + 1;  // keys that it sees
         const size_t slab = ((size_t)b * p.kv_heads + kvh) * (size_t)p.max_seq;
 
+        SegmentWord word;
+        if (pieces > 1 && tid == 0) word.request(p.words + segment * kWordPitch, p.launch_id);
         // q as the operand that the keys' words pair with
         u32x4_t q[D / 32];
         float q_sum[kG] = {};
@@ -564,8 +622,7 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4>())) void cache_attend
                 load_v<D, C>(x, v, (t0 + wave) * kStep, len, n, quad);
             }
         }
-        SegmentWord word{(word_t*)(p.words + segment * kWordPitch), p.launch_id};
-        if (pieces > 1 && tid == 0) word.claim();
+        if (pieces > 1 && tid == 0) word.replace();
         if constexpr (!Q4) {
 #pragma unroll
             for (int c = 0; c < D / 32; c++) q[c] = nat[c];
@@ -708,6 +765,7 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4>())) void cache_attend
             __syncthreads();  // (the next piece's requests land where the fold was)
             continue;
         }
+        if (tid == 0) word.settle();
         if (tid < rows) put2(rs, mine + 4u * (uint32_t)(p.part_rows * D + 2 * tid), m_wg, l_wg);  // (tid < kR: n is tid)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
@@ -779,17 +837,32 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4>())) void cache_attend
     }
 }
 
-// The keys' weights from the scores and the rows' statistics.  Grid (1024 keys, kv heads, batch).
+// The keys' weights from the scores and the rows' statistics.  Grid (1024 keys, kv heads, batch), four keys a thread; the heads' scores
+// are asked for four at a time.
 __global__ __launch_bounds__(256) void cache_weigh_kernel(CacheAttendParams p) {
-    const int kvh = blockIdx.y, b = blockIdx.z, len = len_of(p, b);
-    const size_t sums = ((size_t)b * p.kv_heads + kvh) * (size_t)p.max_seq;
-    for (int j = (int)blockIdx.x * 1024 + (int)threadIdx.x, e = 0; e < 4 && j < len; e++, j += 256) {
-        float w = p.weights_in ? p.weights_in[sums + j] : 0.0f, sum = 0.0f;
+    const int kvh = blockIdx.y, b = blockIdx.z, len = len_of(p, b), j = (int)blockIdx.x * 1024 + 4 * (int)threadIdx.x;
+    if (j >= len) return;
+    const size_t sums = ((size_t)b * p.kv_heads + kvh) * (size_t)p.max_seq + j, row0 = (size_t)b * p.heads + kvh * p.group;
+    const float* scores = p.scores + row0 * p.max_seq + j;
+    const float* stats = p.stats + 2 * row0;
+    auto part = [&](float y, int h) __attribute__((always_inline)) { return __builtin_amdgcn_exp2f((y - stats[2 * h]) * p.scale_log2e) * stats[2 * h + 1]; };
+    if (j + 4 <= len) {
+        f32x4_t w = {0, 0, 0, 0};
+        if (p.weights_in) w = *(const f32x4_any*)(p.weights_in + sums);
+        f32x4_t sum = {0, 0, 0, 0};
+#pragma unroll 4
         for (int h = 0; h < p.group; h++) {
-            const size_t row = (size_t)b * p.heads + kvh * p.group + h;
-            sum += __builtin_amdgcn_exp2f((p.scores[row * p.max_seq + j] - p.stats[2 * row]) * p.scale_log2e) * p.stats[2 * row + 1];
+            const f32x4_t y = *(const f32x4_any*)(scores + (size_t)h * p.max_seq);
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum[e] += part(y[e], h);
         }
-        p.weights_out[sums + j] = w + sum;
+        *(f32x4_any*)(p.weights_out + sums) = w + sum;
+        return;
+    }
+    for (int e = 0; j + e < len; e++) {
+        float sum = 0.0f;
+        for (int h = 0; h < p.group; h++) sum += part(scores[(size_t)h * p.max_seq + e], h);
+        p.weights_out[sums + e] = (p.weights_in ? p.weights_in[sums + e] : 0.0f) + sum;
     }
 }
 
@@ -827,7 +900,7 @@ AttendPlan plan_attend(int64_t batch, int64_t seq_new, int64_t heads, int64_t kv
     a.rows = seq_new * (heads / kv_heads);
     a.n_tiles = (a.rows + 15) / 16;
     a.segments = batch * kv_heads * a.n_tiles;
-    a.steps = a.segments * ((max_seq + kStep - 1) / kStep);
+    a.steps = a.segments * ((max_seq + kStep - 1) / kStep + kStart);
     a.groups = (int)std::min<int64_t>(groups_at_once(dim, q4), std::max<int64_t>((a.steps + kWaves - 1) / kWaves, 1));
     a.part_rows = (int)std::min<int64_t>(16, a.rows);
     auto round = [](size_t x) { return (x + 255) / 256 * 256; };

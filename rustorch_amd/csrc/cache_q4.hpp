@@ -70,6 +70,7 @@ struct CacheAttendParams {
     int n_tiles;  // of 16 of them
     int n_groups;  // workgroups launched
     int span_min;  // one takes at least this many steps of 32 keys
+    int few_pieces;  // into about how many a segment is cut where that leaves them short
     float scale_log2e;
     float* part;    // partials: (n_groups + segments) slots of part_rows * (dim + 2) floats, the rows and behind them their (m, l)
     int part_rows;  // min(16, rows)

@@ -91,9 +91,20 @@ struct Span {
 // Lengths 64 at a time, the first of them once for both walks.
 __device__ __forceinline__ Span span_of(const CacheAttendParams& p, int group, int lane) {
     const int per = p.kv_heads * p.n_tiles;
+    Span s;
+    if (p.batch == 1) {  // (one scalar load)
+        int len = p.kv_len;
+        if (p.kv_lens) len = min(max(*(const __attribute__((address_space(4))) int32_t*)p.kv_lens, 0), p.max_seq);
+        s.empty = len == 0;
+        s.total = places_of(len) * per;
+        const int most = steps_of(len);
+        s.size = max(max(p.span_min, quotient(s.total + p.n_groups - 1, p.n_groups)), max(min(quotient(most + p.few_pieces - 1, p.few_pieces), 64), (most + kMaxPieces - 3) / (kMaxPieces - 2)));
+        s.b = s.first = 0;
+        s.len = len;
+        return s;
+    }
     auto len_at = [&](int b0) { return b0 + lane < p.batch ? len_of(p, b0 + lane) : 0; };
     const int len0 = len_at(0), ends0 = lane_sums(places_of(len0));
-    Span s;
     s.empty = __ballot(len0 == 0);
     int sum = __builtin_amdgcn_readlane(ends0, 63), most = lane_max(len0);
     for (int b0 = 64; b0 < p.batch; b0 += 64) {
@@ -104,7 +115,7 @@ __device__ __forceinline__ Span span_of(const CacheAttendParams& p, int group, i
     most = steps_of(most);
     s.total = sum * per;
     // (the steps of a segment touch at most steps / size + 2 spans)
-    s.size = max(max(p.span_min, quotient(s.total + p.n_groups - 1, p.n_groups)), max(min((most + 31) / 32, 64), (most + kMaxPieces - 3) / (kMaxPieces - 2)));
+    s.size = max(max(p.span_min, quotient(s.total + p.n_groups - 1, p.n_groups)), max(min(quotient(most + p.few_pieces - 1, p.few_pieces), 64), (most + kMaxPieces - 3) / (kMaxPieces - 2)));
     s.b = s.first = s.len = 0;
     const long long at = (long long)group * s.size;
     if (at >= s.total) return s;
@@ -220,6 +231,7 @@ template <int D>
 struct Ring {
     static constexpr int kRow = D / 2, kStages = 2, kG = D / 64;
     static constexpr int kRows = 32 * kRow, kPairs = D == 256 ? 512 : 256;  // bytes of K or V, of their pairs
+    static_assert(kStages == 2, "the waits of the walk");
     static constexpr int kStage = 2 * kRows + 2 * kPairs;
     static constexpr int kLoads = 2 * (kRows / 1024) + 2 * (kPairs / 256);  // requests a stage
     // the source of what lands at byte `at` of 16 rows
@@ -249,12 +261,12 @@ struct RingLanes {  // byte offsets of a lane's requests
 };
 
 // The requests of one step: keys [key0, key0 + 32) of a slab of `len` keys.  What lies behind the last key lands as zeros, but for pairs
-// of another group's first keys, which no visible key's place takes.  key0 >= len: all zeros, nothing is read.
+// of another group's first keys, which no visible key's place takes.  key0 < len.
 template <int D>
 __device__ __forceinline__ void ring_load(const RingLanes<D>& at, uint32_t lds, const uint8_t* k, const uint8_t* v, const uint32_t* kp, const uint32_t* vp, int max_seq, int key0, int len) {
     using R = Ring<D>;
-    const int keys = max(0, min(kStep, len - key0));
-    const size_t from = keys ? (size_t)key0 : 0;
+    const int keys = min(kStep, len - key0);
+    const size_t from = (size_t)key0;
     const uint32_t bytes = (uint32_t)keys * R::kRow;
     const u32x4_t krs = make_rsrc(k + from * R::kRow, bytes), vrs = make_rsrc(v + from * R::kRow, bytes);
 #pragma unroll
@@ -262,7 +274,7 @@ __device__ __forceinline__ void ring_load(const RingLanes<D>& at, uint32_t lds, 
         buffer_to_lds(krs, at.k[i], 0u, lds + 1024u * i);
         buffer_to_lds(vrs, at.v[i], 0u, lds + R::kRows + 1024u * i);
     }
-    const uint32_t pair_bytes = keys ? 4u * (uint32_t)keys + (D > 64 ? 4u * (uint32_t)max_seq : 0u) : 0u;
+    const uint32_t pair_bytes = 4u * (uint32_t)keys + (D > 64 ? 4u * (uint32_t)max_seq : 0u);
 #pragma unroll
     for (int i = 0; i < R::kPairs / 256; i++) {
         buffer_to_lds_b32(make_rsrc(kp + from + (size_t)(2 * i) * max_seq, pair_bytes), at.pair, 0u, lds + 2 * R::kRows + 256u * i);
@@ -337,6 +349,31 @@ __device__ __forceinline__ float quad_max(float x) {
     const u32x2_t c = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
     return fmaxf(__uint_as_float(c[0]), __uint_as_float(c[1]));
 }
+// A row of sixteen lanes turned by kBy, and what that makes of columns that lie 16 / C apart: their largest, their sum, in every one.
+template <int kBy>
+__device__ __forceinline__ float turned(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + kBy, 0xf, 0xf, false));
+}
+template <int C>
+__device__ __forceinline__ float columns_max(float x) {
+    if (C >= 2) x = fmaxf(x, turned<8>(x));
+    if (C >= 4) x = fmaxf(x, turned<4>(x));
+    if (C == 16) {
+        x = fmaxf(x, turned<2>(x));
+        x = fmaxf(x, turned<1>(x));
+    }
+    return x;
+}
+template <int C>
+__device__ __forceinline__ float columns_sum(float x) {
+    if (C >= 2) x += turned<8>(x);
+    if (C >= 4) x += turned<4>(x);
+    if (C == 16) {
+        x += turned<2>(x);
+        x += turned<1>(x);
+    }
+    return x;
+}
 __device__ __forceinline__ float quad_sum(float x) {
     const u32x2_t a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     const float y = __uint_as_float(a[0]) + __uint_as_float(a[1]);
@@ -355,8 +392,8 @@ __device__ __forceinline__ float two_terms(float a, float b, uint32_t& hi, uint3
 }
 
 // Waves that an SIMD holds.
-template <int D, bool Q4>
-constexpr int per_simd() { return D == 64 ? 4 : D == 128 ? (Q4 ? 4 : 2) : Q4 ? 2 : 1; }
+template <int D, bool Q4, int C>
+constexpr int per_simd() { return D == 64 ? 4 : D == 128 ? (!Q4 ? 2 : C == 4 ? 4 : 3) : Q4 ? 2 : 1; }
 
 // What a lane has of its query row over the keys it has walked.
 template <int D, bool Q4>
@@ -550,7 +587,7 @@ __device__ __forceinline__ void step(State<D, Q4>& st, const Keys<D, Q4, C>& x, 
 }
 
 template <int D, bool Q4, int C, bool kWeigh>
-__global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4>())) void cache_attend_kernel(CacheAttendParams p) {
+__global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4, C>())) void cache_attend_kernel(CacheAttendParams p) {
     constexpr int kG = Keys<D, Q4, C>::kG, NT = 64 * kWaves, kPitch = D + 4, kR = 16 / C;  // kR query rows
     constexpr int kRingBytes = Q4 ? kWaves * Ring<D>::kStages * Ring<D>::kStage : 0, kFold = kWaves * 16 * kPitch * 4, kFolds = kMaxPieces * 16 * 8 + NT * 16;
     constexpr int kLds = std::max(std::max(kRingBytes, kFold), kFolds);
@@ -615,7 +652,8 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4>())) void cache_attend
         Keys<D, Q4, C> x;
         if constexpr (Q4) {
 #pragma unroll
-            for (int s = 0; s < Ring<D>::kStages; s++) ring_load<D>(lanes, ring + s * Ring<D>::kStage, k, v, kp, vp, p.max_seq, (t0 + wave + s * kWaves) * kStep, t0 + wave + s * kWaves < t1 ? len : 0);
+            for (int s = 0; s < Ring<D>::kStages; s++)
+                if (t0 + wave + s * kWaves < t1) ring_load<D>(lanes, ring + s * Ring<D>::kStage, k, v, kp, vp, p.max_seq, (t0 + wave + s * kWaves) * kStep, len);
         } else {
             if (t0 + wave < t1) {
                 load_k<D, C>(x, k, (t0 + wave) * kStep, len, n, quad);
@@ -660,15 +698,18 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4>())) void cache_attend
             const int key0 = t * kStep;
             float* const to = kWeigh && there ? scores + key0 : nullptr;
             if constexpr (Q4) {
-                // (all but the newest kStages - 1 steps' requests are there)
-                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Ring<D>::kLoads * (Ring<D>::kStages - 1)) : "memory");
+                // (this step's requests are there, if not the next one's)
+                if (t + kWaves < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(Ring<D>::kLoads) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 const unsigned char* const rows = ring_at + stage * Ring<D>::kStage;
                 ring_k<D, C>(x, rows, n, cls, quad);
                 step<D, Q4, C, kCut, kWeigh>(st, x, [] {}, [&]() __attribute__((always_inline)) { ring_v<D, C>(x, rows, n, cls, quad); }, codes, q, q_sum, cls, key0 + 4 * quad, seen, p.scale_log2e, to);
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read before it is written again)
                 const int next = t + Ring<D>::kStages * kWaves;
-                ring_load<D>(lanes, ring + stage * Ring<D>::kStage, k, v, kp, vp, p.max_seq, next * kStep, next < t1 ? len : 0);
-                stage = stage + 1 == Ring<D>::kStages ? 0 : stage + 1;
+                if (next < t1) {
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read before it is written again)
+                    ring_load<D>(lanes, ring + stage * Ring<D>::kStage, k, v, kp, vp, p.max_seq, next * kStep, len);
+                }
+                stage ^= 1;
             } else {
                 const int next = t + kWaves;
                 step<D, Q4, C, kCut, kWeigh>(st, x, [&]() __attribute__((always_inline)) { if (next < t1) load_k<D, C>(x, k, next * kStep, len, n, quad); }, [] {}, codes, q, q_sum, cls, key0 + 4 * quad, seen,
@@ -679,43 +720,43 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4>())) void cache_attend
         };
         while (t < t_whole) take(std::false_type{});
         while (t < t1) take(std::true_type{});
-        if constexpr (Q4) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (what is still under way lands in memory of the fold)
-
         // ---- fold the four waves, and the columns of a row.  (The thread's number anew: what follows from it would be worked out
         // ahead of the steps otherwise, and take their registers.)
         int ft = threadIdx.x;
         asm volatile("" : "+v"(ft));
         const int tid = ft, lane = ft & 63, n = ft & 15, quad = lane >> 4;
-        const float l = quad_sum(st.l);
+        const float m = columns_max<C>(st.m), f = __builtin_amdgcn_exp2f((st.m - m) * p.scale_log2e);
+        const float l = columns_sum<C>(quad_sum(st.l) * f);
         if constexpr (Q4) {
 #pragma unroll
             for (int g = 0; g < kG; g++) {
                 const float off = quad_sum(st.pz[g]) - 24.0f * quad_sum(st.ps[g]);
 #pragma unroll
-                for (int f = 0; f < 4; f++) {
-                    const int byte = D == 64 ? f / 2 : (g & 1) + 2 * (f / 2);
-                    st.o[8 * (D == 64 ? 0 : g / 2) + 2 * byte + f % 2] += off;
+                for (int i = 0; i < 4; i++) {
+                    const int byte = D == 64 ? i / 2 : (g & 1) + 2 * (i / 2);
+                    st.o[8 * (D == 64 ? 0 : g / 2) + 2 * byte + i % 2] += off;
                 }
             }
         }
-        if (quad == 0) {
-            red_m[wave][n] = st.m;
+        if (C > 1)
+#pragma unroll
+            for (int i = 0; i < D / 16; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) st.o[i][e] = columns_sum<C>(st.o[i][e] * f);
+        float* const red = (float*)lds;  // [wave][row][kPitch]
+        if (n < kR && quad == 0) {
+            red_m[wave][n] = m;
             red_l[wave][n] = l;
         }
         __syncthreads();  // also: every wave is done with the ring
-        float m_wg = kNoMax, l_wg = 0.0f;  // of row n % kR
+        float m_wg = red_m[0][n % kR], l_wg = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWaves; w++)
+        for (int w = 1; w < kWaves; w++) m_wg = fmaxf(m_wg, red_m[w][n % kR]);
 #pragma unroll
-            for (int c = 0; c < C; c++) m_wg = fmaxf(m_wg, red_m[w][n % kR + c * kR]);
-#pragma unroll
-        for (int w = 0; w < kWaves; w++)
-#pragma unroll
-            for (int c = 0; c < C; c++) l_wg += red_l[w][n % kR + c * kR] * __builtin_amdgcn_exp2f((red_m[w][n % kR + c * kR] - m_wg) * p.scale_log2e);
-        float* const red = (float*)lds;
-        {
-            const float f = __builtin_amdgcn_exp2f((st.m - m_wg) * p.scale_log2e);
-            float* row = red + (wave * 16 + n) * kPitch;
+        for (int w = 0; w < kWaves; w++) l_wg += red_l[w][n % kR] * __builtin_amdgcn_exp2f((red_m[w][n % kR] - m_wg) * p.scale_log2e);
+        if (n < kR) {
+            const float fw = __builtin_amdgcn_exp2f((m - m_wg) * p.scale_log2e);
+            float* row = red + (wave * kR + n) * kPitch;
 #pragma unroll
             for (int c = 0; c < D / 32; c++) {  // eight dims in a row
                 float y[8];
@@ -723,17 +764,17 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4>())) void cache_attend
                 for (int e = 0; e < 8; e++) {
                     if constexpr (Q4) {
                         const int byte = D == 64 ? c : (c & ~3) | (c & 1) << 1 | (c >> 1 & 1);
-                        y[e] = st.o[2 * byte + e % 2][e / 2] * f;
+                        y[e] = st.o[2 * byte + e % 2][e / 2] * fw;
                     } else {
-                        y[e] = st.o[(8 * c + e) % (D / 16)][(8 * c + e) / (D / 16)] * f;
+                        y[e] = st.o[(8 * c + e) % (D / 16)][(8 * c + e) / (D / 16)] * fw;
                     }
                 }
                 float* dst = row + (Q4 ? 32 * c + 8 * quad : quad * (D / 4) + 8 * c);
                 *(f32x4_t*)dst = f32x4_t{y[0], y[1], y[2], y[3]};
                 *(f32x4_t*)(dst + 4) = f32x4_t{y[4], y[5], y[6], y[7]};
             }
+            if (wave == 0 && quad == 0) inv_l[n] = l_wg == 0.0f ? 0.0f : 1.0f / l_wg;
         }
-        if (wave == 0 && quad == 0 && n < kR) inv_l[n] = l_wg == 0.0f ? 0.0f : 1.0f / l_wg;
         __syncthreads();
         const int rows = min(kR, p.rows - tile * kR);
         const uint32_t slot_bytes = (uint32_t)p.part_rows * (D + 2) * 4;
@@ -748,7 +789,7 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4>())) void cache_attend
             const int row = i / (D / 4), d = 4 * (i % (D / 4));
             f32x4_t o = {0, 0, 0, 0};
 #pragma unroll
-            for (int w = 0; w < kWaves * C; w++) o += *(const f32x4_t*)(red + (w * kR + row) * kPitch + d);
+            for (int w = 0; w < kWaves; w++) o += *(const f32x4_t*)(red + (w * kR + row) * kPitch + d);
             if (pieces == 1) {
                 o *= inv_l[row];
                 *(u32x2_t*)(p.out + out_row(row) + d) = u32x2_t{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
@@ -772,56 +813,62 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4>())) void cache_attend
         if (tid == 0) is_last = word.count(pieces) ? 1 : 0;
         __syncthreads();
         if (is_last) {
-            // ---- the last workgroup of the segment: the weighted sum of its partials, the weights first
-            float* const wgt = (float*)lds;  // [pieces][16] (m, then the factor), l behind
+            // ---- the last workgroup of the segment: the weighted sum of its partials.  Items of four elements, kAhead pieces of each at a
+            // time; where there are fewer items than threads, several threads an item, each with every sub-th piece.  The first are asked
+            // for ahead of the (m, l) that their weights are made of.
+            constexpr int kAhead = 8;
+            float* const wgt = (float*)lds;  // [pieces][16]
             float* const wl = wgt + kMaxPieces * 16;
             f32x4_t* const part = (f32x4_t*)(wl + kMaxPieces * 16);
-            for (int i = tid; i < pieces * rows; i += NT) {
-                const int piece = i / rows, row = i - piece * rows;
-                const u32x2_t ml = get2(rs, (uint32_t)piece * slot_bytes + 4u * (uint32_t)(p.part_rows * D + 2 * row));
-                wgt[piece * 16 + row] = __uint_as_float(ml[0]);
-                wl[piece * 16 + row] = __uint_as_float(ml[1]);
-            }
-            __syncthreads();
-            for (int row = wave; row < rows; row += kWaves) {
-                float m = kNoMax, sum = 0.0f;
-                for (int i = lane; i < pieces; i += 64) m = fmaxf(m, wgt[i * 16 + row]);
+            const int items = rows * (D / 4), sub_n = items >= NT ? 1 : NT / items;
+            const int x0 = sub_n == 1 ? tid : tid % items, sub = sub_n == 1 ? 0 : tid / items;
+            f32x4_t a[kAhead];
+            auto ask = [&](int i, int k0) __attribute__((always_inline)) {  // (row and element follow one another in a slot)
+                const uint32_t from = 16u * (uint32_t)min(i, items - 1);
 #pragma unroll
-                for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-                for (int i = lane; i < pieces; i += 64) {
-                    const float f = __builtin_amdgcn_exp2f((wgt[i * 16 + row] - m) * p.scale_log2e);
-                    wgt[i * 16 + row] = f;
-                    sum += wl[i * 16 + row] * f;
+                for (int e = 0; e < kAhead; e++) a[e] = get4(rs, (uint32_t)min(k0 + e * sub_n, pieces - 1) * slot_bytes + from);
+            };
+            ask(x0, sub);
+            {
+                const int row = tid >> 4, col = tid & 15;  // sixteen lanes a row
+                const bool on = row < rows;
+                float top = kNoMax, sum = 0.0f;
+                for (int k = col; on && k < pieces; k += 16) {
+                    const u32x2_t ml = get2(rs, (uint32_t)k * slot_bytes + 4u * (uint32_t)(p.part_rows * D + 2 * row));
+                    wgt[k * 16 + row] = __uint_as_float(ml[0]);
+                    wl[k * 16 + row] = __uint_as_float(ml[1]);
+                    top = fmaxf(top, __uint_as_float(ml[0]));
                 }
-#pragma unroll
-                for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
-                if (lane == 0) {
+                top = columns_max<16>(top);
+                for (int k = col; on && k < pieces; k += 16) {
+                    const float fk = __builtin_amdgcn_exp2f((wgt[k * 16 + row] - top) * p.scale_log2e);
+                    wgt[k * 16 + row] = fk;
+                    sum += wl[k * 16 + row] * fk;
+                }
+                sum = columns_sum<16>(sum);
+                if (on && col == 0) {
                     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                     inv_l[row] = inv;
                     if (kWeigh) {
                         float* to = p.stats + ((size_t)b * p.heads + kvh * p.group + tile * kR + row) * 2;
-                        to[0] = m;
+                        to[0] = top;
                         to[1] = inv;
                     }
                 }
             }
             __syncthreads();
-            // items of four elements; where there are fewer than threads, several threads an item, each with every sub-th piece
-            const int items = rows * (D / 4), sub_n = items >= NT ? 1 : NT / items;
             for (int i0 = 0; i0 < items; i0 += NT) {
-                const int i = i0 + (sub_n == 1 ? tid : tid % items), sub = sub_n == 1 ? 0 : tid / items;
+                const int i = i0 + x0;
                 const bool on = i < items && sub < sub_n;
-                const int row = on ? i / (D / 4) : 0, d = on ? 4 * (i % (D / 4)) : 0;
+                const int row = on ? i / (D / 4) : 0, d = 4 * (i % (D / 4));
                 f32x4_t o = {0, 0, 0, 0};
-                for (int k0 = sub; on && k0 < pieces; k0 += 8 * sub_n) {  // eight loads at a time
-                    f32x4_t a[8];
+                for (int k0 = sub; on && k0 < pieces; k0 += kAhead * sub_n) {
+                    if (i0 || k0 != sub) ask(i, k0);
 #pragma unroll
-                    for (int e = 0; e < 8; e++) a[e] = get4(rs, (uint32_t)min(k0 + e * sub_n, pieces - 1) * slot_bytes + 4u * (uint32_t)(row * D + d));
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
+                    for (int e = 0; e < kAhead; e++)
                         if (k0 + e * sub_n < pieces) o += a[e] * wgt[(k0 + e * sub_n) * 16 + row];
                 }
-                if (sub_n > 1) {
+                if (sub_n > 1) {  // (one round)
                     part[tid] = o;
                     __syncthreads();
                     if (on && sub == 0)
@@ -889,11 +936,10 @@ struct AttendPlan {
     size_t bytes() const { return part_bytes + word_bytes + score_bytes + stat_bytes; }
 };
 // workgroups that the chip holds at once (a wave of each on every SIMD)
-int groups_at_once(int64_t dim, bool q4) {
-    if (dim == 64) return kCus * per_simd<64, true>();
-    if (dim == 128) return kCus * (q4 ? per_simd<128, true>() : per_simd<128, false>());
-    return kCus * (q4 ? per_simd<256, true>() : per_simd<256, false>());
-}
+template <int D, bool Q4>
+int groups_at_once(int64_t rows) { return kCus * (rows <= 4 ? per_simd<D, Q4, 4>() : rows <= 8 ? per_simd<D, Q4, 2>() : per_simd<D, Q4, 1>()); }
+template <bool Q4>
+int groups_at_once(int64_t dim, int64_t rows) { return dim == 64 ? groups_at_once<64, Q4>(rows) : dim == 128 ? groups_at_once<128, Q4>(rows) : groups_at_once<256, Q4>(rows); }
 // (q4: the same workspace serves either kind of cache, so it is sized for the one with more workgroups)
 AttendPlan plan_attend(int64_t batch, int64_t seq_new, int64_t heads, int64_t kv_heads, int64_t dim, int64_t max_seq, bool weigh, bool q4 = true) {
     AttendPlan a{};
@@ -901,7 +947,7 @@ AttendPlan plan_attend(int64_t batch, int64_t seq_new, int64_t heads, int64_t kv
     a.n_tiles = (a.rows + 15) / 16;
     a.segments = batch * kv_heads * a.n_tiles;
     a.steps = a.segments * ((max_seq + kStep - 1) / kStep + kStart);
-    a.groups = (int)std::min<int64_t>(groups_at_once(dim, q4), std::max<int64_t>((a.steps + kWaves - 1) / kWaves, 1));
+    a.groups = (int)std::min<int64_t>(q4 ? groups_at_once<true>(dim, a.rows) : groups_at_once<false>(dim, a.rows), std::max<int64_t>((a.steps + kWaves - 1) / kWaves, 1));
     a.part_rows = (int)std::min<int64_t>(16, a.rows);
     auto round = [](size_t x) { return (x + 255) / 256 * 256; };
     a.part_bytes = round(((size_t)a.groups + (size_t)a.segments) * (size_t)a.part_rows * (size_t)(dim + 2) * 4);
@@ -944,6 +990,7 @@ int attend_common(void* stream, CacheAttendParams& p, int head_dim, bool q4, boo
     p.n_tiles = (int)a.n_tiles;
     p.n_groups = groups;
     p.span_min = kWaves;
+    p.few_pieces = a.rows <= 4 ? 32 : a.rows <= 8 ? 24 : 16;
     p.scale_log2e = (1.0f / sqrtf((float)head_dim)) * kLog2eHost;
     p.part = (float*)workspace;
     p.part_rows = a.part_rows;

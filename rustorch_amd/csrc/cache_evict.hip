@@ -23,49 +23,38 @@ constexpr int kSelect = 1024, kSelectWaves = kSelect / 64, kPer = 8, kTile = kSe
 constexpr int kBins = 2048;
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // 16 bytes from any word
 
-// The order of the sums as that of whole numbers: NaN counts as -infinity, -0 as 0, the newest tokens' as +infinity.
+// The order of the sums as that of whole numbers: NaN counts as -infinity, -0 as 0, the newest tokens' as +infinity.  0 is no sum's.
 constexpr uint32_t kNewest = 0xff800000u;
-__device__ __forceinline__ uint32_t key_of(float w, int pos, long long newest_out) {
-    if ((long long)pos > newest_out) return kNewest;
-    if (w != w) return 0x007fffffu;
-    const uint32_t u = __float_as_uint(w == 0.0f ? 0.0f : w);
-    return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+__device__ __forceinline__ uint32_t key_of(float w) {
+    const uint32_t u = __float_as_uint(w + 0.0f), x = u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+    return w != w ? 0x007fffffu : x;
 }
 
-// A workgroup's reductions and sums: in a wave, then over the waves' results in `room` (kSelectWaves words), one barrier ahead of
-// their writing and one behind it.
-template <typename T, typename F>
-__device__ __forceinline__ T all_of(T x, F f, T* room) {
+__device__ __forceinline__ uint32_t bits(float x) { return __float_as_uint(x); }
+__device__ __forceinline__ uint32_t bits(int32_t x) { return (uint32_t)x; }
+
+// A workgroup's largest of three numbers and its sums: in a wave, then over the waves' results in `room` (not those of the call
+// before: one barrier is enough then), all of it within registers (lanes_step, cache_q4.hpp).
+__device__ __forceinline__ void largest_of(uint32_t (&x)[3], uint32_t (*room)[kSelectWaves]) {
+    auto f = [](uint32_t a, uint32_t b) __attribute__((always_inline)) { return max(a, b); };
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) x = f(x, __shfl_xor(x, o, 64));
+    for (int i = 0; i < 3; i++) {
+        const uint32_t y = lanes_fold<6>(x[i], f);
+        if ((threadIdx.x & 63) == 63) room[i][threadIdx.x >> 6] = y;
+    }
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = x;
-    __syncthreads();
-    T y = room[threadIdx.x & (kSelectWaves - 1)];
 #pragma unroll
-    for (int o = kSelectWaves / 2; o >= 1; o >>= 1) y = f(y, __shfl_xor(y, o, 64));
-    return y;
+    for (int i = 0; i < 3; i++) x[i] = __builtin_amdgcn_readlane(lanes_fold<4>(room[i][threadIdx.x & (kSelectWaves - 1)], f), kSelectWaves - 1);
 }
 // The sum over the threads before this one; `all`: over all.
 __device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t* room, uint32_t* all) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t end = x;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t y = __shfl_up(end, o, 64);
-        if (lane >= o) end += y;
-    }
-    __syncthreads();
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t end = lane_sums((int)x);
     if (lane == 63) room[wave] = end;
     __syncthreads();
-    uint32_t y = room[lane & (kSelectWaves - 1)];
-#pragma unroll
-    for (int o = 1; o < kSelectWaves; o <<= 1) {
-        const uint32_t z = __shfl_up(y, o, kSelectWaves);
-        if ((lane & (kSelectWaves - 1)) >= o) y += z;
-    }
-    *all = __shfl(y, kSelectWaves - 1, 64);
-    return end - x + (wave ? __shfl(y, wave - 1, 64) : 0u);
+    const uint32_t ends = lane_sums((int)(lane < kSelectWaves ? room[lane] : 0u));
+    *all = __builtin_amdgcn_readlane(ends, kSelectWaves - 1);
+    return end - x + (wave ? __builtin_amdgcn_readlane(ends, wave - 1) : 0u);
 }
 
 // One workgroup a (sequence, kv head), grid (kv heads, batch).  Thread t has the slots 8 t .. 8 t + 7 of a tile of 8192; up to there the keys are
@@ -75,7 +64,8 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t* room, uint3
 // (By fixed bytes from the top most sums share a bin, and a wave's counts in one word wait for each other: 8192 keys 30 us.)
 template <bool kOne>
 __global__ __launch_bounds__(kSelect) void cache_select_kernel(CacheEvictParams p) {
-    __shared__ uint32_t bins[kBins], room[kSelectWaves], chosen[2];
+    __shared__ uint32_t bins[kBins], chosen[2], above_all, room[6][kSelectWaves];
+    __shared__ uint16_t listed[2 * kTile];  // of a tile, in order: the slots that are freed, and behind them the rows that move
     const int tid = threadIdx.x, b = blockIdx.y, head = b * p.n_kv + (int)blockIdx.x;
     const int len = min(max(p.kv_lens[b], 0), p.max_seq);
     const float* w_in = p.weights_in + (size_t)head * p.max_seq;
@@ -83,23 +73,11 @@ __global__ __launch_bounds__(kSelect) void cache_select_kernel(CacheEvictParams 
     float* w_out = p.weights_out + (size_t)head * p.max_seq;
     int32_t* s_out = p.slots_out + (size_t)head * p.max_seq;
     const bool copy_w = w_in != w_out, copy_s = s_in != s_out;
-    if (len <= p.budget || p.budget == 0) {  // all of it stays, or nothing
-        for (int j = tid; j < min(len, p.budget); j += kSelect) {
-            if (copy_w) w_out[j] = w_in[j];
-            if (copy_s) s_out[j] = s_in[j];
-        }
-        if (tid == 0) {
-            p.header[2 * head] = len;
-            p.header[2 * head + 1] = 0;
-        }
-        return;
-    }
-    const int tiles = kOne ? 1 : (len + kTile - 1) / kTile;
     float w[kPer];
     int32_t s[kPer];
-    auto load = [&](int tile) __attribute__((always_inline)) {  // (slots behind the last: what its key is made of does not count)
+    auto load = [&](int tile) __attribute__((always_inline)) {
         const int j0 = tile * kTile + tid * kPer;
-        if (j0 + kPer <= len) {
+        if (j0 + kPer <= p.max_seq) {  // (whatever the length, which is still on its way)
 #pragma unroll
             for (int e = 0; e < kPer; e += 4) {
                 const u32x4_any a = *(const u32x4_any*)(w_in + j0 + e), c = *(const u32x4_any*)(s_in + j0 + e);
@@ -113,107 +91,155 @@ __global__ __launch_bounds__(kSelect) void cache_select_kernel(CacheEvictParams 
         }
 #pragma unroll
         for (int e = 0; e < kPer; e++) {
-            w[e] = j0 + e < len ? w_in[j0 + e] : 0.0f;
-            s[e] = j0 + e < len ? s_in[j0 + e] : INT32_MIN;
+            w[e] = j0 + e < p.max_seq ? w_in[j0 + e] : 0.0f;
+            s[e] = j0 + e < p.max_seq ? s_in[j0 + e] : 0;
         }
     };
-    // the newest token
-    int newest = INT32_MIN;
-    for (int t = 0; t < tiles; t++) {
-        load(t);
-#pragma unroll
-        for (int e = 0; e < kPer; e++) newest = max(newest, s[e]);
-    }
-    newest = all_of(newest, [](int x, int y) { return max(x, y); }, (int*)room);
-    const long long out_from = (long long)newest - p.recent;
     uint32_t key[kPer];
-    auto keys = [&](int tile) __attribute__((always_inline)) {
-        if (!kOne) load(tile);
+    auto sums = [&](int tile) __attribute__((always_inline)) {  // 0 behind the last slot
+        const int there = len - tile * kTile - tid * kPer;
 #pragma unroll
-        for (int e = 0; e < kPer; e++) key[e] = key_of(w[e], s[e], out_from);
+        for (int e = 0; e < kPer; e++) key[e] = e < there ? key_of(w[e]) : 0u;
     };
-    auto in = [&](int tile, int e) __attribute__((always_inline)) { return tile * kTile + tid * kPer + e < len; };
-    // the newest tokens' keys, which are the largest, apart: they would stretch the range of the others
-    uint32_t low = ~0u, high = 0, at_top = 0;
+    if (kOne) load(0);
+    if (len <= p.budget || p.budget == 0) {  // all of it stays, or nothing
+        for (int j = tid; j < min(len, p.budget); j += kSelect) {
+            if (copy_w) w_out[j] = w_in[j];
+            if (copy_s) s_out[j] = s_in[j];
+        }
+        if (tid == 0) {
+            p.header[2 * head] = len;
+            p.header[2 * head + 1] = 0;
+        }
+        return;
+    }
+    const int tiles = kOne ? 1 : (len + kTile - 1) / kTile;
+    bins[tid] = bins[tid + kSelect] = 0;
+    if (tid == 0) above_all = 0;
+    // the newest token (positions as unsigned numbers in their order), and the range of the sums' keys
+    uint32_t most[3] = {0, 0, 0};
     for (int t = 0; t < tiles; t++) {
-        keys(t);
+        if (!kOne) load(t);
+        sums(t);
 #pragma unroll
-        for (int e = 0; e < kPer; e++)
-            if (in(t, e)) {
-                at_top += key[e] == kNewest;
-                if (key[e] != kNewest) {
-                    low = min(low, key[e]);
-                    high = max(high, key[e]);
+        for (int e = 0; e < kPer; e++) {
+            most[0] = max(most[0], key[e] ? bits(s[e]) ^ 0x80000000u : 0u);
+            most[1] = max(most[1], key[e]);
+            most[2] = max(most[2], key[e] ? ~key[e] : 0u);
+        }
+    }
+    largest_of(most, room);
+    const uint32_t newest = most[0] ^ 0x80000000u;
+    uint32_t high = most[1], low = ~most[2];
+    auto newer = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < kPer; e++) key[e] = key[e] && newest - bits(s[e]) < (uint32_t)p.recent ? kNewest : key[e];
+    };
+    auto keys = [&](int tile) __attribute__((always_inline)) {
+        if (kOne) return;
+        load(tile);
+        sums(tile);
+        newer(tile);
+    };
+    if (kOne) newer(0);
+    // The newest tokens' keys lie above the range, and are counted apart the first time.  Of the keys in [low, high] the left-th largest is the
+    // threshold; where all of a bin's stay, what lies below it is one as well, of which none stays.
+    uint32_t left = (uint32_t)p.budget, above_range = 0;
+    for (bool first = true; first || low < high; first = false) {
+        const int shift = max(0, 32 - __builtin_clz((high - low) | 1u) - 11);  // (high - low) >> shift < 2048
+        const uint32_t width = high - low;
+        for (int t = 0; t < tiles; t++) {
+            keys(t);
+            if (width) {
+#pragma unroll
+                for (int e = 0; e < kPer; e++) {
+                    const uint32_t x = key[e] - low;
+                    if (x <= width) atomicAdd(&bins[x >> shift], 1u);
                 }
             }
-    }
-    low = all_of(low, [](uint32_t x, uint32_t y) { return min(x, y); }, room);
-    high = all_of(high, [](uint32_t x, uint32_t y) { return max(x, y); }, room);
-    at_top = all_of(at_top, [](uint32_t x, uint32_t y) { return x + y; }, room);
-    uint32_t left = (uint32_t)p.budget;  // of the keys in [low, high], the left-th largest is the threshold
-    if (left <= at_top) low = high = kNewest;
-    else left -= at_top;
-    while (low < high) {
-        const int shift = max(0, 32 - __builtin_clz(high - low) - 11);  // (high - low) >> shift < 2048
-        bins[tid] = bins[tid + kSelect] = 0;
-        __syncthreads();
-        for (int t = 0; t < tiles; t++) {
-            if (!kOne) keys(t);
+            if (first) {
 #pragma unroll
-            for (int e = 0; e < kPer; e++)
-                if (in(t, e) && key[e] >= low && key[e] <= high) atomicAdd(&bins[(key[e] - low) >> shift], 1u);
+                for (int e = 0; e < kPer; e++) above_range += (uint32_t)__popcll(__ballot(key[e] > high));
+            }
         }
+        if (first && above_range && (tid & 63) == 0) atomicAdd(&above_all, above_range);
         __syncthreads();
+        if (first) {
+            above_range = above_all;
+            if (left <= above_range) {
+                low = kNewest;
+                break;
+            }
+            left -= above_range;
+            if (low == high) break;
+        }
         // thread t has the bins 2047 - 2 t and 2046 - 2 t: those above it are those before it
         const uint32_t c0 = bins[kBins - 1 - 2 * tid], c1 = bins[kBins - 2 - 2 * tid];
+        bins[kBins - 1 - 2 * tid] = bins[kBins - 2 - 2 * tid] = 0;
         uint32_t all;
-        const uint32_t above = sum_before(c0 + c1, room, &all);
+        const uint32_t above = sum_before(c0 + c1, room[3], &all);
         if (above < left && left <= above + c0 + c1) {
             const bool second = left > above + c0;
+            const uint32_t rest = left - above - (second ? c0 : 0u);
             chosen[0] = (uint32_t)(kBins - 1 - 2 * tid) - (second ? 1u : 0u);
-            chosen[1] = left - above - (second ? c0 : 0u);
+            chosen[1] = rest == (second ? c1 : c0) ? 0u : rest;
         }
         __syncthreads();
         const uint32_t bin = chosen[0];
         left = chosen[1];
         high = min(high, low + ((bin + 1) << shift) - 1);  // (no further than the range: low + 2^32 does not come up)
         low += bin << shift;
+        if (left == 0) {
+            low--;
+            break;
+        }
     }
     // in slot order: keys above it stay, and the first `left` that equal it
     uint32_t equal = 0, freed = 0, moved = 0;
     int32_t* from = p.from + (size_t)head * p.most;
     int32_t* to = p.to + (size_t)head * p.most;
     for (int t = 0; t < tiles; t++) {
-        if (!kOne) keys(t);
+        keys(t);
         const int j0 = t * kTile + tid * kPer;
-        uint32_t mine = 0, all;
+        uint32_t keep = 0, all;  // bits of the slots that stay
+        if (left) {
+            uint32_t mine = 0;
 #pragma unroll
-        for (int e = 0; e < kPer; e++) mine += in(t, e) && key[e] == low;
-        uint32_t rank = equal + sum_before(mine, room, &all);
-        equal += all;
-        uint32_t keep = 0, count = 0;  // count: freed slots in the low half, rows that move in the high one (8192 each at most)
+            for (int e = 0; e < kPer; e++) mine += key[e] == low;
+            uint32_t rank = equal + sum_before(mine, room[4], &all);
+            equal += all;
 #pragma unroll
-        for (int e = 0; e < kPer; e++) {
-            const bool eq = key[e] == low, stays = in(t, e) && (key[e] > low || (eq && rank < left));
-            rank += in(t, e) && eq;
-            keep |= (stays ? 1u : 0u) << e;
-            count += in(t, e) && !stays && j0 + e < p.budget ? 1u : 0u;
-            count += stays && j0 + e >= p.budget ? 1u << 16 : 0u;
-        }
-        const uint32_t before = sum_before(count, room, &all);
-        uint32_t at_hole = freed + (before & 0xffffu), at_mover = moved + (before >> 16);
-        freed += all & 0xffffu;
-        moved += all >> 16;
-#pragma unroll
-        for (int e = 0; e < kPer; e++) {
-            const bool stays = keep >> e & 1u, below = j0 + e < p.budget;
-            if (in(t, e) && !stays && below) to[at_hole++] = j0 + e;
-            if (stays && !below) from[at_mover++] = j0 + e;
-            if (stays && below) {
-                if (copy_w) w_out[j0 + e] = w[e];
-                if (copy_s) s_out[j0 + e] = s[e];
+            for (int e = 0; e < kPer; e++) {
+                keep |= (key[e] == low && rank < left ? 1u : 0u) << e;
+                rank += key[e] == low;
             }
         }
+#pragma unroll
+        for (int e = 0; e < kPer; e++) keep |= (key[e] > low ? 1u : 0u) << e;
+        const uint32_t below = (1u << min(max(p.budget - j0, 0), kPer)) - 1u, which = keep ^ below;  // (the budget is less than the length)
+        const uint32_t before = sum_before((uint32_t)__popc(which & below) + ((uint32_t)__popc(which & ~below) << 16), room[5], &all);  // 8192 each at most
+        uint32_t at_hole = before & 0xffffu, at_mover = kTile + (before >> 16);
+#pragma unroll
+        for (int e = 0; e < kPer; e++)
+            if (which >> e & 1u) listed[below >> e & 1u ? at_hole++ : at_mover++] = (uint16_t)(tid * kPer + e);
+        // (freed slots too: a row that moves comes over them later)
+        auto put = [&](auto* to, const auto (&x)[kPer]) __attribute__((always_inline)) {
+            if (j0 + kPer <= p.budget) {
+#pragma unroll
+                for (int e = 0; e < kPer; e += 4) *(u32x4_any*)(to + j0 + e) = u32x4_any{bits(x[e]), bits(x[e + 1]), bits(x[e + 2]), bits(x[e + 3])};
+            } else {
+#pragma unroll
+                for (int e = 0; e < kPer; e++)
+                    if (j0 + e < p.budget) to[j0 + e] = x[e];
+            }
+        };
+        if (copy_w) put(w_out, w);
+        if (copy_s) put(s_out, s);
+        __syncthreads();
+        for (uint32_t i = tid; i < (all & 0xffffu); i += kSelect) to[freed + i] = t * kTile + listed[i];
+        for (uint32_t i = tid; i < all >> 16; i += kSelect) from[moved + i] = t * kTile + listed[kTile + i];
+        freed += all & 0xffffu;
+        moved += all >> 16;
     }
     if (tid == 0) {
         p.header[2 * head] = len;
@@ -221,28 +247,36 @@ __global__ __launch_bounds__(kSelect) void cache_select_kernel(CacheEvictParams 
     }
 }
 
-constexpr int kMoveRows = 32;  // a workgroup
-
-// Grid (kMoveRows moved rows, kv heads, batch).
+// Grid (p.move_rows moved rows, kv heads, batch).  A thread has two pieces of 16 bytes of K's rows and of V's, all four under way at once.
+constexpr int kMovePieces = 512;
 __global__ __launch_bounds__(256) void cache_move_kernel(CacheEvictParams p) {
     const int tid = threadIdx.x, b = blockIdx.z, head = b * p.n_kv + (int)blockIdx.y;
     const int len = p.header[2 * head], moves = p.header[2 * head + 1];
     if (p.new_lens && blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) p.new_lens[b] = min(len, p.budget);
-    const int first = (int)blockIdx.x * kMoveRows, rows = min(kMoveRows, moves - first);
+    const int first = (int)blockIdx.x * p.move_rows, rows = min(p.move_rows, moves - first);
     if (rows <= 0) return;
     const int32_t* from = p.from + (size_t)head * p.most + first;
     const int32_t* to = p.to + (size_t)head * p.most + first;
     const size_t slab = (size_t)head * p.max_seq;
-    const int units = p.row_bytes / 16;
-    uint4* k = (uint4*)(p.k + slab * p.row_bytes);
-    uint4* v = (uint4*)(p.v + slab * p.row_bytes);
-    for (int i = tid; i < rows * units; i += 256) {
-        const int r = i / units, u = i - r * units;
-        const size_t src = (size_t)from[r] * units + u, dst = (size_t)to[r] * units + u;
-        const uint4 a = k[src], c = v[src];
-        k[dst] = a;
-        v[dst] = c;
+    const int shift = __builtin_ctz(p.row_bytes / 16);  // a row is a power of two of pieces
+    u32x4_t* k = (u32x4_t*)(p.k + slab * p.row_bytes);
+    u32x4_t* v = (u32x4_t*)(p.v + slab * p.row_bytes);
+    u32x4_t a[2], c[2];
+    size_t dst[2];
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        const int r = min((tid + 256 * x) >> shift, rows - 1), u = (tid + 256 * x) & ((1 << shift) - 1);
+        const size_t src = ((size_t)from[r] << shift) + u;
+        dst[x] = ((size_t)to[r] << shift) + u;
+        a[x] = k[src];
+        c[x] = v[src];
     }
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+        if ((tid + 256 * x) >> shift < rows) {
+            k[dst[x]] = a[x];
+            v[dst[x]] = c[x];
+        }
     if (p.k_pairs) {
         for (int i = tid; i < rows * p.groups; i += 256) {
             const int g = i / rows, r = i - g * rows;
@@ -252,11 +286,11 @@ __global__ __launch_bounds__(256) void cache_move_kernel(CacheEvictParams p) {
             p.v_pairs[plane + to[r]] = c;
         }
     }
-    if (tid < rows) {
-        const float w = p.weights_in[slab + from[tid]];
-        const int32_t s = p.slots_in[slab + from[tid]];
-        p.weights_out[slab + to[tid]] = w;
-        p.slots_out[slab + to[tid]] = s;
+    for (int i = tid; i < rows; i += 256) {
+        const float w = p.weights_in[slab + from[i]];
+        const int32_t s = p.slots_in[slab + from[i]];
+        p.weights_out[slab + to[i]] = w;
+        p.slots_out[slab + to[i]] = s;
     }
 }
 
@@ -302,11 +336,12 @@ int evict_common(void* stream, CacheEvictParams& p, int head_dim, bool q4, void*
     p.most = a.most;
     p.row_bytes = q4 ? head_dim / 2 : 2 * head_dim;
     p.groups = q4 ? head_dim / 64 : 0;
+    p.move_rows = kMovePieces * 16 / p.row_bytes;
     const hipStream_t s = (hipStream_t)stream;
     if (p.max_seq <= kTile) hipLaunchKernelGGL(cache_select_kernel<true>, dim3(p.n_kv, p.batch), dim3(kSelect), 0, s, p);
     else hipLaunchKernelGGL(cache_select_kernel<false>, dim3(p.n_kv, p.batch), dim3(kSelect), 0, s, p);
     HIP_TRY(hipGetLastError(), "cache_select launch");
-    hipLaunchKernelGGL(cache_move_kernel, dim3(std::max(1, (a.most + kMoveRows - 1) / kMoveRows), p.n_kv, p.batch), dim3(256), 0, s, p);
+    hipLaunchKernelGGL(cache_move_kernel, dim3(std::max(1, (a.most + p.move_rows - 1) / p.move_rows), p.n_kv, p.batch), dim3(256), 0, s, p);
     HIP_TRY(hipGetLastError(), "cache_move launch");
     return RT_OK;
 }

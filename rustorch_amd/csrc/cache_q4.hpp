@@ -21,6 +21,41 @@
 
 namespace rt {
 
+// Over the lanes of a wave within registers, where a shuffle goes through LDS and takes ten times as long: step i brings a lane the value
+// from 1, 2, 4, 8 lanes down its row of 16, from the row before it (second and fourth row), from the lower half (upper half); `none`
+// where there is none.
+template <int kStep>
+__device__ __forceinline__ int lanes_step(int none, int x) {
+    constexpr int kCtrl[6] = {0x111, 0x112, 0x114, 0x118, 0x142, 0x143}, kRows[6] = {0xf, 0xf, 0xf, 0xf, 0xa, 0xc};
+    return __builtin_amdgcn_update_dpp(none, x, kCtrl[kStep], kRows[kStep], 0xf, false);
+}
+// the sum up to and with this lane
+__device__ __forceinline__ int lane_sums(int x) {
+    x += lanes_step<0>(0, x);
+    x += lanes_step<1>(0, x);
+    x += lanes_step<2>(0, x);
+    x += lanes_step<3>(0, x);
+    x += lanes_step<4>(0, x);
+    x += lanes_step<5>(0, x);
+    return x;
+}
+// f over the lanes up to and with this one of its row of 16 (kSteps 4) or of the wave (6), in the last lane of each; f(x, x) = x
+template <int kSteps, typename T, typename F>
+__device__ __forceinline__ T lanes_fold(T x, F f) {
+    x = f(x, (T)lanes_step<0>((int)x, (int)x));
+    x = f(x, (T)lanes_step<1>((int)x, (int)x));
+    x = f(x, (T)lanes_step<2>((int)x, (int)x));
+    x = f(x, (T)lanes_step<3>((int)x, (int)x));
+    if constexpr (kSteps == 6) {
+        x = f(x, (T)lanes_step<4>((int)x, (int)x));
+        x = f(x, (T)lanes_step<5>((int)x, (int)x));
+    }
+    return x;
+}
+__device__ __forceinline__ int lane_max(int x) {
+    return __builtin_amdgcn_readlane(lanes_fold<6>(x, [](int a, int b) __attribute__((always_inline)) { return max(a, b); }), 63);
+}
+
 inline bool cache_q4_dim(int dim) { return dim == 64 || dim == 128 || dim == 256; }
 
 // New rows into a cache, bf16 or 4-bit (cache_append.hip).
@@ -101,6 +136,7 @@ struct CacheEvictParams {
     int batch, n_kv, max_seq, budget, recent;
     int row_bytes;    // of K and of V
     int groups;       // pairs a row has
+    int move_rows;    // rows that a workgroup moves
     int most;         // min(budget, max_seq - budget): rows of a head that can move
 };
 

@@ -57,28 +57,6 @@ __device__ __forceinline__ int quotient(int x, int d) {
     }
     return __builtin_amdgcn_readfirstlane(q);
 }
-// Sums over the lanes up to this one, and the largest of all, within registers.
-template <int kCtrl, int kRows>
-__device__ __forceinline__ int moved(int x) { return __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xf, false); }
-__device__ __forceinline__ int lane_sums(int x) {
-    x += moved<0x111, 0xf>(x);  // from 1, 2, 4, 8 lanes down a row of 16
-    x += moved<0x112, 0xf>(x);
-    x += moved<0x114, 0xf>(x);
-    x += moved<0x118, 0xf>(x);
-    x += moved<0x142, 0xa>(x);  // a row's last lane to the next row; the second row's to the upper half
-    x += moved<0x143, 0xc>(x);
-    return x;
-}
-__device__ __forceinline__ int lane_max(int x) {  // x >= 0
-    x = max(x, moved<0x111, 0xf>(x));
-    x = max(x, moved<0x112, 0xf>(x));
-    x = max(x, moved<0x114, 0xf>(x));
-    x = max(x, moved<0x118, 0xf>(x));
-    x = max(x, moved<0x142, 0xa>(x));
-    x = max(x, moved<0x143, 0xc>(x));
-    return __builtin_amdgcn_readlane(x, 63);
-}
-
 // The list that the workgroups share: of every segment `kStart` places and its steps.  The places stand for what a segment costs
 // besides its steps, so that a span of short sequences is no longer a walk than one of a long one.
 constexpr int kStart = 4;

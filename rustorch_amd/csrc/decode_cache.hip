@@ -6,10 +6,15 @@
 // both products transposed: scores^T = K q^T leaves a lane with the scores of ONE query row for eight keys, which is the operand
 // that out^T = V^T P^T takes, so that nothing of a step crosses lanes but the running maximum.
 //
-// 4-bit rows enter the products as codes: 16 + c is a bf16 whose mantissa the code's bits are (0x4180 | c << 3), and what follows
-// from x = z + s (c - 8) is done on the sums, 64 dims at a time:
-//   score = sum over groups of s (sum q (16 + c) - 24 sum q) + z sum q
-//   out_d = sum over keys of (p s) (16 + c_d) - 24 sum over keys of (p s) + sum over keys of p z
+// 4-bit rows enter the products as the codes themselves: a byte below a byte of zeros is a bf16 of that many times 2^-133, subnormal or of
+// the first binade (the matrix cores take both as they are, products and sums exact as ever), so that a mask, and for every second
+// byte a shift, is all that a pair of codes costs; the high half of a byte stays where it is and counts 16-fold.  The other operand
+// makes up for it: q scaled by the power of two that brings its row's largest value to 2^120 (and by 2^-4 where codes count
+// 16-fold), the weights of V's keys 2^60 times theirs.  What follows from x = z + s (c - 8) is done on the sums, 64 dims at a time:
+//   score = sum over groups of s (sum q c - 8 sum q) + z sum q
+//   out_d = sum over keys of (p s) c_d - 8 sum over keys of (p s) + sum over keys of p z
+// (With codes as the mantissa of 16 + c a pair of codes took a shift and an and-or, 144 of a step's 255 vector instructions at dim 128
+// for 88 of 180 now.)  V's scales may be 2^-60 to 2^58: beyond, p s 2^60 is no bf16, below, its products lose bits.
 // The weights p s are two bf16 terms (16 bits), as are those of a bf16 cache: with one the output's error is half as large again
 // as its own rounding's.
 //
@@ -35,6 +40,7 @@ constexpr int kMaxPieces = 256;  // partials of a segment
 constexpr float kNoMax = -1.0e30f;
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // 16 bytes from any word
 typedef float f32x2_any __attribute__((ext_vector_type(2), aligned(4)));
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
@@ -306,17 +312,18 @@ __device__ __forceinline__ void ring_v(Keys<D, true, C>& t, const unsigned char*
     }
 }
 
-// The codes at bits 4 nib of every second byte as two bf16 numbers 16 + c.  The constants stand in registers: one and-or takes no two
-// literals, and the compiler, which sees through constants, makes two instructions of it.
+// The codes at bits 4 nib of every second byte as two bf16 numbers, c or 16 c times 2^kCodeExp.  The masks stand in registers: as literals
+// they would be a word more of every instruction.
+constexpr int kCodeExp = -133, kWeightExp = 60;  // (weights of 4-bit rows: times 2^kWeightExp)
 struct Codes {
-    uint32_t mask, sixteen;
+    uint32_t low, high;
     __device__ __forceinline__ Codes() {
-        asm volatile("s_mov_b32 %0, 0x780078" : "=s"(mask));
-        asm volatile("v_mov_b32 %0, 0x41804180" : "=v"(sixteen));
+        asm volatile("s_mov_b32 %0, 0xf000f" : "=s"(low));
+        asm volatile("s_mov_b32 %0, 0xf000f0" : "=s"(high));
     }
     template <int kNib>
     __device__ __forceinline__ uint32_t of(uint32_t w) const {
-        return ((kNib == 0 ? w << 3 : w >> (4 * kNib - 3)) & mask) | sixteen;
+        return (kNib >= 2 ? w >> 8 : w) & (kNib & 1 ? high : low);
     }
 };
 
@@ -360,7 +367,7 @@ __device__ __forceinline__ float quad_sum(float x) {
 }
 
 // The hi and lo terms of two weights: hi by truncation, what it leaves by truncation too (16 bits in all).  Returns the sum of the terms:
-// what is taken off for the codes' offsets has to be what went in, or the truncation's bias comes back 24 times.
+// what is taken off for the codes' offsets has to be what went in, or the truncation's bias comes back 8 times.
 __device__ __forceinline__ float two_terms(float a, float b, uint32_t& hi, uint32_t& lo) {
     const float ha = __uint_as_float(__float_as_uint(a) & 0xffff0000u), hb = __uint_as_float(__float_as_uint(b) & 0xffff0000u);
     hi = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
@@ -395,7 +402,7 @@ struct State {
 // behind the last use of K, v_due ahead of V's first.
 template <int D, bool Q4, int C, bool kCut, bool kWeigh, typename KDone, typename VDue>
 __device__ __forceinline__ void step(State<D, Q4>& st, const Keys<D, Q4, C>& x, KDone k_done, VDue v_due, const Codes& codes, const u32x4_t (&q)[D / 32], const float (&q_sum)[Q4 ? D / 64 : 1],
-                                     int cls, int first_key, int seen, float scale_log2e, float* scores) {
+                                     int cls, int first_key, int seen, float scale_log2e, float unscale, float* scores) {
     constexpr int kG = Keys<D, Q4, C>::kG, kO = D / 16, kE = 8 / C;
     float y[kE];
     // of both sixteens' scores, a column's
@@ -409,15 +416,16 @@ __device__ __forceinline__ void step(State<D, Q4>& st, const Keys<D, Q4, C>& x, 
         } else {
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                const float a0 = cls & 1 ? a[0][2 + e] : a[0][e], a1 = cls & 1 ? a[1][2 + e] : a[1][e];
-                to[e] = cls & 2 ? a1 : a0;
+                // (of both sixteens first: two of one register group the compiler takes for an index into it, four selections)
+                const float a0 = cls & 2 ? a[1][e] : a[0][e], a2 = cls & 2 ? a[1][2 + e] : a[0][2 + e];
+                to[e] = cls & 1 ? a2 : a0;
             }
         }
     };
     if constexpr (Q4) {
 #pragma unroll
         for (int g = 0; g < kG; g++) {
-            const float c0 = -24.0f * q_sum[g];
+            const float c0 = -8.0f * q_sum[g];
             f32x4_t a[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -463,16 +471,17 @@ __device__ __forceinline__ void step(State<D, Q4>& st, const Keys<D, Q4, C>& x, 
         if (hid[e]) y[e] = neg_inf();
     }
     if constexpr (kWeigh) {
+        auto full = [&](float x) __attribute__((always_inline)) { return Q4 ? x * unscale : x; };
         if (scores) {
             if constexpr (kCut) {
 #pragma unroll
                 for (int e = 0; e < kE; e++)
-                    if (!hid[e]) scores[place(e)] = y[e];
+                    if (!hid[e]) scores[place(e)] = full(y[e]);
             } else if constexpr (C == 4) {
-                *(f32x2_any*)(scores + place(0)) = f32x2_any{y[0], y[1]};
+                *(f32x2_any*)(scores + place(0)) = f32x2_any{full(y[0]), full(y[1])};
             } else {
 #pragma unroll
-                for (int e = 0; e < kE; e += 4) *(f32x4_any*)(scores + place(e)) = f32x4_any{y[e], y[e + 1], y[e + 2], y[e + 3]};
+                for (int e = 0; e < kE; e += 4) *(f32x4_any*)(scores + place(e)) = f32x4_any{full(y[e]), full(y[e + 1]), full(y[e + 2]), full(y[e + 3])};
             }
         }
     }
@@ -497,7 +506,7 @@ __device__ __forceinline__ void step(State<D, Q4>& st, const Keys<D, Q4, C>& x, 
     float w[kE];
 #pragma unroll
     for (int e = 0; e < kE; e++) {
-        w[e] = __builtin_amdgcn_exp2f((y[e] - st.m) * scale_log2e);
+        w[e] = __builtin_amdgcn_exp2f(fmaf(y[e] - st.m, scale_log2e, Q4 ? (float)kWeightExp : 0.0f));
         st.l += w[e];
     }
     // pairs of weights as the operand's words, zeros in the other columns' places
@@ -613,6 +622,7 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4, C>())) void cache_att
         // q as the operand that the keys' words pair with
         u32x4_t q[D / 32];
         float q_sum[kG] = {};
+        int q_exp = 0;  // scores of 4-bit rows are 2^q_exp times their own
         u32x4_t nat[D / 32];
 #pragma unroll
         for (int c = 0; c < D / 32; c++) {
@@ -643,6 +653,14 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4, C>())) void cache_att
 #pragma unroll
             for (int c = 0; c < D / 32; c++) q[c] = nat[c];
         } else {
+            // the row's largest exponent, of 2^-60 at least (a score of 2^-133 times that much is as good as 0)
+            u16x2_t most = {0, 0};
+#pragma unroll
+            for (int c = 0; c < D / 32; c++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, nat[c][i] & 0x7fff7fffu));
+            const int exponent = max((int)quad_max((float)(max(most[0], most[1]) >> 7)), 67) - 127, up = 120 - exponent;
+            q_exp = up + kCodeExp;
 #pragma unroll
             for (int g = 0; g < kG; g++) {
                 float sum = 0.0f;
@@ -650,17 +668,18 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4, C>())) void cache_att
                 for (int c = 2 * g; c < 2 * g + 2; c++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) sum += bf16_lo(nat[c][i]) + bf16_hi(nat[c][i]);
-                q_sum[g] = quad_sum(sum);
+                q_sum[g] = __builtin_amdgcn_ldexpf(quad_sum(sum), q_exp);
 #pragma unroll
-                for (int par = 0; par < 2; par++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        // dim 64: word (u, c) pairs i's of one chunk; above: chunks 2 g and 2 g + 1 at one i
-                        const uint32_t a = D == 64 ? nat[i & 1][i & 2] : nat[2 * g][i], o = D == 64 ? nat[i & 1][(i & 2) + 1] : nat[2 * g + 1][i];
-                        q[2 * g + par][i] = __builtin_amdgcn_perm(o, a, par ? 0x07060302u : 0x05040100u);
-                    }
+                for (int i = 0; i < 4; i++) {
+                    // dim 64: word (u, c) pairs i's of one chunk; above: chunks 2 g and 2 g + 1 at one i
+                    const uint32_t a = D == 64 ? nat[i & 1][i & 2] : nat[2 * g][i], o = D == 64 ? nat[i & 1][(i & 2) + 1] : nat[2 * g + 1][i];
+                    auto scaled = [&](float x, int by) __attribute__((always_inline)) { return __float_as_uint(__builtin_amdgcn_ldexpf(x, by)); };
+                    q[2 * g][i] = __builtin_amdgcn_perm(scaled(bf16_lo(o), up), scaled(bf16_lo(a), up), 0x07060302u);
+                    q[2 * g + 1][i] = __builtin_amdgcn_perm(scaled(bf16_hi(o), up - 4), scaled(bf16_hi(a), up - 4), 0x07060302u);
+                }
             }
         }
+        const float scale_log2e = Q4 ? __builtin_amdgcn_ldexpf(p.scale_log2e, -q_exp) : p.scale_log2e, unscale = __builtin_amdgcn_ldexpf(1.0f, -q_exp);
         const int all_see = len - p.seq_new + 1;  // keys that every row sees
         float* const scores = kWeigh && there ? p.scores + ((size_t)b * p.heads + head) * (size_t)p.max_seq + 4 * quad : nullptr;
 
@@ -681,7 +700,7 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4, C>())) void cache_att
                 else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 const unsigned char* const rows = ring_at + stage * Ring<D>::kStage;
                 ring_k<D, C>(x, rows, n, cls, quad);
-                step<D, Q4, C, kCut, kWeigh>(st, x, [] {}, [&]() __attribute__((always_inline)) { ring_v<D, C>(x, rows, n, cls, quad); }, codes, q, q_sum, cls, key0 + 4 * quad, seen, p.scale_log2e, to);
+                step<D, Q4, C, kCut, kWeigh>(st, x, [] {}, [&]() __attribute__((always_inline)) { ring_v<D, C>(x, rows, n, cls, quad); }, codes, q, q_sum, cls, key0 + 4 * quad, seen, scale_log2e, unscale, to);
                 const int next = t + Ring<D>::kStages * kWaves;
                 if (next < t1) {
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read before it is written again)
@@ -691,7 +710,7 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4, C>())) void cache_att
             } else {
                 const int next = t + kWaves;
                 step<D, Q4, C, kCut, kWeigh>(st, x, [&]() __attribute__((always_inline)) { if (next < t1) load_k<D, C>(x, k, next * kStep, len, n, quad); }, [] {}, codes, q, q_sum, cls, key0 + 4 * quad, seen,
-                                             p.scale_log2e, to);
+                                             scale_log2e, unscale, to);
                 if (next < t1) load_v<D, C>(x, v, next * kStep, len, n, quad);
             }
             t += kWaves;
@@ -703,16 +722,20 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4, C>())) void cache_att
         int ft = threadIdx.x;
         asm volatile("" : "+v"(ft));
         const int tid = ft, lane = ft & 63, n = ft & 15, quad = lane >> 4;
+        if (Q4 && st.m != kNoMax) st.m = __builtin_amdgcn_ldexpf(st.m, -q_exp);
+        if (Q4) st.l = __builtin_amdgcn_ldexpf(st.l, -kWeightExp);
         const float m = columns_max<C>(st.m), f = __builtin_amdgcn_exp2f((st.m - m) * p.scale_log2e);
         const float l = columns_sum<C>(quad_sum(st.l) * f);
         if constexpr (Q4) {
 #pragma unroll
             for (int g = 0; g < kG; g++) {
-                const float off = quad_sum(st.pz[g]) - 24.0f * quad_sum(st.ps[g]);
+                const float off = __builtin_amdgcn_ldexpf(quad_sum(st.pz[g]) - 8.0f * quad_sum(st.ps[g]), -kWeightExp);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int byte = D == 64 ? i / 2 : (g & 1) + 2 * (i / 2);
-                    st.o[8 * (D == 64 ? 0 : g / 2) + 2 * byte + i % 2] += off;
+                    f32x4_t& o = st.o[8 * (D == 64 ? 0 : g / 2) + 2 * byte + i % 2];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[e] = __builtin_amdgcn_ldexpf(o[e], -kCodeExp - kWeightExp - 4 * (i % 2)) + off;
                 }
             }
         }

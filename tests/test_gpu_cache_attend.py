@@ -234,3 +234,79 @@ def test_rows_past_32_bits():
     want = bf16_values(back.download(np.uint16))
     got = bf16_values(out.download(np.uint16)).reshape(2, d)
     assert np.abs(want).max() > 1 and (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -12).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("heads", [(8, 2), (34, 2)])
+@pytest.mark.parametrize("q_by,k_by,v_by", [(40, -40, 0), (-40, 40, 0), (-70, 70, 0), (90, -90, 0), (0, 0, 50), (0, 0, -50), (-30, 30, 40)])
+def test_powers_of_two_in_q_k_and_v_leave_the_bits(q_by, k_by, v_by, heads, d):
+    """q and K scaled against each other, V by itself: every scale and middle is so many times as large exactly, and so is the output.  (The products of codes
+    and the other operand are scaled into a range of their own; it has to follow the values'.)"""
+    lens = [333, 70]
+    base, c = Case(25, lens, *heads, d, 340), Case(25, lens, *heads, d, 340)
+    for name, by in (("q", q_by), ("k", k_by), ("v", v_by)):
+        setattr(c, name, bf16_bits(bf16_values(getattr(base, name)) * np.float32(2.0 ** by)))
+    a, b = base.q4(), c.q4()
+    assert np.array_equal(a[0], b[0]) and np.array_equal(a[2], b[2])
+    out, sums, _ = weigh(base, a)
+    got, got_sums, _ = weigh(c, b)
+    assert np.array_equal(got, out * np.float32(2.0 ** v_by)) and np.array_equal(got_sums, sums)
+    assert np.array_equal(attend_q4(c, b), got)
+
+
+def test_q_of_zeros_and_of_the_smallest_values():
+    """All keys weigh alike where q is zero, and as good as alike where its values are subnormal numbers."""
+    c = Case(26, [100], 4, 2, 128, 100)
+    caches = c.q4()
+    for bits in (0, 0x8000, 0x0001, 0x8055):
+        c.q = np.full_like(c.q, bits)
+        want = expect_q4(bf16_values(c.q), *caches, c.lens)
+        want.check(attend_q4(c, caches))
+        out, sums, start = weigh(c, caches, "none")
+        want.check(out)
+        want.check_weights(sums, start, c.lens)
+
+
+@pytest.mark.parametrize("kind", ["q4", "weights q4", "weights bf16"])
+def test_replays_over_long_caches(kind):
+    """A segment in many workgroups' pieces, joined by the last of them: recorded once, replayed between eager calls on the same workspace and
+    on another, over lengths that change in between."""
+    from test_gpu_decode_graph import NODE_TYPE_MEMSET, Hip
+
+    ra.init(0)
+    hip, stream, d, n = Hip(), ra.Stream(), 128, 9000
+    b, hq, hkv = 2, 8, 2
+    c = Case(27, [n, n], hq, hkv, d, n)
+    q = ra.HipStorage.from_numpy(c.q)
+    caches = [ra.HipStorage.from_numpy(x) for x in (c.bf16() if kind == "weights bf16" else c.q4())]
+    lens = ra.HipStorage.from_numpy(np.array([n, 17], np.int32))
+    rows = caches if kind == "weights bf16" else [ra.Q4Rows(*caches[:2]), ra.Q4Rows(*caches[2:])]
+    size = K.gqa_decode_q4_workspace_bytes(b, 1, hq, hkv, d, n) if kind == "q4" else K.gqa_decode_weights_workspace_bytes(b, hq, hkv, d, n)
+    spaces = [ra.HipStorage.from_numpy(np.full(size // 4, np.nan, np.float32)) for _ in range(2)]
+    results = [(ra.HipStorage(b * hq * d * 2), ra.HipStorage(b * hkv * n * 4)) for _ in range(2)]
+
+    def call(which, space):
+        out, sums = results[which]
+        if kind == "q4":
+            K.gqa_decode_q4(stream, q, *rows, out, lens, b, 1, hq, hkv, d, n, spaces[space], size)
+        else:
+            (K.gqa_decode_weights_q4 if kind == "weights q4" else K.gqa_decode_weights_bf16)(stream, q, *rows, out, None, sums, lens, b, hq, hkv, d, n, spaces[space], size)
+
+    def seen(which, now):
+        stream.synchronize()
+        sums = results[which][1].download(np.float32).reshape(b, hkv, n)
+        return results[which][0].download(np.uint16), [] if kind == "q4" else [sums[i, :, :x] for i, x in enumerate(now)]
+
+    graph, exe, types = hip.capture(stream, lambda: call(0, 0))
+    assert NODE_TYPE_MEMSET not in types
+    for now in ([n, 17], [n, n], [4097, 8191], [0, n], [n, n]):
+        lens.upload(np.array(now, np.int32))
+        for space in (0, 1, 0):
+            call(1, space)
+            want = seen(1, now)
+            for _ in range(2):
+                hip.launch(exe, stream)
+                got = seen(0, now)
+                assert np.array_equal(got[0], want[0]), now
+                assert all(np.array_equal(x, y) for x, y in zip(got[1], want[1])), now
+    hip.destroy(graph, exe)

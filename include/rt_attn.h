@@ -454,7 +454,8 @@ size_t rt_gqa_decode_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_k
  * A row's number there is not its position any more: new rows are appended behind the last (`rows` below), keys having their
  * position in them by the rotation.  Rows behind a sequence's last are never written but by an append.
  *
- * All are asynchronous on `stream`, allocate nothing and may be recorded into a HIP graph.  What a call needs besides its
+ * All are asynchronous on `stream`, allocate nothing and may be recorded into a HIP graph.  batch, n_heads, n_kv and seq_new up to
+ * 65535 each; max_seq up to 2^29 where rows are attended to or taken out (RT_ERR_UNSUPPORTED beyond).  What a call needs besides its
  * tensors is the caller's `workspace` (device memory, 16-byte aligned), which it works in alone and keeps nothing in: calls that
  * may overlap (other streams, graphs replayed side by side) have workspaces of their own. */
 
@@ -500,8 +501,10 @@ int rt_kv_cache_read_q4(void *stream, const void *codes, const uint32_t *pairs, 
 /* rt_gqa_decode_chunk_bf16 over a 4-bit cache: q/out bf16 [batch, seq_new, n_heads, head_dim], seq_new = 1 for a decode step;
  * kv_lens device int32[batch] = keys in the cache including the new ones (counts above max_seq are max_seq, below 0 are 0), or
  * NULL: every sequence has `kv_len`.  Position s of sequence b sees keys [0, kv_lens[b] - seq_new + s]; one that sees none gives
- * +0.0.  kv head = h / (n_heads / n_kv), any number of heads a group.  f32 accumulation and softmax, weights of 16 bits, one rounding to
- * bf16 at the end.  The last bits of a sequence may depend on what else is in the batch (how its keys are cut into spans); the
+ * +0.0.  kv head = h / (n_heads / n_kv), any number of heads a group; seq_new * n_heads * head_dim < 2^31.  f32 accumulation and
+ * softmax, weights of 16 bits, one rounding to bf16 at the end.  V's values may be as large as
+ * 2^60 over the number of keys (a sum beyond is NaN) and are told apart down to 2^-50; q and K may be anything.  64 dims that read as NaN make all scores of their key NaN, or in V those dims of the
+ * positions that see them.  The last bits of a sequence may depend on what else is in the batch (how its keys are cut into spans); the
  * same call gives the same bits every time.  workspace: rt_gqa_decode_q4_workspace_bytes(...) bytes (RT_ERR_WORKSPACE_TOO_SMALL). */
 size_t rt_gqa_decode_q4_workspace_bytes(int32_t batch, int32_t seq_new, int32_t n_heads, int32_t n_kv,
                                         int32_t head_dim, int32_t max_seq);
@@ -514,7 +517,8 @@ int rt_gqa_decode_q4(void *stream, const void *q, const void *k_codes, const uin
  * rt_gqa_decode_batched_bf16) that also sums what each key draws:
  *   weights_out[b, kvh, j] = weights_in[b, kvh, j] + sum over the query heads h of kvh of softmax weight (h, j)     for j < kv_lens[b]
  * f32 [batch, n_kv, max_seq]; weights_in == NULL counts as zeros, and is weights_out itself or shares no memory with it; entries
- * j >= kv_lens[b] of weights_out stay as they are.  Over a bf16 cache [batch, n_kv, max_seq, head_dim] or a 4-bit one.  workspace:
+ * j >= kv_lens[b] of weights_out stay as they are.  Over a bf16 cache [batch, n_kv, max_seq, head_dim] or a 4-bit one; a dim in which a
+ * visible V row of a bf16 cache is infinite or NaN comes out NaN.  workspace:
  * rt_gqa_decode_weights_workspace_bytes(...) bytes (it holds the scores: batch * n_heads * max_seq floats, among others). */
 size_t rt_gqa_decode_weights_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim,
                                              int32_t max_seq);

@@ -312,7 +312,7 @@ int evict_common(void* stream, CacheEvictParams& p, int head_dim, bool q4, void*
     if (p.batch < 0 || p.n_kv < 0 || head_dim < 0 || p.max_seq < 0) return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "negative dimension");
     if (head_dim == 0) return fail(err, RT_ERR_ZERO_DIM, -1, 0, 0, "head_dim must be > 0");
     if (!cache_q4_dim(head_dim)) return fail(err, RT_ERR_UNSUPPORTED, -1, 256, (uint64_t)head_dim, "these kernels cover head_dim 64, 128 and 256");
-    if (p.batch > 65535 || p.n_kv > 65535 || (int64_t)p.batch * p.n_kv > 0x3fffffff) return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "shape too large for the launch grid");
+    if (p.batch > 65535 || p.n_kv > 65535 || (int64_t)p.batch * p.n_kv > 0x3fffffff || p.max_seq > (1 << 29)) return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "shape too large for the launch grid");
     if (p.budget < 0 || p.recent < 0 || p.recent > p.budget)
         return fail(err, RT_ERR_UNSUPPORTED, -1, (uint64_t)(int64_t)p.budget, (uint64_t)(int64_t)p.recent, "budget must be >= recent >= 0");
     if (p.batch == 0 || p.n_kv == 0) return RT_OK;

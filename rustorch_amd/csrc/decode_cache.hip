@@ -10,11 +10,12 @@
 // the first binade (the matrix cores take both as they are, products and sums exact as ever), so that a mask, and for every second
 // byte a shift, is all that a pair of codes costs; the high half of a byte stays where it is and counts 16-fold.  The other operand
 // makes up for it: q scaled by the power of two that brings its row's largest value to 2^120 (and by 2^-4 where codes count
-// 16-fold), the weights of V's keys 2^60 times theirs.  What follows from x = z + s (c - 8) is done on the sums, 64 dims at a time:
+// 16-fold), V's scales, which the weights take along, by 2^60.  What follows from x = z + s (c - 8) is done on the sums, 64 dims at a time:
 //   score = sum over groups of s (sum q c - 8 sum q) + z sum q
 //   out_d = sum over keys of (p s) c_d - 8 sum over keys of (p s) + sum over keys of p z
 // (With codes as the mantissa of 16 + c a pair of codes took a shift and an and-or, 144 of a step's 255 vector instructions at dim 128
-// for 88 of 180 now.)  V's scales may be 2^-60 to 2^58: beyond, p s 2^60 is no bf16, below, its products lose bits.
+// for 88 of 180 now.)  So V's scales have a range: below 2^-50 the
+// products lose bits, and sum of p s 2^60 has to stay below 2^127, where p is 2^8 at most.
 // The weights p s are two bf16 terms (16 bits), as are those of a bf16 cache: with one the output's error is half as large again
 // as its own rounding's.
 //
@@ -314,7 +315,10 @@ __device__ __forceinline__ void ring_v(Keys<D, true, C>& t, const unsigned char*
 
 // The codes at bits 4 nib of every second byte as two bf16 numbers, c or 16 c times 2^kCodeExp.  The masks stand in registers: as literals
 // they would be a word more of every instruction.
-constexpr int kCodeExp = -133, kWeightExp = 60;  // (weights of 4-bit rows: times 2^kWeightExp)
+constexpr int kCodeExp = -133, kScaleExp = 60;
+// A pair's scale, for V, times 2^kScaleExp: by its exponent's bits, one instruction.  (0 becomes 2^-67, so that a code
+// counts 2^-127 of its offset there.)
+__device__ __forceinline__ float v_scale(uint32_t pair) { return __uint_as_float((pair << 16) + ((uint32_t)kScaleExp << 23)); }
 struct Codes {
     uint32_t low, high;
     __device__ __forceinline__ Codes() {
@@ -506,7 +510,7 @@ __device__ __forceinline__ void step(State<D, Q4>& st, const Keys<D, Q4, C>& x, 
     float w[kE];
 #pragma unroll
     for (int e = 0; e < kE; e++) {
-        w[e] = __builtin_amdgcn_exp2f(fmaf(y[e] - st.m, scale_log2e, Q4 ? (float)kWeightExp : 0.0f));
+        w[e] = __builtin_amdgcn_exp2f((y[e] - st.m) * scale_log2e);
         st.l += w[e];
     }
     // pairs of weights as the operand's words, zeros in the other columns' places
@@ -538,7 +542,7 @@ __device__ __forceinline__ void step(State<D, Q4>& st, const Keys<D, Q4, C>& x, 
             float s[kE];
 #pragma unroll
             for (int e = 0; e < kE; e++) {
-                s[e] = hid[e] ? 0.0f : w[e] * bf16_lo(x.vs[g][e]);  // (what a hidden row holds stays out, were it NaN)
+                s[e] = hid[e] ? 0.0f : w[e] * v_scale(x.vs[g][e]);  // (what a hidden row holds stays out, were it NaN)
                 if (kCut) st.pz[g] += hid[e] ? 0.0f : w[e] * bf16_hi(x.vs[g][e]);
                 else st.pz[g] = fmaf(w[e], bf16_hi(x.vs[g][e]), st.pz[g]);
             }
@@ -723,19 +727,18 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4, C>())) void cache_att
         asm volatile("" : "+v"(ft));
         const int tid = ft, lane = ft & 63, n = ft & 15, quad = lane >> 4;
         if (Q4 && st.m != kNoMax) st.m = __builtin_amdgcn_ldexpf(st.m, -q_exp);
-        if (Q4) st.l = __builtin_amdgcn_ldexpf(st.l, -kWeightExp);
         const float m = columns_max<C>(st.m), f = __builtin_amdgcn_exp2f((st.m - m) * p.scale_log2e);
         const float l = columns_sum<C>(quad_sum(st.l) * f);
         if constexpr (Q4) {
 #pragma unroll
             for (int g = 0; g < kG; g++) {
-                const float off = __builtin_amdgcn_ldexpf(quad_sum(st.pz[g]) - 8.0f * quad_sum(st.ps[g]), -kWeightExp);
+                const float off = quad_sum(st.pz[g]) - __builtin_amdgcn_ldexpf(quad_sum(st.ps[g]), 3 - kScaleExp);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int byte = D == 64 ? i / 2 : (g & 1) + 2 * (i / 2);
                     f32x4_t& o = st.o[8 * (D == 64 ? 0 : g / 2) + 2 * byte + i % 2];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[e] = __builtin_amdgcn_ldexpf(o[e], -kCodeExp - kWeightExp - 4 * (i % 2)) + off;
+                    for (int e = 0; e < 4; e++) o[e] = __builtin_amdgcn_ldexpf(o[e], -kCodeExp - kScaleExp - 4 * (i % 2)) + off;
                 }
             }
         }

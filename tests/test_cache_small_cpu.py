@@ -90,6 +90,8 @@ def test_attend_refusals():
     assert f(d=0)[0] == L.RT_ERR_ZERO_DIM
     assert f(d=96)[0] == f(b=-1)[0] == f(b=65536)[0] == f(s=65536)[0] == f(q=P + 2)[0] == L.RT_ERR_UNSUPPORTED
     assert f(b=60000, n=2 ** 31 - 1)[0] == L.RT_ERR_UNSUPPORTED  # more steps than an int counts
+    assert f(n=2 ** 29 + 1)[0] == f(b=1, s=65535, hq=512, hkv=1)[0] == L.RT_ERR_UNSUPPORTED
+    assert f(b=1, hkv=1, n=2 ** 29)[0] in OK
     rc, err = f(lens=None, kv_len=101)
     assert rc == L.RT_ERR_KV_OVERFLOW and (err.expected, err.got) == (100, 101)
     assert f(lens=None, kv_len=2, s=3)[0] == L.RT_ERR_KV_OVERFLOW
@@ -134,6 +136,7 @@ def test_evict_refusals(name):
     rc, err = f(recent=11)
     assert rc == L.RT_ERR_UNSUPPORTED and (err.expected, err.got) == (10, 11)
     assert f(budget=-1, recent=0)[0] == f(recent=-1)[0] == L.RT_ERR_UNSUPPORTED
+    assert f(n=2 ** 29 + 1)[0] == L.RT_ERR_UNSUPPORTED and f(n=2 ** 29, w_in=1 << 50, s_in=1 << 51, w_out=1 << 52, s_out=1 << 53, size=1 << 50)[0] in OK
     assert f(b=0)[0] == L.RT_OK
     for missing in ("k", "w_in", "s_in", "w_out", "s_out", "lens"):
         assert f(**{missing: None})[0] == L.RT_ERR_NULL_POINTER

@@ -254,6 +254,17 @@ def test_powers_of_two_in_q_k_and_v_leave_the_bits(q_by, k_by, v_by, heads, d):
     assert np.array_equal(attend_q4(c, b), got)
 
 
+@pytest.mark.parametrize("spread", [0.0, 1.0, 40.0])
+@pytest.mark.parametrize("by", [43, -50])
+def test_v_at_the_ends_of_its_range_over_many_keys(by, spread):
+    """8192 keys: values of up to 2^60 / 8192 (2^47: 4 x 4 times 2^43), and down to 2^-50."""
+    base, c = Case(28, [8192], 8, 2, 128, 8192, spread=spread), Case(28, [8192], 8, 2, 128, 8192, spread=spread)
+    v = np.clip(bf16_values(base.v), -16, 16)
+    base.v, c.v = bf16_bits(v), bf16_bits(v * np.float32(2.0 ** by))
+    out = attend_q4(base, base.q4())
+    assert np.isfinite(out).all() and np.array_equal(attend_q4(c, c.q4()), out * np.float32(2.0 ** by))
+
+
 def test_q_of_zeros_and_of_the_smallest_values():
     """All keys weigh alike where q is zero, and as good as alike where its values are subnormal numbers."""
     c = Case(26, [100], 4, 2, 128, 100)

@@ -104,8 +104,7 @@ struct CacheAttendParams {
     int rows;     // seq_new * group query rows of a kv head
     int n_tiles;  // of 16 of them
     int n_groups;  // workgroups launched
-    int span_min;  // one takes at least this many steps of 32 keys
-    int few_pieces;  // into about how many a segment is cut where that leaves them short
+    float span_root;  // one takes at least this many times the root of the longest sequence's steps of 32 keys
     float scale_log2e;
     float* part;    // partials: (n_groups + segments) slots of part_rows * (dim + 2) floats, the rows and behind them their (m, l)
     int part_rows;  // min(16, rows)

@@ -66,13 +66,20 @@ __device__ __forceinline__ int quotient(int x, int d) {
 }
 // The list that the workgroups share: of every segment `kStart` places and its steps.  The places stand for what a segment costs
 // besides its steps, so that a span of short sequences is no longer a walk than one of a long one.
-constexpr int kStart = 4;
+constexpr int kStart = 16;
 __device__ __forceinline__ int places_of(int len) { return len ? kStart + steps_of(len) : 0; }
 struct Span {
     int total, size;    // places of all; of a span
     int b, first, len;  // the sequence that holds the span's first place, the first place of that sequence, its length
     uint64_t empty;     // of the first 64 sequences, those without keys
 };
+// Places a span, of `total` and a longest sequence of `most` steps: what one of all workgroups gets, but no fewer than a join is worth --
+// a segment of few spans is a long walk, one of many a long join: their sum is least around the root of its steps (p.span_root) -- and
+// never more of them than kMaxPieces (the steps of a segment touch at most most / size + 2).
+__device__ __forceinline__ int span_size(const CacheAttendParams& p, int total, int most) {
+    const int root = __builtin_amdgcn_readfirstlane((int)(__builtin_amdgcn_sqrtf((float)most) * p.span_root + 0.5f * kWaves)) & -kWaves;
+    return max(max(kWaves, quotient(total + p.n_groups - 1, p.n_groups)), max(root, (most + kMaxPieces - 3) / (kMaxPieces - 2)));
+}
 // Lengths 64 at a time, the first of them once for both walks.
 __device__ __forceinline__ Span span_of(const CacheAttendParams& p, int group, int lane) {
     const int per = p.kv_heads * p.n_tiles;
@@ -83,7 +90,7 @@ __device__ __forceinline__ Span span_of(const CacheAttendParams& p, int group, i
         s.empty = len == 0;
         s.total = places_of(len) * per;
         const int most = steps_of(len);
-        s.size = max(max(p.span_min, quotient(s.total + p.n_groups - 1, p.n_groups)), max(min(quotient(most + p.few_pieces - 1, p.few_pieces), 64), (most + kMaxPieces - 3) / (kMaxPieces - 2)));
+        s.size = span_size(p, s.total, most);
         s.b = s.first = 0;
         s.len = len;
         return s;
@@ -99,8 +106,7 @@ __device__ __forceinline__ Span span_of(const CacheAttendParams& p, int group, i
     }
     most = steps_of(most);
     s.total = sum * per;
-    // (the steps of a segment touch at most steps / size + 2 spans)
-    s.size = max(max(p.span_min, quotient(s.total + p.n_groups - 1, p.n_groups)), max(min(quotient(most + p.few_pieces - 1, p.few_pieces), 64), (most + kMaxPieces - 3) / (kMaxPieces - 2)));
+    s.size = span_size(p, s.total, most);
     s.b = s.first = s.len = 0;
     const long long at = (long long)group * s.size;
     if (at >= s.total) return s;
@@ -382,7 +388,7 @@ __device__ __forceinline__ float two_terms(float a, float b, uint32_t& hi, uint3
 
 // Waves that an SIMD holds.
 template <int D, bool Q4, int C>
-constexpr int per_simd() { return D == 64 ? 4 : D == 128 ? (!Q4 ? 2 : C == 4 ? 4 : 3) : Q4 ? 2 : 1; }
+constexpr int per_simd() { return D == 64 ? 4 : D == 128 ? (!Q4 || C == 1 ? 2 : 3) : Q4 && C > 1 ? 2 : 1; }
 
 // What a lane has of its query row over the keys it has walked.
 template <int D, bool Q4>
@@ -993,8 +999,7 @@ int attend_common(void* stream, CacheAttendParams& p, int head_dim, bool q4, boo
     p.rows = (int)a.rows;
     p.n_tiles = (int)a.n_tiles;
     p.n_groups = groups;
-    p.span_min = kWaves;
-    p.few_pieces = a.rows <= 4 ? 32 : a.rows <= 8 ? 24 : 16;
+    p.span_root = a.rows <= 4 ? 0.66f : 1.0f;
     p.scale_log2e = (1.0f / sqrtf((float)head_dim)) * kLog2eHost;
     p.part = (float*)workspace;
     p.part_rows = a.part_rows;

@@ -104,6 +104,7 @@ struct CacheAttendParams {
     int rows;     // seq_new * group query rows of a kv head
     int n_tiles;  // of 16 of them
     int n_groups;  // workgroups launched
+    int n_long;  // of them at work where sequences are long
     float span_root;  // one takes at least this many times the root of the longest sequence's steps of 32 keys
     float scale_log2e;
     float* part;    // partials: (n_groups + segments) slots of part_rows * (dim + 2) floats, the rows and behind them their (m, l)

@@ -67,6 +67,7 @@ __device__ __forceinline__ int quotient(int x, int d) {
 // The list that the workgroups share: of every segment `kStart` places and its steps.  The places stand for what a segment costs
 // besides its steps, so that a span of short sequences is no longer a walk than one of a long one.
 constexpr int kStart = 16;
+constexpr int kLong = 64;  // steps a sequence, see per_cu
 __device__ __forceinline__ int places_of(int len) { return len ? kStart + steps_of(len) : 0; }
 struct Span {
     int total, size;    // places of all; of a span
@@ -77,8 +78,9 @@ struct Span {
 // a segment of few spans is a long walk, one of many a long join: their sum is least around the root of its steps (p.span_root) -- and
 // never more of them than kMaxPieces (the steps of a segment touch at most most / size + 2).
 __device__ __forceinline__ int span_size(const CacheAttendParams& p, int total, int most) {
+    const int groups = total >= (long long)(kStart + kLong) * p.kv_heads * p.n_tiles * p.batch ? p.n_long : p.n_groups;
     const int root = __builtin_amdgcn_readfirstlane((int)(__builtin_amdgcn_sqrtf((float)most) * p.span_root + 0.5f * kWaves)) & -kWaves;
-    return max(max(kWaves, quotient(total + p.n_groups - 1, p.n_groups)), max(root, (most + kMaxPieces - 3) / (kMaxPieces - 2)));
+    return max(max(kWaves, quotient(total + groups - 1, groups)), max(root, (most + kMaxPieces - 3) / (kMaxPieces - 2)));
 }
 // Lengths 64 at a time, the first of them once for both walks.
 __device__ __forceinline__ Span span_of(const CacheAttendParams& p, int group, int lane) {
@@ -386,9 +388,9 @@ __device__ __forceinline__ float two_terms(float a, float b, uint32_t& hi, uint3
     return (ha + __uint_as_float(__float_as_uint(la) & 0xffff0000u)) + (hb + __uint_as_float(__float_as_uint(lb) & 0xffff0000u));
 }
 
-// Waves that an SIMD holds.
+// Waves that an SIMD can hold: as many as have their registers without spills.
 template <int D, bool Q4, int C>
-constexpr int per_simd() { return D == 64 ? 4 : D == 128 ? (!Q4 || C == 1 ? 2 : 3) : Q4 && C > 1 ? 2 : 1; }
+constexpr int per_simd() { return D == 64 ? 4 : !Q4 ? 256 / D : (D == 128 ? 3 : 2) - (C == 1 ? 1 : 0); }
 
 // What a lane has of its query row over the keys it has walked.
 template <int D, bool Q4>
@@ -945,11 +947,13 @@ struct AttendPlan {
     size_t part_bytes, word_bytes, score_bytes, stat_bytes;
     size_t bytes() const { return part_bytes + word_bytes + score_bytes + stat_bytes; }
 };
-// workgroups that the chip holds at once (a wave of each on every SIMD)
-template <int D, bool Q4>
-int groups_at_once(int64_t rows) { return kCus * (rows <= 4 ? per_simd<D, Q4, 4>() : rows <= 8 ? per_simd<D, Q4, 2>() : per_simd<D, Q4, 1>()); }
-template <bool Q4>
-int groups_at_once(int64_t dim, int64_t rows) { return dim == 64 ? groups_at_once<64, Q4>(rows) : dim == 128 ? groups_at_once<128, Q4>(rows) : groups_at_once<256, Q4>(rows); }
+// Workgroups a CU, each with a wave on every SIMD: two steps under way a wave keep the memory busy with few waves, and each more is a
+// span more to start and to join.  4-bit rows, a CU with 1 / 2 / 3 / 4: dim 128, 64 sequences of 512 .. 8192 keys 78 / 67 / 70 / 77 us, one
+// with 16 query rows a head 19.5 / 20.4 / 25.5 / 25.5, 8 such 76 / 63 / 72 / 68; dim 256, 16 sequences of 8192 61 / 65 / 74 / 69;
+// dim 64, 64 of 4096 43 / 29 / 34 / 34, but 16 of 37 .. 3001 19.2 / 16.5 / 17.5 / 15.5 and 256 of up to 300 38 / 27 / 24 / 24, where the starts of
+// sequences count for more: two where they are of kLong steps on average, else four.  bf16 rows: dim 64, 16 sequences of 4000
+// 32.2 / 30.4 / - / 31.4; dim 128 63.2 / 64.1 / 67.6.
+constexpr int per_cu(int64_t dim, bool q4) { return q4 ? (dim == 64 ? 4 : dim == 128 ? 2 : 1) : dim == 64 ? 2 : 1; }
 // (q4: the same workspace serves either kind of cache, so it is sized for the one with more workgroups)
 AttendPlan plan_attend(int64_t batch, int64_t seq_new, int64_t heads, int64_t kv_heads, int64_t dim, int64_t max_seq, bool weigh, bool q4 = true) {
     AttendPlan a{};
@@ -957,7 +961,7 @@ AttendPlan plan_attend(int64_t batch, int64_t seq_new, int64_t heads, int64_t kv
     a.n_tiles = (a.rows + 15) / 16;
     a.segments = batch * kv_heads * a.n_tiles;
     a.steps = a.segments * ((max_seq + kStep - 1) / kStep + kStart);
-    a.groups = (int)std::min<int64_t>(q4 ? groups_at_once<true>(dim, a.rows) : groups_at_once<false>(dim, a.rows), std::max<int64_t>((a.steps + kWaves - 1) / kWaves, 1));
+    a.groups = (int)std::min<int64_t>(kCus * per_cu(dim, q4), std::max<int64_t>((a.steps + kWaves - 1) / kWaves, 1));
     a.part_rows = (int)std::min<int64_t>(16, a.rows);
     auto round = [](size_t x) { return (x + 255) / 256 * 256; };
     a.part_bytes = round(((size_t)a.groups + (size_t)a.segments) * (size_t)a.part_rows * (size_t)(dim + 2) * 4);
@@ -999,6 +1003,7 @@ int attend_common(void* stream, CacheAttendParams& p, int head_dim, bool q4, boo
     p.rows = (int)a.rows;
     p.n_tiles = (int)a.n_tiles;
     p.n_groups = groups;
+    p.n_long = q4 && head_dim == 64 ? std::min(groups, 2 * kCus) : groups;
     p.span_root = a.rows <= 4 ? 0.66f : 1.0f;
     p.scale_log2e = (1.0f / sqrtf((float)head_dim)) * kLog2eHost;
     p.part = (float*)workspace;

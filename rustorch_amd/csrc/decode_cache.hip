@@ -197,7 +197,8 @@ struct Keys {
     uint32_t ks[kG][kE], vs[kG][kE];  // pairs of the lane's keys
 };
 
-// bf16 rows come through registers, K's of the next step as soon as this step's scores are there and V's as soon as its products are.
+// bf16 rows come through registers, K's of the next step as soon as this step's scores are there and V's as soon as its products are.  V's
+// past the caches, whole lines a request (16 sequences of 4000 at dim 128 63 -> 49 us); K's, whose lines take two requests, through them.
 template <int D, int C>
 __device__ __forceinline__ void load_k(Keys<D, false, C>& t, const uint8_t* k, int key0, int len, int n, int quad) {
 #pragma unroll
@@ -213,7 +214,8 @@ __device__ __forceinline__ void load_v(Keys<D, false, C>& t, const uint8_t* v, i
     for (int e = 0; e < 8; e++) {
         const uint8_t* row = v + (size_t)min(key0 + 16 * (e / 4) + 4 * quad + e % 4, len - 1) * (2 * D);
 #pragma unroll
-        for (int i = 0; i < D / 32; i++) t.v[e][i] = ((const uint32_t*)(row + (D / 8) * n))[i];
+        for (int i = 0; i < D / 128; i++) *(u32x4_t*)(t.v[e] + 4 * i) = __builtin_nontemporal_load((const u32x4_t*)(row + 256 * i + 16 * n));
+        if constexpr (D == 64) *(u32x2_t*)t.v[e] = __builtin_nontemporal_load((const u32x2_t*)(row + 8 * n));
     }
 }
 
@@ -255,7 +257,9 @@ struct RingLanes {  // byte offsets of a lane's requests
 
 // The requests of one step: keys [key0, key0 + 32) of a slab of `len` keys.  What lies behind the last key lands as zeros, but for pairs
 // of another group's first keys, which no visible key's place takes.  key0 < len.
-template <int D>
+// kOnce: past the caches, rows that no other workgroup asks for (64 sequences of 8192 keys 108 -> 98 us; with 64 query rows a head, whose
+// keys four workgroups walk, 64 -> 69).
+template <int D, bool kOnce>
 __device__ __forceinline__ void ring_load(const RingLanes<D>& at, uint32_t lds, const uint8_t* k, const uint8_t* v, const uint32_t* kp, const uint32_t* vp, int max_seq, int key0, int len) {
     using R = Ring<D>;
     const int keys = min(kStep, len - key0);
@@ -264,8 +268,13 @@ __device__ __forceinline__ void ring_load(const RingLanes<D>& at, uint32_t lds, 
     const u32x4_t krs = make_rsrc(k + from * R::kRow, bytes), vrs = make_rsrc(v + from * R::kRow, bytes);
 #pragma unroll
     for (int i = 0; i < R::kRows / 1024; i++) {
-        buffer_to_lds(krs, at.k[i], 0u, lds + 1024u * i);
-        buffer_to_lds(vrs, at.v[i], 0u, lds + R::kRows + 1024u * i);
+        if constexpr (kOnce) {
+            buffer_to_lds_past(krs, at.k[i], 0u, lds + 1024u * i);
+            buffer_to_lds_past(vrs, at.v[i], 0u, lds + R::kRows + 1024u * i);
+        } else {
+            buffer_to_lds(krs, at.k[i], 0u, lds + 1024u * i);
+            buffer_to_lds(vrs, at.v[i], 0u, lds + R::kRows + 1024u * i);
+        }
     }
     const uint32_t pair_bytes = 4u * (uint32_t)keys + (D > 64 ? 4u * (uint32_t)max_seq : 0u);
 #pragma unroll
@@ -576,7 +585,7 @@ __device__ __forceinline__ void step(State<D, Q4>& st, const Keys<D, Q4, C>& x, 
         u32x4_t p_hi, p_lo;
         operand(w, p_hi, p_lo);
 #pragma unroll
-        for (int d = 0; d < kO; d++) {  // dim n * (D / 16) + d
+        for (int d = 0; d < kO; d++) {  // dim n * (D / 16) + d; of 256, of the lower and of the upper 128 in turn
             u32x4_t a;
 #pragma unroll
             for (int i = 0; i < 4; i++) a[i] = __builtin_amdgcn_perm(x.v[2 * i + 1][d / 2], x.v[2 * i][d / 2], d & 1 ? 0x07060302u : 0x05040100u);
@@ -653,7 +662,7 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4, C>())) void cache_att
         if constexpr (Q4) {
 #pragma unroll
             for (int s = 0; s < Ring<D>::kStages; s++)
-                if (t0 + wave + s * kWaves < t1) ring_load<D>(lanes, ring + s * Ring<D>::kStage, k, v, kp, vp, p.max_seq, (t0 + wave + s * kWaves) * kStep, len);
+                if (t0 + wave + s * kWaves < t1) ring_load<D, (C > 1)>(lanes, ring + s * Ring<D>::kStage, k, v, kp, vp, p.max_seq, (t0 + wave + s * kWaves) * kStep, len);
         } else {
             if (t0 + wave < t1) {
                 load_k<D, C>(x, k, (t0 + wave) * kStep, len, n, quad);
@@ -716,7 +725,7 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4, C>())) void cache_att
                 const int next = t + Ring<D>::kStages * kWaves;
                 if (next < t1) {
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (read before it is written again)
-                    ring_load<D>(lanes, ring + stage * Ring<D>::kStage, k, v, kp, vp, p.max_seq, next * kStep, len);
+                    ring_load<D, (C > 1)>(lanes, ring + stage * Ring<D>::kStage, k, v, kp, vp, p.max_seq, next * kStep, len);
                 }
                 stage ^= 1;
             } else {
@@ -781,7 +790,7 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4, C>())) void cache_att
                         y[e] = st.o[(8 * c + e) % (D / 16)][(8 * c + e) / (D / 16)] * fw;
                     }
                 }
-                float* dst = row + (Q4 ? 32 * c + 8 * quad : quad * (D / 4) + 8 * c);
+                float* dst = row + (Q4 ? 32 * c + 8 * quad : D == 256 ? 128 * (c & 1) + 32 * quad + 8 * (c >> 1) : quad * (D / 4) + 8 * c);
                 *(f32x4_t*)dst = f32x4_t{y[0], y[1], y[2], y[3]};
                 *(f32x4_t*)(dst + 4) = f32x4_t{y[4], y[5], y[6], y[7]};
             }

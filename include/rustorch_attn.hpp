@@ -577,6 +577,12 @@ private:
 
 // ---- LlmKernels: the attention launchers (llm_kernels.rs:874-958), raw device addresses and i32 dims ----------
 
+// One of K and V held in 4 bits (include/rt_attn.h, "caches that are kept small"): device addresses.
+struct Q4Rows {
+    void* codes;
+    uint32_t* pairs;
+};
+
 struct LlmKernels {
     static void kv_append_bf16(void* stream, void* k_cache, void* v_cache, const void* k_in, const void* v_in, int32_t pos,
                                int32_t n_kv, int32_t head_dim, int32_t max_seq) {
@@ -652,6 +658,129 @@ struct LlmKernels {
                                                    n_heads, n_kv, head_dim, max_seq, &e),
                           e);
     }
+    // Caches that are kept small, no counterparts in the reference.  qk_norm_rope_kv_append_bf16 into a 4-bit cache, or into a bf16
+    // one whose rows are not the positions (`rows`, device int32[batch]); slots and weights [batch, n_kv, max_seq] or nullptr.
+    static void qk_norm_rope_kv_append_q4(void* stream, const void* q, void* q_out, const void* k_in, const void* v_in,
+                                          const Q4Rows& k_cache, const Q4Rows& v_cache, const int32_t* positions, int32_t pos,
+                                          const int32_t* rows, int32_t* slots, float* weights, const float* q_gamma,
+                                          const float* k_gamma, float eps, RoPE& rope, int32_t batch, int32_t n_heads,
+                                          int32_t n_kv, int32_t head_dim, int32_t max_seq, int32_t seq = 1) {
+        check_rows(positions, pos, rows, rope, max_seq, seq);
+        rt_err_detail e;
+        detail::check_prepare(
+            rt_qk_norm_rope_kv_append_q4(stream, q, q_out, k_in, v_in, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs,
+                                         positions, pos, rows, slots, weights, q_gamma, k_gamma, eps,
+                                         (const float*)rope.device_cos(), (const float*)rope.device_sin(),
+                                         (int32_t)rope.max_seq(), batch, seq, n_heads, n_kv, head_dim, max_seq, &e),
+            e);
+    }
+    static void qk_norm_rope_kv_append_rows_bf16(void* stream, const void* q, void* q_out, const void* k_in, const void* v_in,
+                                                 void* k_cache, void* v_cache, const int32_t* positions, int32_t pos,
+                                                 const int32_t* rows, int32_t* slots, float* weights, const float* q_gamma,
+                                                 const float* k_gamma, float eps, RoPE& rope, int32_t batch, int32_t n_heads,
+                                                 int32_t n_kv, int32_t head_dim, int32_t max_seq, int32_t seq = 1) {
+        check_rows(positions, pos, rows, rope, max_seq, seq);
+        rt_err_detail e;
+        detail::check_prepare(
+            rt_qk_norm_rope_kv_append_rows_bf16(stream, q, q_out, k_in, v_in, k_cache, v_cache, positions, pos, rows, slots, weights,
+                                                q_gamma, k_gamma, eps, (const float*)rope.device_cos(),
+                                                (const float*)rope.device_sin(), (int32_t)rope.max_seq(), batch, seq, n_heads,
+                                                n_kv, head_dim, max_seq, &e),
+            e);
+    }
+    // KVLayerCache::append of bf16 rows into a 4-bit cache; lengths in elements.
+    static void kv_cache_append_q4(void* stream, const Q4Rows& k_cache, const Q4Rows& v_cache, const void* new_k, size_t new_k_len,
+                                   const void* new_v, size_t new_v_len, size_t batch, size_t n_heads, size_t max_seq,
+                                   size_t head_dim, size_t current_len, size_t seq_added) {
+        rt_err_detail e;
+        detail::check_prepare(rt_kv_cache_append_q4_dev(stream, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, new_k,
+                                                        new_k_len, new_v, new_v_len, batch, n_heads, max_seq, head_dim,
+                                                        current_len, seq_added, &e),
+                              e);
+    }
+    // rows [row, row + n_rows) of every sequence, or from rows[b] on, as bf16 [batch, n_kv, n_rows, head_dim]
+    static void kv_cache_read_q4(void* stream, const Q4Rows& cache, void* out, const int32_t* rows, int32_t row, int32_t n_rows,
+                                 int32_t batch, int32_t n_kv, int32_t head_dim, int32_t max_seq) {
+        rt_err_detail e;
+        detail::check_prepare(rt_kv_cache_read_q4(stream, cache.codes, cache.pairs, out, rows, row, n_rows, batch, n_kv, head_dim,
+                                                  max_seq, &e),
+                              e);
+    }
+    static size_t gqa_decode_q4_workspace_bytes(int32_t batch, int32_t seq_new, int32_t n_heads, int32_t n_kv, int32_t head_dim,
+                                                int32_t max_seq) {
+        return rt_gqa_decode_q4_workspace_bytes(batch, seq_new, n_heads, n_kv, head_dim, max_seq);
+    }
+    // gqa_decode_chunk_bf16 over a 4-bit cache
+    static void gqa_decode_q4(void* stream, const void* q, const Q4Rows& k_cache, const Q4Rows& v_cache, void* out,
+                              const int32_t* kv_lens, int32_t kv_len, int32_t batch, int32_t seq_new, int32_t n_heads,
+                              int32_t n_kv, int32_t head_dim, int32_t max_seq, void* workspace, size_t workspace_bytes) {
+        rt_err_detail e;
+        detail::check_gqa(rt_gqa_decode_q4(stream, q, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, out, kv_lens,
+                                           kv_len, batch, seq_new, n_heads, n_kv, head_dim, max_seq, workspace, workspace_bytes,
+                                           &e),
+                          e);
+    }
+    // A decode step that also sums what each key draws (weights_in nullptr: from zeros), over a bf16 or a 4-bit cache.
+    static size_t gqa_decode_weights_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim,
+                                                     int32_t max_seq) {
+        return rt_gqa_decode_weights_workspace_bytes(batch, n_heads, n_kv, head_dim, max_seq);
+    }
+    static void gqa_decode_weights_bf16(void* stream, const void* q, const void* k_cache, const void* v_cache, void* out,
+                                        const float* weights_in, float* weights_out, const int32_t* kv_lens, int32_t batch,
+                                        int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t max_seq, void* workspace,
+                                        size_t workspace_bytes) {
+        rt_err_detail e;
+        detail::check_gqa(rt_gqa_decode_weights_bf16(stream, q, k_cache, v_cache, out, weights_in, weights_out, kv_lens, batch,
+                                                     n_heads, n_kv, head_dim, max_seq, workspace, workspace_bytes, &e),
+                          e);
+    }
+    static void gqa_decode_weights_q4(void* stream, const void* q, const Q4Rows& k_cache, const Q4Rows& v_cache, void* out,
+                                      const float* weights_in, float* weights_out, const int32_t* kv_lens, int32_t batch,
+                                      int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t max_seq, void* workspace,
+                                      size_t workspace_bytes) {
+        rt_err_detail e;
+        detail::check_gqa(rt_gqa_decode_weights_q4(stream, q, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, out,
+                                                   weights_in, weights_out, kv_lens, batch, n_heads, n_kv, head_dim, max_seq,
+                                                   workspace, workspace_bytes, &e),
+                          e);
+    }
+    // Cuts every sequence to `budget` rows: the `recent` newest tokens' and those with the largest sums of weights.
+    static size_t kv_evict_workspace_bytes(int32_t batch, int32_t n_kv, int32_t max_seq, int32_t budget) {
+        return rt_kv_evict_workspace_bytes(batch, n_kv, max_seq, budget);
+    }
+    static void kv_evict_bf16(void* stream, void* k_cache, void* v_cache, const float* weights_in, const int32_t* slots_in,
+                              float* weights_out, int32_t* slots_out, const int32_t* kv_lens, int32_t* new_lens, int32_t batch,
+                              int32_t n_kv, int32_t head_dim, int32_t max_seq, int32_t budget, int32_t recent, void* workspace,
+                              size_t workspace_bytes) {
+        rt_err_detail e;
+        detail::check_device(rt_kv_evict_bf16(stream, k_cache, v_cache, weights_in, slots_in, weights_out, slots_out, kv_lens,
+                                              new_lens, batch, n_kv, head_dim, max_seq, budget, recent, workspace,
+                                              workspace_bytes, &e),
+                             e);
+    }
+    static void kv_evict_q4(void* stream, const Q4Rows& k_cache, const Q4Rows& v_cache, const float* weights_in,
+                            const int32_t* slots_in, float* weights_out, int32_t* slots_out, const int32_t* kv_lens,
+                            int32_t* new_lens, int32_t batch, int32_t n_kv, int32_t head_dim, int32_t max_seq, int32_t budget,
+                            int32_t recent, void* workspace, size_t workspace_bytes) {
+        rt_err_detail e;
+        detail::check_device(rt_kv_evict_q4(stream, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, weights_in, slots_in,
+                                            weights_out, slots_out, kv_lens, new_lens, batch, n_kv, head_dim, max_seq, budget,
+                                            recent, workspace, workspace_bytes, &e),
+                             e);
+    }
+
+private:
+    // the checks of a host position, before anything touches the device
+    static void check_rows(const int32_t* positions, int32_t pos, const int32_t* rows, const RoPE& rope, int32_t max_seq, int32_t seq) {
+        if (positions) return;
+        const int64_t end = (int64_t)pos + seq;
+        if (pos < 0 || end > (int64_t)rope.max_seq())
+            throw RoPEError(RoPEError::Kind::PositionOverflow, rope.max_seq(), (size_t)end,
+                            "rope: position " + std::to_string(end) + " exceeds max_seq " + std::to_string(rope.max_seq()));
+        if (!rows && end > max_seq) throw KVCacheOverflow((size_t)end, (size_t)max_seq);
+    }
+
+public:
     // No counterpart in the reference: adds `delta` to n int32 values on the device, on `stream` -- the positions and
     // context lengths of a decode loop recorded into a HIP graph advance inside the graph.
     static void i32_add_dev(void* stream, int32_t* values, size_t n, int32_t delta) {

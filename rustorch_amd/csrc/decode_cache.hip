@@ -10,18 +10,22 @@
 // the first binade (the matrix cores take both as they are, products and sums exact as ever), so that a mask, and for every second
 // byte a shift, is all that a pair of codes costs; the high half of a byte stays where it is and counts 16-fold.  The other operand
 // makes up for it: q scaled by the power of two that brings its row's largest value to 2^120 (and by 2^-4 where codes count
-// 16-fold), V's scales, which the weights take along, by 2^60.  What follows from x = z + s (c - 8) is done on the sums, 64 dims at a time:
+// 16-fold), the weights that meet V's codes by 2^60.  What follows from x = z + s (c - 8) is done on the sums, 64 dims at a time:
 //   score = sum over groups of s (sum q c - 8 sum q) + z sum q
 //   out_d = sum over keys of (p s) c_d - 8 sum over keys of (p s) + sum over keys of p z
 // (With codes as the mantissa of 16 + c a pair of codes took a shift and an and-or, 144 of a step's 255 vector instructions at dim 128
-// for 88 of 180 now.)  So V's scales have a range: below 2^-50 the
-// products lose bits, and sum of p s 2^60 has to stay below 2^127, where p is 2^8 at most.
+// for 88 of 180 now.)  So V's scales have a range: below
+// 2^-50 the products lose bits, and the sum of p s 2^60 has to stay below 2^127, where p is 2^8 at most.
 // The weights p s are two bf16 terms (16 bits), as are those of a bf16 cache: with one the output's error is half as large again
 // as its own rounding's.
 //
 // The steps of all (sequence, kv head, 16 query rows) segments form one list that is cut into equal spans, one a workgroup of four
 // waves, which deal the steps of a segment among themselves and fold what they have through LDS.  A segment that lies in one span
 // is written at once; of the others every workgroup leaves an unnormalised partial, and the one that finishes last folds them.
+//
+// Bound by the rows' bytes where there are many: 64 sequences of 8192 keys, 32 heads on 8 of 128, 604 MB in 97 us (6.2 TB/s), of 512 .. 8192 keys
+// 322 MB in 60 us; by the start and the join where there are few: one sequence of 2048 keys 9.1 us, of which 2.8 pass before the
+// first row is there and 2 in the join.
 #include <algorithm>
 #include <type_traits>
 
@@ -65,7 +69,9 @@ __device__ __forceinline__ int quotient(int x, int d) {
     return __builtin_amdgcn_readfirstlane(q);
 }
 // The list that the workgroups share: of every segment `kStart` places and its steps.  The places stand for what a segment costs
-// besides its steps, so that a span of short sequences is no longer a walk than one of a long one.
+// besides its steps, so that a span of short sequences is no longer a walk than one of a long one: us for 0 / 4 / 8 / 16 / 32 places, 256
+// sequences of up to 300 keys at dim 64 46 / 25.7 / 25.0 / 24.5 / 24.9, 16 of 37 .. 3001 21.1 / 18.1 / 17.9 / 15.7 / 16.3, 32 of 500 .. 4096 at dim 128
+// - / 27.8 / 27.4 / 26.4 / 26.2.
 constexpr int kStart = 16;
 constexpr int kLong = 64;  // steps a sequence, see per_cu
 __device__ __forceinline__ int places_of(int len) { return len ? kStart + steps_of(len) : 0; }
@@ -75,7 +81,8 @@ struct Span {
     uint64_t empty;     // of the first 64 sequences, those without keys
 };
 // Places a span, of `total` and a longest sequence of `most` steps: what one of all workgroups gets, but no fewer than a join is worth --
-// a segment of few spans is a long walk, one of many a long join: their sum is least around the root of its steps (p.span_root) -- and
+// a segment of few spans is a long walk, one of many a long join: their sum is least around the root of its steps (p.span_root; one
+// sequence of 8192 keys, 32 heads on 8 of 128, in 8 / 16 / 21 / 32 / 64 pieces 16.9 / 11.7 / 12.0 / 13.1 / 16.3 us) -- and
 // never more of them than kMaxPieces (the steps of a segment touch at most most / size + 2).
 __device__ __forceinline__ int span_size(const CacheAttendParams& p, int total, int most) {
     const int groups = total >= (long long)(kStart + kLong) * p.kv_heads * p.n_tiles * p.batch ? p.n_long : p.n_groups;
@@ -189,7 +196,8 @@ struct SegmentWord {
 // Up to four or eight query rows leave most of the sixteen columns of a product idle, and what is done a (row, key) -- scales, exponentials,
 // the weights' terms -- would be done for all sixteen.  There a row has C = 4 or 2 columns, n, n + 16 / C, ..., and each of them takes a
 // C-th of a lane's eight keys: the others' weights are zeros in its operand, and its part of the row has a maximum and a sum of its own,
-// folded with the waves' at the end.  (Scores of all eight are there anyway: selecting them costs less than finishing them.)
+// folded with the waves' at the end.  (Scores of all eight are there anyway: selecting them costs less than finishing them.  Four rows
+// with C = 1 / 2 / 4: 64 sequences of 512 .. 8192 keys, dim 128 91 / 78 / 77 us, 64 of 4096 at dim 64 40 / 35 / 33, 16 of 8192 at dim 256 138 / 70 / 67.)
 template <int D, bool Q4, int C>
 struct Keys {
     static constexpr int kKw = Q4 ? D / 32 : D / 8, kVw = Q4 ? (D + 127) / 128 : D / 32, kG = Q4 ? D / 64 : 1, kE = 8 / C;
@@ -332,10 +340,7 @@ __device__ __forceinline__ void ring_v(Keys<D, true, C>& t, const unsigned char*
 
 // The codes at bits 4 nib of every second byte as two bf16 numbers, c or 16 c times 2^kCodeExp.  The masks stand in registers: as literals
 // they would be a word more of every instruction.
-constexpr int kCodeExp = -133, kScaleExp = 60;
-// A pair's scale, for V, times 2^kScaleExp: by its exponent's bits, one instruction.  (0 becomes 2^-67, so that a code
-// counts 2^-127 of its offset there.)
-__device__ __forceinline__ float v_scale(uint32_t pair) { return __uint_as_float((pair << 16) + ((uint32_t)kScaleExp << 23)); }
+constexpr int kCodeExp = -133, kScaleExp = 60;  // (kScaleExp: as 0x1p60f too)
 struct Codes {
     uint32_t low, high;
     __device__ __forceinline__ Codes() {
@@ -507,7 +512,8 @@ __device__ __forceinline__ void step(State<D, Q4>& st, const Keys<D, Q4, C>& x, 
         }
     }
     // The running maximum, common to the four lanes of a column.  It follows the scores only where they have risen by 8 in the exponent
-    // of two: up to there the weights, all of them f32 or two bf16 terms, are as exact, and sums are scaled once or twice a span.
+    // of two: up to there the weights, all of them f32 or two bf16 terms, are as exact, and sums are scaled once or twice a span
+    // (64 query heads on 8, 64 sequences of 8192 keys: 137 us, 144 where every rise counts).
     float top = y[0];
 #pragma unroll
     for (int e = 1; e < kE; e++) top = fmaxf(top, y[e]);
@@ -559,7 +565,7 @@ __device__ __forceinline__ void step(State<D, Q4>& st, const Keys<D, Q4, C>& x, 
             float s[kE];
 #pragma unroll
             for (int e = 0; e < kE; e++) {
-                s[e] = hid[e] ? 0.0f : w[e] * v_scale(x.vs[g][e]);  // (what a hidden row holds stays out, were it NaN)
+                s[e] = hid[e] ? 0.0f : w[e] * 0x1p60f * bf16_lo(x.vs[g][e]);  // (what a hidden row holds stays out, were it NaN)
                 if (kCut) st.pz[g] += hid[e] ? 0.0f : w[e] * bf16_hi(x.vs[g][e]);
                 else st.pz[g] = fmaf(w[e], bf16_hi(x.vs[g][e]), st.pz[g]);
             }

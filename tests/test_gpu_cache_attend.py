@@ -321,3 +321,13 @@ def test_replays_over_long_caches(kind):
                 assert np.array_equal(got[0], want[0]), now
                 assert all(np.array_equal(x, y) for x, y in zip(got[1], want[1])), now
     hip.destroy(graph, exe)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_constant_rows_of_v_come_out_as_they_are(d):
+    """A group of equal values has s = 0: zeros give zeros, not what a scale of next to nothing would leave."""
+    c = Case(29, [300, 1, 33], 8, 2, d, 300)
+    v = np.repeat(np.array([0.0, -3.0, 1.5, 0.0], np.float32)[: max(d // 64, 1)], 64)
+    c.v = bf16_bits(np.broadcast_to(v, c.v.shape))
+    out, _, _ = weigh(c, c.q4())
+    assert np.array_equal(out, np.broadcast_to(v, out.shape)) and np.array_equal(attend_q4(c, c.q4()), out)

@@ -42,7 +42,7 @@ constexpr int kStep = 32;       // keys a step
 constexpr int kWaves = 4;        // a workgroup
 constexpr int kCus = 256;
 constexpr int kMaxPieces = 256;  // partials of a segment
-constexpr float kNoMax = -1.0e30f;
+constexpr float kNoMax = -3.0e38f;
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // 16 bytes from any word
 typedef float f32x2_any __attribute__((ext_vector_type(2), aligned(4)));
 typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));

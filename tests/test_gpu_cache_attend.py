@@ -323,6 +323,20 @@ def test_replays_over_long_caches(kind):
     hip.destroy(graph, exe)
 
 
+def test_scores_far_below_zero_are_scores():
+    """Scores of -2^62, -2^63, ...: the least of them in size draws everything."""
+    c = Case(30, [40], 4, 2, 128, 40)
+    c.q = bf16_bits(np.full(c.q.shape, 2.0 ** -60))
+    c.k = bf16_bits(np.broadcast_to(-(2.0 ** 115) * (1 + np.arange(40, dtype=np.float64))[::-1][:, None], c.k.shape))
+    caches = c.q4()
+    out, sums, _ = weigh(c, caches, "none")
+    from _cache import values
+    want = np.repeat(values(*caches[2:])[0, :, 39], 2, axis=0)
+    assert (np.abs(out[0, 0] - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -12 * np.abs(want).max()).all()
+    assert np.array_equal(sums[0, :, 39], [2, 2]) and not sums[0, :, :39].any()
+    assert np.array_equal(attend_q4(c, caches), out)
+
+
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_constant_rows_of_v_come_out_as_they_are(d):
     """A group of equal values has s = 0: zeros give zeros, not what a scale of next to nothing would leave."""

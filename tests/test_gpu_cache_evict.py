@@ -114,3 +114,36 @@ def test_a_row_a_token():
                 w[i, j, :budget], slots[i, j, :budget] = w[i, j, source[i, j]], slots[i, j, source[i, j]]
                 w[i, j, budget], slots[i, j, budget] = 0, slots[i, j, :budget].max() + 1
         w[:, :, :33] += rng.random((2, 2, 33)).astype(np.float32)
+
+
+@pytest.mark.parametrize("n", [8191, 8192, 8193, 20000])
+@pytest.mark.parametrize("budget", [1, 8000, 8191, 8192, 12000])
+def test_around_the_slots_that_registers_hold(n, budget):
+    """Threads of eight slots each, tiles of 8192, equal sums on both sides of their ends."""
+    w, slots, lens, rng = state(37, [n, n - 3, min(budget + 1, n)], 1, n)
+    check(w, slots, lens, budget, min(budget, 500), 64, True, rng, in_place=budget < 8192)
+
+
+@pytest.mark.parametrize("n", [5000, 9000])
+def test_sums_a_bit_apart_and_far_apart(n):
+    """Every range that the counts divide: sums that differ in their last bit, beside some from all over f32."""
+    w, slots, lens, rng = state(38, [n] * 4, 1, n, ties=False)
+    near = (np.uint32(0x40490FDB) + rng.permutation(n).astype(np.uint32)).view(np.float32)
+    w[0, 0] = near
+    w[1, 0] = np.where(rng.random(n) < 0.3, np.ldexp(rng.standard_normal(n), rng.integers(-140, 120, n)), near)
+    w[2, 0] = rng.integers(0, 2 ** 32, n, dtype=np.uint64).astype(np.uint32).view(np.float32)
+    w[3, 0] = np.where(rng.random(n) < 0.5, np.float32(1), np.float32(1 + 2.0 ** -23))
+    for budget, recent in ((1, 0), (n // 3, 40), (n - 1, 0)):
+        check(w, slots, lens, budget, recent, 64, False, rng)
+
+
+def test_positions_at_the_ends_of_32_bits():
+    for low in (-2 ** 31, 2 ** 31 - 300):
+        w, slots, lens, rng = state(39, [300, 200], 2, 300)
+        slots[:] = (low + np.argsort(rng.random(slots.shape), axis=-1)).astype(np.int64)
+        check(w, slots, lens, 120, 50, 64, False, rng)
+    w, slots, lens, rng = state(40, [300], 1, 300)
+    slots[0, 0, ::2] = -2 ** 31 + np.arange(150)
+    slots[0, 0, 1::2] = 2 ** 31 - 150 + np.arange(150)
+    check(w, slots, lens, 100, 30, 64, False, rng)
+    check(w, slots, lens, 200, 160, 64, False, rng)

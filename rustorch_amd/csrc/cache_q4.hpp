@@ -12,7 +12,7 @@
 // Codes: [batch, kv heads, max_seq, dim / 2] bytes.  Byte i n + p of a row, n = dim / 32, holds the dims 32 c + 2 i (low bits) and
 // 32 c + 2 i + 1, where c is p with its two lowest bits exchanged (c = p for n = 2).  A lane of a matrix instruction that owns four
 // consecutive i has the operand of a 64-dim group in the low bits of every second byte, so that two codes come out of a word with
-// one shift and one and-or.
+// a mask, and a shift for the odd bytes.
 // Pairs: [batch, kv heads, dim / 64, max_seq] words, s in the low half: a group's pairs of neighbouring rows are neighbours.
 #pragma once
 #include <hip/hip_runtime.h>

@@ -345,3 +345,22 @@ def test_constant_rows_of_v_come_out_as_they_are(d):
     c.v = bf16_bits(np.broadcast_to(v, c.v.shape))
     out, _, _ = weigh(c, c.q4())
     assert np.array_equal(out, np.broadcast_to(v, out.shape)) and np.array_equal(attend_q4(c, c.q4()), out)
+
+
+@pytest.mark.parametrize("d,b,hq,hkv", [(64, 16, 8, 4), (128, 10, 8, 4), (256, 6, 6, 2)])
+def test_batches_that_fill_the_chip(d, b, hq, hkv):
+    """More steps than workgroups take at their least: spans that end inside sequences, of which some are empty or short."""
+    lens = [2600 + 17 * i for i in range(b)]
+    lens[3], lens[b // 2] = 0, 5
+    c = Case(31, lens, hq, hkv, d, 2900)
+    caches = c.q4()
+    want = expect_q4(bf16_values(c.q), *caches, c.lens)
+    want.check(attend_q4(c, caches))
+    out, sums, start = weigh(c, caches)
+    want.check(out)
+    want.check_weights(sums, start, c.lens)
+    caches = c.bf16()
+    want = expect_bf16(bf16_values(c.q), *(bf16_values(x) for x in caches), c.lens)
+    out, sums, start = weigh(c, caches)
+    want.check(out)
+    want.check_weights(sums, start, c.lens)

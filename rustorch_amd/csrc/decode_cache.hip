@@ -363,7 +363,7 @@ __device__ __forceinline__ float quad_max(float x) {
 // A row of sixteen lanes turned by kBy, and what that makes of columns that lie 16 / C apart: their largest, their sum, in every one.
 template <int kBy>
 __device__ __forceinline__ float turned(float x) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + kBy, 0xf, 0xf, false));
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + kBy, 0xf, 0xf, true));
 }
 template <int C>
 __device__ __forceinline__ float columns_max(float x) {
@@ -753,15 +753,17 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4, C>())) void cache_att
         const float m = columns_max<C>(st.m), f = __builtin_amdgcn_exp2f((st.m - m) * p.scale_log2e);
         const float l = columns_sum<C>(quad_sum(st.l) * f);
         if constexpr (Q4) {
+            static_assert(-kCodeExp - kScaleExp == 73);
+            const float whole[2] = {0x1p73f * f, 0x1p69f * f};
 #pragma unroll
             for (int g = 0; g < kG; g++) {
-                const float off = quad_sum(st.pz[g]) - __builtin_amdgcn_ldexpf(quad_sum(st.ps[g]), 3 - kScaleExp);
+                const float off = (quad_sum(st.pz[g]) - __builtin_amdgcn_ldexpf(quad_sum(st.ps[g]), 3 - kScaleExp)) * f;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int byte = D == 64 ? i / 2 : (g & 1) + 2 * (i / 2);
                     f32x4_t& o = st.o[8 * (D == 64 ? 0 : g / 2) + 2 * byte + i % 2];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[e] = __builtin_amdgcn_ldexpf(o[e], -kCodeExp - kScaleExp - 4 * (i % 2)) + off;
+                    for (int e = 0; e < 4; e++) o[e] = fmaf(o[e], whole[i % 2], off);
                 }
             }
         }
@@ -769,7 +771,7 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4, C>())) void cache_att
 #pragma unroll
             for (int i = 0; i < D / 16; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) st.o[i][e] = columns_sum<C>(st.o[i][e] * f);
+                for (int e = 0; e < 4; e++) st.o[i][e] = columns_sum<C>(Q4 ? st.o[i][e] : st.o[i][e] * f);
         float* const red = (float*)lds;  // [wave][row][kPitch]
         if (n < kR && quad == 0) {
             red_m[wave][n] = m;

@@ -46,6 +46,7 @@ constexpr float kNoMax = -3.0e38f;
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // 16 bytes from any word
 typedef float f32x2_any __attribute__((ext_vector_type(2), aligned(4)));
 typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
@@ -686,23 +687,29 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4, C>())) void cache_att
             for (int c = 0; c < D / 32; c++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, nat[c][i] & 0x7fff7fffu));
-            const int exponent = max((int)quad_max((float)(max(most[0], most[1]) >> 7)), 67) - 127, up = 120 - exponent;
+            const int field = max((int)quad_max((float)(max(most[0], most[1]) >> 7)), 67), up = 247 - field;
             q_exp = up + kCodeExp;
+            // By their exponents' bits: what is 0 or subnormal becomes 2^-67 of the largest value or less.  A row with values above 2^110, or
+            // that are no numbers, is NaN.
+            const u16x2_t by0 = {(uint16_t)(up << 7), (uint16_t)(up << 7)}, by1 = {(uint16_t)((up - 4) << 7), (uint16_t)((up - 4) << 7)};
+            auto scaled = [](uint32_t w, u16x2_t by) __attribute__((always_inline)) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(u16x2_t, w) + by); };
 #pragma unroll
             for (int g = 0; g < kG; g++) {
-                float sum = 0.0f;
+                float sum = field > 237 ? quiet_nan() : 0.0f;
 #pragma unroll
                 for (int c = 2 * g; c < 2 * g + 2; c++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) sum += bf16_lo(nat[c][i]) + bf16_hi(nat[c][i]);
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t two = nat[c][i];
+                        sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, two), bf16x2_t{(__bf16)1.0f, (__bf16)1.0f}, sum, false);
+                    }
                 q_sum[g] = __builtin_amdgcn_ldexpf(quad_sum(sum), q_exp);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     // dim 64: word (u, c) pairs i's of one chunk; above: chunks 2 g and 2 g + 1 at one i
                     const uint32_t a = D == 64 ? nat[i & 1][i & 2] : nat[2 * g][i], o = D == 64 ? nat[i & 1][(i & 2) + 1] : nat[2 * g + 1][i];
-                    auto scaled = [&](float x, int by) __attribute__((always_inline)) { return __float_as_uint(__builtin_amdgcn_ldexpf(x, by)); };
-                    q[2 * g][i] = __builtin_amdgcn_perm(scaled(bf16_lo(o), up), scaled(bf16_lo(a), up), 0x07060302u);
-                    q[2 * g + 1][i] = __builtin_amdgcn_perm(scaled(bf16_hi(o), up - 4), scaled(bf16_hi(a), up - 4), 0x07060302u);
+                    q[2 * g][i] = scaled(__builtin_amdgcn_perm(o, a, 0x05040100u), by0);
+                    q[2 * g + 1][i] = scaled(__builtin_amdgcn_perm(o, a, 0x07060302u), by1);
                 }
             }
         }
@@ -914,7 +921,8 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4, C>())) void cache_att
 }
 
 // The keys' weights from the scores and the rows' statistics.  Grid (1024 keys, kv heads, batch), four keys a thread; the heads' scores
-// are asked for four at a time.
+// are asked for four at a time.  Bound by the launch and one chain of reads (one sequence of 8192 keys 3.9 us) or, in a batch, by the scores' bytes
+// (32 of 300 .. 4096, 32 heads 5.6 us).  A launch of its own, since a weight needs its row's maximum over all spans.
 __global__ __launch_bounds__(256) void cache_weigh_kernel(CacheAttendParams p) {
     const int kvh = blockIdx.y, b = blockIdx.z, len = len_of(p, b), j = (int)blockIdx.x * 1024 + 4 * (int)threadIdx.x;
     if (j >= len) return;

@@ -323,6 +323,18 @@ def test_replays_over_long_caches(kind):
     hip.destroy(graph, exe)
 
 
+@pytest.mark.parametrize("value", [2.0 ** 112, -(2.0 ** 127), np.inf, -np.inf, np.nan])
+def test_a_row_of_q_beyond_its_range_is_nan_and_no_other(value):
+    c = Case(32, [150], 8, 2, 128, 150)
+    caches = c.q4()
+    out, sums, _ = weigh(c, caches, "none")
+    c.q[0, 0, 2, 77] = bf16_bits(np.float32(value))
+    got, got_sums, _ = weigh(c, caches, "none")
+    assert np.isnan(got[0, 0, 2]).all() and np.isnan(got_sums[0, 0]).all()
+    rest = np.delete(np.arange(8), 2)
+    assert np.array_equal(got[0, 0, rest], out[0, 0, rest]) and np.array_equal(got_sums[0, 1], sums[0, 1])
+
+
 def test_scores_far_below_zero_are_scores():
     """Scores of -2^62, -2^63, ...: the least of them in size draws everything."""
     c = Case(30, [40], 4, 2, 128, 40)

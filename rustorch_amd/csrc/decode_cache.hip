@@ -24,7 +24,7 @@
 // is written at once; of the others every workgroup leaves an unnormalised partial, and the one that finishes last folds them.
 //
 // Bound by the rows' bytes where there are many: 64 sequences of 8192 keys, 32 heads on 8 of 128, 604 MB in 97 us (6.2 TB/s), of 512 .. 8192 keys
-// 322 MB in 60 us; by the start and the join where there are few: one sequence of 2048 keys 9.1 us, of which 2.8 pass before the
+// 322 MB in 60 us; by the start and the join where there are few: one sequence of 2048 keys 8.8 us, of which 2.8 pass before the
 // first row is there and 2 in the join.
 #include <algorithm>
 #include <type_traits>

@@ -504,7 +504,8 @@ int rt_kv_cache_read_q4(void *stream, const void *codes, const uint32_t *pairs, 
  * +0.0.  kv head = h / (n_heads / n_kv), any number of heads a group; seq_new * n_heads * head_dim < 2^31.  f32 accumulation and
  * softmax, weights of 16 bits, one rounding to bf16 at the end.  V's values may be as large as
  * 2^60 over the number of keys (a sum beyond is NaN) and are told apart down to 2^-50; q may be as large as 2^110 (a row
- * beyond it is NaN), K anything.  64 dims that read as NaN make all scores of their key NaN, or in V those dims of the
+ * beyond it is NaN), K anything: a score is a sum in f32, off besides by 2^-132 of its row's largest |q| times its key's largest |k| at
+ * most, and what is 0 in q adds nothing to it.  64 dims that read as NaN make all scores of their key NaN, or in V those dims of the
  * positions that see them.  The last bits of a sequence may depend on what else is in the batch (how its keys are cut into spans); the
  * same call gives the same bits every time.  workspace: rt_gqa_decode_q4_workspace_bytes(...) bytes (RT_ERR_WORKSPACE_TOO_SMALL). */
 size_t rt_gqa_decode_q4_workspace_bytes(int32_t batch, int32_t seq_new, int32_t n_heads, int32_t n_kv,

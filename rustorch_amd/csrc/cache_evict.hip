@@ -62,8 +62,11 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t* room, uint3
 // The budget-th largest key is found by counts: the range that the keys in question span is cut into 2048 bins, and the bin it falls in is
 // the next range -- three times at most, since 2048^3 > 2^32, and twice as a rule, since bins that follow the keys' own range hold few of them.
 // (By fixed bytes from the top most sums share a bin, and a wave's counts in one word wait for each other: 8192 keys 30 us.)
-// 8192 slots of 8 heads to 2048: 8.2 us, of which 1.9 until the sums are there, 1.8 for the counts, 2.2 for the lists; bound by the instructions of the one CU that
+// 8192 slots of 8 heads to 2048: 8.4 us, of which 1.9 until the sums are there, 1.8 for the counts, 2.2 for the lists; bound by the instructions of the one CU that
 // a head has and by its barriers (14.5 us with the sums over threads through LDS and a barrier on either side of each).
+// kOne goes by the cache's rows, which the host knows, not by the lengths: with a cache of 8193 rows the whole eviction of those 8192 takes 15.0 us for
+// 12.1, of 4096 rows in a cache of 16384 13.5 for 11.0, of 32 x 300 .. 4096 in such a cache 38 for 33.  Longer heads, 8 of them: 16384 rows to 4096
+// 24.5 us, 65536 to 8192 68, by the one workgroup a head.
 template <bool kOne>
 __global__ __launch_bounds__(kSelect) void cache_select_kernel(CacheEvictParams p) {
     __shared__ uint32_t bins[kBins], chosen[2], above_all, room[6][kSelectWaves];
@@ -250,7 +253,7 @@ __global__ __launch_bounds__(kSelect) void cache_select_kernel(CacheEvictParams 
 }
 
 // Grid (p.move_rows moved rows, kv heads, batch).  A thread has two pieces of 16 bytes of K's rows and of V's, all four under way at once.
-// 32 sequences of 300 .. 4096 rows to 1500, 8 heads of 128 in bf16: 26.6 us for about 110 MB both ways (4.1 TB/s).
+// 32 sequences of 300 .. 4096 rows to 1500, 8 heads of 128 in bf16: 26.6 us for 125 MB both ways (4.7 TB/s), a copy's rate.
 constexpr int kMovePieces = 512;
 __global__ __launch_bounds__(256) void cache_move_kernel(CacheEvictParams p) {
     const int tid = threadIdx.x, b = blockIdx.z, head = b * p.n_kv + (int)blockIdx.y;

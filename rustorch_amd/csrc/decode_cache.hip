@@ -24,8 +24,9 @@
 // is written at once; of the others every workgroup leaves an unnormalised partial, and the one that finishes last folds them.
 //
 // Bound by the rows' bytes where there are many: 64 sequences of 8192 keys, 32 heads on 8 of 128, 604 MB in 97 us (6.2 TB/s), of 512 .. 8192 keys
-// 322 MB in 60 us; by the start and the join where there are few: one sequence of 2048 keys 8.8 us, of which 2.8 pass before the
-// first row is there and 2 in the join.
+// 322 MB in 59 us; by the start and the join where there are few: one sequence of 2048 keys 8.9 us, of which 2.8 pass before the
+// first row is there and 2 in the join; by the steps' vector instructions where there are many query rows a kv head, since every sixteen
+// of them walk, unpack and scale the same keys anew: 16 / 64 / 128 new positions over 8192 keys, 32 heads on 8 of 128, 19 / 36 / 59 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -917,8 +918,9 @@ __global__ __launch_bounds__(64 * kWaves, (per_simd<D, Q4, C>())) void cache_att
 }
 
 // The keys' weights from the scores and the rows' statistics.  Grid (1024 keys, kv heads, batch), four keys a thread; the heads' scores
-// are asked for four at a time.  Bound by the launch and one chain of reads (one sequence of 8192 keys 3.9 us) or, in a batch, by the scores' bytes
-// (32 of 300 .. 4096, 32 heads 5.6 us).  A launch of its own, since a weight needs its row's maximum over all spans.
+// are asked for four at a time.  Bound by the launch and one chain of reads (one sequence of 8192 keys 4.0 us) or, in a batch, by the scores' bytes
+// (32 of 300 .. 4096, 32 heads 5.8 us).  A launch of its own, since a weight needs its row's maximum over all spans.  (The workgroup that ends a
+// segment has that maximum; with up to sixteen heads a kv head it could sum the segment's weights itself.  Not tried.)
 __global__ __launch_bounds__(256) void cache_weigh_kernel(CacheAttendParams p) {
     const int kvh = blockIdx.y, b = blockIdx.z, len = len_of(p, b), j = (int)blockIdx.x * 1024 + 4 * (int)threadIdx.x;
     if (j >= len) return;
@@ -1025,6 +1027,10 @@ int attend_common(void* stream, CacheAttendParams& p, int head_dim, bool q4, boo
     p.n_tiles = (int)a.n_tiles;
     p.n_groups = groups;
     p.n_long = q4 && head_dim == 64 ? std::min(groups, 2 * kCus) : groups;
+    // Of four rows a piece's partial is short and is worth fewer steps than of sixteen.  us for 0.5 / 0.66 / 1 / 1.4 times the root, one sequence: 32 heads
+    // on 8 of 128, 2048 keys 8.9 / 8.9 / 9.6 / 10.3, 8192 12.7 / 11.7 / 11.4 / 12.8, 32768 18.7 / 18.6 / 18.8 / 18.9; 16 heads of 64, 16384 keys
+    // 12.1 / 12.1 / 12.8 / 13.6.  More rows, 8192 keys at dim 128: 8 rows 14.4 / 12.6 / 12.4 / 13.9, 16 18.6 / 15.7 / 14.9 / 16.5, 17 16.1 / 15.3 / 14.7 / 16.3,
+    // 64 19.3 / 19.3 / 19.3 / 21.5.
     p.span_root = a.rows <= 4 ? 0.66f : 1.0f;
     p.scale_log2e = (1.0f / sqrtf((float)head_dim)) * kLog2eHost;
     p.part = (float*)workspace;

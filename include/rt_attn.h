@@ -434,6 +434,70 @@ int rt_gqa_decode_batched_bf16_noalloc(void *stream, const void *q, const void *
 size_t rt_gqa_decode_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim,
                                      int32_t max_seq);
 
+/* ---- many requests side by side: packed prompts, and caches in pages ------------------------------ */
+
+/* No counterparts in the reference, which serves one request at a time from a cache of its own.
+ *
+ * Packed tokens: the tokens of all sequences one behind the other, [tokens, heads, head_dim], as the projections leave them.  `starts`,
+ * device int32[batch + 1], are the first token of each sequence and the end of the last: sequence b has the tokens starts[b] ..
+ * starts[b + 1] - 1, none where the two are equal.  Tokens ahead of the first sequence or behind the last belong to none: rows of
+ * theirs are neither read into others' results nor written.
+ *
+ * A cache in pages: K and V are [n_pages, n_kv, page_size, head_dim] of bf16, page_size a power of two from 16 to 1024, and
+ * `page_table` is device int32[batch, table_pages]: row r of sequence b lies in page page_table[b, r / page_size], there in row
+ * r % page_size of each kv head.  An entry outside 0 .. n_pages - 1 is no page: rows that would go there are not written, and keys there
+ * are not seen.  Several sequences may have a page in common.  head_dim up to 256, a multiple of 16; batch, n_heads and n_kv up to 65535.
+ *
+ * All are asynchronous on `stream`, allocate nothing and may be recorded into a HIP graph. */
+
+/* rt_qk_norm_rope_kv_append_bf16 for packed tokens and a cache in pages, with the same arithmetic, bit for bit.  q [tokens, n_heads,
+ * head_dim] goes rotated to q_out, which is q itself or shares no memory with it; k_in, v_in [tokens, n_kv, head_dim] go to the pages, and
+ * rotated k to k_out too, which is NULL, k_in itself or shares no memory with it (what rt_flash_forward_packed_bf16_dev takes).
+ * Token s of sequence b is row p_b + s of the sequence, p_b = positions[b] (device int32[batch]) or `pos` for all; with starts == NULL every
+ * sequence has tokens / batch tokens (1 for a decode step).
+ * Its rotary position is its row, or, with n_axes of 1 to 4, axis_positions[a, token] (device int32[n_axes, tokens]) on axis a: the first
+ * sections[0] pairs of a head (pair i: dims i and i + head_dim / 2) turn with axis 0, the next sections[1] with axis 1, and so on (host
+ * int32[n_axes], their sum head_dim / 2, any of them 0; RT_ERR_ROPE_WRONG_INPUT_LEN otherwise).
+ * A token whose position the tables do not have is left as it is, everywhere; one whose row has no page (behind the table, negative,
+ * or an entry that is no page) is rotated and not stored.  No two tokens of a call may go to one row of a page; what is shared stays as it
+ * is.  A host `pos` is checked (RT_ERR_ROPE_POSITION_OVERFLOW, then RT_ERR_KV_OVERFLOW; with `starts`, its lowest row alone).  All tensors
+ * 16-byte aligned (gammas and tables 4); outputs and pages share no memory with each other or with other inputs (RT_ERR_UNSUPPORTED). */
+int rt_qk_norm_rope_kv_append_paged_bf16(void *stream, const void *q, void *q_out, const void *k_in, void *k_out,
+                                         const void *v_in, void *k_pages, void *v_pages, const int32_t *page_table,
+                                         const int32_t *starts, const int32_t *positions, int32_t pos,
+                                         const int32_t *axis_positions, const int32_t *sections, int32_t n_axes,
+                                         const float *q_gamma, const float *k_gamma, float eps, const float *cos_table,
+                                         const float *sin_table, int32_t table_rows, int32_t tokens, int32_t batch,
+                                         int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t n_pages,
+                                         int32_t page_size, int32_t table_pages, rt_err_detail *err);
+
+/* Causal attention of whole prompts, packed: shape = {batch: sequences, heads, seq: tokens of all, dim}; q/out [seq, heads, dim], k/v [seq,
+ * n_kv_heads, dim] (0 = heads), all bf16; token i of a sequence sees its tokens 0 .. i and no other sequence's.  Rows equal
+ * rt_flash_forward_bnhd_bf16_dev of the sequence alone up to the last bits (which may depend on what else is in the launch, as with that
+ * entry), and rt_set_strict_non_finite_v holds here too.  dim up to 256, a multiple of 8, tensors 16-byte aligned, k and v below
+ * 4 GiB each, out apart from the inputs (RT_ERR_UNSUPPORTED). */
+int rt_flash_forward_packed_bf16_dev(void *stream, const rt_attention_shape *shape, uint64_t n_kv_heads, const void *q,
+                                     const void *k, const void *v, const int32_t *starts, void *out, rt_err_detail *err);
+
+/* rt_gqa_decode_batched_bf16 over a cache in pages, for a batch that may share a prefix: q/out bf16 [batch, n_heads, head_dim], kv_lens
+ * device int32[batch] = keys of each sequence (counts above table_pages * page_size are that, below 0 are 0).  With P =
+ * shared_lens[0] (device int32[1]) or, with shared_lens == NULL, `shared_len` (0: nothing in common), every sequence of at least P keys has
+ * its first P in common with the others: they are read once for all of them, through page_table[0]; its own, from P on, and
+ * all keys of shorter sequences, through the sequence's row of the table.  P need not end with a page.  A sequence that sees no key (no
+ * keys, or none in pages) gives rows of +0.0.  kv head = h / (n_heads / n_kv), any number of heads a group.  f32 accumulation and
+ * softmax, weights of one bf16 each, one rounding to bf16 at the end.  What is not seen does not count, whatever it holds; a dim in which a
+ * V row that is seen is infinite or NaN comes out infinite or NaN.  The last bits of a sequence may depend on what else is in the batch (how its keys are cut into spans); the same call gives the same bits
+ * every time.  table_pages * page_size up to 2^28.  `workspace`: rt_gqa_decode_paged_workspace_bytes(...) bytes of device memory, 16-byte
+ * aligned (RT_ERR_WORKSPACE_TOO_SMALL), which the call works in alone and keeps nothing in: calls that may overlap (other streams,
+ * graphs replayed side by side) have workspaces of their own. */
+size_t rt_gqa_decode_paged_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim,
+                                           int32_t page_size, int32_t table_pages);
+int rt_gqa_decode_paged_bf16(void *stream, const void *q, const void *k_pages, const void *v_pages, void *out,
+                             const int32_t *page_table, const int32_t *kv_lens, const int32_t *shared_lens,
+                             int32_t shared_len, int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim,
+                             int32_t n_pages, int32_t page_size, int32_t table_pages, void *workspace,
+                             size_t workspace_bytes, rt_err_detail *err);
+
 /* ---- caches that are kept small: 4-bit rows, and rows taken out ---------------------------------- */
 
 /* No counterparts in the reference, whose caches are f32 or bf16 and keep every row.

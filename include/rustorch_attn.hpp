@@ -583,6 +583,13 @@ struct Q4Rows {
     uint32_t* pairs;
 };
 
+// K and V of a cache in pages: [n_pages, n_kv, page_size, head_dim] of bf16 (include/rt_attn.h).
+struct KVPages {
+    void* k;
+    void* v;
+    int32_t n_pages, page_size;
+};
+
 struct LlmKernels {
     static void kv_append_bf16(void* stream, void* k_cache, void* v_cache, const void* k_in, const void* v_in, int32_t pos,
                                int32_t n_kv, int32_t head_dim, int32_t max_seq) {
@@ -767,6 +774,51 @@ struct LlmKernels {
                                             weights_out, slots_out, kv_lens, new_lens, batch, n_kv, head_dim, max_seq, budget,
                                             recent, workspace, workspace_bytes, &e),
                              e);
+    }
+
+    // Norm, rotation and append of packed tokens [tokens, heads, head_dim] into pages; rotated k goes to k_out too, where it is not nullptr.
+    // starts (device [batch + 1], nullptr: tokens / batch each) are the sequences' first tokens, positions (device, or pos) the rows of
+    // those; with sections, a head's pairs for each of up to four axes, the rotary positions are axis_positions [axes, tokens].
+    static void qk_norm_rope_kv_append_paged_bf16(void* stream, const void* q, void* q_out, const void* k_in, void* k_out, const void* v_in,
+                                                  const KVPages& pages, const int32_t* page_table, int32_t table_pages,
+                                                  const int32_t* starts, const int32_t* positions, int32_t pos,
+                                                  const int32_t* axis_positions, const std::vector<int32_t>& sections,
+                                                  const float* q_gamma, const float* k_gamma, float eps, RoPE& rope, int32_t tokens,
+                                                  int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim) {
+        if (sections.empty())
+            check_rows(positions, pos, nullptr, rope, table_pages * pages.page_size, starts || batch <= 0 ? 0 : tokens / batch);
+        rt_err_detail e;
+        detail::check_prepare(
+            rt_qk_norm_rope_kv_append_paged_bf16(stream, q, q_out, k_in, k_out, v_in, pages.k, pages.v, page_table, starts, positions, pos,
+                                                 axis_positions, sections.empty() ? nullptr : sections.data(), (int32_t)sections.size(),
+                                                 q_gamma, k_gamma, eps, (const float*)rope.device_cos(), (const float*)rope.device_sin(),
+                                                 (int32_t)rope.max_seq(), tokens, batch, n_heads, n_kv, head_dim, pages.n_pages,
+                                                 pages.page_size, table_pages, &e),
+            e);
+    }
+    // A decode step over pages; the first shared_len keys (or shared_lens[0], on the device) of every sequence that has as many are those of
+    // the first row of the table, and are read once.
+    static size_t gqa_decode_paged_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t page_size,
+                                                   int32_t table_pages) {
+        return rt_gqa_decode_paged_workspace_bytes(batch, n_heads, n_kv, head_dim, page_size, table_pages);
+    }
+    static void gqa_decode_paged_bf16(void* stream, const void* q, const KVPages& pages, void* out, const int32_t* page_table,
+                                      int32_t table_pages, const int32_t* kv_lens, const int32_t* shared_lens, int32_t shared_len,
+                                      int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim, void* workspace,
+                                      size_t workspace_bytes) {
+        rt_err_detail e;
+        detail::check_gqa(rt_gqa_decode_paged_bf16(stream, q, pages.k, pages.v, out, page_table, kv_lens, shared_lens, shared_len, batch,
+                                                   n_heads, n_kv, head_dim, pages.n_pages, pages.page_size, table_pages, workspace,
+                                                   workspace_bytes, &e),
+                          e);
+    }
+    // Causal attention of prompts packed one behind the other: shape.batch sequences of shape.seq tokens in all, q/out [seq, heads, dim],
+    // k/v [seq, n_kv_heads, dim]; starts (device [batch + 1]) are their first tokens.
+    static void flash_forward_packed_bf16(void* stream, const AttentionShape& shape, size_t n_kv_heads, const void* q, const void* k,
+                                          const void* v, const int32_t* starts, void* out) {
+        const rt_attention_shape s = shape.c();
+        rt_err_detail e;
+        detail::check_attention(rt_flash_forward_packed_bf16_dev(stream, &s, n_kv_heads, q, k, v, starts, out, &e), e);
     }
 
 private:

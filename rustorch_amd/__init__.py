@@ -8,7 +8,7 @@ from . import _lib
 from .attention import (AttentionShape, Mask, flash_backward, flash_backward_f32_dev, flash_backward_saved_f32_dev,
                         flash_forward_stats_f32_dev,
                         flash_backward_workspace_bytes, flash_forward, flash_forward_bf16_dev, flash_forward_bnhd_bf16_dev,
-                        flash_forward_bnhd_f32_dev, flash_forward_f32_dev, flash_forward_masked,
+                        flash_forward_bnhd_f32_dev, flash_forward_f32_dev, flash_forward_masked, flash_forward_packed_bf16_dev,
                         flash_forward_varlen_bf16_dev, flash_forward_window_bf16_dev, mha_attention_f32, mha_attention_route, mha_flash_forward_f32, mha_forward_masked_bf16_dev, mha_forward_masked_f32_dev,
                         mha_forward_masked_f32)
 from .device import (HipStorage, Stream, debug_f32_split_products, debug_f32_wide_gradients, debug_force_bf16_prefill_kernel, i32_add_dev, init,
@@ -18,8 +18,8 @@ from .errors import (AttentionError, BufferShapeMismatch, DeviceError, GQAError,
                      MaskError, OutputShapeMismatch, Overflow, PaddingLengthMismatch, PositionOverflow, RoPEError,
                      RopeWrongInputLen, WrongInputLen, ZeroDim)
 from .gqa import gqa_forward_f32, gqa_forward_f32_dev
-from .kv_cache import KVCache
-from .llm_kernels import LlmKernels, Q4Rows
+from .kv_cache import KVCache, PagedKVCache
+from .llm_kernels import KVPages, LlmKernels, Q4Rows
 from .masks import MASK_NEG, bool_to_additive, causal_mask, sliding_window_mask
 from .rope import RoPE
 

@@ -29,6 +29,7 @@ SYMBOLS = (
     "rt_qk_norm_rope_kv_append_q4", "rt_qk_norm_rope_kv_append_rows_bf16", "rt_kv_cache_append_q4_dev", "rt_kv_cache_read_q4",
     "rt_gqa_decode_q4", "rt_gqa_decode_q4_workspace_bytes", "rt_gqa_decode_weights_bf16", "rt_gqa_decode_weights_q4",
     "rt_gqa_decode_weights_workspace_bytes", "rt_kv_evict_bf16", "rt_kv_evict_q4", "rt_kv_evict_workspace_bytes",
+    "rt_qk_norm_rope_kv_append_paged_bf16", "rt_flash_forward_packed_bf16_dev", "rt_gqa_decode_paged_bf16", "rt_gqa_decode_paged_workspace_bytes",
 )
 
 RT_OK = 0
@@ -127,8 +128,12 @@ def lib():
     L.rt_gqa_decode_weights_bf16.argtypes = [vp] * 8 + [i32] * 5 + [vp, sz, errp]
     L.rt_gqa_decode_weights_q4.argtypes = [vp] * 10 + [i32] * 5 + [vp, sz, errp]
     L.rt_kv_evict_bf16.argtypes = [vp] * 9 + [i32] * 6 + [vp, sz, errp]
+    L.rt_qk_norm_rope_kv_append_paged_bf16.argtypes = [vp] * 11 + [i32, vp, vp, i32, vp, vp, f32, vp, vp] + [i32] * 9 + [errp]
+    L.rt_flash_forward_packed_bf16_dev.argtypes = [vp, shp, u64, vp, vp, vp, vp, vp, errp]
+    L.rt_gqa_decode_paged_bf16.argtypes = [vp] * 8 + [i32] * 8 + [vp, sz, errp]
     L.rt_kv_evict_q4.argtypes = [vp] * 11 + [i32] * 6 + [vp, sz, errp]
-    for name, n in (("rt_gqa_decode_q4_workspace_bytes", 6), ("rt_gqa_decode_weights_workspace_bytes", 5), ("rt_kv_evict_workspace_bytes", 4)):
+    for name, n in (("rt_gqa_decode_q4_workspace_bytes", 6), ("rt_gqa_decode_weights_workspace_bytes", 5), ("rt_kv_evict_workspace_bytes", 4),
+                    ("rt_gqa_decode_paged_workspace_bytes", 6)):
         getattr(L, name).argtypes = [i32] * n
         getattr(L, name).restype = sz
     L.rt_buf_alloc.argtypes = [sz, errp]

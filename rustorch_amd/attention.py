@@ -159,6 +159,12 @@ def flash_forward_varlen_bf16_dev(shape, q, k, v, seq_lens_dev, out, zero_padded
                                                     int(bool(zero_padded_rows)), out))
 
 
+def flash_forward_packed_bf16_dev(shape, q, k, v, starts_dev, out, n_kv_heads=0, stream=None):
+    """Causal attention of prompts packed one behind the other: shape.batch sequences of shape.seq tokens in all, q/out [seq, heads,
+    dim], k/v [seq, n_kv_heads, dim] (0 = heads); starts_dev, device int32[batch + 1], are the sequences' first tokens."""
+    check(L.native.rt_flash_forward_packed_bf16_dev(stream, shape, n_kv_heads, q, k, v, starts_dev, out))
+
+
 # ---- [batch, seq, heads, dim] tensors: the layout MultiHeadAttention keeps its projections in --------------
 
 

@@ -117,13 +117,14 @@ std::atomic<int> g_strict_v{0};
 // After a causal forward, when the strict switch is on: the pass that gives query rows the reference's NaN for
 // non-finite V elements at keys they do not see (the forward kernels skip those key tiles).
 int strict_pass(hipStream_t stream, const rt_attention_shape* s, uint64_t n_kv_heads, const void* v, void* out,
-                const int32_t* seq_lens, int mask_kind, bool bnhd, bool bf16, rt_err_detail* err) {
+                const int32_t* seq_lens, int mask_kind, bool bnhd, bool bf16, rt_err_detail* err, const int32_t* starts = nullptr) {
     if (mask_kind != rt::kMaskCausal && mask_kind != rt::kMaskVarlenCausal) return RT_OK;
     if (!g_strict_v.load(std::memory_order_relaxed)) return RT_OK;
     rt::StrictVParams p{};
     p.v = v;
     p.out = out;
     p.seq_lens = seq_lens;
+    p.starts = starts;
     p.batch = (int)s->batch;
     p.heads = (int)s->heads;
     p.kv_heads = (int)n_kv_heads;
@@ -136,6 +137,7 @@ int strict_pass(hipStream_t stream, const rt_attention_shape* s, uint64_t n_kv_h
         p.lo = rt::layout_bhnd((long long)s->heads, (long long)s->seq, p.dim);
         p.lkv = rt::layout_bhnd((long long)n_kv_heads, (long long)s->seq, p.dim);
     }
+    if (starts) p.lo.batch_stride = p.lkv.batch_stride = 0;
     HIP_TRY(rt::launch_strict_hidden_v(stream, p, bf16), "strict_hidden_v launch");
     return RT_OK;
 }
@@ -1633,6 +1635,52 @@ RT_API int rt_flash_forward_varlen_bf16_dev(void* stream, const rt_attention_sha
 }
 
 // ---- decode, device pointers -------------------------------------------------------------------------
+
+RT_API int rt_flash_forward_packed_bf16_dev(void* stream, const rt_attention_shape* shape, uint64_t n_kv_heads,
+                                            const void* q, const void* k, const void* v, const int32_t* starts, void* out,
+                                            rt_err_detail* err) {
+    clear_err(err);
+    if (!shape) return fail(err, RT_ERR_NULL_POINTER, -1, 0, 0, "shape is NULL");
+    if (shape->dim == 0) return fail(err, RT_ERR_ZERO_DIM, -1, 0, 0, "dim must be > 0");
+    if (n_kv_heads == 0) n_kv_heads = shape->heads;
+    if (shape->seq == 0 || shape->batch == 0 || shape->heads == 0) return RT_OK;
+    int rc = check_flash_dims(shape, n_kv_heads, err);
+    if (rc) return rc;
+    if (shape->dim > 256 || shape->dim % 8 != 0)
+        return fail(err, RT_ERR_UNSUPPORTED, -1, 256, shape->dim, "packed prompts cover head dims up to 256, multiples of 8");
+    if (!rt::flash_tile_bf16_addressable((long long)shape->seq, (long long)(n_kv_heads * shape->dim)))
+        return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "k and v of a call must be below 4 GiB each");
+    if (!q || !k || !v || !out || !starts) return fail(err, RT_ERR_NULL_POINTER, -1, 0, 0, "NULL buffer");
+    if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15)
+        return fail(err, RT_ERR_UNSUPPORTED, -1, 16, 0, "q, k, v and out must be 16-byte aligned");
+    const size_t rows = (size_t)shape->seq * shape->dim * 2, q_bytes = rows * shape->heads, kv_bytes = rows * n_kv_heads;
+    if (rt::overlap(out, q_bytes, q, q_bytes) || rt::overlap(out, q_bytes, k, kv_bytes) || rt::overlap(out, q_bytes, v, kv_bytes))
+        return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "out must share no memory with the inputs");
+    rc = ensure_device(err);
+    if (rc) return rc;
+    rt::FlashTileParams t{};
+    t.q = (const uint16_t*)q;
+    t.k = (const uint16_t*)k;
+    t.v = (const uint16_t*)v;
+    t.out = (uint16_t*)out;
+    t.starts = starts;
+    t.batch = (int)shape->batch;
+    t.heads = (int)shape->heads;
+    t.kv_heads = (int)n_kv_heads;
+    t.group = (int)(shape->heads / n_kv_heads);
+    t.pack = 1;
+    t.n_cus = g_num_cus;
+    t.seq_q = t.seq_kv = (int)shape->seq;
+    t.dim = (int)shape->dim;
+    t.mask = rt::kMaskPacked;
+    t.ref_bc = 1;
+    t.scale = 1.0f / sqrtf((float)shape->dim);
+    t.scale_log2e = t.scale * rt::kLog2eHost;
+    t.lq = t.lo = rt::layout_bnhd((long long)shape->heads, 0, t.dim);
+    t.lkv = rt::layout_bnhd((long long)n_kv_heads, 0, t.dim);
+    HIP_TRY(rt::launch_flash_tile_bf16((hipStream_t)stream, t), "flash_tile_bf16 launch");
+    return strict_pass((hipStream_t)stream, shape, n_kv_heads, v, out, nullptr, rt::kMaskCausal, true, true, err, starts);
+}
 
 RT_API int rt_kv_append_bf16(void* stream, void* k_cache, void* v_cache, const void* k_in, const void* v_in,
                              int32_t pos, int32_t n_kv, int32_t head_dim, int32_t max_seq, rt_err_detail* err) {

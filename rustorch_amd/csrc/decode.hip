@@ -1001,10 +1001,16 @@ __global__ __launch_bounds__(256) void strict_hidden_v_kernel(StrictVParams p) {
     const int group = p.heads / p.kv_heads;
     int n_keys = p.seq, n_q = p.seq;
     if (p.seq_lens) n_keys = n_q = min(max(p.seq_lens[b], 0), p.seq);
+    size_t row0 = 0;
+    if (p.starts) {
+        const int first = min(max(p.starts[b], 0), p.seq);
+        row0 = (size_t)first;
+        n_keys = n_q = min(max(p.starts[b + 1], first), p.seq) - first;
+    }
     __shared__ int last_bad[512];
     for (int c = tid; c < p.dim; c += 256) last_bad[c] = -1;
     __syncthreads();
-    const T* vb = (const T*)p.v + (size_t)b * p.lkv.batch_stride + (size_t)kvh * p.lkv.head_stride;
+    const T* vb = (const T*)p.v + (size_t)b * p.lkv.batch_stride + (size_t)kvh * p.lkv.head_stride + row0 * p.lkv.row_pitch;
     // thread t looks at columns t % cw + k * cw of rows t / cw + k * (256 / cw): consecutive lanes, consecutive addresses
     const int cw = p.dim >= 256 ? 256 : (p.dim >= 128 ? 128 : (p.dim >= 64 ? 64 : (p.dim >= 32 ? 32 : 16)));
     const int rows_per_pass = 256 / cw;
@@ -1025,7 +1031,7 @@ __global__ __launch_bounds__(256) void strict_hidden_v_kernel(StrictVParams p) {
         const int hidden_rows = min(last_bad[c] - off, n_q);  // rows 0 .. hidden_rows-1 do not see that key
         if (hidden_rows <= 0) continue;
         for (int g = 0; g < group; g++) {
-            T* ob = (T*)p.out + (size_t)b * p.lo.batch_stride + (size_t)(kvh * group + g) * p.lo.head_stride + c;
+            T* ob = (T*)p.out + (size_t)b * p.lo.batch_stride + (size_t)(kvh * group + g) * p.lo.head_stride + row0 * p.lo.row_pitch + c;
             for (int i = tid; i < hidden_rows; i += 256) {
                 if constexpr (sizeof(T) == 2) ob[(size_t)i * p.lo.row_pitch] = (T)0x7fc0u;
                 else ob[(size_t)i * p.lo.row_pitch] = __uint_as_float(0x7fc00000u);

@@ -1,0 +1,880 @@
+// A decode step over a cache in pages, for a batch that may share a prefix:
+//
+//   out_b = softmax(q_b K_b^T / sqrt(dim)) V_b        K_b = [the prefix's rows; the sequence's own], looked up page by page
+//
+// A wave walks steps of 32 keys of one kv head by the matrix cores, both products transposed as in decode_cache.hip: scores^T = K q^T
+// leaves a lane with the scores of ONE query row for eight keys, which is the operand that out^T = V^T P^T takes, so that nothing of
+// a step crosses lanes but the running maximum.  A step's two sixteens of rows lie in a page each, whose place is looked up ahead; K
+// and V come through descriptors that end with the last key's row, so that rows behind it are zeros and are not read.
+//
+// A sequence's own keys meet the up to sixteen query rows of one kv head.  The prefix's keys meet those of the whole batch: the rows of
+// all sequences that share it form tiles of 16 kTiles rows, whose operands wait in LDS, and a step's keys are asked for once for a tile.
+// Both kinds of segments, (kv head, tile) of the prefix and (sequence, kv head), form one list of steps that is cut into equal
+// spans, one a workgroup of four waves, which deal the steps of a segment among themselves and fold what they have through LDS.  What a
+// workgroup finishes of a sequence it writes at once, where that is all there is; otherwise it leaves a partial (o, m, l) and counts
+// its steps, and the workgroup that completes the sequence's count folds the partials.
+//
+// The weights meet V as one bf16 each, rounded to nearest, as in the prefill kernels: 2^-9 of a weight, and errors of many keys cancel.
+#include <algorithm>
+#include <type_traits>
+
+#include "cache_paged.hpp"
+#include "rt_common.hpp"
+#include "rt_host.hpp"
+#include "rt_kernels.hpp"
+
+namespace rt {
+
+namespace {
+
+constexpr int kStep = 32;   // keys a step
+constexpr int kWaves = 4;   // a workgroup
+constexpr int kCus = 256;
+constexpr int kMaxPieces = 256;  // partials of a sequence's kv head: half of the prefix, half of its own keys, or all of its own
+constexpr float kNoMax = -3.0e38f;
+typedef float f32x2p __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2p __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t two_bf16(float lo, float hi) {  // to nearest even
+    const f32x2p x = {lo, hi};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2p));
+}
+// x / d for 0 <= x < 2^31, 0 < d, by a reciprocal in f32 and what it is off by
+__device__ __forceinline__ int quotient(int x, int d) {
+    int q = (int)((float)x * __builtin_amdgcn_rcpf((float)d));
+    int r = x - q * d;
+    while (r < 0) {
+        q--;
+        r += d;
+    }
+    while (r >= d) {
+        q++;
+        r -= d;
+    }
+    return __builtin_amdgcn_readfirstlane(q);
+}
+
+// ---- over lanes, within registers (the steps of a prefix sum are those of cache_q4.hpp) ------------------------------------
+template <int kStepNo>
+__device__ __forceinline__ int lanes_from(int none, int x) {
+    constexpr int kCtrl[6] = {0x111, 0x112, 0x114, 0x118, 0x142, 0x143}, kRows[6] = {0xf, 0xf, 0xf, 0xf, 0xa, 0xc};
+    return __builtin_amdgcn_update_dpp(none, x, kCtrl[kStepNo], kRows[kStepNo], 0xf, false);
+}
+__device__ __forceinline__ int lane_sums(int x) {  // up to and with this lane
+    x += lanes_from<0>(0, x);
+    x += lanes_from<1>(0, x);
+    x += lanes_from<2>(0, x);
+    x += lanes_from<3>(0, x);
+    x += lanes_from<4>(0, x);
+    x += lanes_from<5>(0, x);
+    return x;
+}
+__device__ __forceinline__ int lane_max(int x) {
+    x = max(x, lanes_from<0>(x, x));
+    x = max(x, lanes_from<1>(x, x));
+    x = max(x, lanes_from<2>(x, x));
+    x = max(x, lanes_from<3>(x, x));
+    x = max(x, lanes_from<4>(x, x));
+    x = max(x, lanes_from<5>(x, x));
+    return __builtin_amdgcn_readlane(x, 63);
+}
+// of the four lanes of a query row (rows of 16 lanes swapped, then halves of the wave)
+template <typename F>
+__device__ __forceinline__ float over_quads(float x, F f) {
+    const u32x2_t a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const float y = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const u32x2_t c = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+    return f(__uint_as_float(c[0]), __uint_as_float(c[1]));
+}
+__device__ __forceinline__ float quad_max(float x) {
+    return over_quads(x, [](float a, float b) __attribute__((always_inline)) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float quad_sum(float x) {
+    return over_quads(x, [](float a, float b) __attribute__((always_inline)) { return a + b; });
+}
+// a row of sixteen lanes turned by kBy, and of columns that lie 16 / C apart their largest or their sum, in every one
+template <int kBy>
+__device__ __forceinline__ float turned(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + kBy, 0xf, 0xf, true));
+}
+template <int C>
+__device__ __forceinline__ float columns_max(float x) {
+    if (C >= 2) x = fmaxf(x, turned<8>(x));
+    if (C >= 4) x = fmaxf(x, turned<4>(x));
+    if (C == 16) {
+        x = fmaxf(x, turned<2>(x));
+        x = fmaxf(x, turned<1>(x));
+    }
+    return x;
+}
+template <int C>
+__device__ __forceinline__ float columns_sum(float x) {
+    if (C >= 2) x += turned<8>(x);
+    if (C >= 4) x += turned<4>(x);
+    if (C == 16) {
+        x += turned<2>(x);
+        x += turned<1>(x);
+    }
+    return x;
+}
+
+// ---- the list that the workgroups share -----------------------------------------------------------------------------------
+// Of every segment kStart places, which stand for what it costs besides its steps, and its steps.
+constexpr int kStart = 16;
+__device__ __forceinline__ int steps_up_to(int key) { return (key + kStep - 1) / kStep; }
+struct Own {  // a sequence's own keys
+    int len, lo;  // [lo, len); lo: the prefix's length where it shares it, else 0
+    __device__ __forceinline__ Own(int n, int shared) : len(n), lo(n >= shared ? shared : 0) {}
+    __device__ __forceinline__ int first() const { return lo / kStep; }
+    __device__ __forceinline__ int steps() const { return len > lo ? steps_up_to(len) - first() : 0; }
+    __device__ __forceinline__ int places() const { return len > lo ? steps() + kStart : 0; }
+};
+__device__ __forceinline__ int len_of(const PagedDecodeParams& p, int b) { return min(max(p.kv_lens[b], 0), p.max_len); }
+
+struct Span {
+    int total, size;     // places of all; of a span
+    int shared;          // the prefix's length; 0: nobody shares one
+    int pre_places;      // places of a (kv head, tile) of the prefix
+    int pre_total;       // of all of them
+    int b, first, len;   // the sequence that holds the span's first place, where it starts, its length
+    uint64_t empty;      // of the first 64 sequences, those without keys
+    int begin, end;
+};
+// The span of `group`, of workgroups that are numbered as they come.  A prefix's tiles read the same keys: their spans go to workgroups of
+// one XCD, an eighth of the list each.
+template <bool kShared>
+__device__ __forceinline__ Span span_of(const PagedDecodeParams& p, int& group, int lane) {
+    const int per = p.kv_heads * p.chunks;
+    Span s;
+    s.shared = !kShared ? 0 : min(max(p.shared_lens ? *(const __attribute__((address_space(4))) int32_t*)p.shared_lens : p.shared_len, 0), p.max_len);
+    auto len_at = [&](int b0) { return b0 + lane < p.batch ? len_of(p, b0 + lane) : -1; };  // (behind the last: no sequence)
+    auto places = [&](int len) { return len < 0 ? 0 : Own(len, s.shared).places(); };
+    const int len0 = len_at(0), ends0 = lane_sums(places(len0));
+    s.empty = __ballot(len0 == 0);
+    int sum = __builtin_amdgcn_readlane(ends0, 63), most = lane_max(len0 < 0 ? 0 : Own(len0, s.shared).steps());
+    bool any = kShared && __any(len0 >= s.shared);
+    for (int b0 = 64; b0 < p.batch; b0 += 64) {
+        const int len = len_at(b0);
+        sum += __builtin_amdgcn_readlane(lane_sums(places(len)), 63);
+        most = max(most, lane_max(len < 0 ? 0 : Own(len, s.shared).steps()));
+        any = any || (kShared && __any(len >= s.shared));
+    }
+    if (!any) s.shared = 0;  // (then every `lo` was 0 already)
+    s.pre_places = s.shared > 0 ? kStart + steps_up_to(s.shared) : 0;
+    s.pre_total = s.pre_places * p.kv_heads * p.n_tiles;
+    most = max(most, s.shared > 0 ? steps_up_to(s.shared) : 0);
+    s.total = s.pre_total + sum * per;
+    // what one of all workgroups gets, but no fewer than a join is worth (a segment of few spans is a long walk, one of many a long join:
+    // their sum is least around the root of its steps), and never more of them than a sequence may have
+    const int pieces = s.shared > 0 ? kMaxPieces / 2 : kMaxPieces;
+    const int root = __builtin_amdgcn_readfirstlane((int)(__builtin_amdgcn_sqrtf((float)most) * p.span_root + 0.5f * kWaves)) & -kWaves;
+    s.size = max(max(kWaves, quotient(s.total + p.n_groups - 1, p.n_groups)), max(root, (most + pieces - 3) / (pieces - 2)));
+    if (s.shared > 0) {
+        const int active = quotient(s.total + s.size - 1, s.size), eighth = (active + 7) / 8;  // (n_groups divides by eight)
+        group = group / 8 < eighth ? (group & 7) * eighth + group / 8 : 0x7fffffff;
+    }
+    s.b = s.first = s.len = 0;
+    const long long at = (long long)group * s.size;
+    s.begin = (int)min(at, (long long)s.total);
+    s.end = (int)min((long long)s.total, at + s.size);
+    if (s.begin >= s.total) return s;
+    // the first sequence that has a place from `begin` on
+    int before = s.pre_total, len = len0, ends = ends0;
+    for (int b0 = 0;;) {
+        const uint64_t past = __ballot(before + ends * per > max(s.begin, s.pre_total));
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            s.b = b0 + l;
+            s.len = __builtin_amdgcn_readlane(len, l);
+            s.first = before + (__builtin_amdgcn_readlane(ends, l) - Own(s.len, s.shared).places()) * per;
+            return s;
+        }
+        before += __builtin_amdgcn_readlane(ends, 63) * per;
+        b0 += 64;
+        if (b0 >= p.batch) return s;  // (a list of prefixes alone)
+        len = len_at(b0);
+        ends = lane_sums(places(len));
+    }
+}
+
+// ---- partials that another workgroup of the launch reads: device scope both ways, as in decode_cache.hip ---------------------
+constexpr int kScopeDevice = 16;  // sc1
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, kBufferFlags);
+}
+__device__ __forceinline__ void put4(__amdgpu_buffer_rsrc_t rs, uint32_t byte, f32x4_t v) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), rs, byte, 0, kScopeDevice);
+}
+__device__ __forceinline__ void put2(__amdgpu_buffer_rsrc_t rs, uint32_t byte, float a, float b) {
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(a), __float_as_uint(b)}, rs, byte, 0, kScopeDevice);
+}
+__device__ __forceinline__ f32x4_t get4(__amdgpu_buffer_rsrc_t rs, uint32_t byte) {
+    return __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, byte, 0, kScopeDevice));
+}
+__device__ __forceinline__ u32x2_t get2(__amdgpu_buffer_rsrc_t rs, uint32_t byte) { return __builtin_amdgcn_raw_buffer_load_b64(rs, byte, 0, kScopeDevice); }
+
+// The word through which the workgroups of a (sequence, kv head, piece of its heads) learn which of them is the last: (launch id | steps
+// done).  It lies in the caller's workspace, which holds anything: every workgroup makes sure, ahead of its own count, that the word
+// carries this launch's id.  The last one leaves 0 there, so that a recorded launch, which brings its id along on every replay,
+// finds none of its own counts.  Behind the word: where the sequence's own partials are, left by those that count its own steps.
+typedef unsigned long long word_t;
+constexpr int kWordPitch = 128;  // bytes: atomics on one line wait for each other
+constexpr int kCountBits = 24;
+constexpr word_t kCountMask = ((word_t)1 << kCountBits) - 1;
+struct UnitWord {
+    word_t* at;
+    word_t id, seen, got;
+    __device__ __forceinline__ bool ours(word_t x) const { return ((x ^ id) & ~kCountMask) == 0; }
+    // what is there, asked for ahead of the rows; it is replaced behind their requests, and whether that has held is looked at ahead of
+    // the count: neither is waited for by itself
+    __device__ __forceinline__ void request(void* word, word_t launch_id) {
+        at = (word_t*)word;
+        id = launch_id;
+        seen = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __device__ __forceinline__ void replace() {
+        got = seen;
+        __hip_atomic_compare_exchange_strong(at, &got, ours(seen) ? seen : id, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __device__ __forceinline__ void settle() {
+        while (got != seen && !ours(got)) {  // (fails only if another workgroup was first, whose id is this one, or with another launch's word)
+            seen = got;
+            replace();
+        }
+    }
+    // counts `steps` of `all`; true for the workgroup that completes them
+    __device__ __forceinline__ bool count(int steps, int all) {
+        const word_t old = __hip_atomic_fetch_add(at, (word_t)steps, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool last = (int)(old & kCountMask) + steps == all;
+        if (last) __hip_atomic_store(at, (word_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return last;
+    }
+};
+
+// ---- what a lane holds of 32 keys ------------------------------------------------------------------------------------------
+// As an operand of scores^T, keys are rows: lane (n, quad) has key n of either sixteen, and a quarter of each 32 dims.  As an operand of
+// out^T, dims are rows and keys the products' inner index: lane (n, quad) has dims by n of the eight keys 4 quad + {0..3}, 16 + those, in the
+// order in which scores^T leaves their weights.
+//
+// Up to four or eight query rows leave most of the sixteen columns of a product idle, and what is done a (row, key) would be done for all
+// sixteen: there a row has C = 4 or 2 columns, n, n + 16 / C, ..., each of which takes a C-th of a lane's eight keys, as in decode_cache.hip.
+template <int D>
+struct Keys {
+    uint32_t k[2][D / 8], v[8][D / 32];
+};
+// Byte offsets of a lane's requests from the first row of a sixteen.  kWhole: dim is D; else what lies behind a row's end is behind the
+// descriptor's too.
+constexpr uint32_t kNowhere = 0x80000000u;
+template <int D, bool kWhole>
+struct Lanes {
+    static constexpr int kK = kWhole ? 1 : D / 32, kV = kWhole || D < 256 ? 1 : 2;
+    uint32_t k[kK], v[4][kV];
+    __device__ __forceinline__ Lanes(int n, int quad, uint32_t row_bytes) {
+#pragma unroll
+        for (int c = 0; c < kK; c++) k[c] = kWhole || 64u * c + 16u * quad < row_bytes ? n * row_bytes + 64u * c + 16u * quad : kNowhere;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int i = 0; i < kV; i++) {
+                const uint32_t at = 256u * i + (D == 64 ? 8u : 16u) * n;
+                v[e][i] = kWhole || at < row_bytes ? (4u * quad + e) * row_bytes + at : kNowhere;
+            }
+    }
+};
+
+// A walk over the keys [lo, hi) of one kv head of one sequence's pages, the wave's steps first, first + kWaves, ... below `end`.
+template <int D, bool kWhole>
+struct Walk {
+    const PagedDecodeParams& p;
+    const int32_t* table;  // the sequence's
+    const int kvh, lo, hi, first, end, lane;
+    const uint32_t row_bytes;
+    int entry[2];  // lane i: the pages of the two sixteens of the wave's i-th step from the last refill on
+    __amdgpu_buffer_rsrc_t ks[2], vs[2];
+    uint32_t seen;  // of the step whose place was taken last: a bit for every key that is there
+
+    __device__ __forceinline__ Walk(const PagedDecodeParams& params, const int32_t* row, int kv_head, int from, int to, int step0, int step1, int l)
+        : p(params), table(row), kvh(kv_head), lo(from), hi(to), first(step0), end(step1), lane(l), row_bytes(2u * (uint32_t)(kWhole ? D : params.dim)) {}
+    __device__ __forceinline__ void refill(int t) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const long long row = (long long)(t + kWaves * lane) * kStep + 16 * h;
+            entry[h] = table[(int)min(row >> p.page_shift, (long long)p.table_pages - 1)];
+        }
+    }
+    // the descriptors of step t, the wave's i-th
+    __device__ __forceinline__ void place(int t, int i) {
+        if ((i & 63) == 0) refill(t);
+        seen = 0;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int page = __builtin_amdgcn_readlane(entry[h], i & 63), row = t * kStep + 16 * h;
+            const bool there = page >= 0 && page < p.n_pages;
+            const uint32_t in_page = (uint32_t)row & ((1u << p.page_shift) - 1);
+            const uint64_t at = ((((uint64_t)(there ? page : 0) * (uint32_t)p.kv_heads + (uint32_t)kvh) << p.page_shift) + in_page) * row_bytes;
+            const int rows = there ? min(max(hi - row, 0), 16) : 0, skip = min(max(lo - row, 0), 16);
+            ks[h] = rsrc_of((const char*)p.k_pages + at, (uint32_t)rows * row_bytes);
+            vs[h] = rsrc_of((const char*)p.v_pages + at, (uint32_t)rows * row_bytes);
+            seen |= (((1u << rows) - 1) & ~((1u << skip) - 1)) << (16 * h);
+        }
+    }
+    __device__ __forceinline__ void load_k(Keys<D>& x, const Lanes<D, kWhole>& at) const {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int c = 0; c < D / 32; c++)
+                *(u32x4_t*)(x.k[h] + 4 * c) = __builtin_amdgcn_raw_buffer_load_b128(ks[h], kWhole ? at.k[0] + 64u * c : at.k[kWhole ? 0 : c], 0, 0);
+    }
+    // kOnce: past the caches, rows that no other workgroup asks for
+    template <bool kOnce>
+    __device__ __forceinline__ void load_v(Keys<D>& x, const Lanes<D, kWhole>& at) const {
+        constexpr int kAux = kOnce ? 2 : 0;  // nt
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if constexpr (D == 64) {
+                *(u32x2_t*)x.v[e] = __builtin_amdgcn_raw_buffer_load_b64(vs[e / 4], at.v[e % 4][0], 0, kAux);
+            } else {
+#pragma unroll
+                for (int i = 0; i < D / 128; i++)
+                    *(u32x4_t*)(x.v[e] + 4 * i) = __builtin_amdgcn_raw_buffer_load_b128(vs[e / 4], kWhole ? at.v[e % 4][0] + 256u * i : at.v[e % 4][kWhole || D < 256 ? 0 : i], 0, kAux);
+            }
+        }
+    }
+};
+
+// What a lane has of its query row over the keys it has walked.
+template <int D>
+struct State {
+    float m, l;
+    f32x4_t o[D / 16];
+    __device__ __forceinline__ void reset() {
+        m = kNoMax;
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) o[i] = f32x4_t{0, 0, 0, 0};
+    }
+};
+
+// One step for NT tiles of sixteen query rows, whose operands q_of(tile, c) gives.  k_done is called behind the last use of K.
+template <int D, int C, int NT, typename QOf, typename KDone>
+__device__ __forceinline__ void step(State<D> (&st)[NT], Keys<D>& x, QOf q_of, KDone k_done, uint32_t seen, int cls, int quad, float scale_log2e) {
+    static_assert(C == 1 || NT == 1);
+    constexpr int kE = 8 / C;
+    float y[NT][kE];
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+        f32x4_t a[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+        for (int c = 0; c < D / 32; c++) {
+            const u32x4_t q = q_of(i, c);
+#pragma unroll
+            for (int h = 0; h < 2; h++) a[h] = mfma(*(const u32x4_t*)(x.k[h] + 4 * c), q, a[h]);
+        }
+        if constexpr (C == 1) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[i][e] = a[e / 4][e % 4];
+        } else if constexpr (C == 2) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[i][e] = cls ? a[1][e] : a[0][e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                // (of both sixteens first: two of one register group the compiler takes for an index into it, four selections)
+                const float a0 = cls & 2 ? a[1][e] : a[0][e], a2 = cls & 2 ? a[1][2 + e] : a[0][2 + e];
+                y[i][e] = cls & 1 ? a2 : a0;
+            }
+        }
+    }
+    // the lane's keys, of its eight slots; a key that is not there has no weight, and zeros in V, whatever lies there
+    auto place = [&](int e) __attribute__((always_inline)) { return C == 1 ? 16 * (e / 4) + e % 4 : C == 2 ? 16 * cls + e : 16 * (cls >> 1) + 2 * (cls & 1) + e; };
+    if (seen != ~0u) {
+        const uint32_t mine = seen >> (4 * quad);
+#pragma unroll
+        for (int e = 0; e < kE; e++) {
+            const bool hid = !(mine >> place(e) & 1);
+#pragma unroll
+            for (int i = 0; i < NT; i++) y[i][e] = hid ? neg_inf() : y[i][e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const bool hid = !(mine >> (16 * (e / 4) + e % 4) & 1);
+#pragma unroll
+            for (int w = 0; w < D / 32; w++) x.v[e][w] = hid ? 0u : x.v[e][w];
+        }
+    }
+    k_done();
+    u32x4_t w[NT];
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+        // The running maximum, common to the four lanes of a column.  It follows the scores only where they have risen by 8 in the exponent
+        // of two: up to there sums of weights in f32 and weights of 8 bits are as exact, and sums are scaled once or twice a span.
+        float top = y[i][0];
+#pragma unroll
+        for (int e = 1; e < kE; e++) top = fmaxf(top, y[i][e]);
+        top = quad_max(top);
+        if (__any((top - st[i].m) * scale_log2e > 8.0f)) {
+            const float m_new = fmaxf(st[i].m, top), alpha = __builtin_amdgcn_exp2f((st[i].m - m_new) * scale_log2e);
+            st[i].m = m_new;
+            st[i].l *= alpha;
+#pragma unroll
+            for (int d = 0; d < D / 16; d++) st[i].o[d] *= alpha;
+        }
+        float f[kE];
+#pragma unroll
+        for (int e = 0; e < kE; e++) {
+            f[e] = __builtin_amdgcn_exp2f((y[i][e] - st[i].m) * scale_log2e);
+            st[i].l += f[e];
+        }
+        // pairs of weights as the operand's words, zeros in the other columns' places
+#pragma unroll
+        for (int k = 0; k < kE / 2; k++) {
+            const uint32_t two = two_bf16(f[2 * k], f[2 * k + 1]);
+            if constexpr (C == 1) {
+                w[i][k] = two;
+            } else {
+#pragma unroll
+                for (int c = 0; c < C; c++) w[i][c * (kE / 2) + k] = cls == c ? two : 0u;
+            }
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < D / 16; d++) {  // dim n * (D / 16) + d; of 256, of the lower and of the upper 128 in turn
+        u32x4_t a;
+#pragma unroll
+        for (int i = 0; i < 4; i++) a[i] = __builtin_amdgcn_perm(x.v[2 * i + 1][d / 2], x.v[2 * i][d / 2], d & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int i = 0; i < NT; i++) st[i].o[d] = mfma(a, w[i], st[i].o[d]);
+    }
+}
+
+template <int D, int C, int NT, bool kWhole, bool kOnce, typename QOf>
+__device__ __forceinline__ void walk(State<D> (&st)[NT], Walk<D, kWhole>& at, const Lanes<D, kWhole>& lanes, QOf q_of, int cls, int quad, float scale_log2e) {
+    if (at.first >= at.end) return;
+    Keys<D> x;
+    int i = 0;
+    at.place(at.first, 0);
+    at.load_k(x, lanes);
+    at.template load_v<kOnce>(x, lanes);
+    for (int t = at.first; t < at.end; t += kWaves) {
+        const uint32_t seen = at.seen;
+        const bool more = t + kWaves < at.end;
+        step<D, C, NT>(st, x, q_of, [&]() __attribute__((always_inline)) {
+            if (more) {
+                at.place(t + kWaves, ++i);
+                at.load_k(x, lanes);
+            }
+        }, seen, cls, quad, scale_log2e);
+        if (more) at.template load_v<kOnce>(x, lanes);
+    }
+}
+
+// Tiles of sixteen query rows that a prefix's step serves.
+template <int D>
+constexpr int prefix_tiles() { return D == 256 ? 2 : 4; }
+
+template <int D, int C, bool kWhole, bool kShared>
+__global__ __launch_bounds__(64 * kWaves, kShared || D == 256 ? 1 : 2) void paged_decode_kernel(PagedDecodeParams p) {
+    constexpr int NT = 64 * kWaves, kPitch = D + 4, kR = 16 / C, kTiles = prefix_tiles<D>();
+    constexpr int kFold = kWaves * 16 * kPitch * 4, kFolds = kMaxPieces * 16 * 8 + NT * 16, kLds = std::max(kFold, kFolds);
+    constexpr int kQPitch = 2 * D + 16;  // bytes
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kLds];
+    __shared__ __attribute__((aligned(16))) unsigned char prefix_q[kShared ? 16 * kTiles * kQPitch : 16];
+    __shared__ float red_m[kWaves][16], red_l[kWaves][16], inv_l[16];
+    __shared__ int is_last[64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, quad = lane >> 4, cls = n / kR;
+    const int per = p.kv_heads * p.chunks, dim = kWhole ? D : p.dim;
+    int group = blockIdx.x;
+    const Span span = span_of<kShared>(p, group, lane);
+    // sequences without keys, dealt to the workgroups: rows of zeros
+    for (int b = blockIdx.x; b < p.batch; b += (int)gridDim.x)
+        if (b < 64 ? (span.empty >> b & 1) != 0 : len_of(p, b) == 0)
+            for (int i = tid; i < p.heads * (dim / 8); i += NT) *(u32x4_t*)(p.out + (size_t)b * p.heads * dim + 8 * i) = u32x4_t{0, 0, 0, 0};
+    if (span.begin >= span.total) return;
+    int at = span.begin, b = span.b, first = span.first, len = span.len;
+
+    const Lanes<D, kWhole> lanes(n, quad, 2u * (uint32_t)dim);
+    // slots of partials: of the prefix's, then of the sequences'.  A piece's is (workgroup + segment): along the list each further piece
+    // advances one or the other.
+    const uint32_t pre_slot = (uint32_t)(16 * kTiles) * (D + 2) * 4, own_slot = (uint32_t)p.rows * (D + 2) * 4;
+    const int pre_segments = p.kv_heads * p.n_tiles;
+    char* const pre_part = (char*)p.part;
+    char* const own_part = pre_part + (kShared ? (size_t)(p.n_groups + pre_segments) * pre_slot : 0);
+    float* const red = (float*)lds;  // [wave][row][kPitch]
+
+    // A tile's rows, folded over the columns and the waves of the workgroup: to_row(row, d, values of four dims, m, l).
+    auto fold = [&](State<D>& st, auto c_of, int rows, auto to_row, auto to_ml) __attribute__((always_inline)) {
+        constexpr int kC = decltype(c_of)::value, kRows = 16 / kC;
+        const float m = columns_max<kC>(st.m), f = __builtin_amdgcn_exp2f((st.m - m) * p.scale_log2e);
+        const float l = columns_sum<kC>(quad_sum(st.l) * f);
+        if (kC > 1)
+#pragma unroll
+            for (int i = 0; i < D / 16; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) st.o[i][e] = columns_sum<kC>(st.o[i][e] * f);
+        if (n < kRows && quad == 0) {
+            red_m[wave][n] = m;
+            red_l[wave][n] = l;
+        }
+        __syncthreads();
+        float m_wg = red_m[0][n % kRows], l_wg = 0.0f;
+#pragma unroll
+        for (int w = 1; w < kWaves; w++) m_wg = fmaxf(m_wg, red_m[w][n % kRows]);
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) l_wg += red_l[w][n % kRows] * __builtin_amdgcn_exp2f((red_m[w][n % kRows] - m_wg) * p.scale_log2e);
+        if (n < kRows) {
+            const float fw = __builtin_amdgcn_exp2f((m - m_wg) * p.scale_log2e);
+            float* row = red + (wave * kRows + n) * kPitch;
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) {  // eight dims in a row
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] = st.o[(8 * c + e) % (D / 16)][(8 * c + e) / (D / 16)] * fw;
+                float* dst = row + (D == 256 ? 128 * (c & 1) + 32 * quad + 8 * (c >> 1) : quad * (D / 4) + 8 * c);
+                *(f32x4_t*)dst = f32x4_t{y[0], y[1], y[2], y[3]};
+                *(f32x4_t*)(dst + 4) = f32x4_t{y[4], y[5], y[6], y[7]};
+            }
+            if (wave == 0 && quad == 0) {
+                inv_l[n] = l_wg == 0.0f ? 0.0f : 1.0f / l_wg;
+                if (n < rows) to_ml(n, m_wg, l_wg);
+            }
+        }
+        __syncthreads();
+        for (int i = tid; i < rows * (D / 4); i += NT) {
+            const int row = i / (D / 4), d = 4 * (i % (D / 4));
+            f32x4_t o = {0, 0, 0, 0};
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) o += *(const f32x4_t*)(red + (w * kRows + row) * kPitch + d);
+            to_row(row, d, o);
+        }
+        __syncthreads();
+    };
+    auto put_out = [&](int seq, int head, int d, f32x4_t o) __attribute__((always_inline)) {
+        if (kWhole || d < dim) *(u32x2_t*)(p.out + ((size_t)seq * p.heads + head) * dim + d) = u32x2_t{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
+    };
+    // All partials of `rows` heads from `head` on of sequence `seq`: n_pre of the prefix, rows of theirs from pre_row on, and n_own.
+    auto join = [&](int seq, int head, int rows, __amdgpu_buffer_rsrc_t pre, int n_pre, int pre_row, __amdgpu_buffer_rsrc_t own, int n_own) __attribute__((always_inline)) {
+        constexpr int kAhead = 8;
+        float* const wgt = (float*)lds;  // [pieces][16]
+        float* const wl = wgt + kMaxPieces * 16;
+        f32x4_t* const part = (f32x4_t*)(wl + kMaxPieces * 16);
+        const int pieces = n_pre + n_own, items = rows * (D / 4), sub_n = items >= NT ? 1 : NT / items;
+        const int x0 = sub_n == 1 ? tid : tid % items, sub = sub_n == 1 ? 0 : tid / items;
+        f32x4_t a[kAhead];
+        auto ask = [&](int i, int k0) __attribute__((always_inline)) {  // (row and element follow one another in a slot)
+            const uint32_t from = 16u * (uint32_t)min(i, items - 1);
+#pragma unroll
+            for (int e = 0; e < kAhead; e++) {
+                const int k = min(k0 + e * sub_n, pieces - 1);
+                a[e] = kShared && k < n_pre ? get4(pre, (uint32_t)k * pre_slot + (uint32_t)(pre_row * D * 4) + from) : get4(own, (uint32_t)(k - n_pre) * own_slot + from);
+            }
+        };
+        ask(x0, sub);
+        {
+            const int row = tid >> 4, col = tid & 15;  // sixteen lanes a row
+            const bool on = row < rows;
+            float top = kNoMax, sum = 0.0f;
+            for (int k = col; on && k < pieces; k += 16) {
+                const u32x2_t ml = kShared && k < n_pre ? get2(pre, (uint32_t)k * pre_slot + 4u * (uint32_t)(16 * kTiles * D + 2 * (pre_row + row)))
+                                                        : get2(own, (uint32_t)(k - n_pre) * own_slot + 4u * (uint32_t)(p.rows * D + 2 * row));
+                wgt[k * 16 + row] = __uint_as_float(ml[0]);
+                wl[k * 16 + row] = __uint_as_float(ml[1]);
+                top = fmaxf(top, __uint_as_float(ml[0]));
+            }
+            top = columns_max<16>(top);
+            for (int k = col; on && k < pieces; k += 16) {
+                const float fk = __builtin_amdgcn_exp2f((wgt[k * 16 + row] - top) * p.scale_log2e);
+                wgt[k * 16 + row] = fk;
+                sum += wl[k * 16 + row] * fk;
+            }
+            sum = columns_sum<16>(sum);
+            if (on && col == 0) inv_l[row] = sum == 0.0f ? 0.0f : 1.0f / sum;
+        }
+        __syncthreads();
+        for (int i0 = 0; i0 < items; i0 += NT) {
+            const int i = i0 + x0;
+            const bool on = i < items && sub < sub_n;
+            const int row = on ? i / (D / 4) : 0, d = 4 * (i % (D / 4));
+            f32x4_t o = {0, 0, 0, 0};
+            for (int k0 = sub; on && k0 < pieces; k0 += kAhead * sub_n) {
+                if (i0 || k0 != sub) ask(i, k0);
+#pragma unroll
+                for (int e = 0; e < kAhead; e++)
+                    if (k0 + e * sub_n < pieces) o += a[e] * wgt[(k0 + e * sub_n) * 16 + row];
+            }
+            if (sub_n > 1) {  // (one round)
+                part[tid] = o;
+                __syncthreads();
+                if (on && sub == 0)
+                    for (int e = 1; e < sub_n; e++) o += part[e * items + tid];
+            }
+            if (on && sub == 0) put_out(seq, head + row, d, o * inv_l[row]);
+        }
+        __syncthreads();
+    };
+    // where the prefix's partials for a kv head's tile are
+    auto pre_pieces = [&](int seg, int& w0) __attribute__((always_inline)) {
+        const int f = seg * span.pre_places;
+        w0 = quotient(f + kStart, span.size);
+        return quotient(f + span.pre_places - 1, span.size) - w0 + 1;
+    };
+    auto word_of = [&](int seq, int head_of_kv, int piece) { return p.words + (((size_t)seq * p.kv_heads + head_of_kv) * p.chunks + piece) * kWordPitch; };
+
+    while (at < span.end) {
+        if (kShared && at < span.pre_total) {
+            // ---- a piece of the prefix
+            const int seg = quotient(at, span.pre_places), seg_first = seg * span.pre_places;
+            const int t0 = max(at - seg_first - kStart, 0), t1 = min(span.pre_places, span.end - seg_first) - kStart;
+            at = min(seg_first + span.pre_places, span.end);
+            if (t1 <= 0) continue;  // (places alone)
+            const int kvh = quotient(seg, p.n_tiles), tile = seg - kvh * p.n_tiles;
+            int w0;
+            const int pieces = pre_pieces(seg, w0);
+            // the tile's units, (sequence, piece of the kv head's query heads): unit `tid` is this thread's to count
+            const int unit0 = tile * p.per_tile, units = min(p.per_tile, p.batch * p.chunks - unit0);
+            const int my_seq = (unit0 + tid) / p.chunks, my_piece = unit0 + tid - my_seq * p.chunks;
+            const int my_len = tid < units ? len_of(p, my_seq) : -1;
+            const bool mine = tid < units && my_len >= span.shared;
+            UnitWord word;
+            if (mine) word.request(word_of(my_seq, kvh, my_piece), p.launch_id);
+            // operands of q: row i of the tile is head i % rows of unit i / rows
+            const int group_rows = p.rows;
+            for (int i = tid; i < 16 * kTiles * (D / 8); i += NT) {
+                const int row = i / (D / 8), c = i % (D / 8), u = row / group_rows, r = row - u * group_rows;
+                const int seq = (unit0 + u) / p.chunks, h = (unit0 + u - seq * p.chunks) * group_rows + r;
+                u32x4_t q = {0, 0, 0, 0};
+                if (u < units && h < p.group && (kWhole || 8 * c < dim)) q = *(const u32x4_t*)(p.q + ((size_t)seq * p.heads + kvh * p.group + h) * dim + 8 * c);
+                *(u32x4_t*)(prefix_q + row * kQPitch + 16 * c) = q;
+            }
+            if (mine) word.replace();
+            __syncthreads();
+            State<D> st[kTiles];
+#pragma unroll
+            for (int i = 0; i < kTiles; i++) st[i].reset();
+            {
+                Walk<D, kWhole> w(p, p.page_table, kvh, 0, span.shared, t0 + wave, t1, lane);
+                walk<D, 1, kTiles, kWhole, false>(st, w, lanes, [&](int i, int c) __attribute__((always_inline)) {
+                    return *(const u32x4_t*)(prefix_q + (16 * i + n) * kQPitch + 64 * c + 16 * quad);
+                }, 0, quad, p.scale_log2e);
+            }
+            const __amdgpu_buffer_rsrc_t rs = rsrc_of(pre_part + ((size_t)w0 + seg) * pre_slot, (uint32_t)pieces * pre_slot);
+            const uint32_t to = (uint32_t)(group - w0) * pre_slot;
+#pragma unroll
+            for (int i = 0; i < kTiles; i++)
+                fold(st[i], std::integral_constant<int, 1>{}, 16,
+                     [&](int row, int d, f32x4_t o) __attribute__((always_inline)) { put4(rs, to + 4u * (uint32_t)((16 * i + row) * D + d), o); },
+                     [&](int row, float m, float l) __attribute__((always_inline)) { put2(rs, to + 4u * (uint32_t)(16 * kTiles * D + 2 * (16 * i + row)), m, l); });
+            if (mine) word.settle();
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (tid < 64) is_last[tid] = 0;
+            if (mine) is_last[tid] = word.count(t1 - t0, steps_up_to(span.shared) + Own(my_len, span.shared).steps()) ? 1 : 0;
+            __syncthreads();
+            for (int u = 0; u < units; u++) {
+                if (!is_last[u]) continue;
+                const int seq = (unit0 + u) / p.chunks, piece = unit0 + u - seq * p.chunks, head = piece * p.rows;
+                int own_n = 0, own_w0 = 0;
+                const int own_steps = Own(len_of(p, seq), span.shared).steps();
+                if (own_steps > 0) {
+                    const int* where = (const int*)(word_of(seq, kvh, piece) + 8);
+                    own_w0 = __hip_atomic_load(where, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    own_n = __hip_atomic_load(where + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    own_w0 = __builtin_amdgcn_readfirstlane(own_w0);
+                    own_n = __builtin_amdgcn_readfirstlane(own_n);
+                }
+                const size_t segment = (size_t)seq * per + (size_t)kvh * p.chunks + piece;
+                join(seq, kvh * p.group + head, min(p.rows, p.group - head), rs, pieces, u * p.rows, rsrc_of(own_part + ((size_t)own_w0 + segment) * own_slot, (uint32_t)own_n * own_slot), own_n);
+            }
+            continue;
+        }
+        // ---- a piece of a sequence's own keys
+        const Own own(len, span.shared);
+        const int places = own.places();
+        if (at >= first + places * per) {  // the next sequence
+            first += places * per;
+            b++;
+            len = len_of(p, b);
+            continue;
+        }
+        const int seg = quotient(at - first, places), seg_first = first + seg * places;
+        const int t0 = max(at - seg_first - kStart, 0), t1 = min(places, span.end - seg_first) - kStart;
+        at = min(seg_first + places, span.end);
+        if (t1 <= 0) continue;  // (places alone)
+        const int kvh = p.chunks == 1 ? seg : quotient(seg, p.chunks), piece = seg - kvh * p.chunks;
+        const int w0 = quotient(seg_first + kStart, span.size), pieces = quotient(seg_first + places - 1, span.size) - w0 + 1;
+        const size_t segment = (size_t)b * per + seg;
+        const bool alone = pieces == 1 && own.lo == 0;
+        const int head = piece * p.rows, rows = min(p.rows, p.group - head);  // of the kv head's query heads
+        const bool there = n % kR < rows;
+
+        UnitWord word;
+        if (!alone && tid == 0) word.request(word_of(b, kvh, piece), p.launch_id);
+        u32x4_t q[D / 32];
+        const uint16_t* q_row = p.q + ((size_t)b * p.heads + kvh * p.group + head + (there ? n % kR : 0)) * dim;
+#pragma unroll
+        for (int c = 0; c < D / 32; c++) {
+            q[c] = u32x4_t{0, 0, 0, 0};
+            if (there && (kWhole || 32 * c + 8 * quad < dim)) q[c] = *(const u32x4_t*)(q_row + 32 * c + 8 * quad);
+        }
+        if (!alone && tid == 0) word.replace();
+        State<D> st[1];
+        st[0].reset();
+        {
+            Walk<D, kWhole> w(p, p.page_table + (size_t)b * p.table_pages, kvh, own.lo, len, own.first() + t0 + wave, own.first() + t1, lane);
+            walk<D, C, 1, kWhole, true>(st, w, lanes, [&](int, int c) __attribute__((always_inline)) { return q[c]; }, cls, quad, p.scale_log2e);
+        }
+        const __amdgpu_buffer_rsrc_t rs = rsrc_of(own_part + ((size_t)w0 + segment) * own_slot, (uint32_t)pieces * own_slot);
+        const uint32_t to = (uint32_t)(group - w0) * own_slot;
+        fold(st[0], std::integral_constant<int, C>{}, rows,
+             [&](int row, int d, f32x4_t o) __attribute__((always_inline)) {
+                 if (alone) put_out(b, kvh * p.group + head + row, d, o * inv_l[row]);
+                 else put4(rs, to + 4u * (uint32_t)(row * D + d), o);
+             },
+             [&](int row, float m, float l) __attribute__((always_inline)) {
+                 if (!alone) put2(rs, to + 4u * (uint32_t)(p.rows * D + 2 * row), m, l);
+             });
+        if (alone) continue;
+        if (tid == 0) {
+            word.settle();
+            if (kShared && own.lo > 0) {  // for whoever joins them
+                int* where = (int*)(word_of(b, kvh, piece) + 8);
+                __hip_atomic_store(where, w0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(where + 1, pieces, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (tid == 0) is_last[0] = word.count(t1 - t0, own.steps() + (own.lo > 0 ? steps_up_to(span.shared) : 0)) ? 1 : 0;
+        __syncthreads();
+        if (is_last[0]) {
+            int n_pre = 0, pre_w0 = 0, pre_row = 0;
+            __amdgpu_buffer_rsrc_t pre = rs;
+            if (kShared && own.lo > 0) {
+                const int unit = b * p.chunks + piece, tile = quotient(unit, p.per_tile), pre_seg = kvh * p.n_tiles + tile;
+                n_pre = pre_pieces(pre_seg, pre_w0);
+                pre_row = (unit - tile * p.per_tile) * p.rows;
+                pre = rsrc_of(pre_part + ((size_t)pre_w0 + pre_seg) * pre_slot, (uint32_t)n_pre * pre_slot);
+            }
+            join(b, kvh * p.group + head, rows, pre, n_pre, pre_row, rs, pieces);
+        }
+        __syncthreads();
+    }
+}
+
+template <int D, bool kWhole, bool kShared>
+hipError_t launch_as(hipStream_t stream, const PagedDecodeParams& p) {
+    const dim3 grid(p.n_groups), block(64 * kWaves);
+    if (p.rows <= 4) hipLaunchKernelGGL((paged_decode_kernel<D, 4, kWhole, kShared>), grid, block, 0, stream, p);
+    else if (p.rows <= 8) hipLaunchKernelGGL((paged_decode_kernel<D, 2, kWhole, kShared>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((paged_decode_kernel<D, 1, kWhole, kShared>), grid, block, 0, stream, p);
+    return hipGetLastError();
+}
+template <int D>
+hipError_t launch_dim(hipStream_t stream, const PagedDecodeParams& p, bool shared) {
+    if (p.dim == D) return shared ? launch_as<D, true, true>(stream, p) : launch_as<D, true, false>(stream, p);
+    return shared ? launch_as<D, false, true>(stream, p) : launch_as<D, false, false>(stream, p);
+}
+
+// Workgroups a CU, each with a wave on every SIMD.
+constexpr int per_cu(int64_t dim, bool shared) { return shared || dim == 256 ? 1 : 2; }
+// Segments, steps and workgroups of a call at its longest, and what its workspace holds.
+struct Plan {
+    int64_t chunks, rows, per_tile, n_tiles, own_segments, pre_segments, places;
+    int dim, groups;  // dim: the kernel's
+    size_t part_bytes, word_bytes;
+};
+Plan plan_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_t max_len) {
+    Plan a{};
+    const int64_t group = heads / kv_heads;
+    a.dim = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
+    a.chunks = (group + 15) / 16;
+    a.rows = (group + a.chunks - 1) / a.chunks;
+    const int64_t tile_rows = a.dim == 256 ? 32 : 64;
+    a.per_tile = tile_rows / a.rows;
+    a.n_tiles = (batch * a.chunks + a.per_tile - 1) / a.per_tile;
+    a.own_segments = batch * kv_heads * a.chunks;
+    a.pre_segments = kv_heads * a.n_tiles;
+    const int64_t steps = max_len / kStep + 2 + kStart;
+    a.places = (a.own_segments + a.pre_segments) * steps;
+    a.groups = (int)std::min<int64_t>(2 * kCus, std::max<int64_t>((a.places + kWaves - 1) / kWaves, 1));
+    a.groups = (a.groups + 7) / 8 * 8;
+    auto round = [](size_t x) { return (x + 255) / 256 * 256; };
+    a.part_bytes = round((size_t)(a.groups + a.pre_segments) * (size_t)tile_rows * (size_t)(a.dim + 2) * 4 + (size_t)(a.groups + a.own_segments) * (size_t)a.rows * (size_t)(a.dim + 2) * 4);
+    a.word_bytes = (size_t)a.own_segments * kWordPitch;
+    return a;
+}
+static_assert(prefix_tiles<64>() == 4 && prefix_tiles<128>() == 4 && prefix_tiles<256>() == 2, "the plan's rows of a tile");
+
+}  // namespace
+
+}  // namespace rt
+
+using namespace rt;
+
+RT_API size_t rt_gqa_decode_paged_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t page_size, int32_t table_pages) {
+    if (batch <= 0 || n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || !cache_paged_dim(head_dim) || !cache_page_size(page_size) || table_pages < 0) return 0;
+    const Plan a = plan_of(batch, n_heads, n_kv, head_dim, (int64_t)table_pages * page_size);
+    return a.part_bytes + a.word_bytes;
+}
+
+RT_API int rt_gqa_decode_paged_bf16(void* stream, const void* q, const void* k_pages, const void* v_pages, void* out, const int32_t* page_table,
+                                    const int32_t* kv_lens, const int32_t* shared_lens, int32_t shared_len, int32_t batch, int32_t n_heads,
+                                    int32_t n_kv, int32_t head_dim, int32_t n_pages, int32_t page_size, int32_t table_pages,
+                                    void* workspace, size_t workspace_bytes, rt_err_detail* err) {
+    clear_err(err);
+    if (batch < 0 || n_heads < 0 || n_kv < 0 || head_dim < 0 || n_pages < 0 || table_pages < 0) return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "negative dimension");
+    if (n_kv == 0 || n_heads % n_kv != 0)
+        return fail(err, RT_ERR_HEAD_COUNT_MISMATCH, -1, (uint64_t)n_heads, (uint64_t)n_kv, "n_heads not divisible by n_kv");
+    if (head_dim == 0) return fail(err, RT_ERR_ZERO_DIM, -1, 0, 0, "head_dim must be > 0");
+    if (!cache_paged_dim(head_dim)) return fail(err, RT_ERR_UNSUPPORTED, -1, 256, (uint64_t)head_dim, "pages have head_dim up to 256, a multiple of 16");
+    if (!cache_page_size(page_size)) return fail(err, RT_ERR_UNSUPPORTED, -1, kPageMax, (uint64_t)(int64_t)page_size, "page_size must be a power of two, 16 to 1024");
+    const int64_t max_len = (int64_t)table_pages * page_size;
+    if (!shared_lens && (shared_len < 0 || shared_len > max_len))
+        return fail(err, RT_ERR_KV_OVERFLOW, -1, (uint64_t)max_len, (uint64_t)(int64_t)shared_len, "a prefix behind the page table");
+    if (batch == 0 || n_heads == 0) return RT_OK;
+    const Plan a = plan_of(batch, n_heads, n_kv, head_dim, max_len);
+    if (batch > 65535 || n_heads > 65535 || max_len > (1 << 28) || a.places > 0x7fffffffll - (1 << 20))
+        return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "shape too large for the launch grid");
+    if (!q || !out || !kv_lens || (max_len > 0 && (!page_table || (n_pages > 0 && (!k_pages || !v_pages))))) return fail(err, RT_ERR_NULL_POINTER, -1, 0, 0, "NULL buffer");
+    if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out) & 15) return fail(err, RT_ERR_UNSUPPORTED, -1, 16, 0, "q, out and the pages must be 16-byte aligned");
+    const size_t need = a.part_bytes + a.word_bytes;
+    if (!workspace || workspace_bytes < need)
+        return fail(err, RT_ERR_WORKSPACE_TOO_SMALL, -1, need, workspace ? workspace_bytes : 0, "workspace too small");
+    if ((uintptr_t)workspace & 15) return fail(err, RT_ERR_WORKSPACE_TOO_SMALL, -1, 16, (uint64_t)((uintptr_t)workspace & 15), "workspace must be 16-byte aligned");
+    int rc = ensure_device(err);
+    if (rc) return rc;
+    PagedDecodeParams p{};
+    p.q = (const uint16_t*)q;
+    p.k_pages = (const uint16_t*)k_pages;
+    p.v_pages = (const uint16_t*)v_pages;
+    p.out = (uint16_t*)out;
+    p.page_table = page_table;
+    p.kv_lens = kv_lens;
+    p.shared_lens = shared_lens;
+    p.shared_len = shared_len;
+    p.batch = batch;
+    p.heads = n_heads;
+    p.kv_heads = n_kv;
+    p.dim = head_dim;
+    p.n_pages = n_pages;
+    p.table_pages = table_pages;
+    p.page_shift = __builtin_ctz((unsigned)page_size);
+    p.max_len = (int)max_len;
+    p.group = n_heads / n_kv;
+    p.chunks = (int)a.chunks;
+    p.rows = (int)a.rows;
+    p.per_tile = (int)a.per_tile;
+    p.n_tiles = (int)a.n_tiles;
+    p.span_root = a.rows <= 4 ? 0.66f : 1.0f;
+    p.scale_log2e = (1.0f / sqrtf((float)head_dim)) * kLog2eHost;
+    p.part = (float*)workspace;
+    p.words = (unsigned char*)workspace + a.part_bytes;
+    p.launch_id = next_launch_id() << 16;  // (its low 24 bits zero)
+    const bool shared = shared_lens || shared_len > 0;
+    p.n_groups = std::min(a.groups, kCus * per_cu(a.dim, shared));
+    const hipStream_t s = (hipStream_t)stream;
+    HIP_TRY(a.dim == 64 ? launch_dim<64>(s, p, shared) : a.dim == 128 ? launch_dim<128>(s, p, shared) : launch_dim<256>(s, p, shared), "paged_decode launch");
+    return RT_OK;
+}

@@ -26,6 +26,7 @@
 #include "rt_common.hpp"
 #include "rt_kernels.hpp"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace rt {
@@ -142,12 +143,65 @@ __device__ __forceinline__ TilePlace t_place_by_length(const int32_t* lens, int 
     return TilePlace{b, tile, __builtin_amdgcn_readlane(len, b)};
 }
 
+// Where a workgroup works that takes the `pos`-th query tile of sequences packed one behind the other: starts[b] .. starts[b + 1] are the
+// tokens of sequence b (read as ascending and within the tokens there are, whatever they hold).  Of up to 64 sequences the tiles are
+// ordered by their number downwards, which is their cost: the highest number at which no more than `pos` tiles have been passed by is found
+// bit by bit, a sum over the lanes a bit.  Of more, sequence by sequence, each from its last tile on.  b < 0: there is no such tile.
+struct PackedPlace {
+    int b, tile, first, len;
+};
+__device__ __forceinline__ int t_lane_sums(int x) {  // up to and with this lane
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return x;
+}
+__device__ __forceinline__ PackedPlace t_place_packed(const int32_t* starts, int batch, int tokens, int pos, int lane) {
+    for (int b0 = 0; b0 < batch; b0 += 64) {
+        const bool on = b0 + lane < batch;
+        const int from = on ? starts[b0 + lane] : 0, to = on ? starts[b0 + lane + 1] : 0;
+        const int first = min(max(from, 0), tokens), len = min(max(to, first), tokens) - first, n = (len + TROWS - 1) / TROWS;
+        const int ends = t_lane_sums(n), all = __builtin_amdgcn_readlane(ends, 63);
+        if (pos >= all) {
+            pos -= all;
+            continue;
+        }
+        uint64_t has;
+        int at = pos, tile = -1;
+        if (batch <= 64) {
+            // tiles numbered `number` or more, of all sequences: the highest number of which there are more than `pos`
+            auto from_number = [&](int number) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(t_lane_sums(max(n - number, 0)), 63); };
+            int number = 0, passed = 0;  // (pos < all: number 0 is one)
+            for (int bit = 1 << (31 - __builtin_clz(__builtin_amdgcn_readfirstlane(all))); bit; bit >>= 1)
+                if (from_number(number + bit) > pos) number += bit;
+            passed = from_number(number + 1);
+            has = __ballot(n > number);
+            at = pos - passed;
+            tile = number;
+        } else {
+            has = __ballot(ends > pos);
+            at = 0;
+        }
+        const int below = __builtin_amdgcn_mbcnt_hi((uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0u));
+        const uint64_t one = has & __ballot(below == at);
+        const int l = one ? __builtin_ctzll(one) : 0;
+        if (tile < 0) tile = __builtin_amdgcn_readlane(ends, l) - 1 - pos;
+        return PackedPlace{b0 + l, tile, __builtin_amdgcn_readlane(first, l), __builtin_amdgcn_readlane(len, l)};
+    }
+    return PackedPlace{-1, 0, 0, 0};
+}
+
 // How K/V tiles come into LDS: through registers, or straight there with rows of DP columns or with rows of fewer.
 enum TileWay : int { kTilesRegs = 0, kTilesDirect = 1, kTilesDirectPart = 2 };
 
 // MODE: kMaskNone, kMaskCausal, kMaskPadding.  BIAS: an additive f32 score bias is applied (then MODE is kMaskNone).
 // PACKED: query rows run over (position, head of the GQA group) (then MODE is kMaskCausal and there is no bias).
 // The grid is (heads or kv heads, batch, query tiles): no division stands between a workgroup and its first load.
+// kMaskPacked: causal, sequences one behind the other; the grid is (heads, places in the list of all sequences' query tiles), and the
+// sequence's first row takes the place of the batch stride.
 //
 // The key walk of a wave is a software pipeline over 32-key items, one step per item j:
 //
@@ -206,7 +260,8 @@ __global__ __launch_bounds__(HALVES ? 512 : TileCfg<DP>::THREADS, HALVES ? 2 : B
     constexpr int CH = DP / 8;         // 16-byte chunks per (padded) row
     constexpr int CHUNKS = KT * CH;    // chunks of one matrix's tile
     constexpr int NL = (CHUNKS + TTHREADS - 1) / TTHREADS;  // chunks a thread moves per matrix per tile
-    constexpr bool kCausal = MODE == kMaskCausal;
+    constexpr bool kSeqs = MODE == kMaskPacked;
+    constexpr bool kCausal = MODE == kMaskCausal || kSeqs;
     constexpr int PF = Cfg::PF;        // register sets of tiles in flight behind the two LDS stages
     static_assert(2 * DT == KS, "one P.V matrix instruction per score matrix instruction");
     // Through registers, head dims above 128 do not have those for two score tiles and their operands in flight beside the tiles'
@@ -251,7 +306,7 @@ __global__ __launch_bounds__(HALVES ? 512 : TileCfg<DP>::THREADS, HALVES ? 2 : B
     // ((batch, head) pairs, or (batch, kv head) when rows are packed) divide by 8, all query tiles of a unit land on
     // one XCD and share K and V through its L2.
     const int G = PACKED ? p.pack : 1;  // heads per packed row block (1: rows are positions of one head)
-    const int rows_total = p.seq_q * G;
+    int rows_total = p.seq_q * G;
     // The heads of a GQA group follow one another at a distance of kv_heads in the grid, so that a group lands on one XCD
     // (or on those its kv heads leave it) and shares its keys through that L2: grid position x is head x / kv_heads of
     // group x % kv_heads (kv_magic = 2^32 / kv_heads + 1, exact below 2^16 heads; 0 where every head has its own keys).
@@ -264,7 +319,7 @@ __global__ __launch_bounds__(HALVES ? 512 : TileCfg<DP>::THREADS, HALVES ? 2 : B
     // all sequences' query tiles by their number, which is their cost: the last tile of the longest sequence first, the tiles
     // of padded rows only last.  Ranked within their own sequence, the second and third tile of the longest one waited behind
     // first tiles of short ones.
-    constexpr bool kByLength = kCausal && !PACKED && !SPLIT && !WIN;
+    constexpr bool kByLength = MODE == kMaskCausal && !PACKED && !SPLIT && !WIN;
     TilePlace place{-1, 0, 0};
     // (what the first requests need of the arguments is loaded ahead of the branch, not once more behind it)
     if (kByLength) asm volatile("" ::"s"(p.k), "s"(p.v), "s"(p.lkv.batch_stride), "s"(p.lkv.head_stride), "s"(p.lkv.row_pitch), "s"(p.seq_kv), "s"(p.dim));
@@ -272,11 +327,20 @@ __global__ __launch_bounds__(HALVES ? 512 : TileCfg<DP>::THREADS, HALVES ? 2 : B
         place = t_place_by_length(p.q_lens, (int)gridDim.y, p.seq_q, (int)(blockIdx.y + gridDim.y * blockIdx.z), lane);
         b = place.b;
     }
+    PackedPlace seq{0, 0, 0, 0};
+    if constexpr (kSeqs) {
+        seq = t_place_packed(p.starts, p.batch, p.seq_q, (int)(blockIdx.y + gridDim.y * blockIdx.z), lane);
+        if (seq.b < 0) return;
+        b = seq.b;
+        rows_total = seq.len;
+    }
+    // where the sequence's row 0 lies in a tensor, of head 0
+    auto base_of = [&](const TensorLayout& l) __attribute__((always_inline)) { return kSeqs ? (size_t)seq.first * (size_t)l.row_pitch : (size_t)b * l.batch_stride; };
     const int h0 = PACKED ? hx * G : hx;  // head of a row with g = 0
     const int D = p.dim;
 
-    const uint16_t* __restrict__ Kg = p.k + (size_t)b * p.lkv.batch_stride + (size_t)kvh * p.lkv.head_stride;
-    const uint16_t* __restrict__ Vg = p.v + (size_t)b * p.lkv.batch_stride + (size_t)kvh * p.lkv.head_stride;
+    const uint16_t* __restrict__ Kg = p.k + base_of(p.lkv) + (size_t)kvh * p.lkv.head_stride;
+    const uint16_t* __restrict__ Vg = p.v + base_of(p.lkv) + (size_t)kvh * p.lkv.head_stride;
 
     // ---- tile movement: chunk c = tid + TTHREADS n of a tile is (row c / CH, 16-byte chunk c % CH).  A tile
     // travels global -> registers -> LDS.  LDS holds two stages of each matrix; PF register sets per matrix hold
@@ -353,7 +417,7 @@ __global__ __launch_bounds__(HALVES ? 512 : TileCfg<DP>::THREADS, HALVES ? 2 : B
     // once the length is known, those of K are masked in the score tile whatever they hold.  (A span of the keys
     // starts where the sequence's own length puts it: its requests wait for the lengths.)
     const uint32_t tile_bytes_g = (uint32_t)KT * kv_pitch * 2u;  // from a tile's first row to the next tile's, in memory
-    if (!SPLIT && !WIN && !HALVES) {
+    if (!SPLIT && !WIN && !HALVES && !kSeqs) {
         const uint32_t all_bytes = p.seq_kv > 0 ? ((uint32_t)(p.seq_kv - 1) * kv_pitch + (uint32_t)D) * 2u : 0u;
         if constexpr (DIRECT) {
             const u32x4_t Kall = make_rsrc(Kg, all_bytes), Vall = make_rsrc(Vg, all_bytes);
@@ -386,9 +450,9 @@ __global__ __launch_bounds__(HALVES ? 512 : TileCfg<DP>::THREADS, HALVES ? 2 : B
     auto len_at = [](const int32_t* a, int i) __attribute__((always_inline)) {
         return ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)a)[i];
     };
-    const int q_len_raw = p.q_lens ? (kByLength && place.b >= 0 ? place.len : len_at(p.q_lens, b)) : p.seq_q;
+    const int q_len_raw = kSeqs ? seq.len : p.q_lens ? (kByLength && place.b >= 0 ? place.len : len_at(p.q_lens, b)) : p.seq_q;
     // (a padded batch of self-attention hands over one array for both: one dependent load instead of two in a row)
-    const int kv_len_raw = p.kv_lens ? (p.kv_lens == p.q_lens ? q_len_raw : len_at(p.kv_lens, b)) : p.seq_kv;
+    const int kv_len_raw = kSeqs ? seq.len : p.kv_lens ? (p.kv_lens == p.q_lens ? q_len_raw : len_at(p.kv_lens, b)) : p.seq_kv;
     const int n_q = min(max(q_len_raw, 0), p.seq_q);  // valid query positions
     int n_keys = min(max(kv_len_raw, 0), p.seq_kv);  // keys that exist
     int qtile = SPLIT ? zz / p.n_splits : zz;
@@ -403,11 +467,12 @@ __global__ __launch_bounds__(HALVES ? 512 : TileCfg<DP>::THREADS, HALVES ? 2 : B
         qtile = rank < n_qt ? n_qt - 1 - rank : rank;
         if (kByLength && place.b >= 0) qtile = place.qtile;
     }
+    if (kSeqs) qtile = seq.tile;
     const int q0 = qtile * TROWS;
     // which 32 query rows of the tile a wave owns.  Wave w runs on SIMD w % 4, and under a causal mask the rows at
     // the end of a tile see more keys than those at its start: the assignment rotates from workgroup to workgroup
     // so that no SIMD collects the long rows of every tile.
-    const int wq = (wave + hx + b + (int)blockIdx.z) & 3;
+    const int wq = (wave + hx + b + (kSeqs ? qtile : (int)blockIdx.z)) & 3;
     int off = n_keys - n_q;  // causal: the last valid query sees every key
 
     // keys the workgroup walks
@@ -483,11 +548,11 @@ __global__ __launch_bounds__(HALVES ? 512 : TileCfg<DP>::THREADS, HALVES ? 2 : B
     const __amdgpu_buffer_rsrc_t Kbuf = __builtin_amdgcn_make_buffer_rsrc((void*)Kg, 0, slab_bytes, kBufferFlags);
     const __amdgpu_buffer_rsrc_t Vbuf = __builtin_amdgcn_make_buffer_rsrc((void*)Vg, 0, slab_bytes, kBufferFlags);
     const u32x4_t Kd = make_rsrc(Kg, slab_bytes), Vd = make_rsrc(Vg, slab_bytes);  // (DIRECT: the same descriptors as scalars)
-    if (DIRECT && (SPLIT || WIN || HALVES)) {
+    if (DIRECT && (SPLIT || WIN || HALVES || kSeqs)) {
         dl_tile(Kd, dl_k, dl_k_on, 0u, 0u);
         dl_tile(Vd, dl_v, dl_v_on, 0u, 2u * STAGE_B);
         dl_tile(Kd, dl_k, dl_k_on, tile_bytes_g, STAGE_B);
-    } else if (SPLIT || WIN) {  // tile 0 (K and V) and K of tile 1 of the span / of the window
+    } else if (SPLIT || WIN || kSeqs) {  // tile 0 (K and V) and K of tile 1 of the span / of the window
 #pragma unroll
         for (int n = 0; n < NL; n++) {
             kreg[0][n] = __builtin_amdgcn_raw_buffer_load_b128(Kbuf, ld_off[n], 0, 0);
@@ -593,7 +658,7 @@ __global__ __launch_bounds__(HALVES ? 512 : TileCfg<DP>::THREADS, HALVES ? 2 : B
         // (the query row is read without a test: a row past the tensor reads the tensor's last row)
         const int r_q = min(r, rows_total - 1);
         const int s_q = G > 1 ? r_q / G : r_q;
-        const size_t q_off = (size_t)b * p.lq.batch_stride + (size_t)(h0 + (r_q - s_q * G)) * p.lq.head_stride + (size_t)s_q * p.lq.row_pitch;
+        const size_t q_off = base_of(p.lq) + (size_t)(h0 + (r_q - s_q * G)) * p.lq.head_stride + (size_t)s_q * p.lq.row_pitch;
 
         // BIAS (scores = (q . k) * scale + bias, crates/rustorch-nn/src/attention.rs:378-392, kept in the natural domain so
         // that a bias of -1e4 weighs as it does in the reference): f32 rows of seq_kv per (batch, head), or one matrix for
@@ -664,7 +729,7 @@ __global__ __launch_bounds__(HALVES ? 512 : TileCfg<DP>::THREADS, HALVES ? 2 : B
             const int r_first = q0 + 32 * wq, n_rows = max(min(32, rows_total - r_first), 0);
             const uint32_t q_pitch = (uint32_t)p.lq.row_pitch;
             const bool many = WIN && (uint64_t)gridDim.x * gridDim.y * gridDim.z > (uint64_t)p.n_cus * Cfg::OCC_DIRECT;
-            const u32x4_t Qd = make_rsrc(p.q + (size_t)b * p.lq.batch_stride + (size_t)h0 * p.lq.head_stride + (size_t)min(r_first, rows_total - 1) * q_pitch,
+            const u32x4_t Qd = make_rsrc(p.q + base_of(p.lq) + (size_t)h0 * p.lq.head_stride + (size_t)min(r_first, rows_total - 1) * q_pitch,
                                          n_rows > 0 ? ((uint32_t)(n_rows - 1) * q_pitch + (uint32_t)D) * 2u : 0u);
 #pragma unroll
             for (int n = 0; n < Lds::Q_REQUESTS; n++) {
@@ -1355,7 +1420,7 @@ __global__ __launch_bounds__(HALVES ? 512 : TileCfg<DP>::THREADS, HALVES ? 2 : B
         constexpr int RS = 64 / CH;  // rows per store instruction
         const int row0 = (int)((unsigned)lane / (unsigned)CH), ch = (int)((unsigned)lane % (unsigned)CH);
         const int rr0 = q0 + 32 * wq + row0;
-        uint16_t* dst = p.out + (size_t)b * p.lo.batch_stride + (size_t)h0 * p.lo.head_stride + (size_t)rr0 * p.lo.row_pitch + 8 * ch;
+        uint16_t* dst = p.out + base_of(p.lo) + (size_t)h0 * p.lo.head_stride + (size_t)rr0 * p.lo.row_pitch + 8 * ch;
         const size_t step = (size_t)RS * (size_t)p.lo.row_pitch;
         const uint16_t* src = obuf + row0 * LDK + 8 * ch;
         const bool col_ok = 8 * ch < D;
@@ -1383,7 +1448,7 @@ __global__ __launch_bounds__(HALVES ? 512 : TileCfg<DP>::THREADS, HALVES ? 2 : B
             u32x4_t val = {f2, f2, f2, f2};
             if (n_loop > 0) val = *(const u32x4_t*)(obuf + row * LDK + 8 * ch);
             if (rr < rows_total && 8 * ch < D) {
-                uint16_t* dst = p.out + (size_t)b * p.lo.batch_stride + (size_t)(h0 + gg) * p.lo.head_stride +
+                uint16_t* dst = p.out + base_of(p.lo) + (size_t)(h0 + gg) * p.lo.head_stride +
                                 (size_t)sp * p.lo.row_pitch + 8 * ch;
                 store_row(dst, val);
             }
@@ -1984,7 +2049,7 @@ __global__ __launch_bounds__(256, 2) void flash_wide_bf16_kernel(FlashTileParams
 // stores, 2 32/8 1501 128 took 45.9 for 45.6, small calls with a branch a store 2 to 4 % longer.  Above head dim 128 without the choice: plainly
 // under a window (4 40/8 2653 256 window 476 425 us, past the caches 437), past the caches otherwise (1 8/2 1024 256 46.9 -> 46.7).
 static bool out_goes_past(const FlashTileParams& p) {
-    const double written = 2.0 * p.batch * p.heads * (double)p.seq_q * p.dim;
+    const double written = 2.0 * (p.mask == kMaskPacked ? 1 : p.batch) * p.heads * (double)p.seq_q * p.dim;
     return written > 6.0 * (1 << 20);
 }
 
@@ -2030,6 +2095,7 @@ hipError_t launch_tiles(hipStream_t stream, const FlashTileParams& p, dim3 grid)
     }
     if (p.mask == kMaskNone) return launch_one<DP, kMaskNone, false, false, false, false, TILES>(stream, p, grid);
     if (p.mask == kMaskCausal) return launch_one<DP, kMaskCausal, false, false, false, false, TILES>(stream, p, grid);
+    if (p.mask == kMaskPacked) return launch_one<DP, kMaskPacked, false, false, false, false, TILES>(stream, p, grid);
     return hipErrorInvalidValue;
 }
 // Two halves of the walk (head dims 64 and 128 exactly, up to 32, and 65 to 96): where every workgroup has a CU to itself and
@@ -2042,6 +2108,7 @@ template <int DP, int TILES>
 hipError_t launch_halves(hipStream_t stream, const FlashTileParams& p, dim3 grid) {
     if (p.bias) return launch_one<DP, kMaskNone, true, false, false, false, TILES, true>(stream, p, grid);
     if (p.mask == kMaskNone) return launch_one<DP, kMaskNone, false, false, false, false, TILES, true>(stream, p, grid);
+    if (p.mask == kMaskPacked) return launch_one<DP, kMaskPacked, false, false, false, false, TILES, true>(stream, p, grid);
     return launch_one<DP, kMaskCausal, false, false, false, false, TILES, true>(stream, p, grid);
 }
 // Up to 1.9 causal workgroups a CU: the long tiles are dispatched first, so that a long walk in halves and a short one behind
@@ -2058,6 +2125,7 @@ hipError_t launch_halves(hipStream_t stream, const FlashTileParams& p, dim3 grid
 static bool takes_halves(const FlashTileParams& p, dim3 grid) {
     if (p.pack != 1 || p.decode_rows || p.window != 0 || p.mask == kMaskPadding || p.seq_kv < (p.dim <= 64 ? kHalvesFrom64 : kHalvesFrom)) return false;
     const unsigned long long units = (unsigned long long)grid.x * grid.y, n = units * grid.z, n_cus = (unsigned long long)p.n_cus;
+    if (p.mask == kMaskPacked) return n <= n_cus && flash_tile_bf16_packed_len(p) >= (p.dim <= 64 ? kHalvesFrom64 : kHalvesFrom);
     if (n <= n_cus) return true;
     if (p.mask != kMaskCausal || 10 * n > 19 * n_cus) return false;
     if (p.dim > 64) return grid.z >= 18 || (grid.z >= 11 && units % 8 == 0 && 8 * units <= n_cus && 4 * n <= 7 * n_cus);
@@ -2200,10 +2268,16 @@ hipError_t launch_flash_tile_bf16(hipStream_t stream, const FlashTileParams& par
     if (p.n_splits > 1 && ((long long)p.batch * p.kv_heads > 65535 || (rows + 31) / 32 > 65535 || rows * (long long)p.pack >= 1ll << 32 ||
                            (long long)p.batch * p.kv_heads * p.kv_heads >= 1ll << 32 || (long long)p.n_splits * p.dim >= 1ll << 25))
         return hipErrorInvalidValue;
-    if (p.batch > 65535 || n_qtiles * p.n_splits > 65535 || heads_u > 65535 || p.group < 1) return hipErrorInvalidValue;  // grid limits
+    if (p.batch > 65535 || heads_u > 65535 || p.group < 1) return hipErrorInvalidValue;  // grid limits
+    // (packed sequences: a place for every tile there can be, whose rows are 128 each but for a sequence's last)
+    const long long places = p.seq_q / TROWS + std::min<long long>(p.batch, p.seq_q), deep = (places + 65534) / 65535;
+    if (p.mask != kMaskPacked && n_qtiles * p.n_splits > 65535) return hipErrorInvalidValue;
+    if (p.mask == kMaskPacked && (!p.starts || p.seq_q != p.seq_kv || p.pack > 1 || p.decode_rows || p.bias || p.window || p.n_splits > 1 || p.q_lens || p.kv_lens || deep > 65535))
+        return hipErrorInvalidValue;
     set_grid_order(p, n_qtiles * p.n_splits);
     if (tiles_by_length(p, n_qtiles)) p.n_qtiles = -1;
     dim3 grid((unsigned)heads_u, (unsigned)p.batch, (unsigned)(n_qtiles * p.n_splits));
+    if (p.mask == kMaskPacked) grid = dim3((unsigned)heads_u, (unsigned)((places + deep - 1) / deep), (unsigned)deep);
     if (p.dim <= 32) return launch_dp<32>(stream, p, grid);
     if (p.dim <= 64) return launch_dp<64>(stream, p, grid);
     if (p.dim <= 96) return launch_dp<96>(stream, p, grid);

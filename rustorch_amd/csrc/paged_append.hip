@@ -1,0 +1,331 @@
+// New rows of packed tokens into a cache in pages: per-head RMSNorm of q and k, half-split RoPE with one position a token or one on each
+// of several axes, and the append, as in prepare.hip (steps 2a, 2b, 3 of LlamaModel::decode_step,
+// crates/rustorch-llm/src/model.rs:575-636), where the tokens of all sequences follow one another ([tokens, heads, dim], what the
+// projections leave) and a row's place is looked up in its sequence's page table.
+//
+//   x' = gamma x / sqrt(mean x^2 + eps)        pair i (dims i and i + D / 2) turned by the angle table[position on the pair's axis, i]
+//
+// The f32 arithmetic is the reference's, rounding for rounding (this file too is compiled without contraction): the sum of squares
+// runs in index order, so that a row has the bits that prepare.hip gives it.
+//
+// A wave takes a token: its sequence, place and angles are found once, as scalars and a lane's registers, and serve all of the token's
+// rows, which follow one another in memory.  D / 16 lanes a row (4, 8 or 16 of them set aside): lane j has the dims 8 j .. 8 j + 7 and
+// their partners D / 2 on, 16 bytes a request.  The sum of squares goes from lane to lane within registers: at stage i lane i's value is
+// that of dims 0 .. 8 i + 7, added one by one, and moves on; what the other lanes add meanwhile is thrown away.
+#include <algorithm>
+
+#include "cache_paged.hpp"
+#include "rt_common.hpp"
+#include "rt_host.hpp"
+
+#pragma clang fp contract(off)
+
+namespace rt {
+
+namespace {
+
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // 16 bytes from any word
+
+__device__ __forceinline__ float from_lane_below(float x) {  // within a row of sixteen lanes
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x111, 0xf, 0xf, true));
+}
+
+// U rows a lane at once.  Grid (tokens / waves of a workgroup, pieces of a token's rows).
+template <int kLanes, int U, bool kAxes>
+__global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p) {
+    constexpr int kRows = 64 / kLanes;  // a wave's, a pass
+    const int lane = threadIdx.x & 63, j = lane % kLanes, r = lane / kLanes;
+    const int t = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6)));
+    if (t >= p.tokens) return;
+    const int D = p.dim, half = D / 2, nl = D / 16, all = p.n_heads + 2 * p.n_kv;
+    const int pass0 = (int)blockIdx.y * p.per, passes = min((all + kRows - 1) / kRows, pass0 + p.per);
+    const bool in_row = j < nl;  // (a head dim of no power of two leaves lanes over)
+    const int d0 = in_row ? 8 * j : 0;
+
+    u32x4_t raw[U][2];
+    auto place = [&](int pass, int u, int& hh) __attribute__((always_inline)) {  // the lane's row
+        hh = (pass + u) * kRows + r;
+        return pass + u < passes && hh < all;
+    };
+    auto load = [&](int pass) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            int hh;
+            const bool on = place(pass, u, hh);
+            hh = on ? hh : 0;
+            const bool is_q = hh < p.n_heads, is_v = hh >= p.n_heads + p.n_kv;
+            const uint16_t* src = is_q ? p.q + ((size_t)t * p.n_heads + hh) * D : (is_v ? p.v_in + ((size_t)t * p.n_kv + (hh - p.n_heads - p.n_kv)) * D : p.k_in + ((size_t)t * p.n_kv + (hh - p.n_heads)) * D);
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                raw[u][e] = u32x4_t{0, 0, 0, 0};
+                if (on && in_row) raw[u][e] = *(const u32x4_t*)(src + d0 + e * half);
+            }
+        }
+    };
+    load(pass0);
+
+    // the token's sequence, row and page
+    int b, first;
+    if (p.starts) {
+        b = 0;
+        for (int b0 = 0; b0 < p.batch; b0 += 64) {  // sequences that end ahead of it
+            const int n = __popcll(__ballot(b0 + lane < p.batch && p.starts[min(b0 + lane, p.batch - 1) + 1] <= t));
+            b += n;
+            if (n < 64) break;
+        }
+        b = __builtin_amdgcn_readfirstlane(b);
+        if (b >= p.batch) return;  // behind the last sequence
+        first = p.starts[b];
+        if (first > t) return;  // ahead of the first
+    } else {
+        b = t / p.each;
+        first = b * p.each;
+    }
+    const long long row = (long long)(p.positions ? p.positions[b] : p.pos) + ((long long)t - first);
+    const bool in_table = row >= 0 && row >> p.page_shift < p.table_pages;
+    const int page = in_table ? p.page_table[(size_t)b * p.table_pages + (size_t)(row >> p.page_shift)] : -1;
+    const bool stored = page >= 0 && page < p.n_pages;
+    // its angles; a token whose position the tables do not have is left as it is
+    float cs[8], sn[8];
+    if constexpr (kAxes) {
+        int at[kMaxAxes];
+#pragma unroll
+        for (int a = 0; a < kMaxAxes; a++) at[a] = a < p.n_axes ? p.axes[(size_t)a * p.tokens + t] : 0;
+        bool ok = true;
+#pragma unroll
+        for (int a = 0; a < kMaxAxes; a++) ok = ok && at[a] >= 0 && at[a] < p.table_rows;
+        if (!ok) return;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int i = d0 + e;
+            int pos = at[0];
+#pragma unroll
+            for (int a = 1; a < kMaxAxes; a++) pos = i >= p.ends[a - 1] ? at[a] : pos;
+            cs[e] = p.cos_table[(size_t)pos * half + i];
+            sn[e] = p.sin_table[(size_t)pos * half + i];
+        }
+    } else {
+        if (row < 0 || row >= p.table_rows) return;
+        const size_t at = (size_t)row * half + d0;
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            const f32x4_t c = *(const f32x4_any*)(p.cos_table + at + e), s = *(const f32x4_any*)(p.sin_table + at + e);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                cs[e + i] = c[i];
+                sn[e + i] = s[i];
+            }
+        }
+    }
+    const size_t page_row = stored ? (size_t)page * p.n_kv << p.page_shift : 0;  // of head 0's first row
+    const size_t in_page = (size_t)(row & ((1ll << p.page_shift) - 1));
+
+    for (int pass = pass0; pass < passes; pass += U) {
+        if (pass != pass0) load(pass);
+        float x[U][2][8];
+        const float* gamma[U];
+        bool any_norm = false;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            int hh;
+            const bool on = place(pass, u, hh);
+            gamma[u] = !on || hh >= p.n_heads + p.n_kv ? nullptr : hh < p.n_heads ? p.q_gamma : p.k_gamma;
+            any_norm = any_norm || gamma[u];
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    x[u][e][2 * i] = bf16_lo(raw[u][e][i]);
+                    x[u][e][2 * i + 1] = bf16_hi(raw[u][e][i]);
+                }
+        }
+        if (__any(any_norm)) {
+            float sum[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) sum[u] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float sq[U][8], at[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    at[u] = sum[u];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) sq[u][i] = x[u][e][i] * x[u][e][i];
+                }
+                for (int stage = 0; stage < nl; stage++)
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        float s = at[u];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) s = s + sq[u][i];
+                        sum[u] = s;
+                        at[u] = from_lane_below(s);
+                    }
+#pragma unroll
+                for (int u = 0; u < U; u++) sum[u] = __shfl(sum[u], r * kLanes + nl - 1, 64);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (!gamma[u]) continue;
+                const float inv_d = 1.0f / (float)D;
+                const float inv_rms = 1.0f / sqrtf(sum[u] * inv_d + p.eps);
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int i = 0; i < 8; i += 4) {
+                        const f32x4_t g = *(const f32x4_any*)(gamma[u] + e * half + d0 + i);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) x[u][e][i + k] = x[u][e][i + k] * inv_rms * g[k];
+                    }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            int hh;
+            if (!place(pass, u, hh) || !in_row) continue;
+            const bool is_q = hh < p.n_heads, is_v = hh >= p.n_heads + p.n_kv;
+            const int h = is_q ? hh : is_v ? hh - p.n_heads - p.n_kv : hh - p.n_heads;
+            u32x4_t o[2] = {raw[u][0], raw[u][1]};
+            if (!is_v) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float y0[2], y1[2];
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const int e = 2 * i + k;
+                        const float x0 = x[u][0][e], x1 = x[u][1][e];
+                        y0[k] = x0 * cs[e] - x1 * sn[e];
+                        y1[k] = x1 * cs[e] + x0 * sn[e];
+                    }
+                    o[0][i] = pack_bf16x2(y0[0], y0[1]);
+                    o[1][i] = pack_bf16x2(y1[0], y1[1]);
+                }
+            }
+            if (is_q || (!is_v && p.k_out)) {
+                uint16_t* dst = is_q ? p.q_out + ((size_t)t * p.n_heads + h) * D : p.k_out + ((size_t)t * p.n_kv + h) * D;
+                *(u32x4_t*)(dst + d0) = o[0];
+                *(u32x4_t*)(dst + d0 + half) = o[1];
+            }
+            if (!is_q && stored) {
+                uint16_t* dst = (is_v ? p.v_pages : p.k_pages) + (page_row + ((size_t)h << p.page_shift) + in_page) * D;
+                *(u32x4_t*)(dst + d0) = o[0];
+                *(u32x4_t*)(dst + d0 + half) = o[1];
+            }
+        }
+    }
+}
+
+template <int kLanes, int U>
+hipError_t launch_as(hipStream_t stream, const PagedAppendParams& p, dim3 grid, dim3 block) {
+    if (p.axes) hipLaunchKernelGGL((paged_append_kernel<kLanes, U, true>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((paged_append_kernel<kLanes, U, false>), grid, block, 0, stream, p);
+    return hipGetLastError();
+}
+template <int kLanes>
+hipError_t launch_lanes(hipStream_t stream, PagedAppendParams p) {
+    const int passes = (p.n_heads + 2 * p.n_kv + 64 / kLanes - 1) / (64 / kLanes);
+    const bool few = p.tokens <= 256;
+    p.per = few ? 1 : passes;
+    const int waves = few ? 1 : 4;
+    const dim3 grid((unsigned)((p.tokens + waves - 1) / waves), (unsigned)((passes + p.per - 1) / p.per)), block(64 * waves);
+    return few ? launch_as<kLanes, 1>(stream, p, grid, block) : launch_as<kLanes, 2>(stream, p, grid, block);
+}
+hipError_t launch_paged_append(hipStream_t stream, const PagedAppendParams& p) {
+    return p.dim <= 64 ? launch_lanes<4>(stream, p) : p.dim <= 128 ? launch_lanes<8>(stream, p) : launch_lanes<16>(stream, p);
+}
+
+}  // namespace
+
+}  // namespace rt
+
+using namespace rt;
+
+RT_API int rt_qk_norm_rope_kv_append_paged_bf16(void* stream, const void* q, void* q_out, const void* k_in, void* k_out, const void* v_in,
+                                                void* k_pages, void* v_pages, const int32_t* page_table, const int32_t* starts,
+                                                const int32_t* positions, int32_t pos, const int32_t* axis_positions,
+                                                const int32_t* sections, int32_t n_axes, const float* q_gamma, const float* k_gamma,
+                                                float eps, const float* cos_table, const float* sin_table, int32_t table_rows,
+                                                int32_t tokens, int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim,
+                                                int32_t n_pages, int32_t page_size, int32_t table_pages, rt_err_detail* err) {
+    clear_err(err);
+    if (tokens < 0 || batch < 0 || n_heads < 0 || n_kv < 0 || head_dim < 0 || n_pages < 0 || table_pages < 0 || table_rows < 0 || n_axes < 0)
+        return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "negative dimension");
+    if (head_dim == 0) return fail(err, RT_ERR_ZERO_DIM, -1, 0, 0, "head_dim must be > 0");
+    if (!cache_paged_dim(head_dim)) return fail(err, RT_ERR_UNSUPPORTED, -1, 256, (uint64_t)head_dim, "pages have head_dim up to 256, a multiple of 16");
+    if (!cache_page_size(page_size)) return fail(err, RT_ERR_UNSUPPORTED, -1, kPageMax, (uint64_t)(int64_t)page_size, "page_size must be a power of two, 16 to 1024");
+    if (n_heads > 65535 || n_kv > 65535 || (int64_t)table_pages * page_size > 0x7fffffffll) return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "shape too large for the launch grid");
+    PagedAppendParams p{};
+    if (n_axes > 0) {
+        if (n_axes > kMaxAxes) return fail(err, RT_ERR_UNSUPPORTED, -1, kMaxAxes, (uint64_t)n_axes, "at most four axes");
+        if (!sections) return fail(err, RT_ERR_NULL_POINTER, -1, 0, 0, "NULL sections");
+        int64_t sum = 0;
+        for (int a = 0; a < n_axes; a++) {
+            if (sections[a] < 0) return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "negative dimension");
+            sum += sections[a];
+            p.ends[a] = (int)std::min<int64_t>(sum, head_dim);
+        }
+        if (sum != head_dim / 2) return fail(err, RT_ERR_ROPE_WRONG_INPUT_LEN, -1, (uint64_t)(head_dim / 2), (uint64_t)sum, "the sections' sum must be head_dim / 2");
+        for (int a = n_axes; a < kMaxAxes; a++) p.ends[a] = head_dim;
+    }
+    if (!starts && batch > 0 && tokens % batch != 0)
+        return fail(err, RT_ERR_WRONG_INPUT_LEN, RT_WHICH_Q, (uint64_t)batch, (uint64_t)tokens, "without starts every sequence has tokens / batch tokens");
+    if (!positions) {  // rope.rs:179-184, then kv_cache.rs:84-89
+        const int64_t last = (int64_t)pos + (starts || batch == 0 ? 0 : tokens / batch);
+        if (pos < 0 || (n_axes == 0 && last > table_rows))
+            return fail(err, RT_ERR_ROPE_POSITION_OVERFLOW, -1, (uint64_t)table_rows, (uint64_t)last, "positions outside the RoPE tables");
+        if (last > (int64_t)table_pages * page_size)
+            return fail(err, RT_ERR_KV_OVERFLOW, -1, (uint64_t)((int64_t)table_pages * page_size), (uint64_t)last, "rows behind the page table");
+    }
+    if (batch == 0 || tokens == 0 || n_heads + n_kv == 0) return RT_OK;
+    if ((n_heads > 0 && (!q || !q_out)) || (n_kv > 0 && (!k_in || !v_in || ((!k_pages || !v_pages) && n_pages > 0) || (!page_table && table_pages > 0))) || !cos_table || !sin_table ||
+        (n_axes > 0 && !axis_positions))
+        return fail(err, RT_ERR_NULL_POINTER, -1, 0, 0, "NULL buffer");
+    if (((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k_in | (uintptr_t)k_out | (uintptr_t)v_in | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15)
+        return fail(err, RT_ERR_UNSUPPORTED, -1, 16, 0, "q, k, v and the pages must be 16-byte aligned");
+    const size_t q_bytes = (size_t)tokens * n_heads * head_dim * 2, kv_bytes = (size_t)tokens * n_kv * head_dim * 2;
+    const size_t page_bytes = (size_t)n_pages * n_kv * page_size * head_dim * 2;
+    if ((q != q_out && overlap(q, q_bytes, q_out, q_bytes)) || (k_out && k_out != k_in && overlap(k_in, kv_bytes, k_out, kv_bytes)))
+        return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "q_out must be q, and k_out k_in, or share no memory with it");
+    const struct {
+        const void* at;
+        size_t n;
+    } written[4] = {{q_out, q_bytes}, {k_out, k_out ? kv_bytes : 0}, {k_pages, page_bytes}, {v_pages, page_bytes}}, read[3] = {{q, q_bytes}, {k_in, kv_bytes}, {v_in, kv_bytes}};
+    for (int i = 0; i < 4; i++) {
+        for (int k = i + 1; k < 4; k++)
+            if (overlap(written[i].at, written[i].n, written[k].at, written[k].n)) return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "outputs and pages must share no memory");
+        for (int k = 0; k < 3; k++)
+            if ((i >= 2 || k != i) && overlap(written[i].at, written[i].n, read[k].at, read[k].n)) return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "outputs and pages must share no memory with the inputs");
+    }
+    int rc = ensure_device(err);
+    if (rc) return rc;
+    p.q = (const uint16_t*)q;
+    p.q_out = (uint16_t*)q_out;
+    p.k_in = (const uint16_t*)k_in;
+    p.k_out = (uint16_t*)k_out;
+    p.v_in = (const uint16_t*)v_in;
+    p.k_pages = (uint16_t*)k_pages;
+    p.v_pages = (uint16_t*)v_pages;
+    p.page_table = page_table;
+    p.starts = starts;
+    p.positions = positions;
+    p.pos = pos;
+    p.axes = n_axes > 0 ? axis_positions : nullptr;
+    p.n_axes = n_axes;
+    p.q_gamma = q_gamma;
+    p.k_gamma = k_gamma;
+    p.eps = eps;
+    p.cos_table = cos_table;
+    p.sin_table = sin_table;
+    p.table_rows = table_rows;
+    p.tokens = tokens;
+    p.batch = batch;
+    p.each = tokens / batch;
+    p.n_heads = n_heads;
+    p.n_kv = n_kv;
+    p.dim = head_dim;
+    p.n_pages = n_pages;
+    p.table_pages = table_pages;
+    p.page_shift = __builtin_ctz((unsigned)page_size);
+    HIP_TRY(launch_paged_append((hipStream_t)stream, p), "paged_append launch");
+    return RT_OK;
+}

@@ -197,6 +197,9 @@ PyMethodDef methods[] = {
     RT_BIND(rt_gqa_decode_weights_q4),
     RT_BIND(rt_kv_evict_bf16),
     RT_BIND(rt_kv_evict_q4),
+    RT_BIND(rt_qk_norm_rope_kv_append_paged_bf16),
+    RT_BIND(rt_flash_forward_packed_bf16_dev),
+    RT_BIND(rt_gqa_decode_paged_bf16),
     RT_BIND_HOST(rt_flash_forward_masked_f32),
     RT_BIND_HOST(rt_flash_backward_f32),
     RT_BIND_HOST(rt_gqa_forward_f32),

@@ -6,8 +6,9 @@
 
 namespace rt {
 
-// 0..2 are rt_mask_kind of the C ABI; 3 is the padded-batch mode (per-sequence length + causal).
-enum MaskKind : int { kMaskNone = 0, kMaskCausal = 1, kMaskPadding = 2, kMaskVarlenCausal = 3 };
+// 0..2 are rt_mask_kind of the C ABI; 3 is the padded-batch mode (per-sequence length + causal), 4 that of sequences packed one behind
+// the other (causal).
+enum MaskKind : int { kMaskNone = 0, kMaskCausal = 1, kMaskPadding = 2, kMaskVarlenCausal = 3, kMaskPacked = 4 };
 constexpr float kLog2eHost = 1.4426950408889634f;
 
 // Where element [b, h, row, 0] of a 4-D attention tensor sits (in elements): rows of `dim` contiguous
@@ -188,14 +189,18 @@ struct FlashTileParams {
     // head sets it.
     int decode_rows;
     int n_cus;  // CUs of the device (0: unknown)
+    const int32_t* starts;  // kMaskPacked: device int32[batch + 1], the first token of each sequence; seq_q = seq_kv = all tokens
 };
 static_assert(offsetof(FlashTileParams, q) == 64 && offsetof(FlashTileParams, q_lens) == 128, "lines of the arguments");
 bool flash_tile_bf16_supported(int dim);
+// Packed sequences are as long as launches can tell: the tokens there are for each.
+inline int flash_tile_bf16_packed_len(const FlashTileParams& p) { return p.seq_kv / (p.batch > 0 ? p.batch : 1); }
 // Head dims above 128: tiles straight to LDS?  (Why the lines lie there: takes_tiles_direct, flash_bf16_tile.hip.)
 inline bool flash_tile_bf16_direct(const FlashTileParams& p) {
     const bool packed = p.pack > 1 || p.decode_rows, unknown = packed && p.kv_lens;  // lengths on the device: the new positions' at least
     const long long rows = (long long)p.seq_q * p.pack, keys = unknown ? p.seq_q : p.seq_kv, units = (long long)p.batch * (packed ? p.kv_heads : p.heads) * ((rows + 127) / 128);
     if (p.bias) return false;
+    if (p.mask == kMaskPacked) return flash_tile_bf16_packed_len(p) >= 96;
     if (p.n_splits > 1) return !unknown && keys / p.n_splits >= 256 && rows > (p.pack > 1 ? 64 : 96);
     const long long n_cus = p.n_cus > 0 ? p.n_cus : 256;
     if (keys < (unknown ? 256 : packed ? 140 : p.q_lens && 2 * units > n_cus ? 160 : 96)) return false;
@@ -257,6 +262,7 @@ struct StrictVParams {
     const int32_t* seq_lens;
     int batch, heads, kv_heads, seq, dim;
     TensorLayout lkv, lo;
+    const int32_t* starts;  // optional (packed sequences): device int32[batch + 1], their first rows; then `seq` rows in all
 };
 hipError_t launch_strict_hidden_v(hipStream_t stream, const StrictVParams& p, bool bf16);
 

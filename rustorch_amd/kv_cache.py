@@ -8,13 +8,18 @@ is trimmed or copied out before attention.
 
 With dtype "q4" a layer's buffers are `Q4Rows`, rows of 4 bits, which the `_q4` calls of `LlmKernels` take; `append` takes bf16
 rows there and rounds them.
+
+`PagedKVCache` (no counterpart in the reference) holds many sequences of different lengths in pages, which the `_paged` calls of
+`LlmKernels` take.
 """
 from __future__ import annotations
+
+import numpy as np
 
 from . import _lib as L
 from .device import HipStorage
 from .errors import LayerOutOfRange, Overflow, check
-from .llm_kernels import LlmKernels, Q4Rows
+from .llm_kernels import KVPages, LlmKernels, Q4Rows
 
 _ELEM = {"bf16": 2, "f32": 4, "q4": 2}  # bytes an element of what is appended
 
@@ -85,3 +90,100 @@ class KVCache:
     def dims(self):
         """`(batch, n_heads, max_seq, head_dim)`, or None without layers (kv_cache.rs:223-226)."""
         return self._dims if self._layers else None
+
+
+class PagedKVCache:
+    """Sequences in pages: per layer a `KVPages`, and one page table for all of them.  A sequence has a row of the table from `add` to
+    `remove`; `reserve` gives it pages ahead of the append, `advance` counts the rows that every layer has appended.  Whole pages of a
+    prefix are shared (`add(prefix_of=..., shared=...)`) and live as long as a sequence has them."""
+
+    def __init__(self, num_layers: int, max_sequences: int, n_heads: int, head_dim: int, n_pages: int, page_size: int = 64,
+                 table_pages: int | None = None):
+        self.page_size, self.n_pages = page_size, n_pages
+        self.table_pages = n_pages if table_pages is None else table_pages
+        self._layers = [KVPages.zeros(n_pages, n_heads, page_size, head_dim) for _ in range(num_layers)]
+        self._free = list(range(n_pages - 1, -1, -1))
+        self._uses = np.zeros(n_pages, dtype=np.int32)
+        self._table = np.full((max_sequences, self.table_pages), -1, dtype=np.int32)
+        self._lens = np.full(max_sequences, -1, dtype=np.int32)  # -1: no sequence
+
+    def num_layers(self) -> int:
+        return len(self._layers)
+
+    def layer(self, layer_idx: int) -> KVPages:
+        if not 0 <= layer_idx < len(self._layers):
+            raise LayerOutOfRange(layer_idx, len(self._layers))
+        return self._layers[layer_idx]
+
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _check(self, seq: int):
+        if not 0 <= seq < len(self._lens) or self._lens[seq] < 0:
+            raise KeyError(f"no sequence {seq}")
+
+    def add(self, prefix_of: int | None = None, shared: int = 0) -> int:
+        """A new sequence, empty, or with the first `shared` rows of another, whose pages it has in common: whole pages."""
+        if shared % self.page_size:
+            raise ValueError(f"a shared prefix ends with a page: {shared} rows of pages of {self.page_size}")
+        if shared:
+            self._check(prefix_of)
+            if not 0 < shared <= self._lens[prefix_of]:
+                raise Overflow(shared, int(self._lens[prefix_of]))
+        free = np.flatnonzero(self._lens < 0)
+        if not free.size:
+            raise Overflow(len(self._lens) + 1, len(self._lens))
+        seq, n = int(free[0]), shared // self.page_size
+        if n:
+            self._table[seq, :n] = self._table[prefix_of, :n]
+            self._uses[self._table[seq, :n]] += 1
+        self._lens[seq] = shared
+        return seq
+
+    def reserve(self, seq: int, rows: int) -> None:
+        """Pages for `rows` more rows; all of them or, with Overflow, none."""
+        self._check(seq)
+        if rows < 0:
+            raise ValueError(f"rows must not be negative, got {rows}")
+        have, need = int((self._table[seq] >= 0).sum()), -(-(int(self._lens[seq]) + rows) // self.page_size)
+        if need > self.table_pages or need - have > len(self._free):
+            raise Overflow(int(self._lens[seq]) + rows, min(self.table_pages, have + len(self._free)) * self.page_size)
+        for c in range(have, need):
+            self._table[seq, c] = page = self._free.pop()
+            self._uses[page] = 1
+
+    def advance(self, seq: int, rows: int) -> None:
+        self._check(seq)
+        end, room = int(self._lens[seq]) + rows, int((self._table[seq] >= 0).sum()) * self.page_size
+        if rows < 0 or end > room:
+            raise Overflow(end, room)
+        self._lens[seq] = end
+
+    def remove(self, seq: int) -> None:
+        """The sequence's row of the table is free, and so are the pages that nobody else has."""
+        self._check(seq)
+        for page in self._table[seq][self._table[seq] >= 0].tolist():
+            self._uses[page] -= 1
+            if self._uses[page] == 0:
+                self._free.append(page)
+        self._table[seq], self._lens[seq] = -1, -1
+
+    def length(self, seq: int) -> int:
+        self._check(seq)
+        return int(self._lens[seq])
+
+    def table(self, seqs, write_from=None) -> np.ndarray:
+        """int32 [len(seqs), table_pages], the `page_table` of a call for these sequences.  write_from: for each of them the row from which
+        the call may write; whole pages ahead of it are left out, so that an append keeps off what is shared."""
+        for seq in seqs:
+            self._check(seq)
+        table = self._table[list(seqs)].copy()
+        for i, row in enumerate(write_from if write_from is not None else ()):
+            table[i, :row // self.page_size] = -1
+        return table
+
+    def lengths(self, seqs) -> np.ndarray:
+        """int32 [len(seqs)], the rows that each has."""
+        for seq in seqs:
+            self._check(seq)
+        return self._lens[list(seqs)].copy()

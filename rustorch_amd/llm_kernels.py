@@ -28,6 +28,22 @@ class Q4Rows:
         return cls(HipStorage.zeros(rows * head_dim // 2, stream), HipStorage.zeros(rows * (head_dim // 64) * 4, stream))
 
 
+class KVPages:
+    """K and V of a cache in pages, the cache argument of the `_paged` calls: device buffers [n_pages, n_kv, page_size, head_dim]
+    of bf16, page_size a power of two from 16 to 1024.  Row r of sequence b lies in page `page_table[b, r // page_size]` (device
+    int32 [batch, table_pages]; an entry that is no page, such as -1, stands for rows that are not there)."""
+
+    __slots__ = ("k", "v", "n_pages", "page_size")
+
+    def __init__(self, k, v, n_pages: int, page_size: int):
+        self.k, self.v, self.n_pages, self.page_size = k, v, n_pages, page_size
+
+    @classmethod
+    def zeros(cls, n_pages: int, n_kv: int, page_size: int, head_dim: int, stream=None) -> "KVPages":
+        n_bytes = n_pages * n_kv * page_size * head_dim * 2
+        return cls(HipStorage.zeros(n_bytes, stream), HipStorage.zeros(n_bytes, stream), n_pages, page_size)
+
+
 def _host_or_dev(x):
     """(device address, host value) of an argument that is an int for every sequence or a device int32[batch] buffer."""
     return (None, int(x)) if isinstance(x, (int, np.integer)) else (x, 0)
@@ -215,3 +231,36 @@ class LlmKernels:
         check(L.native.rt_kv_evict_q4(stream, k_cache.codes, k_cache.pairs, v_cache.codes, v_cache.pairs, weights_in, slots_in,
                                       weights_out, slots_out, kv_lens, new_lens, batch, n_kv, head_dim, max_seq, budget, recent,
                                       workspace, workspace_bytes))
+
+    # ---- many requests side by side (no counterparts in the reference): packed tokens, and caches in pages ----
+
+    @staticmethod
+    def qk_norm_rope_kv_append_paged_bf16(stream, q, q_out, k_in, v_in, pages, page_table, table_pages, positions, rope, tokens,
+                                          batch, n_heads, n_kv, head_dim, starts=None, k_out=None, q_gamma=None, k_gamma=None,
+                                          eps=1e-6, axis_positions=None, sections=None):
+        """`qk_norm_rope_kv_append_bf16` for packed tokens ([tokens, heads, head_dim]) and a cache in pages (`KVPages`); q goes to
+        `q_out` and, where it is given, rotated k to `k_out`; each may be its input.  `starts`, device int32[batch + 1], are the
+        sequences' first tokens (None: tokens / batch each); `positions`, an int or a device int32[batch] buffer, the row of a sequence's
+        first token.  With `sections`, pairs of a head for each of up to four axes, a token's rotary positions are
+        `axis_positions`, device int32[len(sections), tokens], and not its row."""
+        ptr, pos = _host_or_dev(positions)
+        sections = None if sections is None else np.ascontiguousarray(sections, dtype=np.int32)
+        cos, sin = rope.device_tables()
+        check(L.native.rt_qk_norm_rope_kv_append_paged_bf16(
+            stream, q, q_out, k_in, k_out, v_in, pages.k, pages.v, page_table, starts, ptr, pos, axis_positions,
+            None if sections is None else sections.ctypes.data, 0 if sections is None else sections.size, q_gamma, k_gamma, eps, cos, sin,
+            rope.max_seq, tokens, batch, n_heads, n_kv, head_dim, pages.n_pages, pages.page_size, table_pages))
+
+    @staticmethod
+    def gqa_decode_paged_workspace_bytes(batch, n_heads, n_kv, head_dim, page_size, table_pages) -> int:
+        return L.lib().rt_gqa_decode_paged_workspace_bytes(batch, n_heads, n_kv, head_dim, page_size, table_pages)
+
+    @staticmethod
+    def gqa_decode_paged_bf16(stream, q, pages, out, page_table, table_pages, kv_lens, batch, n_heads, n_kv, head_dim, workspace,
+                              workspace_bytes, shared_len=0):
+        """`gqa_decode_batched_bf16` over a cache in pages: q/out [batch, n_heads, head_dim], kv_lens device int32[batch].  The
+        first `shared_len` keys (an int or a device int32[1] buffer) of every sequence that has as many are the same for all, in the
+        pages of `page_table[0]`, and are read once."""
+        ptr, shared = _host_or_dev(shared_len)
+        check(L.native.rt_gqa_decode_paged_bf16(stream, q, pages.k, pages.v, out, page_table, kv_lens, ptr, shared, batch, n_heads, n_kv,
+                                                head_dim, pages.n_pages, pages.page_size, table_pages, workspace, workspace_bytes))

@@ -1,0 +1,112 @@
+// Tests of the C++ host mirror's calls for packed tokens and caches in pages (include/rustorch_attn.hpp).
+//   paged_mirror_test errors   what they refuse, and as what: needs no GPU
+//   paged_mirror_test gpu      append, attention of the prompts, decode steps with a shared prefix
+#include <cmath>
+#include <cstdio>
+#include <cstring>
+#include <vector>
+
+#include "rustorch_attn.hpp"
+
+using namespace rustorch_attn;
+
+static int g_failed = 0;
+#define CHECK(cond)                                                     \
+    do {                                                                \
+        if (!(cond)) {                                                  \
+            std::printf("FAIL %s:%d: %s\n", __FILE__, __LINE__, #cond); \
+            ++g_failed;                                                 \
+        }                                                               \
+    } while (0)
+
+template <typename E, typename F>
+static bool throws(F&& f) {
+    try {
+        f();
+    } catch (const E&) {
+        return true;
+    } catch (...) {
+    }
+    return false;
+}
+
+static void errors() {
+    alignas(16) static int32_t some[64];
+    const KVPages pages{some, some, 4, 16};
+    RoPE rope(64, 16);
+    const size_t many = (size_t)1 << 40;
+    CHECK(throws<RoPEError>([&] { LlmKernels::qk_norm_rope_kv_append_paged_bf16(nullptr, some, some, some, nullptr, some, pages, some, 4, nullptr, nullptr, 16, nullptr, {}, nullptr, nullptr, 1e-6f, rope, 1, 1, 1, 1, 64); }));
+    CHECK(throws<KVCacheOverflow>([&] { LlmKernels::qk_norm_rope_kv_append_paged_bf16(nullptr, some, some, some, nullptr, some, KVPages{some, some, 4, 8}, some, 1, nullptr, nullptr, 8, nullptr, {}, nullptr, nullptr, 1e-6f, rope, 1, 1, 1, 1, 64); }));
+    CHECK(throws<GQAError>([&] { LlmKernels::gqa_decode_paged_bf16(nullptr, some, pages, some, some, 4, some, nullptr, 0, 1, 4, 3, 64, some, many); }));
+    CHECK(throws<AttentionError>([&] { LlmKernels::flash_forward_packed_bf16(nullptr, AttentionShape::make(1, 4, 8, 0), 4, some, some, some, some, some); }));
+    CHECK(LlmKernels::gqa_decode_paged_workspace_bytes(2, 4, 2, 64, 16, 8) > 0 && LlmKernels::gqa_decode_paged_workspace_bytes(2, 4, 2, 64, 17, 8) == 0);
+}
+
+template <typename T>
+static HipStorage up(const std::vector<T>& v) {
+    HipStorage s(v.size() * sizeof(T));
+    rt_err_detail e;
+    detail::check_device(rt_memcpy_h2d(s.ptr(), v.data(), v.size() * sizeof(T), nullptr, &e), e);
+    detail::check_device(rt_stream_synchronize(nullptr, &e), e);
+    return s;
+}
+static std::vector<uint16_t> back(const HipStorage& s, size_t n) {
+    std::vector<uint16_t> v(n);
+    rt_err_detail e;
+    detail::check_device(rt_memcpy_d2h(v.data(), s.ptr(), n * 2, nullptr, &e), e);
+    detail::check_device(rt_stream_synchronize(nullptr, &e), e);
+    return v;
+}
+static uint16_t bits(float x) {  // of numbers that are bf16
+    uint32_t u;
+    std::memcpy(&u, &x, 4);
+    return (uint16_t)(u >> 16);
+}
+static float value(uint16_t b) {
+    const uint32_t u = (uint32_t)b << 16;
+    float x;
+    std::memcpy(&x, &u, 4);
+    return x;
+}
+
+// Two prompts of 40 and 21 tokens whose q and k are zeros, so that every key weighs the same, and whose V is the token's number in every dim: an
+// output is the mean of the numbers up to it.  Then a step of each behind the first 16 tokens of the first prompt, which both share.
+static void gpu() {
+    const int heads = 4, kv = 2, d = 64, tokens = 61, page = 16;
+    RoPE rope(d, 64);
+    std::vector<uint16_t> v_in(tokens * kv * d);
+    for (int t = 0; t < tokens; t++)
+        for (int i = 0; i < kv * d; i++) v_in[t * kv * d + i] = bits((float)(t < 40 ? t : t - 40));
+    HipStorage q = up(std::vector<uint16_t>(tokens * heads * d)), k = up(std::vector<uint16_t>(tokens * kv * d)), v = up(v_in), out(tokens * heads * d * 2);
+    HipStorage starts = up(std::vector<int32_t>{0, 40, 61}), rows = up(std::vector<int32_t>{0, 0});
+    HipStorage k_pages(5 * kv * page * d * 2), v_pages(5 * kv * page * d * 2);
+    HipStorage write = up(std::vector<int32_t>{4, 0, 2, -1, 3, -1}), read = up(std::vector<int32_t>{4, 0, 2, 4, 3, -1});
+    const KVPages pages{k_pages.ptr(), v_pages.ptr(), 5, page};
+    LlmKernels::qk_norm_rope_kv_append_paged_bf16(nullptr, q.ptr(), q.ptr(), k.ptr(), k.ptr(), v.ptr(), pages, (int32_t*)write.ptr(), 3, (int32_t*)starts.ptr(), (int32_t*)rows.ptr(), 0, nullptr, {}, nullptr,
+                                                  nullptr, 1e-6f, rope, tokens, 2, heads, kv, d);
+    LlmKernels::flash_forward_packed_bf16(nullptr, AttentionShape::make(2, heads, tokens, d), kv, q.ptr(), k.ptr(), v.ptr(), (int32_t*)starts.ptr(), out.ptr());
+    const std::vector<uint16_t> got = back(out, tokens * heads * d);
+    for (int t = 0; t < tokens; t++)
+        for (int i = 0; i < heads * d; i++) {
+            const double mean = 0.5 * (t < 40 ? t : t - 40);
+            CHECK(std::fabs(value(got[t * heads * d + i]) - mean) <= std::ldexp(mean, -7));
+        }
+    HipStorage lens = up(std::vector<int32_t>{40, 21}), one(2 * heads * d * 2), zero = up(std::vector<uint16_t>(2 * heads * d));
+    const size_t bytes = LlmKernels::gqa_decode_paged_workspace_bytes(2, heads, kv, d, page, 3);
+    HipStorage space(bytes);
+    for (int shared : {0, 16}) {
+        LlmKernels::gqa_decode_paged_bf16(nullptr, zero.ptr(), pages, one.ptr(), (int32_t*)read.ptr(), 3, (int32_t*)lens.ptr(), nullptr, shared, 2, heads, kv, d, space.ptr(), bytes);
+        const std::vector<uint16_t> step = back(one, 2 * heads * d);
+        for (int i = 0; i < 2 * heads * d; i++) {
+            const double mean = i < heads * d ? 19.5 : 10.0;
+            CHECK(std::fabs(value(step[i]) - mean) <= std::ldexp(mean, -7));
+        }
+    }
+}
+
+int main(int argc, char** argv) {
+    if (argc > 1 && !std::strcmp(argv[1], "gpu")) gpu();
+    else errors();
+    std::printf(g_failed ? "%d failed\n" : "ok\n", g_failed);
+    return g_failed != 0;
+}

@@ -59,7 +59,8 @@ struct PagedDecodeParams {
     int n_groups;      // workgroups launched
     float span_root, scale_log2e;
     float* part;
-    unsigned char* words;
+    unsigned char* head;   // what one launch leaves for the next
+    unsigned char* words;  // a line for each (sequence, kv head, piece)
     uint64_t launch_id;
 };
 

@@ -11,8 +11,9 @@
 // all sequences that share it form tiles of 16 kTiles rows, whose operands wait in LDS, and a step's keys are asked for once for a tile.
 // Both kinds of segments, (kv head, tile) of the prefix and (sequence, kv head), form one list of steps that is cut into equal
 // spans, one a workgroup of four waves, which deal the steps of a segment among themselves and fold what they have through LDS.  What a
-// workgroup finishes of a sequence it writes at once, where that is all there is; otherwise it leaves a partial (o, m, l) and counts
-// its steps, and the workgroup that completes the sequence's count folds the partials.
+// workgroup finishes of a sequence it writes at once, where that is all there is; otherwise it leaves a partial (o, m, l).  Without a
+// prefix the workgroup that finishes a sequence's kv head last folds its partials.  With one every sequence has at least two, and a
+// prefix's tile is waited for by all of its sequences: there a second launch folds them, side by side.
 //
 // The weights meet V as one bf16 each, rounded to nearest, as in the prefill kernels: 2^-9 of a weight, and errors of many keys cancel.
 #include <algorithm>
@@ -216,14 +217,13 @@ __device__ __forceinline__ f32x4_t get4(__amdgpu_buffer_rsrc_t rs, uint32_t byte
 }
 __device__ __forceinline__ u32x2_t get2(__amdgpu_buffer_rsrc_t rs, uint32_t byte) { return __builtin_amdgcn_raw_buffer_load_b64(rs, byte, 0, kScopeDevice); }
 
-// The word through which the workgroups of a (sequence, kv head, piece of its heads) learn which of them is the last: (launch id | steps
-// done).  It lies in the caller's workspace, which holds anything: every workgroup makes sure, ahead of its own count, that the word
-// carries this launch's id.  The last one leaves 0 there, so that a recorded launch, which brings its id along on every replay,
-// finds none of its own counts.  Behind the word: where the sequence's own partials are, left by those that count its own steps.
+// The word through which the workgroups of a (sequence, kv head, piece of its heads) learn which of them is the last: (launch id | count).
+// It lies in the caller's workspace, which holds anything: every workgroup makes sure, ahead of its own count, that the word carries this
+// launch's id.  The last one leaves 0 there, so that a recorded launch, which brings its id along on every replay, finds none of its own
+// counts.  With a prefix the same line holds where the sequence's own partials are, for the launch that folds them.
 typedef unsigned long long word_t;
 constexpr int kWordPitch = 128;  // bytes: atomics on one line wait for each other
-constexpr int kCountBits = 24;
-constexpr word_t kCountMask = ((word_t)1 << kCountBits) - 1;
+constexpr word_t kCountMask = 0xffff;
 struct UnitWord {
     word_t* at;
     word_t id, seen, got;
@@ -245,14 +245,111 @@ struct UnitWord {
             replace();
         }
     }
-    // counts `steps` of `all`; true for the workgroup that completes them
-    __device__ __forceinline__ bool count(int steps, int all) {
-        const word_t old = __hip_atomic_fetch_add(at, (word_t)steps, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const bool last = (int)(old & kCountMask) + steps == all;
+    // counts one finished partial of `n`; true for the one that completes the set
+    __device__ __forceinline__ bool count(int n) {
+        const word_t old = __hip_atomic_fetch_add(at, (word_t)1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool last = (int)(old & kCountMask) + 1 == n;
         if (last) __hip_atomic_store(at, (word_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         return last;
     }
 };
+// What the first launch leaves for the second: of the list, and of a unit's line.
+struct ListHead {
+    int size, shared, pre_places;
+};
+struct UnitLine {
+    int w0, pieces;  // of its own keys' partials; none: pieces 0.  One alone, and no prefix: written already, pieces -1
+};
+__device__ __forceinline__ void* word_of(const PagedDecodeParams& p, int seq, int kvh, int piece) {
+    return p.words + (((size_t)seq * p.kv_heads + kvh) * p.chunks + piece) * kWordPitch;
+}
+
+// ---- partials ----------------------------------------------------------------------------------------------------------------
+// Slots of the prefix's come first, then those of the sequences'.  A piece's number is (workgroup + segment): along the list each further
+// piece advances one or the other.  A slot: rows of D floats, then their (m, l).
+template <int D>
+constexpr int prefix_tiles() { return D == 256 ? 2 : 4; }  // of sixteen query rows that a prefix's step serves
+template <int D>
+struct Slots {
+    static constexpr int kTileRows = 16 * prefix_tiles<D>();
+    static constexpr uint32_t kPre = (uint32_t)kTileRows * (D + 2) * 4;
+    char *pre, *own;
+    uint32_t own_bytes;
+    __device__ __forceinline__ Slots(const PagedDecodeParams& p, bool shared)
+        : pre((char*)p.part), own((char*)p.part + (shared ? (size_t)(p.n_groups + p.kv_heads * p.n_tiles) * kPre : 0)), own_bytes((uint32_t)p.rows * (D + 2) * 4) {}
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t of_pre(int w0, int segment, int n) const { return rsrc_of(pre + ((size_t)w0 + segment) * kPre, (uint32_t)n * kPre); }
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t of_own(int w0, size_t segment, int n) const { return rsrc_of(own + ((size_t)w0 + segment) * own_bytes, (uint32_t)n * own_bytes); }
+};
+// Four dims of a row of the output.
+__device__ __forceinline__ void put_out(const PagedDecodeParams& p, int dim, int seq, int head, int d, f32x4_t o) {
+    if (d < dim) *(u32x2_t*)(p.out + ((size_t)seq * p.heads + head) * dim + d) = u32x2_t{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
+}
+constexpr int kThreads = 64 * kWaves;
+constexpr int kJoinLds = kMaxPieces * 16 * 8 + kThreads * 16;
+// All partials of `rows` heads from `head` on of sequence `seq`, by the whole workgroup: n_pre of the prefix, rows of theirs from pre_row on, and
+// n_own.  Items of four elements, kAhead pieces of each at a time; where there are fewer items than threads, several threads an item, each
+// with every sub-th piece.  The first are asked for ahead of the (m, l) that their weights are made of.
+template <int D, bool kShared>
+__device__ __forceinline__ void join(const PagedDecodeParams& p, unsigned char* lds, float* inv_l, int dim, int seq, int head, int rows, __amdgpu_buffer_rsrc_t pre, int n_pre, int pre_row, __amdgpu_buffer_rsrc_t own, int n_own) {
+    constexpr int kAhead = 8, NT = kThreads;
+    constexpr uint32_t kPre = Slots<D>::kPre;
+    const uint32_t own_slot = (uint32_t)p.rows * (D + 2) * 4;
+    float* const wgt = (float*)lds;  // [pieces][16]
+    float* const wl = wgt + kMaxPieces * 16;
+    f32x4_t* const part = (f32x4_t*)(wl + kMaxPieces * 16);
+    const int tid = threadIdx.x, pieces = n_pre + n_own, items = rows * (D / 4), sub_n = items >= NT ? 1 : NT / items;
+    const int x0 = sub_n == 1 ? tid : tid % items, sub = sub_n == 1 ? 0 : tid / items;
+    f32x4_t a[kAhead];
+    auto ask = [&](int i, int k0) __attribute__((always_inline)) {  // (row and element follow one another in a slot)
+        const uint32_t from = 16u * (uint32_t)min(i, items - 1);
+#pragma unroll
+        for (int e = 0; e < kAhead; e++) {
+            const int k = min(k0 + e * sub_n, pieces - 1);
+            a[e] = kShared && k < n_pre ? get4(pre, (uint32_t)k * kPre + (uint32_t)(pre_row * D * 4) + from) : get4(own, (uint32_t)(k - n_pre) * own_slot + from);
+        }
+    };
+    ask(x0, sub);
+    {
+        const int row = tid >> 4, col = tid & 15;  // sixteen lanes a row
+        const bool on = row < rows;
+        float top = kNoMax, sum = 0.0f;
+        for (int k = col; on && k < pieces; k += 16) {
+            const u32x2_t ml = kShared && k < n_pre ? get2(pre, (uint32_t)k * kPre + 4u * (uint32_t)(Slots<D>::kTileRows * D + 2 * (pre_row + row)))
+                                                    : get2(own, (uint32_t)(k - n_pre) * own_slot + 4u * (uint32_t)(p.rows * D + 2 * row));
+            wgt[k * 16 + row] = __uint_as_float(ml[0]);
+            wl[k * 16 + row] = __uint_as_float(ml[1]);
+            top = fmaxf(top, __uint_as_float(ml[0]));
+        }
+        top = columns_max<16>(top);
+        for (int k = col; on && k < pieces; k += 16) {
+            const float fk = __builtin_amdgcn_exp2f((wgt[k * 16 + row] - top) * p.scale_log2e);
+            wgt[k * 16 + row] = fk;
+            sum += wl[k * 16 + row] * fk;
+        }
+        sum = columns_sum<16>(sum);
+        if (on && col == 0) inv_l[row] = sum == 0.0f ? 0.0f : 1.0f / sum;
+    }
+    __syncthreads();
+    for (int i0 = 0; i0 < items; i0 += NT) {
+        const int i = i0 + x0;
+        const bool on = i < items && sub < sub_n;
+        const int row = on ? i / (D / 4) : 0, d = 4 * (i % (D / 4));
+        f32x4_t o = {0, 0, 0, 0};
+        for (int k0 = sub; on && k0 < pieces; k0 += kAhead * sub_n) {
+            if (i0 || k0 != sub) ask(i, k0);
+#pragma unroll
+            for (int e = 0; e < kAhead; e++)
+                if (k0 + e * sub_n < pieces) o += a[e] * wgt[(k0 + e * sub_n) * 16 + row];
+        }
+        if (sub_n > 1) {  // (one round)
+            part[tid] = o;
+            __syncthreads();
+            if (on && sub == 0)
+                for (int e = 1; e < sub_n; e++) o += part[e * items + tid];
+        }
+        if (on && sub == 0) put_out(p, dim, seq, head + row, d, o * inv_l[row]);
+    }
+}
 
 // ---- what a lane holds of 32 keys ------------------------------------------------------------------------------------------
 // As an operand of scores^T, keys are rows: lane (n, quad) has key n of either sixteen, and a quarter of each 32 dims.  As an operand of
@@ -406,22 +503,31 @@ __device__ __forceinline__ void step(State<D> (&st)[NT], Keys<D>& x, QOf q_of, K
         }
     }
     k_done();
-    u32x4_t w[NT];
+    // The running maximum, common to the four lanes of a column.  It follows the scores only where they have risen by 8 in the exponent of
+    // two: up to there sums of weights in f32 and weights of 8 bits are as exact, and sums are scaled once or twice a span.
+    float top[NT];
+    bool risen = false;
 #pragma unroll
     for (int i = 0; i < NT; i++) {
-        // The running maximum, common to the four lanes of a column.  It follows the scores only where they have risen by 8 in the exponent
-        // of two: up to there sums of weights in f32 and weights of 8 bits are as exact, and sums are scaled once or twice a span.
-        float top = y[i][0];
+        top[i] = y[i][0];
 #pragma unroll
-        for (int e = 1; e < kE; e++) top = fmaxf(top, y[i][e]);
-        top = quad_max(top);
-        if (__any((top - st[i].m) * scale_log2e > 8.0f)) {
-            const float m_new = fmaxf(st[i].m, top), alpha = __builtin_amdgcn_exp2f((st[i].m - m_new) * scale_log2e);
+        for (int e = 1; e < kE; e++) top[i] = fmaxf(top[i], y[i][e]);
+        top[i] = quad_max(top[i]);
+        risen = risen || (top[i] - st[i].m) * scale_log2e > 8.0f;
+    }
+    if (__any(risen)) {
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+            const float m_new = fmaxf(st[i].m, top[i]), alpha = __builtin_amdgcn_exp2f((st[i].m - m_new) * scale_log2e);
             st[i].m = m_new;
             st[i].l *= alpha;
 #pragma unroll
             for (int d = 0; d < D / 16; d++) st[i].o[d] *= alpha;
         }
+    }
+    u32x4_t w[NT];
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
         float f[kE];
 #pragma unroll
         for (int e = 0; e < kE; e++) {
@@ -471,19 +577,15 @@ __device__ __forceinline__ void walk(State<D> (&st)[NT], Walk<D, kWhole>& at, co
     }
 }
 
-// Tiles of sixteen query rows that a prefix's step serves.
-template <int D>
-constexpr int prefix_tiles() { return D == 256 ? 2 : 4; }
-
 template <int D, int C, bool kWhole, bool kShared>
 __global__ __launch_bounds__(64 * kWaves, kShared || D == 256 ? 1 : 2) void paged_decode_kernel(PagedDecodeParams p) {
-    constexpr int NT = 64 * kWaves, kPitch = D + 4, kR = 16 / C, kTiles = prefix_tiles<D>();
-    constexpr int kFold = kWaves * 16 * kPitch * 4, kFolds = kMaxPieces * 16 * 8 + NT * 16, kLds = std::max(kFold, kFolds);
+    constexpr int NT = kThreads, kPitch = D + 4, kR = 16 / C, kTiles = prefix_tiles<D>();
+    constexpr int kFold = kWaves * 16 * kPitch * 4, kLds = kShared ? kFold : std::max(kFold, kJoinLds);
     constexpr int kQPitch = 2 * D + 16;  // bytes
     __shared__ __attribute__((aligned(16))) unsigned char lds[kLds];
     __shared__ __attribute__((aligned(16))) unsigned char prefix_q[kShared ? 16 * kTiles * kQPitch : 16];
     __shared__ float red_m[kWaves][16], red_l[kWaves][16], inv_l[16];
-    __shared__ int is_last[64];
+    __shared__ int is_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, quad = lane >> 4, cls = n / kR;
     const int per = p.kv_heads * p.chunks, dim = kWhole ? D : p.dim;
     int group = blockIdx.x;
@@ -492,16 +594,12 @@ __global__ __launch_bounds__(64 * kWaves, kShared || D == 256 ? 1 : 2) void page
     for (int b = blockIdx.x; b < p.batch; b += (int)gridDim.x)
         if (b < 64 ? (span.empty >> b & 1) != 0 : len_of(p, b) == 0)
             for (int i = tid; i < p.heads * (dim / 8); i += NT) *(u32x4_t*)(p.out + (size_t)b * p.heads * dim + 8 * i) = u32x4_t{0, 0, 0, 0};
+    if (kShared && blockIdx.x == 0 && tid == 0) *(ListHead*)p.head = ListHead{span.size, span.shared, span.pre_places};
     if (span.begin >= span.total) return;
     int at = span.begin, b = span.b, first = span.first, len = span.len;
 
     const Lanes<D, kWhole> lanes(n, quad, 2u * (uint32_t)dim);
-    // slots of partials: of the prefix's, then of the sequences'.  A piece's is (workgroup + segment): along the list each further piece
-    // advances one or the other.
-    const uint32_t pre_slot = (uint32_t)(16 * kTiles) * (D + 2) * 4, own_slot = (uint32_t)p.rows * (D + 2) * 4;
-    const int pre_segments = p.kv_heads * p.n_tiles;
-    char* const pre_part = (char*)p.part;
-    char* const own_part = pre_part + (kShared ? (size_t)(p.n_groups + pre_segments) * pre_slot : 0);
+    const Slots<D> slots(p, kShared);
     float* const red = (float*)lds;  // [wave][row][kPitch]
 
     // A tile's rows, folded over the columns and the waves of the workgroup: to_row(row, d, values of four dims, m, l).
@@ -551,77 +649,6 @@ __global__ __launch_bounds__(64 * kWaves, kShared || D == 256 ? 1 : 2) void page
         }
         __syncthreads();
     };
-    auto put_out = [&](int seq, int head, int d, f32x4_t o) __attribute__((always_inline)) {
-        if (kWhole || d < dim) *(u32x2_t*)(p.out + ((size_t)seq * p.heads + head) * dim + d) = u32x2_t{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
-    };
-    // All partials of `rows` heads from `head` on of sequence `seq`: n_pre of the prefix, rows of theirs from pre_row on, and n_own.
-    auto join = [&](int seq, int head, int rows, __amdgpu_buffer_rsrc_t pre, int n_pre, int pre_row, __amdgpu_buffer_rsrc_t own, int n_own) __attribute__((always_inline)) {
-        constexpr int kAhead = 8;
-        float* const wgt = (float*)lds;  // [pieces][16]
-        float* const wl = wgt + kMaxPieces * 16;
-        f32x4_t* const part = (f32x4_t*)(wl + kMaxPieces * 16);
-        const int pieces = n_pre + n_own, items = rows * (D / 4), sub_n = items >= NT ? 1 : NT / items;
-        const int x0 = sub_n == 1 ? tid : tid % items, sub = sub_n == 1 ? 0 : tid / items;
-        f32x4_t a[kAhead];
-        auto ask = [&](int i, int k0) __attribute__((always_inline)) {  // (row and element follow one another in a slot)
-            const uint32_t from = 16u * (uint32_t)min(i, items - 1);
-#pragma unroll
-            for (int e = 0; e < kAhead; e++) {
-                const int k = min(k0 + e * sub_n, pieces - 1);
-                a[e] = kShared && k < n_pre ? get4(pre, (uint32_t)k * pre_slot + (uint32_t)(pre_row * D * 4) + from) : get4(own, (uint32_t)(k - n_pre) * own_slot + from);
-            }
-        };
-        ask(x0, sub);
-        {
-            const int row = tid >> 4, col = tid & 15;  // sixteen lanes a row
-            const bool on = row < rows;
-            float top = kNoMax, sum = 0.0f;
-            for (int k = col; on && k < pieces; k += 16) {
-                const u32x2_t ml = kShared && k < n_pre ? get2(pre, (uint32_t)k * pre_slot + 4u * (uint32_t)(16 * kTiles * D + 2 * (pre_row + row)))
-                                                        : get2(own, (uint32_t)(k - n_pre) * own_slot + 4u * (uint32_t)(p.rows * D + 2 * row));
-                wgt[k * 16 + row] = __uint_as_float(ml[0]);
-                wl[k * 16 + row] = __uint_as_float(ml[1]);
-                top = fmaxf(top, __uint_as_float(ml[0]));
-            }
-            top = columns_max<16>(top);
-            for (int k = col; on && k < pieces; k += 16) {
-                const float fk = __builtin_amdgcn_exp2f((wgt[k * 16 + row] - top) * p.scale_log2e);
-                wgt[k * 16 + row] = fk;
-                sum += wl[k * 16 + row] * fk;
-            }
-            sum = columns_sum<16>(sum);
-            if (on && col == 0) inv_l[row] = sum == 0.0f ? 0.0f : 1.0f / sum;
-        }
-        __syncthreads();
-        for (int i0 = 0; i0 < items; i0 += NT) {
-            const int i = i0 + x0;
-            const bool on = i < items && sub < sub_n;
-            const int row = on ? i / (D / 4) : 0, d = 4 * (i % (D / 4));
-            f32x4_t o = {0, 0, 0, 0};
-            for (int k0 = sub; on && k0 < pieces; k0 += kAhead * sub_n) {
-                if (i0 || k0 != sub) ask(i, k0);
-#pragma unroll
-                for (int e = 0; e < kAhead; e++)
-                    if (k0 + e * sub_n < pieces) o += a[e] * wgt[(k0 + e * sub_n) * 16 + row];
-            }
-            if (sub_n > 1) {  // (one round)
-                part[tid] = o;
-                __syncthreads();
-                if (on && sub == 0)
-                    for (int e = 1; e < sub_n; e++) o += part[e * items + tid];
-            }
-            if (on && sub == 0) put_out(seq, head + row, d, o * inv_l[row]);
-        }
-        __syncthreads();
-    };
-    // where the prefix's partials for a kv head's tile are
-    auto pre_pieces = [&](int seg, int& w0) __attribute__((always_inline)) {
-        const int f = seg * span.pre_places;
-        w0 = quotient(f + kStart, span.size);
-        return quotient(f + span.pre_places - 1, span.size) - w0 + 1;
-    };
-    auto word_of = [&](int seq, int head_of_kv, int piece) { return p.words + (((size_t)seq * p.kv_heads + head_of_kv) * p.chunks + piece) * kWordPitch; };
-
     while (at < span.end) {
         if (kShared && at < span.pre_total) {
             // ---- a piece of the prefix
@@ -630,15 +657,9 @@ __global__ __launch_bounds__(64 * kWaves, kShared || D == 256 ? 1 : 2) void page
             at = min(seg_first + span.pre_places, span.end);
             if (t1 <= 0) continue;  // (places alone)
             const int kvh = quotient(seg, p.n_tiles), tile = seg - kvh * p.n_tiles;
-            int w0;
-            const int pieces = pre_pieces(seg, w0);
-            // the tile's units, (sequence, piece of the kv head's query heads): unit `tid` is this thread's to count
+            const int w0 = quotient(seg_first + kStart, span.size), pieces = quotient(seg_first + span.pre_places - 1, span.size) - w0 + 1;
+            // the tile's units, (sequence, piece of the kv head's query heads)
             const int unit0 = tile * p.per_tile, units = min(p.per_tile, p.batch * p.chunks - unit0);
-            const int my_seq = (unit0 + tid) / p.chunks, my_piece = unit0 + tid - my_seq * p.chunks;
-            const int my_len = tid < units ? len_of(p, my_seq) : -1;
-            const bool mine = tid < units && my_len >= span.shared;
-            UnitWord word;
-            if (mine) word.request(word_of(my_seq, kvh, my_piece), p.launch_id);
             // operands of q: row i of the tile is head i % rows of unit i / rows
             const int group_rows = p.rows;
             for (int i = tid; i < 16 * kTiles * (D / 8); i += NT) {
@@ -648,7 +669,6 @@ __global__ __launch_bounds__(64 * kWaves, kShared || D == 256 ? 1 : 2) void page
                 if (u < units && h < p.group && (kWhole || 8 * c < dim)) q = *(const u32x4_t*)(p.q + ((size_t)seq * p.heads + kvh * p.group + h) * dim + 8 * c);
                 *(u32x4_t*)(prefix_q + row * kQPitch + 16 * c) = q;
             }
-            if (mine) word.replace();
             __syncthreads();
             State<D> st[kTiles];
 #pragma unroll
@@ -659,34 +679,13 @@ __global__ __launch_bounds__(64 * kWaves, kShared || D == 256 ? 1 : 2) void page
                     return *(const u32x4_t*)(prefix_q + (16 * i + n) * kQPitch + 64 * c + 16 * quad);
                 }, 0, quad, p.scale_log2e);
             }
-            const __amdgpu_buffer_rsrc_t rs = rsrc_of(pre_part + ((size_t)w0 + seg) * pre_slot, (uint32_t)pieces * pre_slot);
-            const uint32_t to = (uint32_t)(group - w0) * pre_slot;
+            const __amdgpu_buffer_rsrc_t rs = slots.of_pre(w0, seg, pieces);
+            const uint32_t to = (uint32_t)(group - w0) * Slots<D>::kPre;
 #pragma unroll
             for (int i = 0; i < kTiles; i++)
                 fold(st[i], std::integral_constant<int, 1>{}, 16,
                      [&](int row, int d, f32x4_t o) __attribute__((always_inline)) { put4(rs, to + 4u * (uint32_t)((16 * i + row) * D + d), o); },
                      [&](int row, float m, float l) __attribute__((always_inline)) { put2(rs, to + 4u * (uint32_t)(16 * kTiles * D + 2 * (16 * i + row)), m, l); });
-            if (mine) word.settle();
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (tid < 64) is_last[tid] = 0;
-            if (mine) is_last[tid] = word.count(t1 - t0, steps_up_to(span.shared) + Own(my_len, span.shared).steps()) ? 1 : 0;
-            __syncthreads();
-            for (int u = 0; u < units; u++) {
-                if (!is_last[u]) continue;
-                const int seq = (unit0 + u) / p.chunks, piece = unit0 + u - seq * p.chunks, head = piece * p.rows;
-                int own_n = 0, own_w0 = 0;
-                const int own_steps = Own(len_of(p, seq), span.shared).steps();
-                if (own_steps > 0) {
-                    const int* where = (const int*)(word_of(seq, kvh, piece) + 8);
-                    own_w0 = __hip_atomic_load(where, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    own_n = __hip_atomic_load(where + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    own_w0 = __builtin_amdgcn_readfirstlane(own_w0);
-                    own_n = __builtin_amdgcn_readfirstlane(own_n);
-                }
-                const size_t segment = (size_t)seq * per + (size_t)kvh * p.chunks + piece;
-                join(seq, kvh * p.group + head, min(p.rows, p.group - head), rs, pieces, u * p.rows, rsrc_of(own_part + ((size_t)own_w0 + segment) * own_slot, (uint32_t)own_n * own_slot), own_n);
-            }
             continue;
         }
         // ---- a piece of a sequence's own keys
@@ -710,7 +709,7 @@ __global__ __launch_bounds__(64 * kWaves, kShared || D == 256 ? 1 : 2) void page
         const bool there = n % kR < rows;
 
         UnitWord word;
-        if (!alone && tid == 0) word.request(word_of(b, kvh, piece), p.launch_id);
+        if (!kShared && !alone && tid == 0) word.request(word_of(p, b, kvh, piece), p.launch_id);
         u32x4_t q[D / 32];
         const uint16_t* q_row = p.q + ((size_t)b * p.heads + kvh * p.group + head + (there ? n % kR : 0)) * dim;
 #pragma unroll
@@ -718,49 +717,56 @@ __global__ __launch_bounds__(64 * kWaves, kShared || D == 256 ? 1 : 2) void page
             q[c] = u32x4_t{0, 0, 0, 0};
             if (there && (kWhole || 32 * c + 8 * quad < dim)) q[c] = *(const u32x4_t*)(q_row + 32 * c + 8 * quad);
         }
-        if (!alone && tid == 0) word.replace();
+        if (!kShared && !alone && tid == 0) word.replace();
         State<D> st[1];
         st[0].reset();
         {
             Walk<D, kWhole> w(p, p.page_table + (size_t)b * p.table_pages, kvh, own.lo, len, own.first() + t0 + wave, own.first() + t1, lane);
             walk<D, C, 1, kWhole, true>(st, w, lanes, [&](int, int c) __attribute__((always_inline)) { return q[c]; }, cls, quad, p.scale_log2e);
         }
-        const __amdgpu_buffer_rsrc_t rs = rsrc_of(own_part + ((size_t)w0 + segment) * own_slot, (uint32_t)pieces * own_slot);
-        const uint32_t to = (uint32_t)(group - w0) * own_slot;
+        const __amdgpu_buffer_rsrc_t rs = slots.of_own(w0, segment, pieces);
+        const uint32_t to = (uint32_t)(group - w0) * slots.own_bytes;
+        if (kShared && tid == 0) *(UnitLine*)word_of(p, b, kvh, piece) = UnitLine{w0, alone ? -1 : pieces};
         fold(st[0], std::integral_constant<int, C>{}, rows,
              [&](int row, int d, f32x4_t o) __attribute__((always_inline)) {
-                 if (alone) put_out(b, kvh * p.group + head + row, d, o * inv_l[row]);
+                 if (alone) put_out(p, dim, b, kvh * p.group + head + row, d, o * inv_l[row]);
                  else put4(rs, to + 4u * (uint32_t)(row * D + d), o);
              },
              [&](int row, float m, float l) __attribute__((always_inline)) {
                  if (!alone) put2(rs, to + 4u * (uint32_t)(p.rows * D + 2 * row), m, l);
              });
-        if (alone) continue;
-        if (tid == 0) {
-            word.settle();
-            if (kShared && own.lo > 0) {  // for whoever joins them
-                int* where = (int*)(word_of(b, kvh, piece) + 8);
-                __hip_atomic_store(where, w0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                __hip_atomic_store(where + 1, pieces, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-        }
+        if (kShared || alone) continue;
+        if (tid == 0) word.settle();
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (tid == 0) is_last[0] = word.count(t1 - t0, own.steps() + (own.lo > 0 ? steps_up_to(span.shared) : 0)) ? 1 : 0;
+        if (tid == 0) is_last = word.count(pieces) ? 1 : 0;
         __syncthreads();
-        if (is_last[0]) {
-            int n_pre = 0, pre_w0 = 0, pre_row = 0;
-            __amdgpu_buffer_rsrc_t pre = rs;
-            if (kShared && own.lo > 0) {
-                const int unit = b * p.chunks + piece, tile = quotient(unit, p.per_tile), pre_seg = kvh * p.n_tiles + tile;
-                n_pre = pre_pieces(pre_seg, pre_w0);
-                pre_row = (unit - tile * p.per_tile) * p.rows;
-                pre = rsrc_of(pre_part + ((size_t)pre_w0 + pre_seg) * pre_slot, (uint32_t)n_pre * pre_slot);
-            }
-            join(b, kvh * p.group + head, rows, pre, n_pre, pre_row, rs, pieces);
-        }
+        if (is_last) join<D, false>(p, lds, inv_l, dim, b, kvh * p.group + head, rows, rs, 0, 0, rs, pieces);
         __syncthreads();
     }
+}
+
+// With a prefix: a workgroup for each unit, grid (pieces of a kv head's query heads, kv heads, batch).
+template <int D>
+__global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedDecodeParams p) {
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kJoinLds];
+    __shared__ float inv_l[16];
+    const int piece = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+    const ListHead list = *(const ListHead*)p.head;
+    const Own own(len_of(p, b), list.shared);
+    if (own.len == 0) return;  // (written already)
+    const UnitLine line = own.steps() > 0 ? *(const UnitLine*)word_of(p, b, kvh, piece) : UnitLine{0, 0};
+    if (line.pieces < 0) return;
+    const Slots<D> slots(p, true);
+    const int unit = b * p.chunks + piece, tile = quotient(unit, p.per_tile), segment = kvh * p.n_tiles + tile, head = piece * p.rows;
+    int w0 = 0, n_pre = 0;
+    if (own.lo > 0) {
+        const int first = segment * list.pre_places;
+        w0 = quotient(first + kStart, list.size);
+        n_pre = quotient(first + list.pre_places - 1, list.size) - w0 + 1;
+    }
+    join<D, true>(p, lds, inv_l, p.dim, b, kvh * p.group + head, min(p.rows, p.group - head), slots.of_pre(w0, segment, n_pre), n_pre, (unit - tile * p.per_tile) * p.rows,
+                  slots.of_own(line.w0, ((size_t)b * p.kv_heads + kvh) * p.chunks + piece, line.pieces), line.pieces);
 }
 
 template <int D, bool kWhole, bool kShared>
@@ -769,6 +775,7 @@ hipError_t launch_as(hipStream_t stream, const PagedDecodeParams& p) {
     if (p.rows <= 4) hipLaunchKernelGGL((paged_decode_kernel<D, 4, kWhole, kShared>), grid, block, 0, stream, p);
     else if (p.rows <= 8) hipLaunchKernelGGL((paged_decode_kernel<D, 2, kWhole, kShared>), grid, block, 0, stream, p);
     else hipLaunchKernelGGL((paged_decode_kernel<D, 1, kWhole, kShared>), grid, block, 0, stream, p);
+    if (kShared) hipLaunchKernelGGL(paged_join_kernel<D>, dim3(p.chunks, p.kv_heads, p.batch), block, 0, stream, p);
     return hipGetLastError();
 }
 template <int D>
@@ -802,7 +809,7 @@ Plan plan_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_
     a.groups = (a.groups + 7) / 8 * 8;
     auto round = [](size_t x) { return (x + 255) / 256 * 256; };
     a.part_bytes = round((size_t)(a.groups + a.pre_segments) * (size_t)tile_rows * (size_t)(a.dim + 2) * 4 + (size_t)(a.groups + a.own_segments) * (size_t)a.rows * (size_t)(a.dim + 2) * 4);
-    a.word_bytes = (size_t)a.own_segments * kWordPitch;
+    a.word_bytes = (size_t)a.own_segments * kWordPitch + 256;
     return a;
 }
 static_assert(prefix_tiles<64>() == 4 && prefix_tiles<128>() == 4 && prefix_tiles<256>() == 2, "the plan's rows of a tile");
@@ -870,8 +877,9 @@ RT_API int rt_gqa_decode_paged_bf16(void* stream, const void* q, const void* k_p
     p.span_root = a.rows <= 4 ? 0.66f : 1.0f;
     p.scale_log2e = (1.0f / sqrtf((float)head_dim)) * kLog2eHost;
     p.part = (float*)workspace;
-    p.words = (unsigned char*)workspace + a.part_bytes;
-    p.launch_id = next_launch_id() << 16;  // (its low 24 bits zero)
+    p.head = (unsigned char*)workspace + a.part_bytes;
+    p.words = p.head + 256;
+    p.launch_id = next_launch_id() << 8;  // (its low 16 bits zero)
     const bool shared = shared_lens || shared_len > 0;
     p.n_groups = std::min(a.groups, kCus * per_cu(a.dim, shared));
     const hipStream_t s = (hipStream_t)stream;

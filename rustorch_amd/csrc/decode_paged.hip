@@ -268,7 +268,7 @@ __device__ __forceinline__ void* word_of(const PagedDecodeParams& p, int seq, in
 // Slots of the prefix's come first, then those of the sequences'.  A piece's number is (workgroup + segment): along the list each further
 // piece advances one or the other.  A slot: rows of D floats, then their (m, l).
 template <int D>
-constexpr int prefix_tiles() { return D == 256 ? 2 : 4; }  // of sixteen query rows that a prefix's step serves
+constexpr int prefix_tiles() { return D == 256 ? 1 : D == 128 ? 2 : 4; }  // of sixteen query rows that a prefix's step serves
 template <int D>
 struct Slots {
     static constexpr int kTileRows = 16 * prefix_tiles<D>();
@@ -578,7 +578,7 @@ __device__ __forceinline__ void walk(State<D> (&st)[NT], Walk<D, kWhole>& at, co
 }
 
 template <int D, int C, bool kWhole, bool kShared>
-__global__ __launch_bounds__(64 * kWaves, kShared || D == 256 ? 1 : 2) void paged_decode_kernel(PagedDecodeParams p) {
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_kernel(PagedDecodeParams p) {
     constexpr int NT = kThreads, kPitch = D + 4, kR = 16 / C, kTiles = prefix_tiles<D>();
     constexpr int kFold = kWaves * 16 * kPitch * 4, kLds = kShared ? kFold : std::max(kFold, kJoinLds);
     constexpr int kQPitch = 2 * D + 16;  // bytes
@@ -785,7 +785,7 @@ hipError_t launch_dim(hipStream_t stream, const PagedDecodeParams& p, bool share
 }
 
 // Workgroups a CU, each with a wave on every SIMD.
-constexpr int per_cu(int64_t dim, bool shared) { return shared || dim == 256 ? 1 : 2; }
+constexpr int per_cu(int64_t dim, bool shared) { return dim == 256 ? 1 : 2; }
 // Segments, steps and workgroups of a call at its longest, and what its workspace holds.
 struct Plan {
     int64_t chunks, rows, per_tile, n_tiles, own_segments, pre_segments, places;
@@ -798,7 +798,7 @@ Plan plan_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_
     a.dim = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
     a.chunks = (group + 15) / 16;
     a.rows = (group + a.chunks - 1) / a.chunks;
-    const int64_t tile_rows = a.dim == 256 ? 32 : 64;
+    const int64_t tile_rows = a.dim == 256 ? 16 : a.dim == 128 ? 32 : 64;
     a.per_tile = tile_rows / a.rows;
     a.n_tiles = (batch * a.chunks + a.per_tile - 1) / a.per_tile;
     a.own_segments = batch * kv_heads * a.chunks;
@@ -812,7 +812,7 @@ Plan plan_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_
     a.word_bytes = (size_t)a.own_segments * kWordPitch + 256;
     return a;
 }
-static_assert(prefix_tiles<64>() == 4 && prefix_tiles<128>() == 4 && prefix_tiles<256>() == 2, "the plan's rows of a tile");
+static_assert(prefix_tiles<64>() == 4 && prefix_tiles<128>() == 2 && prefix_tiles<256>() == 1, "the plan's rows of a tile");
 
 }  // namespace
 

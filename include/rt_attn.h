@@ -487,7 +487,7 @@ int rt_flash_forward_packed_bf16_dev(void *stream, const rt_attention_shape *sha
  * keys, or none in pages) gives rows of +0.0.  kv head = h / (n_heads / n_kv), any number of heads a group.  f32 accumulation and
  * softmax, weights of one bf16 each, one rounding to bf16 at the end.  What is not seen does not count, whatever it holds; a dim in which a
  * V row that is seen is infinite or NaN comes out infinite or NaN.  The last bits of a sequence may depend on what else is in the batch (how its keys are cut into spans); the same call gives the same bits
- * every time.  table_pages * page_size up to 2^28.  `workspace`: rt_gqa_decode_paged_workspace_bytes(...) bytes of device memory, 16-byte
+ * every time.  table_pages * page_size up to 2^28, a page of K below 2 GiB.  `workspace`: rt_gqa_decode_paged_workspace_bytes(...) bytes of device memory, 16-byte
  * aligned (RT_ERR_WORKSPACE_TOO_SMALL), which the call works in alone and keeps nothing in: calls that may overlap (other streams,
  * graphs replayed side by side) have workspaces of their own. */
 size_t rt_gqa_decode_paged_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim,

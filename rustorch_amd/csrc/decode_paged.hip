@@ -322,7 +322,7 @@ __device__ __forceinline__ void join(const PagedDecodeParams& p, unsigned char* 
         }
         top = columns_max<16>(top);
         for (int k = col; on && k < pieces; k += 16) {
-            const float fk = __builtin_amdgcn_exp2f((wgt[k * 16 + row] - top) * p.scale_log2e);
+            const float fk = __builtin_amdgcn_exp2f(wgt[k * 16 + row] - top);
             wgt[k * 16 + row] = fk;
             sum += wl[k * 16 + row] * fk;
         }
@@ -387,14 +387,17 @@ template <int D, bool kWhole>
 struct Walk {
     const PagedDecodeParams& p;
     const int32_t* table;  // the sequence's
-    const int kvh, lo, hi, first, end, lane;
-    const uint32_t row_bytes;
+    const int lo, hi, first, end, lane;
+    const uint32_t row_bytes, page_bytes;
+    const char *k_head, *v_head;  // the kv head's first row in page 0
     int entry[2];  // lane i: the pages of the two sixteens of the wave's i-th step from the last refill on
     __amdgpu_buffer_rsrc_t ks[2], vs[2];
     uint32_t seen;  // of the step whose place was taken last: a bit for every key that is there
 
     __device__ __forceinline__ Walk(const PagedDecodeParams& params, const int32_t* row, int kv_head, int from, int to, int step0, int step1, int l)
-        : p(params), table(row), kvh(kv_head), lo(from), hi(to), first(step0), end(step1), lane(l), row_bytes(2u * (uint32_t)(kWhole ? D : params.dim)) {}
+        : p(params), table(row), lo(from), hi(to), first(step0), end(step1), lane(l), row_bytes(2u * (uint32_t)(kWhole ? D : params.dim)),
+          page_bytes(((uint32_t)params.kv_heads << params.page_shift) * row_bytes), k_head((const char*)params.k_pages + ((size_t)kv_head << params.page_shift) * row_bytes),
+          v_head((const char*)params.v_pages + ((size_t)kv_head << params.page_shift) * row_bytes) {}
     __device__ __forceinline__ void refill(int t) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -402,20 +405,38 @@ struct Walk {
             entry[h] = table[(int)min(row >> p.page_shift, (long long)p.table_pages - 1)];
         }
     }
-    // the descriptors of step t, the wave's i-th
+    // The descriptors of step t, the wave's i-th.  (What they are made of is said to be the same in all lanes, which the compiler does not
+    // see: it would ask for each lane's descriptor by itself.)
     __device__ __forceinline__ void place(int t, int i) {
         if ((i & 63) == 0) refill(t);
-        seen = 0;
+        const int row = t * kStep;
+        const uint32_t mask = (1u << p.page_shift) - 1;
+        int rows[2], skip[2] = {0, 0};
+        uint64_t at[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int page = __builtin_amdgcn_readlane(entry[h], i & 63), row = t * kStep + 16 * h;
-            const bool there = page >= 0 && page < p.n_pages;
-            const uint32_t in_page = (uint32_t)row & ((1u << p.page_shift) - 1);
-            const uint64_t at = ((((uint64_t)(there ? page : 0) * (uint32_t)p.kv_heads + (uint32_t)kvh) << p.page_shift) + in_page) * row_bytes;
-            const int rows = there ? min(max(hi - row, 0), 16) : 0, skip = min(max(lo - row, 0), 16);
-            ks[h] = rsrc_of((const char*)p.k_pages + at, (uint32_t)rows * row_bytes);
-            vs[h] = rsrc_of((const char*)p.v_pages + at, (uint32_t)rows * row_bytes);
-            seen |= (((1u << rows) - 1) & ~((1u << skip) - 1)) << (16 * h);
+            const uint32_t page = (uint32_t)__builtin_amdgcn_readlane(entry[h], i & 63);
+            const bool there = page < (uint32_t)p.n_pages;
+            at[h] = (uint64_t)(there ? page : 0u) * page_bytes + (((uint32_t)row + 16u * h) & mask) * row_bytes;
+            rows[h] = there ? 16 : 0;
+        }
+        seen = (rows[0] ? 0xffffu : 0u) | (rows[1] ? 0xffff0000u : 0u);
+        if (row < lo || row + kStep > hi) {  // the first or last step of a sequence
+            seen = 0;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                rows[h] = min(max(hi - row - 16 * h, 0), rows[h]);
+                skip[h] = min(max(lo - row - 16 * h, 0), 16);
+                seen |= (((1u << rows[h]) - 1) & ~((1u << skip[h]) - 1)) << (16 * h);
+            }
+            seen = (uint32_t)__builtin_amdgcn_readfirstlane((int)seen);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint64_t from = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at[h] >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at[h]);
+            const uint32_t bytes = (uint32_t)__builtin_amdgcn_readfirstlane(rows[h]) * row_bytes;
+            ks[h] = rsrc_of(k_head + from, bytes);
+            vs[h] = rsrc_of(v_head + from, bytes);
         }
     }
     __device__ __forceinline__ void load_k(Keys<D>& x, const Lanes<D, kWhole>& at) const {
@@ -503,8 +524,8 @@ __device__ __forceinline__ void step(State<D> (&st)[NT], Keys<D>& x, QOf q_of, K
         }
     }
     k_done();
-    // The running maximum, common to the four lanes of a column.  It follows the scores only where they have risen by 8 in the exponent of
-    // two: up to there sums of weights in f32 and weights of 8 bits are as exact, and sums are scaled once or twice a span.
+    // The running maximum, common to the four lanes of a column, in the exponent of two.  It follows the scores only where they have risen by 8 in it: up to
+    // there sums of weights in f32 and weights of 8 bits are as exact, and sums are scaled once or twice a span.
     float top[NT];
     bool risen = false;
 #pragma unroll
@@ -513,12 +534,13 @@ __device__ __forceinline__ void step(State<D> (&st)[NT], Keys<D>& x, QOf q_of, K
 #pragma unroll
         for (int e = 1; e < kE; e++) top[i] = fmaxf(top[i], y[i][e]);
         top[i] = quad_max(top[i]);
-        risen = risen || (top[i] - st[i].m) * scale_log2e > 8.0f;
+        top[i] *= scale_log2e;
+        risen = risen || top[i] - st[i].m > 8.0f;
     }
     if (__any(risen)) {
 #pragma unroll
         for (int i = 0; i < NT; i++) {
-            const float m_new = fmaxf(st[i].m, top[i]), alpha = __builtin_amdgcn_exp2f((st[i].m - m_new) * scale_log2e);
+            const float m_new = fmaxf(st[i].m, top[i]), alpha = __builtin_amdgcn_exp2f(st[i].m - m_new);
             st[i].m = m_new;
             st[i].l *= alpha;
 #pragma unroll
@@ -531,7 +553,7 @@ __device__ __forceinline__ void step(State<D> (&st)[NT], Keys<D>& x, QOf q_of, K
         float f[kE];
 #pragma unroll
         for (int e = 0; e < kE; e++) {
-            f[e] = __builtin_amdgcn_exp2f((y[i][e] - st[i].m) * scale_log2e);
+            f[e] = __builtin_amdgcn_exp2f(fmaf(y[i][e], scale_log2e, -st[i].m));
             st[i].l += f[e];
         }
         // pairs of weights as the operand's words, zeros in the other columns' places
@@ -605,7 +627,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
     // A tile's rows, folded over the columns and the waves of the workgroup: to_row(row, d, values of four dims, m, l).
     auto fold = [&](State<D>& st, auto c_of, int rows, auto to_row, auto to_ml) __attribute__((always_inline)) {
         constexpr int kC = decltype(c_of)::value, kRows = 16 / kC;
-        const float m = columns_max<kC>(st.m), f = __builtin_amdgcn_exp2f((st.m - m) * p.scale_log2e);
+        const float m = columns_max<kC>(st.m), f = __builtin_amdgcn_exp2f(st.m - m);
         const float l = columns_sum<kC>(quad_sum(st.l) * f);
         if (kC > 1)
 #pragma unroll
@@ -621,9 +643,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
 #pragma unroll
         for (int w = 1; w < kWaves; w++) m_wg = fmaxf(m_wg, red_m[w][n % kRows]);
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) l_wg += red_l[w][n % kRows] * __builtin_amdgcn_exp2f((red_m[w][n % kRows] - m_wg) * p.scale_log2e);
+        for (int w = 0; w < kWaves; w++) l_wg += red_l[w][n % kRows] * __builtin_amdgcn_exp2f(red_m[w][n % kRows] - m_wg);
         if (n < kRows) {
-            const float fw = __builtin_amdgcn_exp2f((m - m_wg) * p.scale_log2e);
+            const float fw = __builtin_amdgcn_exp2f(m - m_wg);
             float* row = red + (wave * kRows + n) * kPitch;
 #pragma unroll
             for (int c = 0; c < D / 32; c++) {  // eight dims in a row
@@ -842,7 +864,7 @@ RT_API int rt_gqa_decode_paged_bf16(void* stream, const void* q, const void* k_p
         return fail(err, RT_ERR_KV_OVERFLOW, -1, (uint64_t)max_len, (uint64_t)(int64_t)shared_len, "a prefix behind the page table");
     if (batch == 0 || n_heads == 0) return RT_OK;
     const Plan a = plan_of(batch, n_heads, n_kv, head_dim, max_len);
-    if (batch > 65535 || n_heads > 65535 || max_len > (1 << 28) || a.places > 0x7fffffffll - (1 << 20))
+    if (batch > 65535 || n_heads > 65535 || max_len > (1 << 28) || (int64_t)n_kv * page_size * head_dim >= (1ll << 30) || a.places > 0x7fffffffll - (1 << 20))
         return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "shape too large for the launch grid");
     if (!q || !out || !kv_lens || (max_len > 0 && (!page_table || (n_pages > 0 && (!k_pages || !v_pages))))) return fail(err, RT_ERR_NULL_POINTER, -1, 0, 0, "NULL buffer");
     if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out) & 15) return fail(err, RT_ERR_UNSUPPORTED, -1, 16, 0, "q, out and the pages must be 16-byte aligned");

@@ -7,8 +7,10 @@
 // a step crosses lanes but the running maximum.  A step's two sixteens of rows lie in a page each, whose place is looked up ahead; K
 // and V come through descriptors that end with the last key's row, so that rows behind it are zeros and are not read.
 //
-// A sequence's own keys meet the up to sixteen query rows of one kv head.  The prefix's keys meet those of the whole batch: the rows of
-// all sequences that share it form tiles of 16 kTiles rows, whose operands wait in LDS, and a step's keys are asked for once for a tile.
+// A sequence's own keys meet the up to sixteen query rows of one kv head, through registers.  The prefix's keys meet those of the whole
+// batch, through LDS: the waves of a workgroup have 32 query rows each, of the sequences that share the prefix, in the larger matrix
+// instruction's layout, and walk the same keys, which come straight to LDS once for all four (each wave with steps of its own through
+// registers, sixteen rows an instruction: 36 us for 64 sequences behind 8192 keys alone, at 15 TB/s from the L2s).
 // Both kinds of segments, (kv head, tile) of the prefix and (sequence, kv head), form one list of steps that is cut into equal
 // spans, one a workgroup of four waves, which deal the steps of a segment among themselves and fold what they have through LDS.  What a
 // workgroup finishes of a sequence it writes at once, where that is all there is; otherwise it leaves a partial (o, m, l).  Without a
@@ -20,6 +22,7 @@
 #include <type_traits>
 
 #include "cache_paged.hpp"
+#include "flash_tile_lds.hpp"
 #include "rt_common.hpp"
 #include "rt_host.hpp"
 #include "rt_kernels.hpp"
@@ -164,9 +167,9 @@ __device__ __forceinline__ Span span_of(const PagedDecodeParams& p, int& group, 
         any = any || (kShared && __any(len >= s.shared));
     }
     if (!any) s.shared = 0;  // (then every `lo` was 0 already)
-    s.pre_places = s.shared > 0 ? kStart + steps_up_to(s.shared) : 0;
+    s.pre_places = s.shared > 0 ? kStart + steps_up_to(s.shared) * p.pre_cost : 0;
     s.pre_total = s.pre_places * p.kv_heads * p.n_tiles;
-    most = max(most, s.shared > 0 ? steps_up_to(s.shared) : 0);
+    most = max(most, s.pre_places);
     s.total = s.pre_total + sum * per;
     // what one of all workgroups gets, but no fewer than a join is worth (a segment of few spans is a long walk, one of many a long join:
     // their sum is least around the root of its steps), and never more of them than a sequence may have
@@ -265,47 +268,52 @@ __device__ __forceinline__ void* word_of(const PagedDecodeParams& p, int seq, in
 }
 
 // ---- partials ----------------------------------------------------------------------------------------------------------------
-// Slots of the prefix's come first, then those of the sequences'.  A piece's number is (workgroup + segment): along the list each further
-// piece advances one or the other.  A slot: rows of D floats, then their (m, l).
-template <int D>
-constexpr int prefix_tiles() { return D == 256 ? 1 : D == 128 ? 2 : 4; }  // of sixteen query rows that a prefix's step serves
+// Slots of the prefix's come first, four a piece, one a wave, then those of the sequences'.  A piece's number is (workgroup + segment): along
+// the list each further piece advances one or the other.  A sequence's slot: rows of D floats, then their (m, l).  A wave's: o as the
+// registers hold it, 16 bytes a lane and request, then the rows' (m, l).
+constexpr int kWaveRows = 32;
 template <int D>
 struct Slots {
-    static constexpr int kTileRows = 16 * prefix_tiles<D>();
-    static constexpr uint32_t kPre = (uint32_t)kTileRows * (D + 2) * 4;
+    static constexpr uint32_t kWave = (uint32_t)kWaveRows * (D + 2) * 4, kPre = kWaves * kWave;
     char *pre, *own;
     uint32_t own_bytes;
     __device__ __forceinline__ Slots(const PagedDecodeParams& p, bool shared)
         : pre((char*)p.part), own((char*)p.part + (shared ? (size_t)(p.n_groups + p.kv_heads * p.n_tiles) * kPre : 0)), own_bytes((uint32_t)p.rows * (D + 2) * 4) {}
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t of_pre(int w0, int segment, int n) const { return rsrc_of(pre + ((size_t)w0 + segment) * kPre, (uint32_t)n * kPre); }
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t of_own(int w0, size_t segment, int n) const { return rsrc_of(own + ((size_t)w0 + segment) * own_bytes, (uint32_t)n * own_bytes); }
+    // Byte, in a wave's slot, of four dims from d on of row `row`; of its (m, l).
+    static __device__ __forceinline__ uint32_t at(int row, int d) {  // lane (row, d / 4 % 2) has eight dims' half, d / 8 by d / 8
+        return (uint32_t)(d / 8 * 1024 + ((d / 4 & 1) * 32 + row) * 16);
+    }
+    static __device__ __forceinline__ uint32_t at_ml(int row) { return (uint32_t)(kWaveRows * D * 4 + 8 * row); }
 };
 // Four dims of a row of the output.
 __device__ __forceinline__ void put_out(const PagedDecodeParams& p, int dim, int seq, int head, int d, f32x4_t o) {
     if (d < dim) *(u32x2_t*)(p.out + ((size_t)seq * p.heads + head) * dim + d) = u32x2_t{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
 }
 constexpr int kThreads = 64 * kWaves;
-constexpr int kJoinLds = kMaxPieces * 16 * 8 + kThreads * 16;
-// All partials of `rows` heads from `head` on of sequence `seq`, by the whole workgroup: n_pre of the prefix, rows of theirs from pre_row on, and
-// n_own.  Items of four elements, kAhead pieces of each at a time; where there are fewer items than threads, several threads an item, each
+constexpr int join_lds(int pieces, int rows) { return kThreads * 16 + pieces * rows * 8; }
+// All partials of `rows` heads from `head` on of sequence `seq`, by the whole workgroup: n_pre of the prefix, wave pre_wave's,
+// rows of theirs from pre_row on, and n_own.  Items of four elements, kAhead pieces of each at a time; where there are fewer items than threads, several threads an item, each
 // with every sub-th piece.  The first are asked for ahead of the (m, l) that their weights are made of.
 template <int D, bool kShared>
-__device__ __forceinline__ void join(const PagedDecodeParams& p, unsigned char* lds, float* inv_l, int dim, int seq, int head, int rows, __amdgpu_buffer_rsrc_t pre, int n_pre, int pre_row, __amdgpu_buffer_rsrc_t own, int n_own) {
-    constexpr int kAhead = 8, NT = kThreads;
-    constexpr uint32_t kPre = Slots<D>::kPre;
+__device__ __forceinline__ void join(const PagedDecodeParams& p, unsigned char* lds, float* inv_l, int dim, int seq, int head, int rows, __amdgpu_buffer_rsrc_t pre, int n_pre, int pre_wave, int pre_row, __amdgpu_buffer_rsrc_t own, int n_own) {
+    constexpr int kAhead = 8, NT = kThreads, kMost = kMaxPieces;
+    auto pre_at = [&](int k) __attribute__((always_inline)) { return (uint32_t)(k * kWaves + pre_wave) * Slots<D>::kWave; };
     const uint32_t own_slot = (uint32_t)p.rows * (D + 2) * 4;
-    float* const wgt = (float*)lds;  // [pieces][16]
-    float* const wl = wgt + kMaxPieces * 16;
-    f32x4_t* const part = (f32x4_t*)(wl + kMaxPieces * 16);
+    f32x4_t* const part = (f32x4_t*)lds;
+    float* const wgt = (float*)(part + NT);  // [pieces][p.rows]
+    float* const wl = wgt + kMost * p.rows;
     const int tid = threadIdx.x, pieces = n_pre + n_own, items = rows * (D / 4), sub_n = items >= NT ? 1 : NT / items;
     const int x0 = sub_n == 1 ? tid : tid % items, sub = sub_n == 1 ? 0 : tid / items;
     f32x4_t a[kAhead];
     auto ask = [&](int i, int k0) __attribute__((always_inline)) {  // (row and element follow one another in a slot)
-        const uint32_t from = 16u * (uint32_t)min(i, items - 1);
+        const int it = min(i, items - 1);
+        const uint32_t from = 16u * (uint32_t)it, from_pre = Slots<D>::at(pre_row + it / (D / 4), 4 * (it % (D / 4)));
 #pragma unroll
         for (int e = 0; e < kAhead; e++) {
             const int k = min(k0 + e * sub_n, pieces - 1);
-            a[e] = kShared && k < n_pre ? get4(pre, (uint32_t)k * kPre + (uint32_t)(pre_row * D * 4) + from) : get4(own, (uint32_t)(k - n_pre) * own_slot + from);
+            a[e] = kShared && k < n_pre ? get4(pre, pre_at(k) + from_pre) : get4(own, (uint32_t)(k - n_pre) * own_slot + from);
         }
     };
     ask(x0, sub);
@@ -314,17 +322,17 @@ __device__ __forceinline__ void join(const PagedDecodeParams& p, unsigned char* 
         const bool on = row < rows;
         float top = kNoMax, sum = 0.0f;
         for (int k = col; on && k < pieces; k += 16) {
-            const u32x2_t ml = kShared && k < n_pre ? get2(pre, (uint32_t)k * kPre + 4u * (uint32_t)(Slots<D>::kTileRows * D + 2 * (pre_row + row)))
+            const u32x2_t ml = kShared && k < n_pre ? get2(pre, pre_at(k) + Slots<D>::at_ml(pre_row + row))
                                                     : get2(own, (uint32_t)(k - n_pre) * own_slot + 4u * (uint32_t)(p.rows * D + 2 * row));
-            wgt[k * 16 + row] = __uint_as_float(ml[0]);
-            wl[k * 16 + row] = __uint_as_float(ml[1]);
+            wgt[k * p.rows + row] = __uint_as_float(ml[0]);
+            wl[k * p.rows + row] = __uint_as_float(ml[1]);
             top = fmaxf(top, __uint_as_float(ml[0]));
         }
         top = columns_max<16>(top);
         for (int k = col; on && k < pieces; k += 16) {
-            const float fk = __builtin_amdgcn_exp2f(wgt[k * 16 + row] - top);
-            wgt[k * 16 + row] = fk;
-            sum += wl[k * 16 + row] * fk;
+            const float fk = __builtin_amdgcn_exp2f(wgt[k * p.rows + row] - top);
+            wgt[k * p.rows + row] = fk;
+            sum += wl[k * p.rows + row] * fk;
         }
         sum = columns_sum<16>(sum);
         if (on && col == 0) inv_l[row] = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -339,7 +347,7 @@ __device__ __forceinline__ void join(const PagedDecodeParams& p, unsigned char* 
             if (i0 || k0 != sub) ask(i, k0);
 #pragma unroll
             for (int e = 0; e < kAhead; e++)
-                if (k0 + e * sub_n < pieces) o += a[e] * wgt[(k0 + e * sub_n) * 16 + row];
+                if (k0 + e * sub_n < pieces) o += a[e] * wgt[(k0 + e * sub_n) * p.rows + row];
         }
         if (sub_n > 1) {  // (one round)
             part[tid] = o;
@@ -382,28 +390,30 @@ struct Lanes {
     }
 };
 
-// A walk over the keys [lo, hi) of one kv head of one sequence's pages, the wave's steps first, first + kWaves, ... below `end`.
+// A walk over the keys [lo, hi) of one kv head of one sequence's pages, the wave's steps first, first + stride, ... below `end`.
 template <int D, bool kWhole>
 struct Walk {
     const PagedDecodeParams& p;
     const int32_t* table;  // the sequence's
-    const int lo, hi, first, end, lane;
+    const int lo, hi, first, end, stride, lane;
     const uint32_t row_bytes, page_bytes;
     const char *k_head, *v_head;  // the kv head's first row in page 0
     int entry[2];  // lane i: the pages of the two sixteens of the wave's i-th step from the last refill on
     __amdgpu_buffer_rsrc_t ks[2], vs[2];
     uint32_t seen;  // of the step whose place was taken last: a bit for every key that is there
 
-    __device__ __forceinline__ Walk(const PagedDecodeParams& params, const int32_t* row, int kv_head, int from, int to, int step0, int step1, int l)
-        : p(params), table(row), lo(from), hi(to), first(step0), end(step1), lane(l), row_bytes(2u * (uint32_t)(kWhole ? D : params.dim)),
+    __device__ __forceinline__ Walk(const PagedDecodeParams& params, const int32_t* row, int kv_head, int from, int to, int step0, int step1, int every, int l)
+        : p(params), table(row), lo(from), hi(to), first(step0), end(step1), stride(every), lane(l), row_bytes(2u * (uint32_t)(kWhole ? D : params.dim)),
           page_bytes(((uint32_t)params.kv_heads << params.page_shift) * row_bytes), k_head((const char*)params.k_pages + ((size_t)kv_head << params.page_shift) * row_bytes),
           v_head((const char*)params.v_pages + ((size_t)kv_head << params.page_shift) * row_bytes) {}
     __device__ __forceinline__ void refill(int t) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const long long row = (long long)(t + kWaves * lane) * kStep + 16 * h;
+            const long long row = ((long long)t + stride * lane) * kStep + 16 * h;
             entry[h] = table[(int)min(row >> p.page_shift, (long long)p.table_pages - 1)];
         }
+        // (awaited here: behind the branch that this stands in, the compiler would wait in every step for whatever is under way)
+        asm volatile("" : "+v"(entry[0]), "+v"(entry[1]));
     }
     // The descriptors of step t, the wave's i-th.  (What they are made of is said to be the same in all lanes, which the compiler does not
     // see: it would ask for each lane's descriptor by itself.)
@@ -439,6 +449,20 @@ struct Walk {
             vs[h] = rsrc_of(v_head + from, bytes);
         }
     }
+    // The same of one of the two sixteens, as scalars, for rows that go to LDS; `seen` of both.  (lo is 0.)
+    u32x4_t ring_k, ring_v;
+    __device__ __forceinline__ void place_half(int t, int i, int h) {
+        if ((i & 63) == 0) refill(t);
+        const int row = t * kStep;
+        const uint32_t mask = (1u << p.page_shift) - 1;
+        const uint32_t page0 = (uint32_t)__builtin_amdgcn_readlane(entry[0], i & 63), page1 = (uint32_t)__builtin_amdgcn_readlane(entry[1], i & 63);
+        const int rows0 = page0 < (uint32_t)p.n_pages ? min(max(hi - row, 0), 16) : 0, rows1 = page1 < (uint32_t)p.n_pages ? min(max(hi - row - 16, 0), 16) : 0;
+        seen = (uint32_t)__builtin_amdgcn_readfirstlane((int)(((1u << rows0) - 1) | ((1u << rows1) - 1) << 16));
+        const int rows = h ? rows1 : rows0;
+        const uint64_t at = (uint64_t)(rows ? h ? page1 : page0 : 0u) * page_bytes + (((uint32_t)row + 16u * h) & mask) * row_bytes;
+        ring_k = make_rsrc(k_head + at, (uint32_t)rows * row_bytes);
+        ring_v = make_rsrc(v_head + at, (uint32_t)rows * row_bytes);
+    }
     __device__ __forceinline__ void load_k(Keys<D>& x, const Lanes<D, kWhole>& at) const {
 #pragma unroll
         for (int h = 0; h < 2; h++)
@@ -446,10 +470,9 @@ struct Walk {
             for (int c = 0; c < D / 32; c++)
                 *(u32x4_t*)(x.k[h] + 4 * c) = __builtin_amdgcn_raw_buffer_load_b128(ks[h], kWhole ? at.k[0] + 64u * c : at.k[kWhole ? 0 : c], 0, 0);
     }
-    // kOnce: past the caches, rows that no other workgroup asks for
-    template <bool kOnce>
+    // (past the caches: whole lines that no other workgroup asks for)
     __device__ __forceinline__ void load_v(Keys<D>& x, const Lanes<D, kWhole>& at) const {
-        constexpr int kAux = kOnce ? 2 : 0;  // nt
+        constexpr int kAux = 2;  // nt
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             if constexpr (D == 64) {
@@ -476,46 +499,36 @@ struct State {
     }
 };
 
-// One step for NT tiles of sixteen query rows, whose operands q_of(tile, c) gives.  k_done is called behind the last use of K.
-template <int D, int C, int NT, typename QOf, typename KDone>
-__device__ __forceinline__ void step(State<D> (&st)[NT], Keys<D>& x, QOf q_of, KDone k_done, uint32_t seen, int cls, int quad, float scale_log2e) {
-    static_assert(C == 1 || NT == 1);
+// One step.  k_done is called behind the last use of K.
+template <int D, int C, typename KDone>
+__device__ __forceinline__ void step(State<D>& st, Keys<D>& x, const u32x4_t (&q)[D / 32], KDone k_done, uint32_t seen, int cls, int quad, float scale_log2e) {
     constexpr int kE = 8 / C;
-    float y[NT][kE];
+    f32x4_t a[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-    for (int i = 0; i < NT; i++) {
-        f32x4_t a[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    for (int c = 0; c < D / 32; c++)
 #pragma unroll
-        for (int c = 0; c < D / 32; c++) {
-            const u32x4_t q = q_of(i, c);
+        for (int h = 0; h < 2; h++) a[h] = mfma(*(const u32x4_t*)(x.k[h] + 4 * c), q[c], a[h]);
+    float y[kE];
+    if constexpr (C == 1) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) a[h] = mfma(*(const u32x4_t*)(x.k[h] + 4 * c), q, a[h]);
-        }
-        if constexpr (C == 1) {
+        for (int e = 0; e < 8; e++) y[e] = a[e / 4][e % 4];
+    } else if constexpr (C == 2) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) y[i][e] = a[e / 4][e % 4];
-        } else if constexpr (C == 2) {
+        for (int e = 0; e < 4; e++) y[e] = cls ? a[1][e] : a[0][e];
+    } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[i][e] = cls ? a[1][e] : a[0][e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                // (of both sixteens first: two of one register group the compiler takes for an index into it, four selections)
-                const float a0 = cls & 2 ? a[1][e] : a[0][e], a2 = cls & 2 ? a[1][2 + e] : a[0][2 + e];
-                y[i][e] = cls & 1 ? a2 : a0;
-            }
+        for (int e = 0; e < 2; e++) {
+            // (of both sixteens first: two of one register group the compiler takes for an index into it, four selections)
+            const float a0 = cls & 2 ? a[1][e] : a[0][e], a2 = cls & 2 ? a[1][2 + e] : a[0][2 + e];
+            y[e] = cls & 1 ? a2 : a0;
         }
     }
     // the lane's keys, of its eight slots; a key that is not there has no weight, and zeros in V, whatever lies there
-    auto place = [&](int e) __attribute__((always_inline)) { return C == 1 ? 16 * (e / 4) + e % 4 : C == 2 ? 16 * cls + e : 16 * (cls >> 1) + 2 * (cls & 1) + e; };
     if (seen != ~0u) {
+        auto place = [&](int e) __attribute__((always_inline)) { return C == 1 ? 16 * (e / 4) + e % 4 : C == 2 ? 16 * cls + e : 16 * (cls >> 1) + 2 * (cls & 1) + e; };
         const uint32_t mine = seen >> (4 * quad);
 #pragma unroll
-        for (int e = 0; e < kE; e++) {
-            const bool hid = !(mine >> place(e) & 1);
-#pragma unroll
-            for (int i = 0; i < NT; i++) y[i][e] = hid ? neg_inf() : y[i][e];
-        }
+        for (int e = 0; e < kE; e++) y[e] = mine >> place(e) & 1 ? y[e] : neg_inf();
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const bool hid = !(mine >> (16 * (e / 4) + e % 4) & 1);
@@ -524,88 +537,209 @@ __device__ __forceinline__ void step(State<D> (&st)[NT], Keys<D>& x, QOf q_of, K
         }
     }
     k_done();
-    // The running maximum, common to the four lanes of a column, in the exponent of two.  It follows the scores only where they have risen by 8 in it: up to
-    // there sums of weights in f32 and weights of 8 bits are as exact, and sums are scaled once or twice a span.
-    float top[NT];
-    bool risen = false;
+    // The running maximum, common to the four lanes of a column, in the exponent of two.  It follows the scores only where they have risen
+    // by 8 in it: up to there sums of weights in f32 and weights of 8 bits are as exact, and sums are scaled once or twice a span.
+    float top = y[0];
 #pragma unroll
-    for (int i = 0; i < NT; i++) {
-        top[i] = y[i][0];
+    for (int e = 1; e < kE; e++) top = fmaxf(top, y[e]);
+    top = quad_max(top) * scale_log2e;
+    if (__any(top - st.m > 8.0f)) {
+        const float m_new = fmaxf(st.m, top), alpha = __builtin_amdgcn_exp2f(st.m - m_new);
+        st.m = m_new;
+        st.l *= alpha;
 #pragma unroll
-        for (int e = 1; e < kE; e++) top[i] = fmaxf(top[i], y[i][e]);
-        top[i] = quad_max(top[i]);
-        top[i] *= scale_log2e;
-        risen = risen || top[i] - st[i].m > 8.0f;
+        for (int d = 0; d < D / 16; d++) st.o[d] *= alpha;
     }
-    if (__any(risen)) {
+    float f[kE];
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
-            const float m_new = fmaxf(st[i].m, top[i]), alpha = __builtin_amdgcn_exp2f(st[i].m - m_new);
-            st[i].m = m_new;
-            st[i].l *= alpha;
-#pragma unroll
-            for (int d = 0; d < D / 16; d++) st[i].o[d] *= alpha;
-        }
+    for (int e = 0; e < kE; e++) {
+        f[e] = __builtin_amdgcn_exp2f(fmaf(y[e], scale_log2e, -st.m));
+        st.l += f[e];
     }
-    u32x4_t w[NT];
+    // pairs of weights as the operand's words, zeros in the other columns' places
+    u32x4_t w;
 #pragma unroll
-    for (int i = 0; i < NT; i++) {
-        float f[kE];
+    for (int k = 0; k < kE / 2; k++) {
+        const uint32_t two = two_bf16(f[2 * k], f[2 * k + 1]);
+        if constexpr (C == 1) {
+            w[k] = two;
+        } else {
 #pragma unroll
-        for (int e = 0; e < kE; e++) {
-            f[e] = __builtin_amdgcn_exp2f(fmaf(y[i][e], scale_log2e, -st[i].m));
-            st[i].l += f[e];
-        }
-        // pairs of weights as the operand's words, zeros in the other columns' places
-#pragma unroll
-        for (int k = 0; k < kE / 2; k++) {
-            const uint32_t two = two_bf16(f[2 * k], f[2 * k + 1]);
-            if constexpr (C == 1) {
-                w[i][k] = two;
-            } else {
-#pragma unroll
-                for (int c = 0; c < C; c++) w[i][c * (kE / 2) + k] = cls == c ? two : 0u;
-            }
+            for (int c = 0; c < C; c++) w[c * (kE / 2) + k] = cls == c ? two : 0u;
         }
     }
 #pragma unroll
     for (int d = 0; d < D / 16; d++) {  // dim n * (D / 16) + d; of 256, of the lower and of the upper 128 in turn
-        u32x4_t a;
+        u32x4_t v;
 #pragma unroll
-        for (int i = 0; i < 4; i++) a[i] = __builtin_amdgcn_perm(x.v[2 * i + 1][d / 2], x.v[2 * i][d / 2], d & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-        for (int i = 0; i < NT; i++) st[i].o[d] = mfma(a, w[i], st[i].o[d]);
+        for (int i = 0; i < 4; i++) v[i] = __builtin_amdgcn_perm(x.v[2 * i + 1][d / 2], x.v[2 * i][d / 2], d & 1 ? 0x07060302u : 0x05040100u);
+        st.o[d] = mfma(v, w, st.o[d]);
     }
 }
 
-template <int D, int C, int NT, bool kWhole, bool kOnce, typename QOf>
-__device__ __forceinline__ void walk(State<D> (&st)[NT], Walk<D, kWhole>& at, const Lanes<D, kWhole>& lanes, QOf q_of, int cls, int quad, float scale_log2e) {
+template <int D, int C, bool kWhole>
+__device__ __forceinline__ void walk(State<D>& st, Walk<D, kWhole>& at, const Lanes<D, kWhole>& lanes, const u32x4_t (&q)[D / 32], int cls, int quad, float scale_log2e) {
     if (at.first >= at.end) return;
     Keys<D> x;
     int i = 0;
     at.place(at.first, 0);
     at.load_k(x, lanes);
-    at.template load_v<kOnce>(x, lanes);
+    at.load_v(x, lanes);
     for (int t = at.first; t < at.end; t += kWaves) {
         const uint32_t seen = at.seen;
         const bool more = t + kWaves < at.end;
-        step<D, C, NT>(st, x, q_of, [&]() __attribute__((always_inline)) {
+        step<D, C>(st, x, q, [&]() __attribute__((always_inline)) {
             if (more) {
                 at.place(t + kWaves, ++i);
                 at.load_k(x, lanes);
             }
         }, seen, cls, quad, scale_log2e);
-        if (more) at.template load_v<kOnce>(x, lanes);
+        if (more) at.load_v(x, lanes);
     }
+}
+
+// ---- the prefix: 32 query rows a wave, keys in LDS ------------------------------------------------------------------------------
+__device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+typedef short s16x4p __attribute__((ext_vector_type(4)));
+// within each group of 16 lanes, lane j gets element j % 4 of the 8 bytes that lanes 4 e + j / 4 address, e = 0 .. 3
+__device__ __forceinline__ u32x2_t lds_transposed(const unsigned char* p) {
+    return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4p __attribute__((address_space(3)))*)p));
+}
+// kStages steps of K and V, rows as wide as they are (1 KB a request), their 16-byte pieces exchanged by the row so that neither K's reads (a
+// piece each of 32 rows) nor V's transposing ones (four pieces each of four rows) meet a bank twice: the layout of the tile kernel.
+template <int D, bool kWhole>
+struct Ring {
+    using L = TileLds<D>;
+    static constexpr int kStages = 4, kRow = 2 * D, kHalf = 32 * kRow, kStage = 2 * kHalf, kPieces = D / 8;
+    static constexpr int kLoads = kHalf / 1024 / kWaves;  // requests of K, and of V, a wave and step: eight rows
+    uint32_t lds, k_at, v_at;
+    uint32_t k_from[kLoads], v_from[kLoads];
+    __device__ __forceinline__ Ring(unsigned char* space, int wave, int lane, uint32_t row_bytes) : lds((uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)space) {
+        const int col = lane & 31, hh = lane >> 5, j = lane & 15, g = lane >> 4 & 1, v_row = (j >> 2) + 4 * hh;
+        k_at = (uint32_t)(col * kRow + 16 * (hh ^ L::swz_k(col)));
+        v_at = (uint32_t)(kHalf + v_row * kRow + 16 * ((2 * g + (j >> 1 & 1)) ^ L::swz_v(v_row)) + 8 * (j & 1));
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            const int at = 64 * i + lane, row = 8 * wave + at / kPieces, k_piece = at % kPieces ^ L::swz_k(row), v_piece = at % kPieces ^ L::swz_v(row);
+            k_from[i] = kWhole || 16u * k_piece < row_bytes ? (uint32_t)(row & 15) * row_bytes + 16u * k_piece : kNowhere;
+            v_from[i] = kWhole || 16u * v_piece < row_bytes ? (uint32_t)(row & 15) * row_bytes + 16u * v_piece : kNowhere;
+        }
+    }
+    // the wave's rows of K and of V of the step whose descriptors `at` has
+    __device__ __forceinline__ void load(const Walk<D, kWhole>& at, int stage, int wave) const {
+        const uint32_t to = lds + (uint32_t)(stage * kStage + wave * (kLoads * 1024));
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            buffer_to_lds(at.ring_k, k_from[i], 0u, to + 1024u * i);
+            buffer_to_lds(at.ring_v, v_from[i], 0u, to + (uint32_t)kHalf + 1024u * i);
+        }
+    }
+};
+// What a lane has of its query row, lane % 32, over the keys walked; the row's other lane has the other eight of each sixteen.
+template <int D>
+struct PrefixState {
+    float m, l;
+    f32x16_t o[D / 32];  // o[t][4 j + e]: dim 32 t + 8 j + 4 (lane / 32) + e
+};
+// A step of 32 keys in `stage`.  scores^T leaves the lane keys 8 (i / 4) + 4 (lane / 32) + i % 4, i < 16; eight of them in a row are the
+// operand of out^T for sixteen keys, in an order of keys that the transposing reads of V follow.
+template <int D, bool kWhole>
+__device__ __forceinline__ void prefix_step(PrefixState<D>& st, const u32x4_t (&q)[D / 16], const Ring<D, kWhole>& ring, const unsigned char* stage, uint32_t seen, int hh, float scale_log2e) {
+    f32x16_t s;
+#pragma unroll
+    for (int i = 0; i < 16; i++) s[i] = 0.0f;
+    {
+        u32x4_t a[D / 16];  // (all asked for ahead of the first product)
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) a[k] = *(const u32x4_t*)(stage + (ring.k_at ^ (uint32_t)(32 * k)));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) s = mfma32(a[k], q[k], s);
+    }
+    u32x4_t v[D / 32][2];  // under way during the softmax
+#pragma unroll
+    for (int t = 0; t < D / 32; t++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const unsigned char* const at = stage + (ring.v_at ^ (uint32_t)(64 * t)) + 16 * u * Ring<D, kWhole>::kRow;
+            const u32x2_t lo = lds_transposed(at), hi = lds_transposed(at + 8 * Ring<D, kWhole>::kRow);
+            v[t][u] = u32x4_t{lo[0], lo[1], hi[0], hi[1]};
+        }
+    __builtin_amdgcn_sched_barrier(0);
+    if (seen != ~0u) {
+        const uint32_t mine = seen >> (4 * hh);
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] = mine >> (8 * (i / 4) + i % 4) & 1 ? s[i] : neg_inf();
+    }
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
+    const u32x2_t both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+    top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * scale_log2e;
+    if (__any(top - st.m > 8.0f)) {  // (as in step())
+        const float m_new = fmaxf(st.m, top), alpha = __builtin_amdgcn_exp2f(st.m - m_new);
+        st.m = m_new;
+        st.l *= alpha;
+#pragma unroll
+        for (int t = 0; t < D / 32; t++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) st.o[t][i] *= alpha;
+    }
+    u32x4_t w[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float a = __builtin_amdgcn_exp2f(fmaf(s[8 * u + 2 * i], scale_log2e, -st.m)), b = __builtin_amdgcn_exp2f(fmaf(s[8 * u + 2 * i + 1], scale_log2e, -st.m));
+            st.l += a + b;
+            w[u][i] = two_bf16(a, b);
+        }
+#pragma unroll
+    for (int t = 0; t < D / 32; t++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) st.o[t] = mfma32(v[t][u], w[u], st.o[t]);
+}
+// All four waves over the steps [at.first, at.end), each for its own rows (`rows`: it has some).
+template <int D, bool kWhole>
+__device__ __forceinline__ void prefix_walk(PrefixState<D>& st, Walk<D, kWhole>& at, unsigned char* space, u32x4_t (&q)[D / 16], bool rows, int wave, float scale_log2e) {
+    using R = Ring<D, kWhole>;
+    const R ring(space, wave, at.lane, at.row_bytes);
+    const int steps = at.end - at.first, hh = at.lane >> 5;
+    uint32_t seen[3] = {0, 0, 0};
+    auto request = [&](int i, uint32_t& to) __attribute__((always_inline)) {
+        at.place_half(at.first + i, i, wave >> 1);
+        to = at.seen;
+        ring.load(at, i & 3, wave);
+    };
+    static_assert(R::kStages == 4, "three steps under way, and one that is read");
+    __syncthreads();  // (what lay in LDS before has been read)
+#pragma unroll
+    for (int i = 0; i < 3; i++)
+        if (i < steps) request(i, seen[i]);
+    // q, awaited here: within the steps the compiler, which does not know of the requests to LDS, would wait for those under way with it
+#pragma unroll
+    for (int k = 0; k < D / 16; k++) asm volatile("" : "+v"(q[k]));
+    for (int i = 0; i < steps; i++) {
+        // this step's rows are there, if not the next two's; behind the barrier everybody's are, and nobody reads the last step's any more
+        if (i + 2 < steps) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 * R::kLoads) : "memory");
+        else if (i + 1 < steps) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * R::kLoads) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        const uint32_t now = seen[0];
+        seen[0] = seen[1];
+        seen[1] = seen[2];
+        if (i + 3 < steps) request(i + 3, seen[2]);
+        if (rows) prefix_step<D, kWhole>(st, q, ring, space + (i & 3) * R::kStage, now, hh, scale_log2e);
+    }
+    __syncthreads();
 }
 
 template <int D, int C, bool kWhole, bool kShared>
 __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_kernel(PagedDecodeParams p) {
-    constexpr int NT = kThreads, kPitch = D + 4, kR = 16 / C, kTiles = prefix_tiles<D>();
-    constexpr int kFold = kWaves * 16 * kPitch * 4, kLds = kShared ? kFold : std::max(kFold, kJoinLds);
-    constexpr int kQPitch = 2 * D + 16;  // bytes
-    __shared__ __attribute__((aligned(16))) unsigned char lds[kLds];
-    __shared__ __attribute__((aligned(16))) unsigned char prefix_q[kShared ? 16 * kTiles * kQPitch : 16];
+    constexpr int NT = kThreads, kPitch = D + 4, kR = 16 / C;
+    constexpr int kFold = kWaves * 16 * kPitch * 4, kLds = kShared ? std::max(kFold, Ring<D, kWhole>::kStages * Ring<D, kWhole>::kStage) : std::max(kFold, join_lds(kMaxPieces, kR));
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[kLds];
     __shared__ float red_m[kWaves][16], red_l[kWaves][16], inv_l[16];
     __shared__ int is_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, quad = lane >> 4, cls = n / kR;
@@ -625,28 +759,27 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
     float* const red = (float*)lds;  // [wave][row][kPitch]
 
     // A tile's rows, folded over the columns and the waves of the workgroup: to_row(row, d, values of four dims, m, l).
-    auto fold = [&](State<D>& st, auto c_of, int rows, auto to_row, auto to_ml) __attribute__((always_inline)) {
-        constexpr int kC = decltype(c_of)::value, kRows = 16 / kC;
-        const float m = columns_max<kC>(st.m), f = __builtin_amdgcn_exp2f(st.m - m);
-        const float l = columns_sum<kC>(quad_sum(st.l) * f);
-        if (kC > 1)
+    auto fold = [&](State<D>& st, int rows, auto to_row, auto to_ml) __attribute__((always_inline)) {
+        const float m = columns_max<C>(st.m), f = __builtin_amdgcn_exp2f(st.m - m);
+        const float l = columns_sum<C>(quad_sum(st.l) * f);
+        if (C > 1)
 #pragma unroll
             for (int i = 0; i < D / 16; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) st.o[i][e] = columns_sum<kC>(st.o[i][e] * f);
-        if (n < kRows && quad == 0) {
+                for (int e = 0; e < 4; e++) st.o[i][e] = columns_sum<C>(st.o[i][e] * f);
+        if (n < kR && quad == 0) {
             red_m[wave][n] = m;
             red_l[wave][n] = l;
         }
         __syncthreads();
-        float m_wg = red_m[0][n % kRows], l_wg = 0.0f;
+        float m_wg = red_m[0][n % kR], l_wg = 0.0f;
 #pragma unroll
-        for (int w = 1; w < kWaves; w++) m_wg = fmaxf(m_wg, red_m[w][n % kRows]);
+        for (int w = 1; w < kWaves; w++) m_wg = fmaxf(m_wg, red_m[w][n % kR]);
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) l_wg += red_l[w][n % kRows] * __builtin_amdgcn_exp2f(red_m[w][n % kRows] - m_wg);
-        if (n < kRows) {
+        for (int w = 0; w < kWaves; w++) l_wg += red_l[w][n % kR] * __builtin_amdgcn_exp2f(red_m[w][n % kR] - m_wg);
+        if (n < kR) {
             const float fw = __builtin_amdgcn_exp2f(m - m_wg);
-            float* row = red + (wave * kRows + n) * kPitch;
+            float* row = red + (wave * kR + n) * kPitch;
 #pragma unroll
             for (int c = 0; c < D / 32; c++) {  // eight dims in a row
                 float y[8];
@@ -666,7 +799,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
             const int row = i / (D / 4), d = 4 * (i % (D / 4));
             f32x4_t o = {0, 0, 0, 0};
 #pragma unroll
-            for (int w = 0; w < kWaves; w++) o += *(const f32x4_t*)(red + (w * kRows + row) * kPitch + d);
+            for (int w = 0; w < kWaves; w++) o += *(const f32x4_t*)(red + (w * kR + row) * kPitch + d);
             to_row(row, d, o);
         }
         __syncthreads();
@@ -675,39 +808,45 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
         if (kShared && at < span.pre_total) {
             // ---- a piece of the prefix
             const int seg = quotient(at, span.pre_places), seg_first = seg * span.pre_places;
-            const int t0 = max(at - seg_first - kStart, 0), t1 = min(span.pre_places, span.end - seg_first) - kStart;
+            // steps whose first place is in the span
+            const int all = steps_up_to(span.shared), t0 = (max(at - seg_first - kStart, 0) + p.pre_cost - 1) / p.pre_cost;
+            const int t1 = min(all, (max(min(span.pre_places, span.end - seg_first) - kStart, 0) + p.pre_cost - 1) / p.pre_cost);
+            const bool some = min(span.pre_places, span.end - seg_first) > kStart;  // (else places alone: no piece)
             at = min(seg_first + span.pre_places, span.end);
-            if (t1 <= 0) continue;  // (places alone)
+            if (!some) continue;
             const int kvh = quotient(seg, p.n_tiles), tile = seg - kvh * p.n_tiles;
-            const int w0 = quotient(seg_first + kStart, span.size), pieces = quotient(seg_first + span.pre_places - 1, span.size) - w0 + 1;
-            // the tile's units, (sequence, piece of the kv head's query heads)
-            const int unit0 = tile * p.per_tile, units = min(p.per_tile, p.batch * p.chunks - unit0);
-            // operands of q: row i of the tile is head i % rows of unit i / rows
-            const int group_rows = p.rows;
-            for (int i = tid; i < 16 * kTiles * (D / 8); i += NT) {
-                const int row = i / (D / 8), c = i % (D / 8), u = row / group_rows, r = row - u * group_rows;
-                const int seq = (unit0 + u) / p.chunks, h = (unit0 + u - seq * p.chunks) * group_rows + r;
-                u32x4_t q = {0, 0, 0, 0};
-                if (u < units && h < p.group && (kWhole || 8 * c < dim)) q = *(const u32x4_t*)(p.q + ((size_t)seq * p.heads + kvh * p.group + h) * dim + 8 * c);
-                *(u32x4_t*)(prefix_q + row * kQPitch + 16 * c) = q;
-            }
-            __syncthreads();
-            State<D> st[kTiles];
-#pragma unroll
-            for (int i = 0; i < kTiles; i++) st[i].reset();
+            // the wave's units, (sequence, piece of the kv head's query heads): row i of them is head i % rows of unit i / rows
+            const int unit0 = tile * p.per_tile + wave * p.per_wave, units = min(p.per_wave, p.batch * p.chunks - unit0), col = lane & 31, hh = lane >> 5;
+            u32x4_t q[D / 16];
             {
-                Walk<D, kWhole> w(p, p.page_table, kvh, 0, span.shared, t0 + wave, t1, lane);
-                walk<D, 1, kTiles, kWhole, false>(st, w, lanes, [&](int i, int c) __attribute__((always_inline)) {
-                    return *(const u32x4_t*)(prefix_q + (16 * i + n) * kQPitch + 64 * c + 16 * quad);
-                }, 0, quad, p.scale_log2e);
-            }
-            const __amdgpu_buffer_rsrc_t rs = slots.of_pre(w0, seg, pieces);
-            const uint32_t to = (uint32_t)(group - w0) * Slots<D>::kPre;
+                const int u = col / p.rows, unit = min(unit0 + u, p.batch * p.chunks - 1), seq = unit / p.chunks, h = (unit - seq * p.chunks) * p.rows + col - u * p.rows;
+                const bool there = u < units && h < p.group;
+                const uint16_t* q_row = p.q + ((size_t)seq * p.heads + kvh * p.group + (there ? h : 0)) * dim;
 #pragma unroll
-            for (int i = 0; i < kTiles; i++)
-                fold(st[i], std::integral_constant<int, 1>{}, 16,
-                     [&](int row, int d, f32x4_t o) __attribute__((always_inline)) { put4(rs, to + 4u * (uint32_t)((16 * i + row) * D + d), o); },
-                     [&](int row, float m, float l) __attribute__((always_inline)) { put2(rs, to + 4u * (uint32_t)(16 * kTiles * D + 2 * (16 * i + row)), m, l); });
+                for (int k = 0; k < D / 16; k++) {
+                    q[k] = *(const u32x4_t*)(q_row + (kWhole ? 16 * k + 8 * hh : min(16 * k + 8 * hh, dim - 8)));
+                    if (!there || (!kWhole && 16 * k >= dim)) q[k] = u32x4_t{0, 0, 0, 0};
+                }
+            }
+            PrefixState<D> st;
+            st.m = kNoMax;
+            st.l = 0.0f;
+#pragma unroll
+            for (int t = 0; t < D / 32; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) st.o[t][i] = 0.0f;
+            {
+                Walk<D, kWhole> w(p, p.page_table, kvh, 0, span.shared, t0, t1, 1, lane);
+                prefix_walk<D, kWhole>(st, w, lds, q, units > 0, wave, p.scale_log2e);
+            }
+            if (units <= 0) continue;  // (a wave without rows has its share of the keys' way to LDS)
+            const __amdgpu_buffer_rsrc_t rs = rsrc_of(slots.pre + ((size_t)group + seg) * Slots<D>::kPre + (size_t)wave * Slots<D>::kWave, Slots<D>::kWave);
+            const u32x2_t l = __builtin_amdgcn_permlane32_swap(__float_as_uint(st.l), __float_as_uint(st.l), false, false);
+            if (hh == 0) put2(rs, Slots<D>::at_ml(col), st.m, __uint_as_float(l[0]) + __uint_as_float(l[1]));
+#pragma unroll
+            for (int t = 0; t < D / 32; t++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) put4(rs, (uint32_t)((4 * t + j) * 1024 + lane * 16), f32x4_t{st.o[t][4 * j], st.o[t][4 * j + 1], st.o[t][4 * j + 2], st.o[t][4 * j + 3]});
             continue;
         }
         // ---- a piece of a sequence's own keys
@@ -740,16 +879,16 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
             if (there && (kWhole || 32 * c + 8 * quad < dim)) q[c] = *(const u32x4_t*)(q_row + 32 * c + 8 * quad);
         }
         if (!kShared && !alone && tid == 0) word.replace();
-        State<D> st[1];
-        st[0].reset();
+        State<D> st;
+        st.reset();
         {
-            Walk<D, kWhole> w(p, p.page_table + (size_t)b * p.table_pages, kvh, own.lo, len, own.first() + t0 + wave, own.first() + t1, lane);
-            walk<D, C, 1, kWhole, true>(st, w, lanes, [&](int, int c) __attribute__((always_inline)) { return q[c]; }, cls, quad, p.scale_log2e);
+            Walk<D, kWhole> w(p, p.page_table + (size_t)b * p.table_pages, kvh, own.lo, len, own.first() + t0 + wave, own.first() + t1, kWaves, lane);
+            walk<D, C, kWhole>(st, w, lanes, q, cls, quad, p.scale_log2e);
         }
         const __amdgpu_buffer_rsrc_t rs = slots.of_own(w0, segment, pieces);
         const uint32_t to = (uint32_t)(group - w0) * slots.own_bytes;
         if (kShared && tid == 0) *(UnitLine*)word_of(p, b, kvh, piece) = UnitLine{w0, alone ? -1 : pieces};
-        fold(st[0], std::integral_constant<int, C>{}, rows,
+        fold(st, rows,
              [&](int row, int d, f32x4_t o) __attribute__((always_inline)) {
                  if (alone) put_out(p, dim, b, kvh * p.group + head + row, d, o * inv_l[row]);
                  else put4(rs, to + 4u * (uint32_t)(row * D + d), o);
@@ -763,7 +902,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
         __syncthreads();
         if (tid == 0) is_last = word.count(pieces) ? 1 : 0;
         __syncthreads();
-        if (is_last) join<D, false>(p, lds, inv_l, dim, b, kvh * p.group + head, rows, rs, 0, 0, rs, pieces);
+        if (is_last) join<D, false>(p, lds, inv_l, dim, b, kvh * p.group + head, rows, rs, 0, 0, 0, rs, pieces);
         __syncthreads();
     }
 }
@@ -771,23 +910,26 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
 // With a prefix: a workgroup for each unit, grid (pieces of a kv head's query heads, kv heads, batch).
 template <int D>
 __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedDecodeParams p) {
-    __shared__ __attribute__((aligned(16))) unsigned char lds[kJoinLds];
+    extern __shared__ __attribute__((aligned(16))) unsigned char join_space[];  // join_lds(kMaxPieces, p.rows)
     __shared__ float inv_l[16];
     const int piece = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+    // (all three at once; what a unit's line holds counts where the sequence has keys of its own)
     const ListHead list = *(const ListHead*)p.head;
+    const UnitLine left = *(const UnitLine*)word_of(p, b, kvh, piece);
     const Own own(len_of(p, b), list.shared);
     if (own.len == 0) return;  // (written already)
-    const UnitLine line = own.steps() > 0 ? *(const UnitLine*)word_of(p, b, kvh, piece) : UnitLine{0, 0};
+    const UnitLine line = own.steps() > 0 ? left : UnitLine{0, 0};
     if (line.pieces < 0) return;
     const Slots<D> slots(p, true);
     const int unit = b * p.chunks + piece, tile = quotient(unit, p.per_tile), segment = kvh * p.n_tiles + tile, head = piece * p.rows;
+    const int in_tile = unit - tile * p.per_tile, row_wave = quotient(in_tile, p.per_wave), pre_row = (in_tile - row_wave * p.per_wave) * p.rows;
     int w0 = 0, n_pre = 0;
     if (own.lo > 0) {
         const int first = segment * list.pre_places;
         w0 = quotient(first + kStart, list.size);
         n_pre = quotient(first + list.pre_places - 1, list.size) - w0 + 1;
     }
-    join<D, true>(p, lds, inv_l, p.dim, b, kvh * p.group + head, min(p.rows, p.group - head), slots.of_pre(w0, segment, n_pre), n_pre, (unit - tile * p.per_tile) * p.rows,
+    join<D, true>(p, join_space, inv_l, p.dim, b, kvh * p.group + head, min(p.rows, p.group - head), slots.of_pre(w0, segment, n_pre), n_pre, row_wave, pre_row,
                   slots.of_own(line.w0, ((size_t)b * p.kv_heads + kvh) * p.chunks + piece, line.pieces), line.pieces);
 }
 
@@ -797,7 +939,7 @@ hipError_t launch_as(hipStream_t stream, const PagedDecodeParams& p) {
     if (p.rows <= 4) hipLaunchKernelGGL((paged_decode_kernel<D, 4, kWhole, kShared>), grid, block, 0, stream, p);
     else if (p.rows <= 8) hipLaunchKernelGGL((paged_decode_kernel<D, 2, kWhole, kShared>), grid, block, 0, stream, p);
     else hipLaunchKernelGGL((paged_decode_kernel<D, 1, kWhole, kShared>), grid, block, 0, stream, p);
-    if (kShared) hipLaunchKernelGGL(paged_join_kernel<D>, dim3(p.chunks, p.kv_heads, p.batch), block, 0, stream, p);
+    if (kShared) hipLaunchKernelGGL(paged_join_kernel<D>, dim3(p.chunks, p.kv_heads, p.batch), block, join_lds(kMaxPieces, p.rows), stream, p);
     return hipGetLastError();
 }
 template <int D>
@@ -808,9 +950,10 @@ hipError_t launch_dim(hipStream_t stream, const PagedDecodeParams& p, bool share
 
 // Workgroups a CU, each with a wave on every SIMD.
 constexpr int per_cu(int64_t dim, bool shared) { return dim == 256 ? 1 : 2; }
+constexpr int kPreCost = 2;  // places of a prefix's step
 // Segments, steps and workgroups of a call at its longest, and what its workspace holds.
 struct Plan {
-    int64_t chunks, rows, per_tile, n_tiles, own_segments, pre_segments, places;
+    int64_t chunks, rows, per_wave, per_tile, n_tiles, own_segments, pre_segments, places;
     int dim, groups;  // dim: the kernel's
     size_t part_bytes, word_bytes;
 };
@@ -820,21 +963,20 @@ Plan plan_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_
     a.dim = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
     a.chunks = (group + 15) / 16;
     a.rows = (group + a.chunks - 1) / a.chunks;
-    const int64_t tile_rows = a.dim == 256 ? 16 : a.dim == 128 ? 32 : 64;
-    a.per_tile = tile_rows / a.rows;
+    a.per_wave = kWaveRows / a.rows;
+    a.per_tile = kWaves * a.per_wave;
     a.n_tiles = (batch * a.chunks + a.per_tile - 1) / a.per_tile;
     a.own_segments = batch * kv_heads * a.chunks;
     a.pre_segments = kv_heads * a.n_tiles;
-    const int64_t steps = max_len / kStep + 2 + kStart;
-    a.places = (a.own_segments + a.pre_segments) * steps;
+    const int64_t steps = max_len / kStep + 2;
+    a.places = a.own_segments * (steps + kStart) + a.pre_segments * (steps * kPreCost + kStart);
     a.groups = (int)std::min<int64_t>(2 * kCus, std::max<int64_t>((a.places + kWaves - 1) / kWaves, 1));
     a.groups = (a.groups + 7) / 8 * 8;
     auto round = [](size_t x) { return (x + 255) / 256 * 256; };
-    a.part_bytes = round((size_t)(a.groups + a.pre_segments) * (size_t)tile_rows * (size_t)(a.dim + 2) * 4 + (size_t)(a.groups + a.own_segments) * (size_t)a.rows * (size_t)(a.dim + 2) * 4);
+    a.part_bytes = round((size_t)(a.groups + a.pre_segments) * (size_t)(kWaves * kWaveRows) * (size_t)(a.dim + 2) * 4 + (size_t)(a.groups + a.own_segments) * (size_t)a.rows * (size_t)(a.dim + 2) * 4);
     a.word_bytes = (size_t)a.own_segments * kWordPitch + 256;
     return a;
 }
-static_assert(prefix_tiles<64>() == 4 && prefix_tiles<128>() == 2 && prefix_tiles<256>() == 1, "the plan's rows of a tile");
 
 }  // namespace
 
@@ -894,7 +1036,9 @@ RT_API int rt_gqa_decode_paged_bf16(void* stream, const void* q, const void* k_p
     p.group = n_heads / n_kv;
     p.chunks = (int)a.chunks;
     p.rows = (int)a.rows;
+    p.per_wave = (int)a.per_wave;
     p.per_tile = (int)a.per_tile;
+    p.pre_cost = kPreCost;
     p.n_tiles = (int)a.n_tiles;
     p.span_root = a.rows <= 4 ? 0.66f : 1.0f;
     p.scale_log2e = (1.0f / sqrtf((float)head_dim)) * kLog2eHost;

@@ -145,8 +145,9 @@ __device__ __forceinline__ TilePlace t_place_by_length(const int32_t* lens, int 
 
 // Where a workgroup works that takes the `pos`-th query tile of sequences packed one behind the other: starts[b] .. starts[b + 1] are the
 // tokens of sequence b (read as ascending and within the tokens there are, whatever they hold).  Of up to 64 sequences the tiles are
-// ordered by their number downwards, which is their cost: the highest number at which no more than `pos` tiles have been passed by is found
-// bit by bit, a sum over the lanes a bit.  Of more, sequence by sequence, each from its last tile on.  b < 0: there is no such tile.
+// ordered by their number downwards, which is their cost: a ballot per number, as above, or, where the longest sequence has more than
+// 32 tiles, first the number's bits, a sum over the lanes each.  Of more sequences, one by one, each from its last tile on.  b < 0: there
+// is no such tile.
 struct PackedPlace {
     int b, tile, first, len;
 };
@@ -157,6 +158,15 @@ __device__ __forceinline__ int t_lane_sums(int x) {  // up to and with this lane
     x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
     x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
     x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return x;
+}
+__device__ __forceinline__ int t_lane_max(int x) {  // of non-negative numbers, in the last lane
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));
+    x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
     return x;
 }
 __device__ __forceinline__ PackedPlace t_place_packed(const int32_t* starts, int batch, int tokens, int pos, int lane) {
@@ -172,15 +182,36 @@ __device__ __forceinline__ PackedPlace t_place_packed(const int32_t* starts, int
         uint64_t has;
         int at = pos, tile = -1;
         if (batch <= 64) {
-            // tiles numbered `number` or more, of all sequences: the highest number of which there are more than `pos`
-            auto from_number = [&](int number) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(t_lane_sums(max(n - number, 0)), 63); };
-            int number = 0, passed = 0;  // (pos < all: number 0 is one)
-            for (int bit = 1 << (31 - __builtin_clz(__builtin_amdgcn_readfirstlane(all))); bit; bit >>= 1)
-                if (from_number(number + bit) > pos) number += bit;
-            passed = from_number(number + 1);
-            has = __ballot(n > number);
-            at = pos - passed;
-            tile = number;
+            const int most = __builtin_amdgcn_readlane(t_lane_max(n), 63);
+            tile = most - 1;
+            if (most > 32) {
+                // tiles numbered `number` or more, of all sequences: the highest number of which there are more than `pos`
+                auto from_number = [&](int number) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(t_lane_sums(max(n - number, 0)), 63); };
+                tile = 0;  // (pos < all: number 0 is one)
+                for (int bit = 1 << (31 - __builtin_clz(most)); bit; bit >>= 1)
+                    if (from_number(tile + bit) > pos) tile += bit;
+                at = pos - from_number(tile + 1);
+                has = __ballot(n > tile);
+            } else {
+                has = 0;
+                for (;; tile -= 4) {  // (below tile 0: every lane, but the place is found ahead of that)
+                    int c[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) c[k] = __builtin_popcountll(__ballot(n > tile - k));
+                    const int four = c[0] + c[1] + c[2] + c[3];
+                    if (at < four) {
+#pragma unroll
+                        for (int k = 0; k < 3; k++) {
+                            if (at < c[k]) break;
+                            at -= c[k];
+                            tile--;
+                        }
+                        has = __ballot(n > tile);
+                        break;
+                    }
+                    at -= four;
+                }
+            }
         } else {
             has = __ballot(ends > pos);
             at = 0;

@@ -3,6 +3,8 @@
 calls enqueue and return."""
 from __future__ import annotations
 
+import functools
+
 import numpy as np
 
 from . import _lib as L
@@ -42,6 +44,13 @@ class KVPages:
     def zeros(cls, n_pages: int, n_kv: int, page_size: int, head_dim: int, stream=None) -> "KVPages":
         n_bytes = n_pages * n_kv * page_size * head_dim * 2
         return cls(HipStorage.zeros(n_bytes, stream), HipStorage.zeros(n_bytes, stream), n_pages, page_size)
+
+
+@functools.lru_cache(maxsize=64)
+def _host_i32(values: tuple):
+    """(address, count, what keeps it alive) of host int32 values."""
+    a = np.array(values, dtype=np.int32)
+    return a.ctypes.data, a.size, a
 
 
 def _host_or_dev(x):
@@ -244,11 +253,10 @@ class LlmKernels:
         first token.  With `sections`, pairs of a head for each of up to four axes, a token's rotary positions are
         `axis_positions`, device int32[len(sections), tokens], and not its row."""
         ptr, pos = _host_or_dev(positions)
-        sections = None if sections is None else np.ascontiguousarray(sections, dtype=np.int32)
+        at, n_axes, _ = (None, 0, None) if sections is None else _host_i32(tuple(sections))
         cos, sin = rope.device_tables()
         check(L.native.rt_qk_norm_rope_kv_append_paged_bf16(
-            stream, q, q_out, k_in, k_out, v_in, pages.k, pages.v, page_table, starts, ptr, pos, axis_positions,
-            None if sections is None else sections.ctypes.data, 0 if sections is None else sections.size, q_gamma, k_gamma, eps, cos, sin,
+            stream, q, q_out, k_in, k_out, v_in, pages.k, pages.v, page_table, starts, ptr, pos, axis_positions, at, n_axes, q_gamma, k_gamma, eps, cos, sin,
             rope.max_seq, tokens, batch, n_heads, n_kv, head_dim, pages.n_pages, pages.page_size, table_pages))
 
     @staticmethod

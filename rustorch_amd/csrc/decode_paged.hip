@@ -204,7 +204,8 @@ __device__ __forceinline__ Span span_of(const PagedDecodeParams& p, int& group, 
     }
 }
 
-// ---- partials that another workgroup of the launch reads: device scope both ways, as in decode_cache.hip ---------------------
+// ---- partials: device scope both ways, as in decode_cache.hip.  (Where a second launch reads them they need none; without it 64 sequences
+// behind 8192 keys took 44.5 us instead of 43.6.) ----------------------------------------------------------------------------------
 constexpr int kScopeDevice = 16;  // sc1
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* base, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, kBufferFlags);
@@ -268,7 +269,7 @@ __device__ __forceinline__ void* word_of(const PagedDecodeParams& p, int seq, in
 }
 
 // ---- partials ----------------------------------------------------------------------------------------------------------------
-// Slots of the prefix's come first, four a piece, one a wave, then those of the sequences'.  A piece's number is (workgroup + segment): along
+// Slots of the prefix's come first, one a wave of a piece, then those of the sequences'.  A piece's number is (workgroup + segment): along
 // the list each further piece advances one or the other.  A sequence's slot: rows of D floats, then their (m, l).  A wave's: o as the
 // registers hold it, 16 bytes a lane and request, then the rows' (m, l).
 constexpr int kWaveRows = 32;
@@ -299,7 +300,7 @@ constexpr int join_lds(int pieces, int rows) { return kThreads * 16 + pieces * r
 template <int D, bool kShared>
 __device__ __forceinline__ void join(const PagedDecodeParams& p, unsigned char* lds, float* inv_l, int dim, int seq, int head, int rows, __amdgpu_buffer_rsrc_t pre, int n_pre, int pre_wave, int pre_row, __amdgpu_buffer_rsrc_t own, int n_own) {
     constexpr int kAhead = 8, NT = kThreads, kMost = kMaxPieces;
-    auto pre_at = [&](int k) __attribute__((always_inline)) { return (uint32_t)(k * kWaves + pre_wave) * Slots<D>::kWave; };
+    auto pre_at = [&](int k) __attribute__((always_inline)) { return (uint32_t)k * Slots<D>::kPre + (uint32_t)pre_wave * Slots<D>::kWave; };
     const uint32_t own_slot = (uint32_t)p.rows * (D + 2) * 4;
     f32x4_t* const part = (f32x4_t*)lds;
     float* const wgt = (float*)(part + NT);  // [pieces][p.rows]
@@ -318,16 +319,18 @@ __device__ __forceinline__ void join(const PagedDecodeParams& p, unsigned char* 
     };
     ask(x0, sub);
     {
+        for (int x = tid; x < pieces * p.rows; x += NT) {
+            const int k = x / p.rows, row = x - k * p.rows;
+            const u32x2_t ml = kShared && k < n_pre ? get2(pre, pre_at(k) + Slots<D>::at_ml(pre_row + row))
+                                                    : get2(own, (uint32_t)(k - n_pre) * own_slot + 4u * (uint32_t)(p.rows * D + 2 * row));
+            wgt[x] = __uint_as_float(ml[0]);
+            wl[x] = __uint_as_float(ml[1]);
+        }
+        __syncthreads();
         const int row = tid >> 4, col = tid & 15;  // sixteen lanes a row
         const bool on = row < rows;
         float top = kNoMax, sum = 0.0f;
-        for (int k = col; on && k < pieces; k += 16) {
-            const u32x2_t ml = kShared && k < n_pre ? get2(pre, pre_at(k) + Slots<D>::at_ml(pre_row + row))
-                                                    : get2(own, (uint32_t)(k - n_pre) * own_slot + 4u * (uint32_t)(p.rows * D + 2 * row));
-            wgt[k * p.rows + row] = __uint_as_float(ml[0]);
-            wl[k * p.rows + row] = __uint_as_float(ml[1]);
-            top = fmaxf(top, __uint_as_float(ml[0]));
-        }
+        for (int k = col; on && k < pieces; k += 16) top = fmaxf(top, wgt[k * p.rows + row]);
         top = columns_max<16>(top);
         for (int k = col; on && k < pieces; k += 16) {
             const float fk = __builtin_amdgcn_exp2f(wgt[k * p.rows + row] - top);
@@ -394,31 +397,42 @@ struct Lanes {
 template <int D, bool kWhole>
 struct Walk {
     const PagedDecodeParams& p;
-    const int32_t* table;  // the sequence's
-    const int lo, hi, first, end, stride, lane;
     const uint32_t row_bytes, page_bytes;
+    const int32_t* table;  // the sequence's
+    int lo, hi, first, end, stride, lane;
     const char *k_head, *v_head;  // the kv head's first row in page 0
     int entry[2];  // lane i: the pages of the two sixteens of the wave's i-th step from the last refill on
     __amdgpu_buffer_rsrc_t ks[2], vs[2];
     uint32_t seen;  // of the step whose place was taken last: a bit for every key that is there
 
-    __device__ __forceinline__ Walk(const PagedDecodeParams& params, const int32_t* row, int kv_head, int from, int to, int step0, int step1, int every, int l)
-        : p(params), table(row), lo(from), hi(to), first(step0), end(step1), stride(every), lane(l), row_bytes(2u * (uint32_t)(kWhole ? D : params.dim)),
-          page_bytes(((uint32_t)params.kv_heads << params.page_shift) * row_bytes), k_head((const char*)params.k_pages + ((size_t)kv_head << params.page_shift) * row_bytes),
-          v_head((const char*)params.v_pages + ((size_t)kv_head << params.page_shift) * row_bytes) {}
-    __device__ __forceinline__ void refill(int t) {
+    __device__ __forceinline__ Walk(const PagedDecodeParams& params, int every, int l)
+        : p(params), row_bytes(2u * (uint32_t)(kWhole ? D : params.dim)), page_bytes(((uint32_t)params.kv_heads << params.page_shift) * row_bytes), stride(every), lane(l) {}
+    __device__ __forceinline__ void over(const int32_t* row, int kv_head, int from, int to, int step0, int step1) {
+        table = row;
+        lo = from;
+        hi = to;
+        first = step0;
+        end = step1;
+        k_head = (const char*)p.k_pages + ((size_t)kv_head << p.page_shift) * row_bytes;
+        v_head = (const char*)p.v_pages + ((size_t)kv_head << p.page_shift) * row_bytes;
+    }
+    // entries from step t on, and what has to stand between the request and the first use.  (Awaited there: behind a branch that requests
+    // stand in, the compiler would wait in every step for whatever is under way.)
+    __device__ __forceinline__ void request_entries(int t) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const long long row = ((long long)t + stride * lane) * kStep + 16 * h;
             entry[h] = table[(int)min(row >> p.page_shift, (long long)p.table_pages - 1)];
         }
-        // (awaited here: behind the branch that this stands in, the compiler would wait in every step for whatever is under way)
-        asm volatile("" : "+v"(entry[0]), "+v"(entry[1]));
     }
+    __device__ __forceinline__ void await_entries() { asm volatile("" : "+v"(entry[0]), "+v"(entry[1])); }
     // The descriptors of step t, the wave's i-th.  (What they are made of is said to be the same in all lanes, which the compiler does not
     // see: it would ask for each lane's descriptor by itself.)
     __device__ __forceinline__ void place(int t, int i) {
-        if ((i & 63) == 0) refill(t);
+        if (i && (i & 63) == 0) {
+            request_entries(t);
+            await_entries();
+        }
         const int row = t * kStep;
         const uint32_t mask = (1u << p.page_shift) - 1;
         int rows[2], skip[2] = {0, 0};
@@ -452,7 +466,10 @@ struct Walk {
     // The same of one of the two sixteens, as scalars, for rows that go to LDS; `seen` of both.  (lo is 0.)
     u32x4_t ring_k, ring_v;
     __device__ __forceinline__ void place_half(int t, int i, int h) {
-        if ((i & 63) == 0) refill(t);
+        if (i && (i & 63) == 0) {
+            request_entries(t);
+            await_entries();
+        }
         const int row = t * kStep;
         const uint32_t mask = (1u << p.page_shift) - 1;
         const uint32_t page0 = (uint32_t)__builtin_amdgcn_readlane(entry[0], i & 63), page1 = (uint32_t)__builtin_amdgcn_readlane(entry[1], i & 63);
@@ -577,20 +594,16 @@ __device__ __forceinline__ void step(State<D>& st, Keys<D>& x, const u32x4_t (&q
     }
 }
 
+// x: the first step's rows, under way.
 template <int D, int C, bool kWhole>
-__device__ __forceinline__ void walk(State<D>& st, Walk<D, kWhole>& at, const Lanes<D, kWhole>& lanes, const u32x4_t (&q)[D / 32], int cls, int quad, float scale_log2e) {
-    if (at.first >= at.end) return;
-    Keys<D> x;
+__device__ __forceinline__ void walk(State<D>& st, Walk<D, kWhole>& at, Keys<D>& x, const Lanes<D, kWhole>& lanes, const u32x4_t (&q)[D / 32], int cls, int quad, float scale_log2e) {
     int i = 0;
-    at.place(at.first, 0);
-    at.load_k(x, lanes);
-    at.load_v(x, lanes);
-    for (int t = at.first; t < at.end; t += kWaves) {
+    for (int t = at.first; t < at.end; t += at.stride) {
         const uint32_t seen = at.seen;
-        const bool more = t + kWaves < at.end;
+        const bool more = t + at.stride < at.end;
         step<D, C>(st, x, q, [&]() __attribute__((always_inline)) {
             if (more) {
-                at.place(t + kWaves, ++i);
+                at.place(t + at.stride, ++i);
                 at.load_k(x, lanes);
             }
         }, seen, cls, quad, scale_log2e);
@@ -607,13 +620,13 @@ typedef short s16x4p __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ u32x2_t lds_transposed(const unsigned char* p) {
     return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4p __attribute__((address_space(3)))*)p));
 }
-// kStages steps of K and V, rows as wide as they are (1 KB a request), their 16-byte pieces exchanged by the row so that neither K's reads (a
+// kStages steps of K and V, as many as two workgroups a CU leave room for, rows as wide as they are (1 KB a request), their 16-byte pieces exchanged by the row so that neither K's reads (a
 // piece each of 32 rows) nor V's transposing ones (four pieces each of four rows) meet a bank twice: the layout of the tile kernel.
 template <int D, bool kWhole>
 struct Ring {
     using L = TileLds<D>;
-    static constexpr int kStages = 4, kRow = 2 * D, kHalf = 32 * kRow, kStage = 2 * kHalf, kPieces = D / 8;
-    static constexpr int kLoads = kHalf / 1024 / kWaves;  // requests of K, and of V, a wave and step: eight rows
+    static constexpr int kOwn = 32 / kWaves, kStages = D == 64 ? 8 : 4, kRow = 2 * D, kHalf = 32 * kRow, kStage = 2 * kHalf, kPieces = D / 8;
+    static constexpr int kLoads = kHalf / 1024 / kWaves;  // requests of K, and of V, a wave and step
     uint32_t lds, k_at, v_at;
     uint32_t k_from[kLoads], v_from[kLoads];
     __device__ __forceinline__ Ring(unsigned char* space, int wave, int lane, uint32_t row_bytes) : lds((uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)space) {
@@ -622,7 +635,7 @@ struct Ring {
         v_at = (uint32_t)(kHalf + v_row * kRow + 16 * ((2 * g + (j >> 1 & 1)) ^ L::swz_v(v_row)) + 8 * (j & 1));
 #pragma unroll
         for (int i = 0; i < kLoads; i++) {
-            const int at = 64 * i + lane, row = 8 * wave + at / kPieces, k_piece = at % kPieces ^ L::swz_k(row), v_piece = at % kPieces ^ L::swz_v(row);
+            const int at = 64 * i + lane, row = kOwn * wave + at / kPieces, k_piece = at % kPieces ^ L::swz_k(row), v_piece = at % kPieces ^ L::swz_v(row);
             k_from[i] = kWhole || 16u * k_piece < row_bytes ? (uint32_t)(row & 15) * row_bytes + 16u * k_piece : kNowhere;
             v_from[i] = kWhole || 16u * v_piece < row_bytes ? (uint32_t)(row & 15) * row_bytes + 16u * v_piece : kNowhere;
         }
@@ -706,37 +719,40 @@ template <int D, bool kWhole>
 __device__ __forceinline__ void prefix_walk(PrefixState<D>& st, Walk<D, kWhole>& at, unsigned char* space, u32x4_t (&q)[D / 16], bool rows, int wave, float scale_log2e) {
     using R = Ring<D, kWhole>;
     const R ring(space, wave, at.lane, at.row_bytes);
+    constexpr int kAhead = R::kStages - 1;  // steps under way, beside the one that is read
     const int steps = at.end - at.first, hh = at.lane >> 5;
-    uint32_t seen[3] = {0, 0, 0};
-    auto request = [&](int i, uint32_t& to) __attribute__((always_inline)) {
-        at.place_half(at.first + i, i, wave >> 1);
-        to = at.seen;
-        ring.load(at, i & 3, wave);
+    int seen = 0;  // lane i % 64: of step i
+    auto request = [&](int i) __attribute__((always_inline)) {
+        at.place_half(at.first + i, i, wave * R::kOwn / 16);
+        if (at.lane == (i & 63)) seen = (int)at.seen;
+        ring.load(at, i & kAhead, wave);
     };
-    static_assert(R::kStages == 4, "three steps under way, and one that is read");
+    auto await = [&](auto others) __attribute__((always_inline)) {  // but for as many later steps' requests
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(decltype(others)::value * 2 * R::kLoads) : "memory");
+    };
+    static_assert((R::kStages & kAhead) == 0 && (kAhead - 1) * 2 * R::kLoads < 63);
+    at.request_entries(at.first);
     __syncthreads();  // (what lay in LDS before has been read)
-#pragma unroll
-    for (int i = 0; i < 3; i++)
-        if (i < steps) request(i, seen[i]);
+    at.await_entries();
     // q, awaited here: within the steps the compiler, which does not know of the requests to LDS, would wait for those under way with it
 #pragma unroll
     for (int k = 0; k < D / 16; k++) asm volatile("" : "+v"(q[k]));
+    for (int i = 0; i < min(kAhead, steps); i++) request(i);
     for (int i = 0; i < steps; i++) {
-        // this step's rows are there, if not the next two's; behind the barrier everybody's are, and nobody reads the last step's any more
-        if (i + 2 < steps) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 * R::kLoads) : "memory");
-        else if (i + 1 < steps) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * R::kLoads) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        const uint32_t now = seen[0];
-        seen[0] = seen[1];
-        seen[1] = seen[2];
-        if (i + 3 < steps) request(i + 3, seen[2]);
-        if (rows) prefix_step<D, kWhole>(st, q, ring, space + (i & 3) * R::kStage, now, hh, scale_log2e);
+        // this step's rows are there, if not the next ones'; behind the barrier everybody's are, and nobody reads the last step's any more
+        const int left = steps - 1 - i;
+        if (left >= kAhead - 1) await(std::integral_constant<int, kAhead - 1>{});
+        else if (left >= kAhead / 2) await(std::integral_constant<int, kAhead / 2>{});
+        else if (left >= 1) await(std::integral_constant<int, 1>{});
+        else await(std::integral_constant<int, 0>{});
+        if (i + kAhead < steps) request(i + kAhead);
+        if (rows) prefix_step<D, kWhole>(st, q, ring, space + (i & kAhead) * R::kStage, (uint32_t)__builtin_amdgcn_readlane(seen, i & 63), hh, scale_log2e);
     }
     __syncthreads();
 }
 
 template <int D, int C, bool kWhole, bool kShared>
-__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_kernel(PagedDecodeParams p) {
+__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void paged_decode_kernel(PagedDecodeParams p) {
     constexpr int NT = kThreads, kPitch = D + 4, kR = 16 / C;
     constexpr int kFold = kWaves * 16 * kPitch * 4, kLds = kShared ? std::max(kFold, Ring<D, kWhole>::kStages * Ring<D, kWhole>::kStage) : std::max(kFold, join_lds(kMaxPieces, kR));
     __shared__ __attribute__((aligned(1024))) unsigned char lds[kLds];
@@ -804,16 +820,15 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
         }
         __syncthreads();
     };
-    while (at < span.end) {
-        if (kShared && at < span.pre_total) {
-            // ---- a piece of the prefix
-            const int seg = quotient(at, span.pre_places), seg_first = seg * span.pre_places;
+    // ---- pieces of the prefix
+    if constexpr (kShared) {
+        const int end = min(span.end, span.pre_total);
+        while (at < end) {
+            const int seg = quotient(at, span.pre_places), seg_first = seg * span.pre_places, to = min(seg_first + span.pre_places, end);
             // steps whose first place is in the span
-            const int all = steps_up_to(span.shared), t0 = (max(at - seg_first - kStart, 0) + p.pre_cost - 1) / p.pre_cost;
-            const int t1 = min(all, (max(min(span.pre_places, span.end - seg_first) - kStart, 0) + p.pre_cost - 1) / p.pre_cost);
-            const bool some = min(span.pre_places, span.end - seg_first) > kStart;  // (else places alone: no piece)
-            at = min(seg_first + span.pre_places, span.end);
-            if (!some) continue;
+            const int t0 = (max(at - seg_first - kStart, 0) + p.pre_cost - 1) / p.pre_cost, t1 = min(steps_up_to(span.shared), (max(to - seg_first - kStart, 0) + p.pre_cost - 1) / p.pre_cost);
+            at = to;
+            if (to - seg_first <= kStart) continue;  // (places alone: no piece)
             const int kvh = quotient(seg, p.n_tiles), tile = seg - kvh * p.n_tiles;
             // the wave's units, (sequence, piece of the kv head's query heads): row i of them is head i % rows of unit i / rows
             const int unit0 = tile * p.per_tile + wave * p.per_wave, units = min(p.per_wave, p.batch * p.chunks - unit0), col = lane & 31, hh = lane >> 5;
@@ -835,10 +850,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
             for (int t = 0; t < D / 32; t++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) st.o[t][i] = 0.0f;
-            {
-                Walk<D, kWhole> w(p, p.page_table, kvh, 0, span.shared, t0, t1, 1, lane);
-                prefix_walk<D, kWhole>(st, w, lds, q, units > 0, wave, p.scale_log2e);
-            }
+            Walk<D, kWhole> w(p, 1, lane);
+            w.over(p.page_table, kvh, 0, span.shared, t0, t1);
+            prefix_walk<D, kWhole>(st, w, lds, q, units > 0, wave, p.scale_log2e);
             if (units <= 0) continue;  // (a wave without rows has its share of the keys' way to LDS)
             const __amdgpu_buffer_rsrc_t rs = rsrc_of(slots.pre + ((size_t)group + seg) * Slots<D>::kPre + (size_t)wave * Slots<D>::kWave, Slots<D>::kWave);
             const u32x2_t l = __builtin_amdgcn_permlane32_swap(__float_as_uint(st.l), __float_as_uint(st.l), false, false);
@@ -847,63 +861,109 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void paged_decode_ke
             for (int t = 0; t < D / 32; t++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) put4(rs, (uint32_t)((4 * t + j) * 1024 + lane * 16), f32x4_t{st.o[t][4 * j], st.o[t][4 * j + 1], st.o[t][4 * j + 2], st.o[t][4 * j + 3]});
-            continue;
         }
-        // ---- a piece of a sequence's own keys
-        const Own own(len, span.shared);
-        const int places = own.places();
-        if (at >= first + places * per) {  // the next sequence
-            first += places * per;
-            b++;
-            len = len_of(p, b);
-            continue;
+        if (at >= span.end) return;
+    }
+    // ---- pieces of sequences' own keys.  The next one's page entries are asked for ahead of a piece's steps, its q and first rows behind
+    // them and ahead of the fold.
+    struct Piece {
+        int b, kvh, piece, lo, hi, t0, t1, w0, pieces;
+    };
+    int next_len = len_of(p, min(b + 1, p.batch - 1));
+    auto next = [&](Piece& x) __attribute__((always_inline)) {  // false: there is none
+        while (at < span.end) {
+            const Own own(len, span.shared);
+            const int places = own.places();
+            if (at >= first + places * per) {  // the next sequence
+                first += places * per;
+                b++;
+                len = next_len;
+                next_len = len_of(p, min(b + 1, p.batch - 1));
+                continue;
+            }
+            const int seg = quotient(at - first, places), seg_first = first + seg * places;
+            const int t0 = max(at - seg_first - kStart, 0), t1 = min(places, span.end - seg_first) - kStart;
+            at = min(seg_first + places, span.end);
+            if (t1 <= 0) continue;  // (places alone)
+            x.b = b;
+            x.kvh = p.chunks == 1 ? seg : quotient(seg, p.chunks);
+            x.piece = seg - x.kvh * p.chunks;
+            x.lo = own.lo;
+            x.hi = len;
+            x.t0 = own.first() + t0;
+            x.t1 = own.first() + t1;
+            x.w0 = quotient(seg_first + kStart, span.size);
+            x.pieces = quotient(seg_first + places - 1, span.size) - x.w0 + 1;
+            return true;
         }
-        const int seg = quotient(at - first, places), seg_first = first + seg * places;
-        const int t0 = max(at - seg_first - kStart, 0), t1 = min(places, span.end - seg_first) - kStart;
-        at = min(seg_first + places, span.end);
-        if (t1 <= 0) continue;  // (places alone)
-        const int kvh = p.chunks == 1 ? seg : quotient(seg, p.chunks), piece = seg - kvh * p.chunks;
-        const int w0 = quotient(seg_first + kStart, span.size), pieces = quotient(seg_first + places - 1, span.size) - w0 + 1;
-        const size_t segment = (size_t)b * per + seg;
-        const bool alone = pieces == 1 && own.lo == 0;
-        const int head = piece * p.rows, rows = min(p.rows, p.group - head);  // of the kv head's query heads
+        return false;
+    };
+    Walk<D, kWhole> w(p, kWaves, lane);
+    Keys<D> x;
+    u32x4_t q[D / 32];
+    auto over = [&](const Piece& c) __attribute__((always_inline)) {
+        w.over(p.page_table + (size_t)c.b * p.table_pages, c.kvh, c.lo, c.hi, c.t0 + wave, c.t1);
+        w.request_entries(min(w.first, w.end - 1));
+    };
+    auto rows_of = [&](const Piece& c) { return min(p.rows, p.group - c.piece * p.rows); };  // of the kv head's query heads
+    auto begin = [&](const Piece& c) __attribute__((always_inline)) {
+        const int rows = rows_of(c);
         const bool there = n % kR < rows;
-
-        UnitWord word;
-        if (!kShared && !alone && tid == 0) word.request(word_of(p, b, kvh, piece), p.launch_id);
-        u32x4_t q[D / 32];
-        const uint16_t* q_row = p.q + ((size_t)b * p.heads + kvh * p.group + head + (there ? n % kR : 0)) * dim;
+        const uint16_t* q_row = p.q + ((size_t)c.b * p.heads + c.kvh * p.group + c.piece * p.rows + (there ? n % kR : 0)) * dim;
 #pragma unroll
-        for (int c = 0; c < D / 32; c++) {
-            q[c] = u32x4_t{0, 0, 0, 0};
-            if (there && (kWhole || 32 * c + 8 * quad < dim)) q[c] = *(const u32x4_t*)(q_row + 32 * c + 8 * quad);
+        for (int k = 0; k < D / 32; k++) {
+            q[k] = *(const u32x4_t*)(q_row + (kWhole ? 32 * k + 8 * quad : min(32 * k + 8 * quad, dim - 8)));
+            if (!there || (!kWhole && 32 * k + 8 * quad >= dim)) q[k] = u32x4_t{0, 0, 0, 0};
         }
-        if (!kShared && !alone && tid == 0) word.replace();
+        w.await_entries();
+        if (w.first < w.end) {
+            w.place(w.first, 0);
+            w.load_k(x, lanes);
+            w.load_v(x, lanes);
+        }
+    };
+    Piece now, then;
+    bool any = next(now);
+    if (any) {
+        over(now);
+        begin(now);
+    }
+    while (any) {
+        const bool alone = now.pieces == 1 && now.lo == 0;
+        const int rows = rows_of(now), head = now.kvh * p.group + now.piece * p.rows;
+        UnitWord word;
+        if (!kShared && !alone && tid == 0) word.request(word_of(p, now.b, now.kvh, now.piece), p.launch_id);
+        any = next(then);
         State<D> st;
         st.reset();
-        {
-            Walk<D, kWhole> w(p, p.page_table + (size_t)b * p.table_pages, kvh, own.lo, len, own.first() + t0 + wave, own.first() + t1, kWaves, lane);
-            walk<D, C, kWhole>(st, w, lanes, q, cls, quad, p.scale_log2e);
+        walk<D, C, kWhole>(st, w, x, lanes, q, cls, quad, p.scale_log2e);
+        if (!kShared && !alone && tid == 0) word.replace();
+        if (any) {
+            over(then);
+            begin(then);
         }
-        const __amdgpu_buffer_rsrc_t rs = slots.of_own(w0, segment, pieces);
-        const uint32_t to = (uint32_t)(group - w0) * slots.own_bytes;
-        if (kShared && tid == 0) *(UnitLine*)word_of(p, b, kvh, piece) = UnitLine{w0, alone ? -1 : pieces};
+        const size_t segment = ((size_t)now.b * p.kv_heads + now.kvh) * p.chunks + now.piece;
+        const __amdgpu_buffer_rsrc_t rs = slots.of_own(now.w0, segment, now.pieces);
+        const uint32_t to = (uint32_t)(group - now.w0) * slots.own_bytes;
+        if (kShared && tid == 0) *(UnitLine*)word_of(p, now.b, now.kvh, now.piece) = UnitLine{now.w0, alone ? -1 : now.pieces};
         fold(st, rows,
              [&](int row, int d, f32x4_t o) __attribute__((always_inline)) {
-                 if (alone) put_out(p, dim, b, kvh * p.group + head + row, d, o * inv_l[row]);
+                 if (alone) put_out(p, dim, now.b, head + row, d, o * inv_l[row]);
                  else put4(rs, to + 4u * (uint32_t)(row * D + d), o);
              },
              [&](int row, float m, float l) __attribute__((always_inline)) {
                  if (!alone) put2(rs, to + 4u * (uint32_t)(p.rows * D + 2 * row), m, l);
              });
-        if (kShared || alone) continue;
-        if (tid == 0) word.settle();
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (tid == 0) is_last = word.count(pieces) ? 1 : 0;
-        __syncthreads();
-        if (is_last) join<D, false>(p, lds, inv_l, dim, b, kvh * p.group + head, rows, rs, 0, 0, 0, rs, pieces);
-        __syncthreads();
+        if (!kShared && !alone) {
+            if (tid == 0) word.settle();
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (tid == 0) is_last = word.count(now.pieces) ? 1 : 0;
+            __syncthreads();
+            if (is_last) join<D, false>(p, lds, inv_l, dim, now.b, head, rows, rs, 0, 0, 0, rs, now.pieces);
+            __syncthreads();
+        }
+        now = then;
     }
 }
 
@@ -935,7 +995,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedDecodeParams 
 
 template <int D, bool kWhole, bool kShared>
 hipError_t launch_as(hipStream_t stream, const PagedDecodeParams& p) {
-    const dim3 grid(p.n_groups), block(64 * kWaves);
+    const dim3 grid(p.n_groups), block(kThreads);
     if (p.rows <= 4) hipLaunchKernelGGL((paged_decode_kernel<D, 4, kWhole, kShared>), grid, block, 0, stream, p);
     else if (p.rows <= 8) hipLaunchKernelGGL((paged_decode_kernel<D, 2, kWhole, kShared>), grid, block, 0, stream, p);
     else hipLaunchKernelGGL((paged_decode_kernel<D, 1, kWhole, kShared>), grid, block, 0, stream, p);
@@ -949,7 +1009,7 @@ hipError_t launch_dim(hipStream_t stream, const PagedDecodeParams& p, bool share
 }
 
 // Workgroups a CU, each with a wave on every SIMD.
-constexpr int per_cu(int64_t dim, bool shared) { return dim == 256 ? 1 : 2; }
+constexpr int per_cu(int64_t dim) { return dim == 256 ? 1 : 2; }
 constexpr int kPreCost = 2;  // places of a prefix's step
 // Segments, steps and workgroups of a call at its longest, and what its workspace holds.
 struct Plan {
@@ -1047,7 +1107,7 @@ RT_API int rt_gqa_decode_paged_bf16(void* stream, const void* q, const void* k_p
     p.words = p.head + 256;
     p.launch_id = next_launch_id() << 8;  // (its low 16 bits zero)
     const bool shared = shared_lens || shared_len > 0;
-    p.n_groups = std::min(a.groups, kCus * per_cu(a.dim, shared));
+    p.n_groups = std::min(a.groups, kCus * per_cu(a.dim));
     const hipStream_t s = (hipStream_t)stream;
     HIP_TRY(a.dim == 64 ? launch_dim<64>(s, p, shared) : a.dim == 128 ? launch_dim<128>(s, p, shared) : launch_dim<256>(s, p, shared), "paged_decode launch");
     return RT_OK;

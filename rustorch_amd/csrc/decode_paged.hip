@@ -140,7 +140,7 @@ __device__ __forceinline__ int len_of(const PagedDecodeParams& p, int b) { retur
 
 struct Span {
     int total, size;     // places of all; of a span
-    int shared;          // the prefix's length; 0: nobody shares one
+    int shared, owner;   // the prefix's length; 0: nobody shares one.  The sequence whose pages of it are read
     int pre_places;      // places of a (kv head, tile) of the prefix
     int pre_total;       // of all of them
     int b, first, len;   // the sequence that holds the span's first place, where it starts, its length
@@ -159,14 +159,18 @@ __device__ __forceinline__ Span span_of(const PagedDecodeParams& p, int& group, 
     const int len0 = len_at(0), ends0 = lane_sums(places(len0));
     s.empty = __ballot(len0 == 0);
     int sum = __builtin_amdgcn_readlane(ends0, 63), most = lane_max(len0 < 0 ? 0 : Own(len0, s.shared).steps());
-    bool any = kShared && __any(len0 >= s.shared);
+    auto sharer = [&](int len, int b0) {  // the first of 64 that has the prefix
+        const uint64_t have = __ballot(len >= s.shared);
+        return have ? b0 + __ffsll((unsigned long long)have) - 1 : -1;
+    };
+    s.owner = kShared ? sharer(len0, 0) : -1;
     for (int b0 = 64; b0 < p.batch; b0 += 64) {
         const int len = len_at(b0);
         sum += __builtin_amdgcn_readlane(lane_sums(places(len)), 63);
         most = max(most, lane_max(len < 0 ? 0 : Own(len, s.shared).steps()));
-        any = any || (kShared && __any(len >= s.shared));
+        if (kShared && s.owner < 0) s.owner = sharer(len, b0);
     }
-    if (!any) s.shared = 0;  // (then every `lo` was 0 already)
+    if (s.owner < 0) s.shared = 0;  // (then every `lo` was 0 already)
     s.pre_places = s.shared > 0 ? kStart + steps_up_to(s.shared) * p.pre_cost : 0;
     s.pre_total = s.pre_places * p.kv_heads * p.n_tiles;
     most = max(most, s.pre_places);
@@ -851,7 +855,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void paged_decode_kerne
 #pragma unroll
                 for (int i = 0; i < 16; i++) st.o[t][i] = 0.0f;
             Walk<D, kWhole> w(p, 1, lane);
-            w.over(p.page_table, kvh, 0, span.shared, t0, t1);
+            w.over(p.page_table + (size_t)span.owner * p.table_pages, kvh, 0, span.shared, t0, t1);
             prefix_walk<D, kWhole>(st, w, lds, q, units > 0, wave, p.scale_log2e);
             if (units <= 0) continue;  // (a wave without rows has its share of the keys' way to LDS)
             const __amdgpu_buffer_rsrc_t rs = rsrc_of(slots.pre + ((size_t)group + seg) * Slots<D>::kPre + (size_t)wave * Slots<D>::kWave, Slots<D>::kWave);

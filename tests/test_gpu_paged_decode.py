@@ -79,6 +79,15 @@ def test_long_prefixes(batch, heads, n_kv, dim, shared, own):
     check(normal_bits(rng, batch, heads, dim), pages, n_kv, shared)
 
 
+@pytest.mark.parametrize("ahead", [1, 70])
+def test_a_prefix_behind_sequences_that_do_not_have_it(ahead):
+    """Idle slots and short sequences come first, with rows of the table of their own."""
+    rng = np.random.default_rng(ahead)
+    lens = [0 if i % 3 == 0 else 20 + i for i in range(ahead)] + [200, 99, 130, 100]
+    pages = Pages(rng, lens, 2, 64, 16, 100)
+    check(normal_bits(rng, len(lens), 8, 64), pages, 2, 100)
+
+
 def test_a_prefix_that_nobody_has_whole():
     rng = np.random.default_rng(5)
     pages = Pages(rng, [10, 0, 99], 2, 64, 16)

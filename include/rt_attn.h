@@ -461,7 +461,8 @@ size_t rt_gqa_decode_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_k
  * A token whose position the tables do not have is left as it is, everywhere; one whose row has no page (behind the table, negative,
  * or an entry that is no page) is rotated and not stored.  No two tokens of a call may go to one row of a page; what is shared stays as it
  * is.  A host `pos` is checked (RT_ERR_ROPE_POSITION_OVERFLOW, then RT_ERR_KV_OVERFLOW; with `starts`, its lowest row alone).  All tensors
- * 16-byte aligned (gammas and tables 4); outputs and pages share no memory with each other or with other inputs (RT_ERR_UNSUPPORTED). */
+ * 16-byte aligned (gammas and tables 4); outputs and pages share no memory with each other or with other inputs; tokens up to 2^25
+ * (RT_ERR_UNSUPPORTED). */
 int rt_qk_norm_rope_kv_append_paged_bf16(void *stream, const void *q, void *q_out, const void *k_in, void *k_out,
                                          const void *v_in, void *k_pages, void *v_pages, const int32_t *page_table,
                                          const int32_t *starts, const int32_t *positions, int32_t pos,

@@ -37,7 +37,6 @@ struct PagedAppendParams {
     int tokens, batch, each;  // each: tokens / batch where there are no starts
     int n_heads, n_kv, dim, n_pages, table_pages, page_shift;
     int n_axes, ends[kMaxAxes];  // pairs below ends[i], and not below ends[i - 1], turn with axis i
-    int per;  // set by the launcher: passes a wave makes over a token's rows
 };
 
 // A decode step over pages (decode_paged.hip).

@@ -8,10 +8,20 @@
 // The f32 arithmetic is the reference's, rounding for rounding (this file too is compiled without contraction): the sum of squares
 // runs in index order, so that a row has the bits that prepare.hip gives it.
 //
-// A wave takes a token: its sequence, place and angles are found once, as scalars and a lane's registers, and serve all of the token's
-// rows, which follow one another in memory.  D / 16 lanes a row (4, 8 or 16 of them set aside): lane j has the dims 8 j .. 8 j + 7 and
-// their partners D / 2 on, 16 bytes a request.  The sum of squares goes from lane to lane within registers: at stage i lane i's value is
-// that of dims 0 .. 8 i + 7, added one by one, and moves on; what the other lanes add meanwhile is thrown away.
+// D / 16 lanes a row (4, 8 or 16 of them set aside), so that a wave has 16, 8 or 4 of a token's rows: lane j has the dims 8 j .. 8 j + 7
+// and their partners D / 2 on, 16 bytes a request.  The sum of squares goes from lane to lane within registers: at stage i lane i's value
+// is that of dims 0 .. 8 i + 7, added one by one, and moves on; what the other lanes add meanwhile is thrown away.
+//
+// Bound: HBM where there are many tokens, a chain of reads (sequence, place, angles) where there are few.  A wave looks all that up for
+// its few rows alone and is gone: us in a recorded loop, one pass a wave / all passes of a token by one wave, two at a time: 1 token
+// of 32 + 8 heads of 128 3.5 / 9.4, 256 5.0 / 10.9, 1000 9.8 / 13.6, 4 prompts up to 4096 66.8 / 69.3 (301 MB: 4.5 TB/s), 6 up to 2000
+// of 16 + 16 heads of 64 on three axes 27.9 / 27.1.  The angles of three axes 16 bytes a request where all sections are multiples of
+// four, or word by word: 27.9, 31.1 on the last.
+//
+// Rows go past the caches to the pages, which the attention of the same prompt does not read (call alone and with that attention behind
+// it, us, plainly / past: 8 prompts up to 300 of 32 + 8 heads of 128 12.6, 25.0 / 11.8, 24.2; 6 up to 2000 of 16 + 16 of 64 27.3, 63.9 / 26.8, 63.9;
+// 16 up to 2000 of 32 + 8 100, 318 / 100, 316), and stay in them where it does: with q_out and k_out past them too the call is 2 to 15 %
+// shorter (23.5 for 26.8) and the two together as long or longer (64.4; 4 up to 4096 338 -> 345).
 #include <algorithm>
 
 #include "cache_paged.hpp"
@@ -30,39 +40,25 @@ __device__ __forceinline__ float from_lane_below(float x) {  // within a row of 
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x111, 0xf, 0xf, true));
 }
 
-// U rows a lane at once.  Grid (tokens / waves of a workgroup, pieces of a token's rows).
-template <int kLanes, int U, bool kAxes>
-__global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p) {
-    constexpr int kRows = 64 / kLanes;  // a wave's, a pass
-    const int lane = threadIdx.x & 63, j = lane % kLanes, r = lane / kLanes;
-    const int t = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6)));
-    if (t >= p.tokens) return;
-    const int D = p.dim, half = D / 2, nl = D / 16, all = p.n_heads + 2 * p.n_kv;
-    const int pass0 = (int)blockIdx.y * p.per, passes = min((all + kRows - 1) / kRows, pass0 + p.per);
+// Grid (tokens, passes over a token's rows), a wave each.
+// kAxes: 0: a position a token; else the pairs of a lane that lie side by side, kAxes of them, turn with one axis.
+template <int kLanes, int kAxes>
+__global__ __launch_bounds__(64) void paged_append_kernel(PagedAppendParams p) {
+    constexpr int kRows = 64 / kLanes;  // a wave's
+    const int lane = threadIdx.x, j = lane % kLanes, r = lane / kLanes, t = blockIdx.x, hh = (int)blockIdx.y * kRows + r;
+    const int D = p.dim, half = D / 2, nl = D / 16;
+    // the lane's row
+    const bool on = hh < p.n_heads + 2 * p.n_kv, is_q = hh < p.n_heads, is_v = hh >= p.n_heads + p.n_kv;
+    const int h = is_q ? hh : is_v ? hh - p.n_heads - p.n_kv : hh - p.n_heads;
     const bool in_row = j < nl;  // (a head dim of no power of two leaves lanes over)
     const int d0 = in_row ? 8 * j : 0;
 
-    u32x4_t raw[U][2];
-    auto place = [&](int pass, int u, int& hh) __attribute__((always_inline)) {  // the lane's row
-        hh = (pass + u) * kRows + r;
-        return pass + u < passes && hh < all;
-    };
-    auto load = [&](int pass) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            int hh;
-            const bool on = place(pass, u, hh);
-            hh = on ? hh : 0;
-            const bool is_q = hh < p.n_heads, is_v = hh >= p.n_heads + p.n_kv;
-            const uint16_t* src = is_q ? p.q + ((size_t)t * p.n_heads + hh) * D : (is_v ? p.v_in + ((size_t)t * p.n_kv + (hh - p.n_heads - p.n_kv)) * D : p.k_in + ((size_t)t * p.n_kv + (hh - p.n_heads)) * D);
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                raw[u][e] = u32x4_t{0, 0, 0, 0};
-                if (on && in_row) raw[u][e] = *(const u32x4_t*)(src + d0 + e * half);
-            }
-        }
-    };
-    load(pass0);
+    u32x4_t raw[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    if (on && in_row) {
+        const uint16_t* src = (is_q ? p.q + ((size_t)t * p.n_heads + h) * D : (is_v ? p.v_in : p.k_in) + ((size_t)t * p.n_kv + h) * D) + d0;
+        raw[0] = *(const u32x4_t*)src;
+        raw[1] = *(const u32x4_t*)(src + half);
+    }
 
     // the token's sequence, row and page
     int b, first;
@@ -87,7 +83,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p) 
     const bool stored = page >= 0 && page < p.n_pages;
     // its angles; a token whose position the tables do not have is left as it is
     float cs[8], sn[8];
-    if constexpr (kAxes) {
+    if constexpr (kAxes > 0) {
         int at[kMaxAxes];
 #pragma unroll
         for (int a = 0; a < kMaxAxes; a++) at[a] = a < p.n_axes ? p.axes[(size_t)a * p.tokens + t] : 0;
@@ -95,14 +91,19 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p) 
 #pragma unroll
         for (int a = 0; a < kMaxAxes; a++) ok = ok && at[a] >= 0 && at[a] < p.table_rows;
         if (!ok) return;
+        typedef float piece_t __attribute__((ext_vector_type(kAxes), aligned(4)));
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
+        for (int e = 0; e < 8; e += kAxes) {
             const int i = d0 + e;
             int pos = at[0];
 #pragma unroll
             for (int a = 1; a < kMaxAxes; a++) pos = i >= p.ends[a - 1] ? at[a] : pos;
-            cs[e] = p.cos_table[(size_t)pos * half + i];
-            sn[e] = p.sin_table[(size_t)pos * half + i];
+            const piece_t c = *(const piece_t*)(p.cos_table + (size_t)pos * half + i), s = *(const piece_t*)(p.sin_table + (size_t)pos * half + i);
+#pragma unroll
+            for (int k = 0; k < kAxes; k++) {
+                cs[e + k] = c[k];
+                sn[e + k] = s[k];
+            }
         }
     } else {
         if (row < 0 || row >= p.table_rows) return;
@@ -120,115 +121,78 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams p) 
     const size_t page_row = stored ? (size_t)page * p.n_kv << p.page_shift : 0;  // of head 0's first row
     const size_t in_page = (size_t)(row & ((1ll << p.page_shift) - 1));
 
-    for (int pass = pass0; pass < passes; pass += U) {
-        if (pass != pass0) load(pass);
-        float x[U][2][8];
-        const float* gamma[U];
-        bool any_norm = false;
+    float x[2][8];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            int hh;
-            const bool on = place(pass, u, hh);
-            gamma[u] = !on || hh >= p.n_heads + p.n_kv ? nullptr : hh < p.n_heads ? p.q_gamma : p.k_gamma;
-            any_norm = any_norm || gamma[u];
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x[e][2 * i] = bf16_lo(raw[e][i]);
+            x[e][2 * i + 1] = bf16_hi(raw[e][i]);
+        }
+    const float* const gamma = !on || is_v ? nullptr : is_q ? p.q_gamma : p.k_gamma;
+    if (__any(gamma != nullptr)) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            float sq[8], at = sum;
+#pragma unroll
+            for (int i = 0; i < 8; i++) sq[i] = x[e][i] * x[e][i];
+            for (int stage = 0; stage < nl; stage++) {
+                sum = at;
+#pragma unroll
+                for (int i = 0; i < 8; i++) sum = sum + sq[i];
+                at = from_lane_below(sum);
+            }
+            sum = __shfl(sum, r * kLanes + nl - 1, 64);
+        }
+        if (gamma) {
+            const float inv_d = 1.0f / (float)D;
+            const float inv_rms = 1.0f / sqrtf(sum * inv_d + p.eps);
 #pragma unroll
             for (int e = 0; e < 2; e++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    x[u][e][2 * i] = bf16_lo(raw[u][e][i]);
-                    x[u][e][2 * i + 1] = bf16_hi(raw[u][e][i]);
+                for (int i = 0; i < 8; i += 4) {
+                    const f32x4_t g = *(const f32x4_any*)(gamma + e * half + d0 + i);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) x[e][i + k] = x[e][i + k] * inv_rms * g[k];
                 }
         }
-        if (__any(any_norm)) {
-            float sum[U];
+    }
+    if (!on || !in_row) return;
+    u32x4_t o[2] = {raw[0], raw[1]};
+    if (!is_v) {
 #pragma unroll
-            for (int u = 0; u < U; u++) sum[u] = 0.0f;
+        for (int i = 0; i < 4; i++) {
+            float y0[2], y1[2];
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                float sq[U][8], at[U];
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    at[u] = sum[u];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) sq[u][i] = x[u][e][i] * x[u][e][i];
-                }
-                for (int stage = 0; stage < nl; stage++)
-#pragma unroll
-                    for (int u = 0; u < U; u++) {
-                        float s = at[u];
-#pragma unroll
-                        for (int i = 0; i < 8; i++) s = s + sq[u][i];
-                        sum[u] = s;
-                        at[u] = from_lane_below(s);
-                    }
-#pragma unroll
-                for (int u = 0; u < U; u++) sum[u] = __shfl(sum[u], r * kLanes + nl - 1, 64);
+            for (int k = 0; k < 2; k++) {
+                const int e = 2 * i + k;
+                y0[k] = x[0][e] * cs[e] - x[1][e] * sn[e];
+                y1[k] = x[1][e] * cs[e] + x[0][e] * sn[e];
             }
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                if (!gamma[u]) continue;
-                const float inv_d = 1.0f / (float)D;
-                const float inv_rms = 1.0f / sqrtf(sum[u] * inv_d + p.eps);
-#pragma unroll
-                for (int e = 0; e < 2; e++)
-#pragma unroll
-                    for (int i = 0; i < 8; i += 4) {
-                        const f32x4_t g = *(const f32x4_any*)(gamma[u] + e * half + d0 + i);
-#pragma unroll
-                        for (int k = 0; k < 4; k++) x[u][e][i + k] = x[u][e][i + k] * inv_rms * g[k];
-                    }
-            }
+            o[0][i] = pack_bf16x2(y0[0], y0[1]);
+            o[1][i] = pack_bf16x2(y1[0], y1[1]);
         }
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            int hh;
-            if (!place(pass, u, hh) || !in_row) continue;
-            const bool is_q = hh < p.n_heads, is_v = hh >= p.n_heads + p.n_kv;
-            const int h = is_q ? hh : is_v ? hh - p.n_heads - p.n_kv : hh - p.n_heads;
-            u32x4_t o[2] = {raw[u][0], raw[u][1]};
-            if (!is_v) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    float y0[2], y1[2];
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const int e = 2 * i + k;
-                        const float x0 = x[u][0][e], x1 = x[u][1][e];
-                        y0[k] = x0 * cs[e] - x1 * sn[e];
-                        y1[k] = x1 * cs[e] + x0 * sn[e];
-                    }
-                    o[0][i] = pack_bf16x2(y0[0], y0[1]);
-                    o[1][i] = pack_bf16x2(y1[0], y1[1]);
-                }
-            }
-            if (is_q || (!is_v && p.k_out)) {
-                uint16_t* dst = is_q ? p.q_out + ((size_t)t * p.n_heads + h) * D : p.k_out + ((size_t)t * p.n_kv + h) * D;
-                *(u32x4_t*)(dst + d0) = o[0];
-                *(u32x4_t*)(dst + d0 + half) = o[1];
-            }
-            if (!is_q && stored) {
-                uint16_t* dst = (is_v ? p.v_pages : p.k_pages) + (page_row + ((size_t)h << p.page_shift) + in_page) * D;
-                *(u32x4_t*)(dst + d0) = o[0];
-                *(u32x4_t*)(dst + d0 + half) = o[1];
-            }
-        }
+    }
+    if (is_q || (!is_v && p.k_out)) {
+        uint16_t* dst = (is_q ? p.q_out + ((size_t)t * p.n_heads + h) * D : p.k_out + ((size_t)t * p.n_kv + h) * D) + d0;
+        *(u32x4_t*)dst = o[0];
+        *(u32x4_t*)(dst + half) = o[1];
+    }
+    if (!is_q && stored) {
+        uint16_t* dst = (is_v ? p.v_pages : p.k_pages) + (page_row + ((size_t)h << p.page_shift) + in_page) * D + d0;
+        __builtin_nontemporal_store(o[0], (u32x4_t*)dst);
+        __builtin_nontemporal_store(o[1], (u32x4_t*)(dst + half));
     }
 }
 
-template <int kLanes, int U>
-hipError_t launch_as(hipStream_t stream, const PagedAppendParams& p, dim3 grid, dim3 block) {
-    if (p.axes) hipLaunchKernelGGL((paged_append_kernel<kLanes, U, true>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((paged_append_kernel<kLanes, U, false>), grid, block, 0, stream, p);
-    return hipGetLastError();
-}
 template <int kLanes>
-hipError_t launch_lanes(hipStream_t stream, PagedAppendParams p) {
-    const int passes = (p.n_heads + 2 * p.n_kv + 64 / kLanes - 1) / (64 / kLanes);
-    const bool few = p.tokens <= 256;
-    p.per = few ? 1 : passes;
-    const int waves = few ? 1 : 4;
-    const dim3 grid((unsigned)((p.tokens + waves - 1) / waves), (unsigned)((passes + p.per - 1) / p.per)), block(64 * waves);
-    return few ? launch_as<kLanes, 1>(stream, p, grid, block) : launch_as<kLanes, 2>(stream, p, grid, block);
+hipError_t launch_lanes(hipStream_t stream, const PagedAppendParams& p) {
+    const dim3 grid((unsigned)p.tokens, (unsigned)((p.n_heads + 2 * p.n_kv + 64 / kLanes - 1) / (64 / kLanes))), block(64);
+    if (!p.axes) hipLaunchKernelGGL((paged_append_kernel<kLanes, 0>), grid, block, 0, stream, p);
+    else if ((p.ends[0] | p.ends[1] | p.ends[2]) % 4 == 0) hipLaunchKernelGGL((paged_append_kernel<kLanes, 4>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((paged_append_kernel<kLanes, 1>), grid, block, 0, stream, p);
+    return hipGetLastError();
 }
 hipError_t launch_paged_append(hipStream_t stream, const PagedAppendParams& p) {
     return p.dim <= 64 ? launch_lanes<4>(stream, p) : p.dim <= 128 ? launch_lanes<8>(stream, p) : launch_lanes<16>(stream, p);
@@ -253,7 +217,7 @@ RT_API int rt_qk_norm_rope_kv_append_paged_bf16(void* stream, const void* q, voi
     if (head_dim == 0) return fail(err, RT_ERR_ZERO_DIM, -1, 0, 0, "head_dim must be > 0");
     if (!cache_paged_dim(head_dim)) return fail(err, RT_ERR_UNSUPPORTED, -1, 256, (uint64_t)head_dim, "pages have head_dim up to 256, a multiple of 16");
     if (!cache_page_size(page_size)) return fail(err, RT_ERR_UNSUPPORTED, -1, kPageMax, (uint64_t)(int64_t)page_size, "page_size must be a power of two, 16 to 1024");
-    if (n_heads > 65535 || n_kv > 65535 || (int64_t)table_pages * page_size > 0x7fffffffll) return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "shape too large for the launch grid");
+    if (tokens > (1 << 25) || n_heads > 65535 || n_kv > 65535 || (int64_t)table_pages * page_size > 0x7fffffffll) return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "shape too large for the launch grid");
     PagedAppendParams p{};
     if (n_axes > 0) {
         if (n_axes > kMaxAxes) return fail(err, RT_ERR_UNSUPPORTED, -1, kMaxAxes, (uint64_t)n_axes, "at most four axes");

@@ -45,6 +45,11 @@ def test_append_refuses(more):
     assert append(**more)[0] == L.RT_ERR_UNSUPPORTED
 
 
+def test_append_refuses_more_tokens_than_a_grid_has():
+    rc, err = append(tokens=(1 << 25) + 2, batch=2)
+    assert rc == L.RT_ERR_UNSUPPORTED and b"launch grid" in err.message
+
+
 def test_append_refuses_with_the_reference_errors():
     assert append(dim=0)[0] == L.RT_ERR_ZERO_DIM
     for more in (dict(q=None), dict(q_out=None), dict(k_in=None), dict(v_in=None), dict(kp=None), dict(vp=None), dict(table=None), dict(cos=None), dict(sin=None),

@@ -76,6 +76,11 @@ def test_one_long_sequence_on_few_heads(dim):
     check(dim, [1700], 2, 1, dim)
 
 
+@pytest.mark.parametrize("dim,heads,lens", [(128, 32, [1300]), (64, 16, [900, 130, 1000]), (80, 40, [1200]), (256, 16, [100, 1700])])
+def test_walks_in_halves_two_to_a_cu(dim, heads, lens):
+    check(dim, lens, heads, heads // 4, dim)
+
+
 @pytest.mark.parametrize("dim,heads", [(64, 32), (128, 32), (256, 16)])
 def test_more_tiles_than_the_chip_holds(dim, heads):
     check(dim, [300, 10, 500, 129, 400, 257, 200, 380], heads, heads // 4, dim)

@@ -1078,6 +1078,16 @@ RT_API int rt_gqa_decode_paged_bf16(void* stream, const void* q, const void* k_p
     if (!workspace || workspace_bytes < need)
         return fail(err, RT_ERR_WORKSPACE_TOO_SMALL, -1, need, workspace ? workspace_bytes : 0, "workspace too small");
     if ((uintptr_t)workspace & 15) return fail(err, RT_ERR_WORKSPACE_TOO_SMALL, -1, 16, (uint64_t)((uintptr_t)workspace & 15), "workspace must be 16-byte aligned");
+    // (a workgroup writes its rows while others read theirs)
+    const size_t q_bytes = (size_t)batch * n_heads * head_dim * 2, page_bytes = (size_t)n_pages * n_kv * page_size * head_dim * 2;
+    const struct {
+        const void* at;
+        size_t n;
+    } written[2] = {{out, q_bytes}, {workspace, need}}, read[3] = {{q, q_bytes}, {k_pages, page_bytes}, {v_pages, page_bytes}};
+    bool apart = !overlap(out, q_bytes, workspace, need);
+    for (const auto& w : written)
+        for (const auto& r : read) apart = apart && !overlap(w.at, w.n, r.at, r.n);
+    if (!apart) return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "out and the workspace must share no memory with each other or with the inputs");
     int rc = ensure_device(err);
     if (rc) return rc;
     PagedDecodeParams p{};

@@ -91,6 +91,12 @@ def test_decode_refuses(more):
     assert decode(**more)[0] == L.RT_ERR_UNSUPPORTED
 
 
+@pytest.mark.parametrize("more", [dict(out=P), dict(out=4 * FAR + 64), dict(out=5 * FAR), dict(out=6 * FAR + 256), dict(ws=P), dict(ws=4 * FAR - 256), dict(ws=5 * FAR + 1024)])
+def test_decode_refuses_outputs_over_inputs(more):
+    rc, err = decode(**more)
+    assert rc == L.RT_ERR_UNSUPPORTED and b"share no memory" in err.message
+
+
 def test_decode_refuses_with_the_reference_errors():
     assert decode(dim=0)[0] == L.RT_ERR_ZERO_DIM
     assert decode(heads=4, n_kv=3)[0] == decode(n_kv=0)[0] == L.RT_ERR_HEAD_COUNT_MISMATCH

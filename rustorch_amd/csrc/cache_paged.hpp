@@ -55,7 +55,6 @@ struct PagedDecodeParams {
     int group;         // heads / kv_heads
     int chunks, rows;  // of a kv head's query heads: so many pieces of `rows` each (the last may have fewer), at most 16
     int per_wave, per_tile, n_tiles;  // (sequence, piece) pairs of a wave's rows and of a tile of the prefix; tiles of a kv head
-    int pre_cost;   // places of a prefix's step
     int n_groups;      // workgroups launched
     float span_root, scale_log2e;
     float* part;

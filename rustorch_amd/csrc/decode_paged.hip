@@ -99,35 +99,31 @@ __device__ __forceinline__ float quad_max(float x) {
 __device__ __forceinline__ float quad_sum(float x) {
     return over_quads(x, [](float a, float b) __attribute__((always_inline)) { return a + b; });
 }
-// a row of sixteen lanes turned by kBy, and of columns that lie 16 / C apart their largest or their sum, in every one
+// of a row of sixteen lanes, in every one of them
 template <int kBy>
 __device__ __forceinline__ float turned(float x) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + kBy, 0xf, 0xf, true));
 }
-template <int C>
-__device__ __forceinline__ float columns_max(float x) {
-    if (C >= 2) x = fmaxf(x, turned<8>(x));
-    if (C >= 4) x = fmaxf(x, turned<4>(x));
-    if (C == 16) {
-        x = fmaxf(x, turned<2>(x));
-        x = fmaxf(x, turned<1>(x));
-    }
-    return x;
+__device__ __forceinline__ float sixteen_max(float x) {
+    x = fmaxf(x, turned<8>(x));
+    x = fmaxf(x, turned<4>(x));
+    x = fmaxf(x, turned<2>(x));
+    return fmaxf(x, turned<1>(x));
 }
-template <int C>
-__device__ __forceinline__ float columns_sum(float x) {
-    if (C >= 2) x += turned<8>(x);
-    if (C >= 4) x += turned<4>(x);
-    if (C == 16) {
-        x += turned<2>(x);
-        x += turned<1>(x);
-    }
-    return x;
+__device__ __forceinline__ float sixteen_sum(float x) {
+    x += turned<8>(x);
+    x += turned<4>(x);
+    x += turned<2>(x);
+    return x + turned<1>(x);
 }
 
 // ---- the list that the workgroups share -----------------------------------------------------------------------------------
-// Of every segment kStart places, which stand for what it costs besides its steps, and its steps.
-constexpr int kStart = 16;
+// Of every segment kStart places, which stand for what it costs besides its steps, and its steps; of a prefix's step kPreCost places.
+// us, 4 / 8 / 16 / 24 places a start, the next segment's rows being asked for ahead of a fold: 256 sequences of 100 to 700 keys 81.7 / 82.5 / 84.9 /
+// 88.1, 32 of 100 to 900 without groups 20.7 / 19.4 / 21.1 / 23.0, 64 behind 8192 43.0 / 42.3 / 43.5 / 48.3, 4 of 1000 to 4000 15.0 / 13.9 / 13.9
+// / -, 16 of 500 to 4000 on 2 kv heads 18.4 / 16.2 / 16.2 / 16.1.  1 / 2 / 3 places a prefix's step: 64 behind 8192 48.8 / 42.3 / 45.0, 32
+// behind 4096 26.3 / 22.8 / 25.9, 128 behind 1000 40.9 / 31.4 / 28.3, 16 behind 2000 19.9 / 18.2 / 22.1.
+constexpr int kStart = 8, kPreCost = 2;
 __device__ __forceinline__ int steps_up_to(int key) { return (key + kStep - 1) / kStep; }
 struct Own {  // a sequence's own keys
     int len, lo;  // [lo, len); lo: the prefix's length where it shares it, else 0
@@ -171,15 +167,18 @@ __device__ __forceinline__ Span span_of(const PagedDecodeParams& p, int& group, 
         if (kShared && s.owner < 0) s.owner = sharer(len, b0);
     }
     if (s.owner < 0) s.shared = 0;  // (then every `lo` was 0 already)
-    s.pre_places = s.shared > 0 ? kStart + steps_up_to(s.shared) * p.pre_cost : 0;
+    s.pre_places = s.shared > 0 ? kStart + steps_up_to(s.shared) * kPreCost : 0;
     s.pre_total = s.pre_places * p.kv_heads * p.n_tiles;
     most = max(most, s.pre_places);
     s.total = s.pre_total + sum * per;
     // what one of all workgroups gets, but no fewer than a join is worth (a segment of few spans is a long walk, one of many a long join:
-    // their sum is least around the root of its steps), and never more of them than a sequence may have
+    // their sum is least around the root of its steps: span_root), and never more of them than a sequence may have
     const int pieces = s.shared > 0 ? kMaxPieces / 2 : kMaxPieces;
     const int root = __builtin_amdgcn_readfirstlane((int)(__builtin_amdgcn_sqrtf((float)most) * p.span_root + 0.5f * kWaves)) & -kWaves;
     s.size = max(max(kWaves, quotient(s.total + p.n_groups - 1, p.n_groups)), max(root, (most + pieces - 3) / (pieces - 2)));
+    // more workgroups than CUs, but not about two for each: one for each, and spans that its waves share evenly (us, 1 sequence of 30000 keys
+    // 31.4 -> 27.0, 4 of 1000 to 4000 15.0 -> 13.9, 16 behind 2000 20.5 -> 18.1; heads of 32 on 8 of 128)
+    if (s.total < s.size * (p.n_groups / 8 * 7) && s.total > s.size * kCus) s.size = (quotient(s.total + kCus - 1, kCus) + kWaves - 1) & -kWaves;
     if (s.shared > 0) {
         const int active = quotient(s.total + s.size - 1, s.size), eighth = (active + 7) / 8;  // (n_groups divides by eight)
         group = group / 8 < eighth ? (group & 7) * eighth + group / 8 : 0x7fffffff;
@@ -335,13 +334,13 @@ __device__ __forceinline__ void join(const PagedDecodeParams& p, unsigned char* 
         const bool on = row < rows;
         float top = kNoMax, sum = 0.0f;
         for (int k = col; on && k < pieces; k += 16) top = fmaxf(top, wgt[k * p.rows + row]);
-        top = columns_max<16>(top);
+        top = sixteen_max(top);
         for (int k = col; on && k < pieces; k += 16) {
             const float fk = __builtin_amdgcn_exp2f(wgt[k * p.rows + row] - top);
             wgt[k * p.rows + row] = fk;
             sum += wl[k * p.rows + row] * fk;
         }
-        sum = columns_sum<16>(sum);
+        sum = sixteen_sum(sum);
         if (on && col == 0) inv_l[row] = sum == 0.0f ? 0.0f : 1.0f / sum;
     }
     __syncthreads();
@@ -371,8 +370,9 @@ __device__ __forceinline__ void join(const PagedDecodeParams& p, unsigned char* 
 // out^T, dims are rows and keys the products' inner index: lane (n, quad) has dims by n of the eight keys 4 quad + {0..3}, 16 + those, in the
 // order in which scores^T leaves their weights.
 //
-// Up to four or eight query rows leave most of the sixteen columns of a product idle, and what is done a (row, key) would be done for all
-// sixteen: there a row has C = 4 or 2 columns, n, n + 16 / C, ..., each of which takes a C-th of a lane's eight keys, as in decode_cache.hip.
+// Up to four or eight query rows leave most of the sixteen columns of a product idle.  (Those columns put to use for the exponentials of the
+// rows, with zeros in each other's weights, as decode_cache.hip does where codes have to be unpacked first, was no shorter: 64 sequences of 512
+// to 8192 keys 189.3 us for 188.1, one of 2048 9.8 for 9.2, 16 heads of 64 without groups 25.1 for 24.9.)
 template <int D>
 struct Keys {
     uint32_t k[2][D / 8], v[8][D / 32];
@@ -521,38 +521,23 @@ struct State {
 };
 
 // One step.  k_done is called behind the last use of K.
-template <int D, int C, typename KDone>
-__device__ __forceinline__ void step(State<D>& st, Keys<D>& x, const u32x4_t (&q)[D / 32], KDone k_done, uint32_t seen, int cls, int quad, float scale_log2e) {
-    constexpr int kE = 8 / C;
+template <int D, typename KDone>
+__device__ __forceinline__ void step(State<D>& st, Keys<D>& x, const u32x4_t (&q)[D / 32], KDone k_done, uint32_t seen, int quad, float scale_log2e) {
     f32x4_t a[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
     for (int c = 0; c < D / 32; c++)
 #pragma unroll
         for (int h = 0; h < 2; h++) a[h] = mfma(*(const u32x4_t*)(x.k[h] + 4 * c), q[c], a[h]);
-    float y[kE];
-    if constexpr (C == 1) {
+    float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = a[e / 4][e % 4];
-    } else if constexpr (C == 2) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) y[e] = cls ? a[1][e] : a[0][e];
-    } else {
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            // (of both sixteens first: two of one register group the compiler takes for an index into it, four selections)
-            const float a0 = cls & 2 ? a[1][e] : a[0][e], a2 = cls & 2 ? a[1][2 + e] : a[0][2 + e];
-            y[e] = cls & 1 ? a2 : a0;
-        }
-    }
-    // the lane's keys, of its eight slots; a key that is not there has no weight, and zeros in V, whatever lies there
+    for (int e = 0; e < 8; e++) y[e] = a[e / 4][e % 4];
+    // a key that is not there has no weight, and zeros in V, whatever lies there
     if (seen != ~0u) {
-        auto place = [&](int e) __attribute__((always_inline)) { return C == 1 ? 16 * (e / 4) + e % 4 : C == 2 ? 16 * cls + e : 16 * (cls >> 1) + 2 * (cls & 1) + e; };
         const uint32_t mine = seen >> (4 * quad);
-#pragma unroll
-        for (int e = 0; e < kE; e++) y[e] = mine >> place(e) & 1 ? y[e] : neg_inf();
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const bool hid = !(mine >> (16 * (e / 4) + e % 4) & 1);
+            y[e] = hid ? neg_inf() : y[e];
 #pragma unroll
             for (int w = 0; w < D / 32; w++) x.v[e][w] = hid ? 0u : x.v[e][w];
         }
@@ -562,7 +547,7 @@ __device__ __forceinline__ void step(State<D>& st, Keys<D>& x, const u32x4_t (&q
     // by 8 in it: up to there sums of weights in f32 and weights of 8 bits are as exact, and sums are scaled once or twice a span.
     float top = y[0];
 #pragma unroll
-    for (int e = 1; e < kE; e++) top = fmaxf(top, y[e]);
+    for (int e = 1; e < 8; e++) top = fmaxf(top, y[e]);
     top = quad_max(top) * scale_log2e;
     if (__any(top - st.m > 8.0f)) {
         const float m_new = fmaxf(st.m, top), alpha = __builtin_amdgcn_exp2f(st.m - m_new);
@@ -571,24 +556,15 @@ __device__ __forceinline__ void step(State<D>& st, Keys<D>& x, const u32x4_t (&q
 #pragma unroll
         for (int d = 0; d < D / 16; d++) st.o[d] *= alpha;
     }
-    float f[kE];
+    float f[8];
 #pragma unroll
-    for (int e = 0; e < kE; e++) {
+    for (int e = 0; e < 8; e++) {
         f[e] = __builtin_amdgcn_exp2f(fmaf(y[e], scale_log2e, -st.m));
         st.l += f[e];
     }
-    // pairs of weights as the operand's words, zeros in the other columns' places
-    u32x4_t w;
+    u32x4_t w;  // the weights, as the operand's words
 #pragma unroll
-    for (int k = 0; k < kE / 2; k++) {
-        const uint32_t two = two_bf16(f[2 * k], f[2 * k + 1]);
-        if constexpr (C == 1) {
-            w[k] = two;
-        } else {
-#pragma unroll
-            for (int c = 0; c < C; c++) w[c * (kE / 2) + k] = cls == c ? two : 0u;
-        }
-    }
+    for (int k = 0; k < 4; k++) w[k] = two_bf16(f[2 * k], f[2 * k + 1]);
 #pragma unroll
     for (int d = 0; d < D / 16; d++) {  // dim n * (D / 16) + d; of 256, of the lower and of the upper 128 in turn
         u32x4_t v;
@@ -599,18 +575,18 @@ __device__ __forceinline__ void step(State<D>& st, Keys<D>& x, const u32x4_t (&q
 }
 
 // x: the first step's rows, under way.
-template <int D, int C, bool kWhole>
-__device__ __forceinline__ void walk(State<D>& st, Walk<D, kWhole>& at, Keys<D>& x, const Lanes<D, kWhole>& lanes, const u32x4_t (&q)[D / 32], int cls, int quad, float scale_log2e) {
+template <int D, bool kWhole>
+__device__ __forceinline__ void walk(State<D>& st, Walk<D, kWhole>& at, Keys<D>& x, const Lanes<D, kWhole>& lanes, const u32x4_t (&q)[D / 32], int quad, float scale_log2e) {
     int i = 0;
     for (int t = at.first; t < at.end; t += at.stride) {
         const uint32_t seen = at.seen;
         const bool more = t + at.stride < at.end;
-        step<D, C>(st, x, q, [&]() __attribute__((always_inline)) {
+        step<D>(st, x, q, [&]() __attribute__((always_inline)) {
             if (more) {
                 at.place(t + at.stride, ++i);
                 at.load_k(x, lanes);
             }
-        }, seen, cls, quad, scale_log2e);
+        }, seen, quad, scale_log2e);
         if (more) at.load_v(x, lanes);
     }
 }
@@ -755,14 +731,14 @@ __device__ __forceinline__ void prefix_walk(PrefixState<D>& st, Walk<D, kWhole>&
     __syncthreads();
 }
 
-template <int D, int C, bool kWhole, bool kShared>
+template <int D, bool kWhole, bool kShared>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void paged_decode_kernel(PagedDecodeParams p) {
-    constexpr int NT = kThreads, kPitch = D + 4, kR = 16 / C;
-    constexpr int kFold = kWaves * 16 * kPitch * 4, kLds = kShared ? std::max(kFold, Ring<D, kWhole>::kStages * Ring<D, kWhole>::kStage) : std::max(kFold, join_lds(kMaxPieces, kR));
+    constexpr int NT = kThreads, kPitch = D + 4;
+    constexpr int kFold = kWaves * 16 * kPitch * 4, kLds = kShared ? std::max(kFold, Ring<D, kWhole>::kStages * Ring<D, kWhole>::kStage) : std::max(kFold, join_lds(kMaxPieces, 16));
     __shared__ __attribute__((aligned(1024))) unsigned char lds[kLds];
     __shared__ float red_m[kWaves][16], red_l[kWaves][16], inv_l[16];
     __shared__ int is_last;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, quad = lane >> 4, cls = n / kR;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, quad = lane >> 4;
     const int per = p.kv_heads * p.chunks, dim = kWhole ? D : p.dim;
     int group = blockIdx.x;
     const Span span = span_of<kShared>(p, group, lane);
@@ -778,28 +754,22 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void paged_decode_kerne
     const Slots<D> slots(p, kShared);
     float* const red = (float*)lds;  // [wave][row][kPitch]
 
-    // A tile's rows, folded over the columns and the waves of the workgroup: to_row(row, d, values of four dims, m, l).
+    // A tile's rows, folded over the waves of the workgroup: to_row(row, d, values of four dims, m, l).
     auto fold = [&](State<D>& st, int rows, auto to_row, auto to_ml) __attribute__((always_inline)) {
-        const float m = columns_max<C>(st.m), f = __builtin_amdgcn_exp2f(st.m - m);
-        const float l = columns_sum<C>(quad_sum(st.l) * f);
-        if (C > 1)
-#pragma unroll
-            for (int i = 0; i < D / 16; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) st.o[i][e] = columns_sum<C>(st.o[i][e] * f);
-        if (n < kR && quad == 0) {
-            red_m[wave][n] = m;
+        const float l = quad_sum(st.l);
+        if (quad == 0) {
+            red_m[wave][n] = st.m;
             red_l[wave][n] = l;
         }
         __syncthreads();
-        float m_wg = red_m[0][n % kR], l_wg = 0.0f;
+        float m_wg = red_m[0][n], l_wg = 0.0f;
 #pragma unroll
-        for (int w = 1; w < kWaves; w++) m_wg = fmaxf(m_wg, red_m[w][n % kR]);
+        for (int w = 1; w < kWaves; w++) m_wg = fmaxf(m_wg, red_m[w][n]);
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) l_wg += red_l[w][n % kR] * __builtin_amdgcn_exp2f(red_m[w][n % kR] - m_wg);
-        if (n < kR) {
-            const float fw = __builtin_amdgcn_exp2f(m - m_wg);
-            float* row = red + (wave * kR + n) * kPitch;
+        for (int w = 0; w < kWaves; w++) l_wg += red_l[w][n] * __builtin_amdgcn_exp2f(red_m[w][n] - m_wg);
+        if (n < rows) {
+            const float fw = __builtin_amdgcn_exp2f(st.m - m_wg);
+            float* row = red + (wave * 16 + n) * kPitch;
 #pragma unroll
             for (int c = 0; c < D / 32; c++) {  // eight dims in a row
                 float y[8];
@@ -811,7 +781,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void paged_decode_kerne
             }
             if (wave == 0 && quad == 0) {
                 inv_l[n] = l_wg == 0.0f ? 0.0f : 1.0f / l_wg;
-                if (n < rows) to_ml(n, m_wg, l_wg);
+                to_ml(n, m_wg, l_wg);
             }
         }
         __syncthreads();
@@ -819,7 +789,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void paged_decode_kerne
             const int row = i / (D / 4), d = 4 * (i % (D / 4));
             f32x4_t o = {0, 0, 0, 0};
 #pragma unroll
-            for (int w = 0; w < kWaves; w++) o += *(const f32x4_t*)(red + (w * kR + row) * kPitch + d);
+            for (int w = 0; w < kWaves; w++) o += *(const f32x4_t*)(red + (w * 16 + row) * kPitch + d);
             to_row(row, d, o);
         }
         __syncthreads();
@@ -830,7 +800,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void paged_decode_kerne
         while (at < end) {
             const int seg = quotient(at, span.pre_places), seg_first = seg * span.pre_places, to = min(seg_first + span.pre_places, end);
             // steps whose first place is in the span
-            const int t0 = (max(at - seg_first - kStart, 0) + p.pre_cost - 1) / p.pre_cost, t1 = min(steps_up_to(span.shared), (max(to - seg_first - kStart, 0) + p.pre_cost - 1) / p.pre_cost);
+            const int t0 = (max(at - seg_first - kStart, 0) + kPreCost - 1) / kPreCost, t1 = min(steps_up_to(span.shared), (max(to - seg_first - kStart, 0) + kPreCost - 1) / kPreCost);
             at = to;
             if (to - seg_first <= kStart) continue;  // (places alone: no piece)
             const int kvh = quotient(seg, p.n_tiles), tile = seg - kvh * p.n_tiles;
@@ -912,8 +882,8 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void paged_decode_kerne
     auto rows_of = [&](const Piece& c) { return min(p.rows, p.group - c.piece * p.rows); };  // of the kv head's query heads
     auto begin = [&](const Piece& c) __attribute__((always_inline)) {
         const int rows = rows_of(c);
-        const bool there = n % kR < rows;
-        const uint16_t* q_row = p.q + ((size_t)c.b * p.heads + c.kvh * p.group + c.piece * p.rows + (there ? n % kR : 0)) * dim;
+        const bool there = n < rows;
+        const uint16_t* q_row = p.q + ((size_t)c.b * p.heads + c.kvh * p.group + c.piece * p.rows + (there ? n : 0)) * dim;
 #pragma unroll
         for (int k = 0; k < D / 32; k++) {
             q[k] = *(const u32x4_t*)(q_row + (kWhole ? 32 * k + 8 * quad : min(32 * k + 8 * quad, dim - 8)));
@@ -940,7 +910,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void paged_decode_kerne
         any = next(then);
         State<D> st;
         st.reset();
-        walk<D, C, kWhole>(st, w, x, lanes, q, cls, quad, p.scale_log2e);
+        walk<D, kWhole>(st, w, x, lanes, q, quad, p.scale_log2e);
         if (!kShared && !alone && tid == 0) word.replace();
         if (any) {
             over(then);
@@ -1000,9 +970,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedDecodeParams 
 template <int D, bool kWhole, bool kShared>
 hipError_t launch_as(hipStream_t stream, const PagedDecodeParams& p) {
     const dim3 grid(p.n_groups), block(kThreads);
-    if (p.rows <= 4) hipLaunchKernelGGL((paged_decode_kernel<D, 4, kWhole, kShared>), grid, block, 0, stream, p);
-    else if (p.rows <= 8) hipLaunchKernelGGL((paged_decode_kernel<D, 2, kWhole, kShared>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((paged_decode_kernel<D, 1, kWhole, kShared>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((paged_decode_kernel<D, kWhole, kShared>), grid, block, 0, stream, p);
     if (kShared) hipLaunchKernelGGL(paged_join_kernel<D>, dim3(p.chunks, p.kv_heads, p.batch), block, join_lds(kMaxPieces, p.rows), stream, p);
     return hipGetLastError();
 }
@@ -1012,9 +980,9 @@ hipError_t launch_dim(hipStream_t stream, const PagedDecodeParams& p, bool share
     return shared ? launch_as<D, false, true>(stream, p) : launch_as<D, false, false>(stream, p);
 }
 
-// Workgroups a CU, each with a wave on every SIMD.
+// Workgroups a CU, each with a wave on every SIMD (two of one: 16 heads of 64 without groups 24.9 us, one 32.9; 64 sequences behind 8192 keys 43.3,
+// 48.6; at dim 256 the registers are one's).
 constexpr int per_cu(int64_t dim) { return dim == 256 ? 1 : 2; }
-constexpr int kPreCost = 2;  // places of a prefix's step
 // Segments, steps and workgroups of a call at its longest, and what its workspace holds.
 struct Plan {
     int64_t chunks, rows, per_wave, per_tile, n_tiles, own_segments, pre_segments, places;
@@ -1112,8 +1080,9 @@ RT_API int rt_gqa_decode_paged_bf16(void* stream, const void* q, const void* k_p
     p.rows = (int)a.rows;
     p.per_wave = (int)a.per_wave;
     p.per_tile = (int)a.per_tile;
-    p.pre_cost = kPreCost;
     p.n_tiles = (int)a.n_tiles;
+    // (a join's partials have `rows` rows.  us, 0.66 / 1: 1 sequence of 2048 keys, 32 heads on 8 of 128 9.2 / 10.5; 16 of 500 to
+    // 4000 on 2 18.6 / 16.1, 8 behind 3000, 16 heads on 1 33.6 / 26.1)
     p.span_root = a.rows <= 4 ? 0.66f : 1.0f;
     p.scale_log2e = (1.0f / sqrtf((float)head_dim)) * kLog2eHost;
     p.part = (float*)workspace;

@@ -179,6 +179,10 @@ __device__ __forceinline__ Span span_of(const PagedDecodeParams& p, int& group, 
     // more workgroups than CUs, but not about two for each: one for each, and spans that its waves share evenly (us, 1 sequence of 30000 keys
     // 31.4 -> 27.0, 4 of 1000 to 4000 15.0 -> 13.9, 16 behind 2000 20.5 -> 18.1; heads of 32 on 8 of 128)
     if (s.total < s.size * (p.n_groups / 8 * 7) && s.total > s.size * kCus) s.size = (quotient(s.total + kCus - 1, kCus) + kWaves - 1) & -kWaves;
+    // long spans of dims 65 to 128 without a prefix: one for each too (us, two / one: 64 sequences of 512 to 8192 190.4 / 185.0, 512 of 100 to 1000 206 /
+    // 198, 16 of 8000 100.8 / 98.5, of dim 96 79.8 / 78.7; but 64 without groups of 64 122 / 158; 64 of 200 to 512, spans of 19 places, 26.0
+    // / 26.4)
+    if (!kShared && p.dim > 64 && p.dim <= 128 && s.size >= 32) s.size *= 2;
     if (s.shared > 0) {
         const int active = quotient(s.total + s.size - 1, s.size), eighth = (active + 7) / 8;  // (n_groups divides by eight)
         group = group / 8 < eighth ? (group & 7) * eighth + group / 8 : 0x7fffffff;

@@ -41,7 +41,7 @@ def test_every_page_size(page):
     check(normal_bits(rng, 4, 8, 64), pages, 2)
 
 
-@pytest.mark.parametrize("batch,heads,n_kv,dim,longest", [(1, 32, 8, 128, 5000), (1, 8, 1, 64, 40000), (3, 16, 2, 256, 3000), (70, 8, 2, 64, 400), (200, 4, 1, 128, 90), (33, 32, 8, 128, 700)])
+@pytest.mark.parametrize("batch,heads,n_kv,dim,longest", [(1, 32, 8, 128, 5000), (1, 8, 1, 64, 40000), (3, 16, 2, 256, 3000), (70, 8, 2, 64, 400), (200, 4, 1, 128, 90), (33, 32, 8, 128, 700), (700, 8, 4, 128, 60), (40, 16, 16, 112, 500)])
 def test_long_contexts_and_many_sequences(batch, heads, n_kv, dim, longest):
     rng = np.random.default_rng(batch)
     lens = [longest] + [int(x) for x in rng.integers(0, longest + 1, batch - 1)]

@@ -182,7 +182,7 @@ __device__ __forceinline__ Span span_of(const PagedDecodeParams& p, int& group, 
     // long spans of dims 65 to 128 without a prefix: one for each too (us, two / one: 64 sequences of 512 to 8192 190.4 / 185.0, 512 of 100 to 1000 206 /
     // 198, 16 of 8000 100.8 / 98.5, of dim 96 79.8 / 78.7; but 64 without groups of 64 122 / 158; 64 of 200 to 512, spans of 19 places, 26.0
     // / 26.4)
-    if (!kShared && p.dim > 64 && p.dim <= 128 && s.size >= 32) s.size *= 2;
+    else if (!kShared && p.dim > 64 && p.dim <= 128 && s.size >= 32 && s.total > s.size * kCus) s.size *= 2;
     if (s.shared > 0) {
         const int active = quotient(s.total + s.size - 1, s.size), eighth = (active + 7) / 8;  // (n_groups divides by eight)
         group = group / 8 < eighth ? (group & 7) * eighth + group / 8 : 0x7fffffff;
@@ -302,11 +302,13 @@ __device__ __forceinline__ void put_out(const PagedDecodeParams& p, int dim, int
 constexpr int kThreads = 64 * kWaves;
 constexpr int join_lds(int pieces, int rows) { return kThreads * 16 + pieces * rows * 8; }
 // All partials of `rows` heads from `head` on of sequence `seq`, by the whole workgroup: n_pre of the prefix, wave pre_wave's,
-// rows of theirs from pre_row on, and n_own.  Items of four elements, kAhead pieces of each at a time; where there are fewer items than threads, several threads an item, each
-// with every sub-th piece.  The first are asked for ahead of the (m, l) that their weights are made of.
+// rows of theirs from pre_row on, and n_own.  Items of four elements, kAhead pieces of each at a time (4 for 8: fewer registers, and
+// fewer requests for nothing: 256 sequences behind 500 keys 69.3 -> 65.9 us, 8 of 2000 to 4000 of 64 15.9 -> 14.8); where there are
+// fewer items than threads, several threads an item, each with every sub-th piece.  The first are asked for ahead of the (m, l) that
+// their weights are made of.
 template <int D, bool kShared>
 __device__ __forceinline__ void join(const PagedDecodeParams& p, unsigned char* lds, float* inv_l, int dim, int seq, int head, int rows, __amdgpu_buffer_rsrc_t pre, int n_pre, int pre_wave, int pre_row, __amdgpu_buffer_rsrc_t own, int n_own) {
-    constexpr int kAhead = 8, NT = kThreads, kMost = kMaxPieces;
+    constexpr int kAhead = 4, NT = kThreads, kMost = kMaxPieces;
     auto pre_at = [&](int k) __attribute__((always_inline)) { return (uint32_t)k * Slots<D>::kPre + (uint32_t)pre_wave * Slots<D>::kWave; };
     const uint32_t own_slot = (uint32_t)p.rows * (D + 2) * 4;
     f32x4_t* const part = (f32x4_t*)lds;

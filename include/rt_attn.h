@@ -483,9 +483,10 @@ int rt_flash_forward_packed_bf16_dev(void *stream, const rt_attention_shape *sha
 /* rt_gqa_decode_batched_bf16 over a cache in pages, for a batch that may share a prefix: q/out bf16 [batch, n_heads, head_dim], kv_lens
  * device int32[batch] = keys of each sequence (counts above table_pages * page_size are that, below 0 are 0).  With P =
  * shared_lens[0] (device int32[1]) or, with shared_lens == NULL, `shared_len` (0: nothing in common), every sequence of at least P keys has
- * its first P in common with the others: they are read once for all of them, through the table's row of the first of those sequences; its
- * own, from P on, and all keys of shorter sequences, through the sequence's row.  P need not end with a page.  A sequence that sees no
- * key (no keys, or none in pages) gives rows of +0.0.  kv head = h / (n_heads / n_kv), any number of heads a group.  f32 accumulation and
+ * its first P in common with the others.  A row of the table holds all keys of its sequence; the common ones are read once for all,
+ * through the row of the first sequence that has them, with a P on the device always, with a P that the host gives where that is shorter
+ * than to read them for each.  P need not end with a page: there each sequence's page holds the rows ahead of P too.  A sequence that
+ * sees no key (no keys, or none in pages) gives rows of +0.0.  kv head = h / (n_heads / n_kv), any number of heads a group.  f32 accumulation and
  * softmax, weights of one bf16 each, one rounding to bf16 at the end.  What is not seen does not count, whatever it holds; a dim in which a
  * V row that is seen is infinite or NaN comes out infinite or NaN.  The last bits of a sequence may depend on what else is in the batch
  * (how its keys are cut into spans); the same call gives the same bits every time.  table_pages * page_size up to 2^28, a page of K below

@@ -82,7 +82,7 @@ def expect_decode(q_bits, pages, lens=None, hidden=None):
 
 
 def run_decode(q_bits, pages, n_kv, shared=0, lens=None, table=None, stream=None, out=None, ws=None):
-    """The entry on host arrays; returns bf16 bits [b, heads, d]."""
+    """The entry on host arrays; returns bf16 bits [b, heads, d].  shared: as the entry takes it (on the device: always read once)."""
     b, h, d = q_bits.shape
     table = pages.table if table is None else table
     K = ra.LlmKernels

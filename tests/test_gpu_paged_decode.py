@@ -12,10 +12,16 @@ pytestmark = pytest.mark.gpu
 HEADS = [(8, 8), (32, 8), (28, 4), (16, 2), (40, 8), (34, 2), (20, 1), (5, 1), (16, 1), (17, 1)]
 
 
+def on_device(n):
+    return dev(np.array([n], dtype=np.int32))
+
+
 def check(q, pages, n_kv, shared=0, label="", **more):
-    got = bf16_values(run_decode(q, pages, n_kv, shared, **more))
+    """With a prefix: its length given by the host, which chooses, and on the device, which has it read once."""
     want, sizes = expect_decode(q, pages, more.get("lens"))
-    assert_within_rounding(got, want, sizes, label)
+    for way in (shared, on_device(shared)) if shared else (0,):
+        got = bf16_values(run_decode(q, pages, n_kv, way, **more))
+        assert_within_rounding(got, want, sizes, label)
 
 
 @pytest.mark.parametrize("dim", [64, 128, 256, 16, 80, 96, 112, 160, 192])
@@ -57,7 +63,6 @@ def test_a_shared_prefix(dim, shared):
     pages = Pages(rng, lens, 2, dim, 16, shared)
     q = normal_bits(rng, len(lens), 8, dim)
     check(q, pages, 2, shared)
-    check(q, pages, 2, dev(np.array([shared], dtype=np.int32)), "on the device")
 
 
 @pytest.mark.parametrize("heads,n_kv", HEADS)
@@ -115,14 +120,16 @@ def test_rows_that_have_no_page(shared):
         table[0, 1] = -5
         for i in range(4):
             hidden[i] += list(range(page, 2 * page))
-    got = bf16_values(run_decode(q, pages, 2, shared, table=table))
+    way = on_device(shared) if shared else 0
+    got = bf16_values(run_decode(q, pages, 2, way, table=table))
     want, sizes = expect_decode(q, pages, hidden=hidden)
     assert_within_rounding(got, want, sizes)
-    assert not run_decode(q, pages, 2, shared, table=np.full_like(table, -1)).any()
+    assert not run_decode(q, pages, 2, way, table=np.full_like(table, -1)).any()
 
 
 def test_what_is_not_seen_does_not_count():
-    """Rows behind a sequence's last, other sequences' pages and own copies of shared rows hold NaN or infinities."""
+    """Rows behind a sequence's last, other sequences' pages and, where the prefix is read once, own copies of shared rows hold NaN or
+    infinities."""
     rng = np.random.default_rng(3)
     lens, shared, page = [75, 90, 64, 71], 70, 16
     pages = Pages(rng, lens, 2, 64, page, shared)
@@ -131,7 +138,8 @@ def test_what_is_not_seen_does_not_count():
         pages.k[own, :, :shared % page] = NAN_BITS
         pages.v[own, :, :shared % page] = 0x7F80
     q = normal_bits(rng, 4, 8, 64)
-    check(q, pages, 2, shared)
+    want, sizes = expect_decode(q, pages)
+    assert_within_rounding(bf16_values(run_decode(q, pages, 2, on_device(shared))), want, sizes)
 
 
 def test_infinities_and_nan_that_are_seen():
@@ -169,12 +177,13 @@ def test_the_same_call_gives_the_same_bits_and_any_workspace_will_do():
     lens = [2100, 2001, 3000, 2500]
     pages = Pages(rng, lens, 4, 128, 16, 2000)
     q = normal_bits(rng, 4, 16, 128)
-    first = run_decode(q, pages, 4, 2000)
     n = ra.LlmKernels.gqa_decode_paged_workspace_bytes(4, 16, 4, 128, 16, pages.table_pages)
-    for fill in (0, 0xFF, 0x7F):
-        ws = dev(np.full(n, fill, dtype=np.uint8))
-        for _ in range(3):
-            assert np.array_equal(run_decode(q, pages, 4, 2000, ws=ws), first)
+    for shared in (on_device(2000), 0):
+        first = run_decode(q, pages, 4, shared)
+        for fill in (0, 0xFF, 0x7F):
+            ws = dev(np.full(n, fill, dtype=np.uint8))
+            for _ in range(3):
+                assert np.array_equal(run_decode(q, pages, 4, shared, ws=ws), first)
 
 
 def test_lengths_outside_the_table_count_as_its_ends():

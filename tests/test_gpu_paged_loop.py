@@ -91,9 +91,10 @@ def test_prompts_then_forks_then_recorded_steps(prefix):
     def step(s, x, of, positions, lengths):
         K.qk_norm_rope_kv_append_paged_bf16(s, of[0], of[0], of[1], of[2], x.pages, d_table, 8, positions, rope, b, b, HEADS, N_KV, DIM,
                                             q_gamma=x.d_gammas[0], k_gamma=x.d_gammas[1])
-        K.gqa_decode_paged_bf16(s, of[0], x.pages, of[3], d_table, 8, lengths, b, HEADS, N_KV, DIM, of[4], n, shared_len=prefix)
+        K.gqa_decode_paged_bf16(s, of[0], x.pages, of[3], d_table, 8, lengths, b, HEADS, N_KV, DIM, of[4], n, shared_len=shared)
 
     # a graph for each layer, with a workspace of its own: they may run side by side
+    shared = dev(np.array([prefix], dtype=np.int32)) if prefix else 0
     graphs = [hip.capture(s.handle, lambda s=s, x=x, of=of: step(s.handle, x, of, d_pos, d_lens)) for s, x, of in zip((stream, others), layers, state)]
     for _, _, types in graphs:
         assert NODE_TYPE_MEMSET not in types and len(types) == (3 if prefix else 2)
@@ -113,7 +114,7 @@ def test_prompts_then_forks_then_recorded_steps(prefix):
             assert_within_rounding(bf16_values(got), want, sizes, f"step {i} layer {which}")
             # the same attention again, eagerly, with a workspace that holds something else: the same bits
             ws, out = dev(np.full(n, 0x5A, dtype=np.uint8)), ra.HipStorage(b * HEADS * DIM * 2)
-            K.gqa_decode_paged_bf16(None, of[0], x.pages, out, d_table, 8, d_lens, b, HEADS, N_KV, DIM, ws, n, shared_len=prefix)
+            K.gqa_decode_paged_bf16(None, of[0], x.pages, out, d_table, 8, d_lens, b, HEADS, N_KV, DIM, ws, n, shared_len=shared)
             ra.synchronize()
             assert np.array_equal(out.download(np.uint16).reshape(got.shape), got)
         for buf in (d_pos, d_lens):
@@ -139,6 +140,7 @@ def test_calls_side_by_side_have_the_bits_of_calls_alone():
         lens = [500 + int(x) for x in rng.integers(0, 900, 20)]
         pages, q = Pages(rng, lens, 4, 128, 16, shared), normal_bits(rng, 20, 16, 128)
         n = K.gqa_decode_paged_workspace_bytes(20, 16, 4, 128, 16, pages.table_pages)
+        shared = dev(np.array([shared], dtype=np.int32)) if shared else 0
         sets.append((run_decode(q, pages, 4, shared), [dev(q), pages.dev(), ra.HipStorage(q.nbytes), dev(pages.table), pages.table_pages,
                                                        dev(np.array(lens, dtype=np.int32)), 20, 16, 4, 128, ra.HipStorage(n), n], shared))
     for _ in range(20):

@@ -169,11 +169,11 @@ __device__ __forceinline__ int t_lane_max(int x) {  // of non-negative numbers, 
     x = max(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
     return x;
 }
-__device__ __forceinline__ PackedPlace t_place_packed(const int32_t* starts, int batch, int tokens, int pos, int lane) {
+__device__ __forceinline__ PackedPlace t_place_packed(const int32_t* starts, int batch, int tokens, int group, int pos, int lane) {
     for (int b0 = 0; b0 < batch; b0 += 64) {
         const bool on = b0 + lane < batch;
         const int from = on ? starts[b0 + lane] : 0, to = on ? starts[b0 + lane + 1] : 0;
-        const int first = min(max(from, 0), tokens), len = min(max(to, first), tokens) - first, n = (len + TROWS - 1) / TROWS;
+        const int first = min(max(from, 0), tokens), len = min(max(to, first), tokens) - first, n = (len * group + TROWS - 1) / TROWS;
         const int ends = t_lane_sums(n), all = __builtin_amdgcn_readlane(ends, 63);
         if (pos >= all) {
             pos -= all;
@@ -229,7 +229,7 @@ __device__ __forceinline__ PackedPlace t_place_packed(const int32_t* starts, int
 enum TileWay : int { kTilesRegs = 0, kTilesDirect = 1, kTilesDirectPart = 2 };
 
 // MODE: kMaskNone, kMaskCausal, kMaskPadding.  BIAS: an additive f32 score bias is applied (then MODE is kMaskNone).
-// PACKED: query rows run over (position, head of the GQA group) (then MODE is kMaskCausal and there is no bias).
+// PACKED: query rows run over (position, head of the GQA group) (then MODE is kMaskCausal or kMaskPacked and there is no bias).
 // The grid is (heads or kv heads, batch, query tiles): no division stands between a workgroup and its first load.
 // kMaskPacked: causal, sequences one behind the other; the grid is (heads, places in the list of all sequences' query tiles), and the
 // sequence's first row takes the place of the batch stride.
@@ -360,10 +360,10 @@ __global__ __launch_bounds__(HALVES ? 512 : TileCfg<DP>::THREADS, HALVES ? 2 : B
     }
     PackedPlace seq{0, 0, 0, 0};
     if constexpr (kSeqs) {
-        seq = t_place_packed(p.starts, p.batch, p.seq_q, (int)(blockIdx.y + gridDim.y * blockIdx.z), lane);
+        seq = t_place_packed(p.starts, p.batch, p.seq_q, G, (int)(blockIdx.y + gridDim.y * blockIdx.z), lane);
         if (seq.b < 0) return;
         b = seq.b;
-        rows_total = seq.len;
+        rows_total = seq.len * G;
     }
     // where the sequence's row 0 lies in a tensor, of head 0
     auto base_of = [&](const TensorLayout& l) __attribute__((always_inline)) { return kSeqs ? (size_t)seq.first * (size_t)l.row_pitch : (size_t)b * l.batch_stride; };
@@ -1412,7 +1412,7 @@ __global__ __launch_bounds__(HALVES ? 512 : TileCfg<DP>::THREADS, HALVES ? 2 : B
     // Packed rows are positions of a chunked decode: one that sees no key at all is a row of zeros, as the reference's
     // decode kernels leave it (crates/rustorch-metal/src/kernels.rs:14504-14514: every loop runs zero times), not the
     // NaN row of flash_forward's l > 0 test.  l == 0 exactly when no key was weighed (a visible key gives P >= 1).
-    const float bad = (PACKED && l == 0.0f) ? 0.0f : quiet_nan();
+    const float bad = (PACKED && !kSeqs && l == 0.0f) ? 0.0f : quiet_nan();
     uint16_t* const obuf = (uint16_t*)(lds + wq * Cfg::REGION);
     const float fill = p.zero_padded_rows ? 0.0f : quiet_nan();
     if (n_loop > 0) {
@@ -2111,6 +2111,7 @@ hipError_t launch_packed(hipStream_t stream, const FlashTileParams& p, dim3 grid
         else hipLaunchKernelGGL(flash_split_merge_kernel<false>, at, dim3(256), 0, stream, m);
         return hipGetLastError();
     }
+    if (p.mask == kMaskPacked) return launch_one<DP, kMaskPacked, false, true, false, false, TILES>(stream, p, grid);
     return launch_one<DP, kMaskCausal, false, true, false, false, TILES>(stream, p, grid);
 }
 template <int DP, int TILES>
@@ -2287,13 +2288,28 @@ static bool tiles_by_length(const FlashTileParams& p, long long n_qtiles) {
            n_qtiles * p.batch * p.heads > (long long)p.n_cus * flash_tile_bf16_workgroups(p.dim);
 }
 
+// Sequences one behind the other: rows that run over (position, head of the group)?  A short sequence then fills its tiles, of which all heads of
+// a kv head share one walk.  Where the tiles do not fit the chip at once, up to a mean of 384 tokens; below 128, where a sequence is one tile a
+// head either way, only if there are fewer by 1.4 that way.  us, a head's / a group's, sequences, heads, lengths, head dim: 200 32/8 5-60 128
+// 83.2 / 46.1, 48 32/8 6-51 80 19.0 / 13.2, 54 16/2 2-30 128 13.2 / 8.6, 64 16/8 5-60 64 11.1 / 8.6, 32 24/8 20-100 128 16.2 / 12.1, 100 28/4 1-200 64 36.9 /
+// 29.8, 43 32/2 30-302 96 46.8 / 40.6, 16 16/4 100-300 256 39.0 / 30.7, 6 40/8 100-400 80 17.2 / 14.5, 16 24/8 200-400 128 33.0 / 30.9, 16 32/8 200-500 128
+// 50.8 / 47.8; but 32 16/8 20-120 128 11.0 / 12.3, 8 32/8 350-500 30.2 / 30.6, 8 16/2 64-1024 256 55.2 / 57.1, 16 32/8 101-2000 128 233 / 236, and where they fit 1
+// 32/8 17 6.3 / 7.5, 32 16/8 5-40 8.7 / 9.2, 16 16/2 50-300 64 10.0 / 10.4, 1 34/2 825 (halves) 19.1 / 21.9 (4 32/8 100-400 64 11.1 / 10.3).
+static bool takes_groups(const FlashTileParams& p) {
+    if (p.mask != kMaskPacked || p.group == 1 || (long long)p.seq_q * p.group > 0x7fffff00ll) return false;
+    const double mean = (double)p.seq_q / p.batch / TROWS, tiles = std::max(1.0, mean + 0.5);
+    if (tiles * p.batch * p.heads <= (double)p.n_cus * flash_tile_bf16_workgroups(p.dim)) return false;
+    return mean <= 3.0 && (mean >= 1.0 || tiles * p.group >= 1.4 * (mean * p.group + 0.5));
+}
+
 hipError_t launch_flash_tile_bf16(hipStream_t stream, const FlashTileParams& params) {
     FlashTileParams p = params;
     if (p.batch == 0 || p.heads == 0 || p.seq_q == 0) return hipSuccess;
     if (!flash_tile_bf16_supported(p.dim) || p.pack < 1) return hipErrorInvalidValue;
+    if (takes_groups(p)) p.pack = p.group;
     if (p.bias && (p.mask != kMaskNone || !flash_tile_bf16_bias_addressable(p.seq_kv))) return hipErrorInvalidValue;
     if (!flash_tile_bf16_addressable(p.seq_kv, p.lkv.row_pitch)) return hipErrorInvalidValue;
-    if ((p.pack > 1 || p.decode_rows) && (p.bias || p.mask != kMaskCausal)) return hipErrorInvalidValue;  // packed rows: the chunked decode only
+    if ((p.pack > 1 || p.decode_rows) && (p.bias || (p.mask != kMaskCausal && p.mask != kMaskPacked))) return hipErrorInvalidValue;  // packed rows: the chunked decode and packed sequences only
     if (p.window < 0 || (p.window > 0 && (p.pack > 1 || p.decode_rows || p.bias || p.mask != kMaskCausal || p.n_splits > 1))) return hipErrorInvalidValue;
     const long long rows = (long long)p.seq_q * p.pack;
     const long long n_qtiles = (rows + TROWS - 1) / TROWS;
@@ -2307,9 +2323,9 @@ hipError_t launch_flash_tile_bf16(hipStream_t stream, const FlashTileParams& par
         return hipErrorInvalidValue;
     if (p.batch > 65535 || heads_u > 65535 || p.group < 1) return hipErrorInvalidValue;  // grid limits
     // (packed sequences: a place for every tile there can be, whose rows are 128 each but for a sequence's last)
-    const long long places = p.seq_q / TROWS + std::min<long long>(p.batch, p.seq_q), deep = (places + 65534) / 65535;
+    const long long places = rows / TROWS + std::min<long long>(p.batch, p.seq_q), deep = (places + 65534) / 65535;
     if (p.mask != kMaskPacked && n_qtiles * p.n_splits > 65535) return hipErrorInvalidValue;
-    if (p.mask == kMaskPacked && (!p.starts || p.seq_q != p.seq_kv || p.pack > 1 || p.decode_rows || p.bias || p.window || p.n_splits > 1 || p.q_lens || p.kv_lens || deep > 65535))
+    if (p.mask == kMaskPacked && (!p.starts || p.seq_q != p.seq_kv || (p.pack > 1 && (p.pack != p.group || rows > 0x7fffff00ll)) || p.decode_rows || p.bias || p.window || p.n_splits > 1 || p.q_lens || p.kv_lens || deep > 65535))
         return hipErrorInvalidValue;
     set_grid_order(p, n_qtiles * p.n_splits);
     if (tiles_by_length(p, n_qtiles)) p.n_qtiles = -1;

@@ -86,6 +86,29 @@ def test_more_tiles_than_the_chip_holds(dim, heads):
     check(dim, [300, 10, 500, 129, 400, 257, 200, 380], heads, heads // 4, dim)
 
 
+@pytest.mark.parametrize("dim,heads,n_kv,batch,longest", [(64, 32, 8, 40, 60), (128, 32, 8, 70, 40), (80, 40, 8, 20, 60), (256, 16, 2, 40, 30), (96, 32, 2, 43, 280), (32, 28, 4, 60, 100),
+                                                          (128, 24, 8, 32, 300), (256, 12, 4, 16, 300), (16, 34, 2, 60, 50), (136, 20, 1, 22, 3), (64, 32, 8, 12, 700)])
+def test_many_sequences_of_grouped_heads(dim, heads, n_kv, batch, longest):
+    rng = np.random.default_rng(dim + batch)
+    check(dim, [int(x) for x in rng.integers(0, longest + 1, batch)], heads, n_kv, dim, tail=9, head=3)
+
+
+def test_nan_among_many_sequences_of_grouped_heads():
+    rng = np.random.default_rng(8)
+    lens = [int(x) for x in rng.integers(1, 60, 40)]
+    starts = np.concatenate([[0], np.cumsum(lens)])
+    t, at = int(starts[-1]), int(starts[7])
+    q, k, v = normal_bits(rng, t, 32, 64), normal_bits(rng, t, 8, 64), normal_bits(rng, t, 8, 64)
+    want, size = expect(q, k, v, starts)
+    k[at, 3, 5], v[at + lens[7], 2, 9] = 0x7FC1, 0x7FC1  # its first token's key; the next sequence's first V row
+    got = bf16_values(run(q, k, v, starts))
+    ill = np.zeros(got.shape, dtype=bool)
+    ill[at:at + lens[7], 12:16] = True
+    ill[at + lens[7]:at + lens[7] + lens[8], 8:12, 9] = True
+    assert np.isnan(got[ill]).all()
+    assert_within_rounding(got[~ill], want[~ill], size[~ill])
+
+
 @pytest.mark.parametrize("batch", [63, 64, 65, 150])
 def test_many_sequences(batch):
     rng = np.random.default_rng(batch)

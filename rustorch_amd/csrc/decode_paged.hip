@@ -17,7 +17,11 @@
 // prefix the workgroup that finishes a sequence's kv head last folds its partials.  With one every sequence has at least two, and a
 // prefix's tile is waited for by all of its sequences: there a second launch folds them, side by side.
 //
-// The weights meet V as one bf16 each, rounded to nearest, as in the prefill kernels: 2^-9 of a weight, and errors of many keys cancel.
+// The weights meet V as one bf16 each, rounded to nearest, as in the prefill kernels: off by up to 2^-8 of a weight, and errors of many keys
+// cancel (0.0023 of an output's size against 64 bits, 0.0017 where only the output is rounded).
+//
+// Bound: HBM; latency where there are few keys.  32 heads on 8 of 128: 64 sequences of 512 to 8192 keys 182 us, 6.3 TB/s; 1 of 2048 8.7 us; 64 of
+// 8200 to 8704 of which 8192 are shared 37.8 us, 103 MB.
 #include <algorithm>
 #include <type_traits>
 

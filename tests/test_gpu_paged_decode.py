@@ -150,7 +150,7 @@ def test_infinities_and_nan_that_are_seen():
     q = normal_bits(rng, 3, 4, 64)
     got = bf16_values(run_decode(q, pages, 1))
     want, sizes = expect_decode(q, pages)
-    # (an infinite one may come out NaN: where a row has several columns of a product, the others' weights are zeros)
+    # (an infinite one may come out NaN: a weight that is too small for f32 is zero)
     assert np.isnan(got[1, :, 7]).all() and not np.isfinite(got[2, :, 9]).any()
     got[1, :, 7], got[2, :, 9] = want[1, :, 7], want[2, :, 9]
     assert_within_rounding(got, want, sizes)
@@ -193,3 +193,27 @@ def test_lengths_outside_the_table_count_as_its_ends():
     got = bf16_values(run_decode(q, pages, 1, lens=[2 ** 31 - 1, -7]))
     want, sizes = expect_decode(q, pages, lens=[48, 0])
     assert_within_rounding(got, want, sizes)
+
+
+@pytest.mark.parametrize("shared", [0, 40])
+def test_caches_without_pages(shared):
+    """No page at all, and no column in the table: nothing is seen."""
+    rng = np.random.default_rng(10)
+    q = normal_bits(rng, 3, 8, 64)
+    for n_pages, columns in ((0, 4), (2, 0), (0, 0)):
+        n = ra.LlmKernels.gqa_decode_paged_workspace_bytes(3, 8, 2, 64, 16, columns)
+        out, pool = dev(np.full(q.shape, 0x7B7B, dtype=np.uint16)), dev(np.full((max(n_pages, 1), 2, 16, 64), NAN_BITS, dtype=np.uint16))
+        keep = dev(q), dev(np.zeros((3, max(columns, 1)), dtype=np.int32)), dev(np.array([50, 64, 7], dtype=np.int32)), dev(np.full(n, 0xA5, dtype=np.uint8))
+        ra.LlmKernels.gqa_decode_paged_bf16(None, keep[0], ra.KVPages(pool, pool, n_pages, 16), out, keep[1], columns, keep[2], 3, 8, 2, 64, keep[3], n,
+                                            shared_len=on_device(shared) if shared else 0)
+        ra.synchronize()
+        assert not out.download(np.uint16).any(), (n_pages, columns)
+
+
+def test_a_prefix_that_is_read_once_or_by_each():
+    """The same call with the prefix's length from the host, below and above where it is read once, and on the device."""
+    rng = np.random.default_rng(12)
+    for batch, shared in ((6, 600), (48, 900)):
+        lens = [shared + int(x) for x in rng.integers(0, 90, batch)]
+        pages = Pages(rng, lens, 8, 128, 32, shared)
+        check(normal_bits(rng, batch, 16, 128), pages, 8, shared)

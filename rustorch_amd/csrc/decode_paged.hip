@@ -1097,9 +1097,10 @@ RT_API int rt_gqa_decode_paged_bf16(void* stream, const void* q, const void* k_p
     p.per_wave = (int)a.per_wave;
     p.per_tile = (int)a.per_tile;
     p.n_tiles = (int)a.n_tiles;
-    // (a join's partials have `rows` rows.  us, 0.66 / 1: 1 sequence of 2048 keys, 32 heads on 8 of 128 9.2 / 10.5; 16 of 500 to
-    // 4000 on 2 18.6 / 16.1, 8 behind 3000, 16 heads on 1 33.6 / 26.1)
-    p.span_root = a.rows <= 4 ? 0.66f : 1.0f;
+    // (a join's partials have `rows` rows.  us, 0.66 / 0.8 / 1: 1 sequence of 2048 keys, 32 heads on 8 of 128 9.2 / 10.5 / 10.5; 4 of 1756 to
+    // 8783, 16 on 2 of 64 11.7 / 11.7 / 12.5, 1 of 12000, 32 on 4 of 128 15.7 / 15.7 / 16.5, 2 of 360 to 5412, 20 on 1 of 80 15.8 / 15.1 / 15.1, 8 of
+    // 3010 to 4000, 16 on 1 of 128 15.3 / 15.3 / 14.9)
+    p.span_root = a.rows <= 4 ? 0.66f : 0.8f;
     p.scale_log2e = (1.0f / sqrtf((float)head_dim)) * kLog2eHost;
     p.part = (float*)workspace;
     p.head = (unsigned char*)workspace + a.part_bytes;

@@ -2157,7 +2157,7 @@ hipError_t launch_halves(hipStream_t stream, const FlashTileParams& p, dim3 grid
 // Sequences one behind the other, whose number and sum are known and no more: by their mean length, up to 1.9 workgroups a CU too.  Whole /
 // halves, sequences, heads, lengths: 128 1 32 1300 32.4 / 29.2, 2 16 700-1900 43.1 / 36.8, 4 8 900-1500 35.5 / 31.1, but 2 32 600-800 20.3 / 23.2,
 // 16 8 100-350 13.5 / 17.6; 96 2 20 900-1200 26.0 / 24.6; 80 1 40 1300 29.0 / 29.5, but 3 20 500-700 18.6 / 20.1; 64 1 32 1500 27.9 / 22.9, 3 16
-// 600-900 18.1 / 16.2, 5 16 300-500 12.4 / 12.2, but 8 16 100-330 10.4 / 12.2; of 256 level (3 8 900-1500 53.0 / 53.3).
+// 600-900 18.1 / 16.2, 5 16 300-500 12.4 / 12.2, but 8 16 100-330 10.4 / 12.2.
 static bool takes_halves(const FlashTileParams& p, dim3 grid) {
     if (p.pack != 1 || p.decode_rows || p.window != 0 || p.mask == kMaskPadding || p.seq_kv < (p.dim <= 64 ? kHalvesFrom64 : kHalvesFrom)) return false;
     const unsigned long long units = (unsigned long long)grid.x * grid.y, n = units * grid.z, n_cus = (unsigned long long)p.n_cus;
@@ -2173,8 +2173,8 @@ static bool takes_halves(const FlashTileParams& p, dim3 grid) {
 // 10.5, 256 16.9 / 13.5, but 1 16 65 9.9 / 10.3, 1 16 16 7.4 / 8.5.  A padded batch of more workgroups than half the CUs, whose lengths are less,
 // from 160 (3 28 133 12.6 / 13.6, 2 32 122 at 224 1.06, 4 16 200 1.05 times as fast), a chunk, which requests its first tiles ahead of all else, from
 // 140 (16 8 87 positions over 129, head dim 208, 14.9 / 15.8; 11 8 176 over 176, 144, 1.05 times).  Sequences one behind the other from a mean of 96
-// on, however many (8 16/2 64-1024 69.9 / 57.7, 4 32/8 500-2000 217 / 171, 32 16 200-400 103 /
-// 98, 32 16 100-300 74.2 / 72.7, 1 8/2 120 12.8 / 11.2, but 32 16 20-60, 192, 19.5 / 21.7, 1 8/2 60 9.2 / 9.5).
+// on, however many (8 16/2 64-1024 69.9 / 57.7, 4 32/8 500-2000 217 / 171, 32 16 200-400 103 / 98, 100-300 74.2 / 72.7, 1 8/2 120 12.8 / 11.2, but
+// 32 16 20-60, 192, 19.5 / 21.7, 1 8/2 60 9.2 / 9.5).
 // Where they fill the chip the tiles of 64 keys that are asked for ahead of the walk come from memory at the pace of all of them, and a short walk
 // ends before they have paid.  Causal 16 16 128 14.7 / 15.9, 32 16 200 61.9 / 65.7, 256 70.1 / 72.8, 300 108.6 / 107.5, 520 228 / 224, 4 32 2048 410
 // / 338, head dim 160 32 16 160 45.5 / 48.3, 256 59.4 / 57.7; four query heads a kv head, whose keys the L2s have, 8 32/8 97 12.6 / 12.4, 128 13.7 /

@@ -1,8 +1,11 @@
 """Attention of prompts packed one behind the other, against attention in 64 bits of each sequence alone."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 import rustorch_amd as ra
+from rustorch_amd import _lib as L
 from _cache import bf16_values
 from _gpu import assert_within_rounding
 from _paged import dev, normal_bits
@@ -176,3 +179,27 @@ def test_the_strict_rule_for_non_finite_v():
     assert np.isnan(got[bad]).all() and np.isposinf(got[699, 1, 5])
     bad[699, 1, 5] = True
     assert_within_rounding(got[~bad], want[~bad], size[~bad])
+
+
+@pytest.mark.parametrize("lens", [[60, 40], [5] * 20])
+def test_rows_behind_four_gigabytes(lens):
+    """Queries and outputs of 4.9 GB, of which the last tokens belong to sequences."""
+    rng = np.random.default_rng(13)
+    t, n, h, d = 600000, sum(lens), 32, 128
+    starts = t - n + np.concatenate([[0], np.cumsum(lens)])
+    q, k, v = normal_bits(rng, n, h, d), normal_bits(rng, n, 1, d), normal_bits(rng, n, 1, d)
+    bufs = [ra.HipStorage(t * heads * d * 2) for heads in (h, 1, 1, h)]
+    out = np.full(q.shape, 0x7B7B, dtype=np.uint16)
+
+    def copy(call, buf, host):
+        err, at = L.RtErr(), buf.ptr + buf.byte_len - host.nbytes
+        a, b = (at, host.ctypes.data) if call == "rt_memcpy_h2d" else (host.ctypes.data, at)
+        assert getattr(L.lib(), call)(a, b, host.nbytes, None, C.byref(err)) == 0
+        ra.synchronize()
+
+    for buf, host in zip(bufs, (q, k, v, out)):
+        copy("rt_memcpy_h2d", buf, host)
+    ra.flash_forward_packed_bf16_dev(ra.AttentionShape.new(len(lens), h, t, d), *bufs[:3], dev(starts.astype(np.int32)), bufs[3], n_kv_heads=1)
+    copy("rt_memcpy_d2h", bufs[3], out)
+    want, size = expect(q, k, v, starts - (t - n))
+    assert_within_rounding(bf16_values(out), want, size)

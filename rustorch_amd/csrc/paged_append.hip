@@ -288,7 +288,7 @@ RT_API int rt_qk_norm_rope_kv_append_paged_bf16(void* stream, const void* q, voi
     p.n_kv = n_kv;
     p.dim = head_dim;
     p.n_pages = n_pages;
-    p.table_pages = table_pages;
+    p.table_pages = n_kv > 0 ? table_pages : 0;  // (without kv heads nothing is stored, and the table may be missing)
     p.page_shift = __builtin_ctz((unsigned)page_size);
     HIP_TRY(launch_paged_append((hipStream_t)stream, p), "paged_append launch");
     return RT_OK;

@@ -167,3 +167,14 @@ def test_the_bits_of_the_append_to_a_plain_cache(dim, norm):
     for a, c in ((pages.k, kc), (pages.v, vc)):
         got = a.download(np.uint16).reshape(b, rows // page, hkv, page, dim).transpose(0, 2, 1, 3, 4).reshape(b, hkv, rows, dim)
         assert np.array_equal(got, c.download(np.uint16).reshape(b, hkv, rows, dim))
+
+
+def test_without_kv_heads_q_is_rotated_and_nothing_else_is_asked_for():
+    """No k, v, pages or table: a call whose heads are all query heads."""
+    rng = np.random.default_rng(14)
+    t, heads, dim, rows = 37, 5, 128, 40
+    q, gamma, rope = normal_bits(rng, t, heads, dim), rng.standard_normal(dim, dtype=np.float32), Tables(rng, dim, rows)
+    dq, out = dev(q), dev(np.full_like(q, 0x1234))
+    ra.LlmKernels.qk_norm_rope_kv_append_paged_bf16(None, dq, out, None, None, ra.KVPages(None, None, 0, 16), None, 3, 0, rope, t, 1, heads, 0, dim, q_gamma=dev(gamma), eps=1e-5)
+    ra.synchronize()
+    assert np.array_equal(out.download(np.uint16).reshape(q.shape), rotated(q, gamma, 1e-5, rope.cos[:t], rope.sin[:t]))

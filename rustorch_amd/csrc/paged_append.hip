@@ -234,7 +234,7 @@ RT_API int rt_qk_norm_rope_kv_append_paged_bf16(void* stream, const void* q, voi
     if (!starts && batch > 0 && tokens % batch != 0)
         return fail(err, RT_ERR_WRONG_INPUT_LEN, RT_WHICH_Q, (uint64_t)batch, (uint64_t)tokens, "without starts every sequence has tokens / batch tokens");
     if (!positions) {  // rope.rs:179-184, then kv_cache.rs:84-89
-        const int64_t last = (int64_t)pos + (starts || batch == 0 ? 0 : tokens / batch);
+        const int64_t last = (int64_t)pos + (batch == 0 || tokens == 0 ? 0 : starts ? 1 : tokens / batch);  // (of `starts` no more is known here)
         if (pos < 0 || (n_axes == 0 && last > table_rows))
             return fail(err, RT_ERR_ROPE_POSITION_OVERFLOW, -1, (uint64_t)table_rows, (uint64_t)last, "positions outside the RoPE tables");
         if (last > (int64_t)table_pages * page_size)

@@ -1,5 +1,6 @@
 // Tests of the C++ host mirror's calls for packed tokens and caches in pages (include/rustorch_attn.hpp).
 //   paged_mirror_test errors   what they refuse, and as what: needs no GPU
+//   paged_mirror_test rows     what they say of a host position
 //   paged_mirror_test gpu      append, attention of the prompts, decode steps with a shared prefix
 #include <cmath>
 #include <cstdio>
@@ -40,6 +41,18 @@ static void errors() {
     CHECK(throws<GQAError>([&] { LlmKernels::gqa_decode_paged_bf16(nullptr, some, pages, some, some, 4, some, nullptr, 0, 1, 4, 3, 64, some, many); }));
     CHECK(throws<AttentionError>([&] { LlmKernels::flash_forward_packed_bf16(nullptr, AttentionShape::make(1, 4, 8, 0), 4, some, some, some, some, some); }));
     CHECK(LlmKernels::gqa_decode_paged_workspace_bytes(2, 4, 2, 64, 16, 8) > 0 && LlmKernels::gqa_decode_paged_workspace_bytes(2, 4, 2, 64, 17, 8) == 0);
+}
+
+// A host position, with and without `starts`, against the last row of the tables and of the page table.
+static void rows() {
+    alignas(16) static int32_t some[64];
+    RoPE rope(64, 16);
+    auto call = [&](const int32_t* starts, int32_t pos, const KVPages& pages, int32_t table_pages) {
+        LlmKernels::qk_norm_rope_kv_append_paged_bf16(nullptr, some, some, some, nullptr, some, pages, some, table_pages, starts, nullptr, pos, nullptr, {}, nullptr, nullptr, 1e-6f, rope, 2, 1, 1, 1, 64);
+    };
+    const KVPages wide{some, some, 4, 16}, narrow{some, some, 4, 8};
+    CHECK(throws<RoPEError>([&] { call(some, 16, wide, 4); }) && throws<RoPEError>([&] { call(nullptr, 15, wide, 4); }));
+    CHECK(throws<KVCacheOverflow>([&] { call(some, 8, narrow, 1); }) && throws<KVCacheOverflow>([&] { call(nullptr, 7, narrow, 1); }));
 }
 
 template <typename T>
@@ -106,6 +119,7 @@ static void gpu() {
 
 int main(int argc, char** argv) {
     if (argc > 1 && !std::strcmp(argv[1], "gpu")) gpu();
+    else if (argc > 1 && !std::strcmp(argv[1], "rows")) rows();
     else errors();
     std::printf(g_failed ? "%d failed\n" : "ok\n", g_failed);
     return g_failed != 0;

@@ -17,6 +17,10 @@ def test_cpp_refusals_need_no_gpu():
     run("errors")
 
 
+def test_cpp_host_positions_are_checked():
+    run("rows")
+
+
 @pytest.mark.gpu
 def test_cpp_prompts_and_steps():
     run("gpu")

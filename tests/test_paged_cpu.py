@@ -69,6 +69,14 @@ def test_append_refuses_with_the_reference_errors():
     assert append(positions=None, pos=65, starts=P, table_rows=100)[0] == L.RT_ERR_KV_OVERFLOW
 
 
+def test_append_checks_the_lowest_row_of_packed_sequences():
+    """A host position with `starts`: the row of the first token there may be, ahead of the tables' and the page table's last."""
+    for more, status in ((dict(pos=64), L.RT_ERR_ROPE_POSITION_OVERFLOW), (dict(pos=64, table_rows=65), L.RT_ERR_KV_OVERFLOW), (dict(pos=64, sections=[32], axes=P), L.RT_ERR_KV_OVERFLOW)):
+        rc, err = append(positions=None, starts=P, **more)
+        assert rc == status and (err.expected, err.got) == (64, 65), more
+    assert append(positions=None, starts=P, pos=64, tokens=0)[0] == L.RT_OK
+
+
 def test_append_of_nothing_is_done():
     assert append(tokens=0)[0] == L.RT_OK and append(batch=0, tokens=7)[0] == L.RT_OK and append(heads=0, n_kv=0)[0] == L.RT_OK
 

@@ -786,7 +786,7 @@ struct LlmKernels {
                                                   const float* q_gamma, const float* k_gamma, float eps, RoPE& rope, int32_t tokens,
                                                   int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim) {
         if (sections.empty())
-            check_rows(positions, pos, nullptr, rope, table_pages * pages.page_size, batch <= 0 || tokens <= 0 ? 0 : starts ? 1 : tokens / batch);
+            check_rows(positions, pos, nullptr, rope, (int64_t)table_pages * pages.page_size, batch <= 0 || tokens <= 0 ? 0 : starts ? 1 : tokens / batch);
         rt_err_detail e;
         detail::check_prepare(
             rt_qk_norm_rope_kv_append_paged_bf16(stream, q, q_out, k_in, k_out, v_in, pages.k, pages.v, page_table, starts, positions, pos,
@@ -823,7 +823,7 @@ struct LlmKernels {
 
 private:
     // the checks of a host position, before anything touches the device
-    static void check_rows(const int32_t* positions, int32_t pos, const int32_t* rows, const RoPE& rope, int32_t max_seq, int32_t seq) {
+    static void check_rows(const int32_t* positions, int32_t pos, const int32_t* rows, const RoPE& rope, int64_t max_seq, int32_t seq) {
         if (positions) return;
         const int64_t end = (int64_t)pos + seq;
         if (pos < 0 || end > (int64_t)rope.max_seq())

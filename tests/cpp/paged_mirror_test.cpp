@@ -53,6 +53,8 @@ static void rows() {
     const KVPages wide{some, some, 4, 16}, narrow{some, some, 4, 8};
     CHECK(throws<RoPEError>([&] { call(some, 16, wide, 4); }) && throws<RoPEError>([&] { call(nullptr, 15, wide, 4); }));
     CHECK(throws<KVCacheOverflow>([&] { call(some, 8, narrow, 1); }) && throws<KVCacheOverflow>([&] { call(nullptr, 7, narrow, 1); }));
+    // (page tables of 2^31 and 2^32 rows, which the entry refuses as too large: no position is behind them)
+    for (int32_t table_pages : {1 << 27, 1 << 28}) CHECK(throws<DeviceError>([&] { call(nullptr, 3, wide, table_pages); }));
 }
 
 template <typename T>

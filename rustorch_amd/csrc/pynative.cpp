@@ -39,7 +39,24 @@ bool as_u64(PyObject* o, uint64_t* out) {
 
 // A device address: None, an int (or anything with __index__), a HipStorage (.ptr), a contiguous GPU tensor
 // (.data_ptr()); or a stream: a handle, a ctypes pointer (.value) or an object that stands for one (_as_parameter_).
-PyTypeObject* tensors = nullptr;  // a type whose objects have data_ptr: the last one seen (held)
+bool as_address(PyObject* o, void** out);
+
+// The same of an object whose type had data_ptr the last time, as a tensor has it: without a method object a call.  False, and no
+// exception: anything about it is other than that, and as_address has to look at it by itself.
+bool as_tensor(PyObject* o, void** out) {
+    PyObject* cuda = PyObject_GetAttr(o, s_is_cuda);
+    PyObject* contiguous = cuda == Py_True ? PyObject_CallMethodNoArgs(o, s_is_contiguous) : nullptr;
+    PyObject* r = contiguous == Py_True ? PyObject_CallMethodNoArgs(o, s_data_ptr) : nullptr;
+    uint64_t v = 0;
+    const bool got = r && as_u64(r, &v);
+    Py_XDECREF(cuda);
+    Py_XDECREF(contiguous);
+    Py_XDECREF(r);
+    if (!got) PyErr_Clear();
+    else *out = (void*)(uintptr_t)v;
+    return got;
+}
+PyTypeObject* tensors = nullptr;  // held
 
 bool as_address(PyObject* o, void** out) {
     *out = nullptr;
@@ -50,28 +67,32 @@ bool as_address(PyObject* o, void** out) {
         *out = (void*)(uintptr_t)v;
         return true;
     }
-    PyObject* m = nullptr;
-    if (Py_TYPE(o) != tensors && (m = attr_or_null(o, s_data_ptr))) {  // (found once a type: a method object less a tensor)
-        Py_DECREF(m);
-        Py_INCREF(Py_TYPE(o));
-        Py_XDECREF(tensors);
-        tensors = Py_TYPE(o);
-    }
-    if (Py_TYPE(o) == tensors) {
+    if (Py_TYPE(o) == tensors && as_tensor(o, out)) return true;
+    PyObject* m = attr_or_null(o, s_data_ptr);
+    if (m) {
         PyObject* cuda = PyObject_GetAttr(o, s_is_cuda);
         PyObject* contiguous = cuda == Py_True ? PyObject_CallMethodNoArgs(o, s_is_contiguous) : nullptr;
-        const bool ok = contiguous && (contiguous == Py_True || PyObject_IsTrue(contiguous) == 1);
+        const bool ok = contiguous && PyObject_IsTrue(contiguous) == 1;
         Py_XDECREF(cuda);
         Py_XDECREF(contiguous);
         if (!ok) {
+            Py_DECREF(m);
             if (!PyErr_Occurred()) PyErr_SetString(PyExc_AssertionError, "device entry points take contiguous GPU tensors");
             return false;
         }
-        PyObject* r = PyObject_CallMethodNoArgs(o, s_data_ptr);
+        PyObject* r = PyObject_CallNoArgs(m);
+        Py_DECREF(m);
         const bool got = r && as_u64(r, &v);
         Py_XDECREF(r);
+        if (!got) return false;
         *out = (void*)(uintptr_t)v;
-        return got;
+        if (Py_TYPE(o) != tensors) {
+            Py_INCREF(Py_TYPE(o));
+            PyTypeObject* const before = tensors;
+            tensors = Py_TYPE(o);
+            Py_XDECREF(before);
+        }
+        return true;
     }
     if (PyErr_Occurred()) return false;
     for (PyObject* name : {s_ptr, s_value, s_as_parameter}) {

@@ -32,3 +32,45 @@ def test_native_binding_converts_arguments_and_reports_errors():
         call(None, 16, 16, 16, 16, 8, 2, 1, 64)
     with pytest.raises(TypeError):
         call(None, 16, 16, 16, 16, 8, 2, 1.0, 64, 10)
+
+
+def test_an_address_is_taken_from_each_object_by_itself():
+    """Objects of one class that hold their address in different ways, in any order: what one call saw is nothing to the next."""
+    class Gpu:
+        """A tensor's protocol, or only the address."""
+
+        def __init__(self, tensor, contiguous=True, cuda=True):
+            if tensor:
+                self.is_cuda, self.is_contiguous, self.data_ptr = cuda, (lambda: contiguous), (lambda: 32)
+            else:
+                self.ptr = 48
+
+    call = L.native.rt_gqa_decode_online_bf16
+    mismatch = (L.RT_ERR_HEAD_COUNT_MISMATCH, -1, 8, 3)
+    for buf in (Gpu(False), Gpu(True), Gpu(False), Gpu(True), Gpu(False)):
+        assert call(None, buf, 16, buf, 16, 8, 3, 1, 64, 10)[:4] == mismatch
+    for bad in (Gpu(True, contiguous=False), Gpu(True, cuda=False)):
+        for _ in range(2):
+            with pytest.raises(AssertionError):
+                call(None, bad, 16, 16, 16, 8, 3, 1, 64, 10)
+    broken = Gpu(True)
+    broken.data_ptr = lambda: 1 // 0
+    for _ in range(2):
+        with pytest.raises(ZeroDivisionError):
+            call(None, broken, 16, 16, 16, 8, 3, 1, 64, 10)
+    half = Gpu(False)
+    half.is_cuda = True  # says so, and has an address alone
+    assert call(None, half, 16, half, 16, 8, 3, 1, 64, 10)[:4] == mismatch
+
+
+def test_a_tensor_that_is_not_on_the_gpu_is_refused():
+    torch = pytest.importorskip("torch")
+    call = L.native.rt_gqa_decode_online_bf16
+    for _ in range(2):
+        with pytest.raises(AssertionError):
+            call(None, torch.zeros(4), 16, 16, 16, 8, 3, 1, 64, 10)
+    # (and a class that comes behind it)
+    class Buf:
+        ptr = 16
+
+    assert call(None, Buf(), 16, Buf(), 16, 8, 3, 1, 64, 10)[:4] == (L.RT_ERR_HEAD_COUNT_MISMATCH, -1, 8, 3)

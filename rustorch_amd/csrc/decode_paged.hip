@@ -717,8 +717,9 @@ __device__ __forceinline__ void prefix_walk(PrefixState<D>& st, Walk<D, kWhole>&
         if (at.lane == (i & 63)) seen = (int)at.seen;
         ring.load(at, i & kAhead, wave);
     };
-    auto await = [&](auto others) __attribute__((always_inline)) {  // but for as many later steps' requests
-        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(decltype(others)::value * 2 * R::kLoads) : "memory");
+    // the wave's requests, but for as many later steps', and its reads of the last step, whose place is overwritten behind the barrier
+    auto await = [&](auto others) __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(others)::value * 2 * R::kLoads) : "memory");
     };
     static_assert((R::kStages & kAhead) == 0 && (kAhead - 1) * 2 * R::kLoads < 63);
     at.request_entries(at.first);

@@ -28,3 +28,16 @@ def test_the_build_script_watches_every_source():
     listed = re.search(r"for f in \[(.*?)\] \{.*?rerun-if-changed", text, re.S).group(1)
     assert set(re.findall(r'"([^"]+)"', listed)) == sources | headers | {"Makefile"}
     assert sources == {n for n in os.listdir(CSRC) if n.endswith(".hip")}
+
+
+def test_a_barrier_in_assembly_waits_for_what_it_stands_for():
+    """The compiler counts the waits ahead of its own barriers; one written in assembly has to bring them: for the wave's requests to
+    LDS (some may stay under way) and for its reads of what is overwritten behind it."""
+    found = []
+    for name in sorted(os.listdir(CSRC)):
+        if name.endswith((".hip", ".hpp")):
+            with open(os.path.join(CSRC, name)) as f:
+                found += [(name, text) for text in re.findall(r'\basm\b[^;]*?"([^;]*?s_barrier[^;]*?)"\s*:', f.read(), re.S)]
+    assert found
+    for name, text in found:
+        assert "vmcnt(" in text and "lgkmcnt(0)" in text and text.index("lgkmcnt") < text.index("s_barrier"), (name, text)

@@ -493,7 +493,7 @@ int rt_flash_forward_packed_bf16_dev(void *stream, const rt_attention_shape *sha
  * (how its keys are cut into spans); the same call gives the same bits every time.  table_pages * page_size up to 2^28, a page of K below
  * 2 GiB.  `workspace`: rt_gqa_decode_paged_workspace_bytes(...) bytes of device memory, 16-byte aligned (RT_ERR_WORKSPACE_TOO_SMALL), which
  * the call works in alone and keeps nothing in: calls that may overlap (other streams, graphs replayed side by side) have workspaces of
- * their own.  out and the workspace share no memory with each other, q or the pages (RT_ERR_UNSUPPORTED). */
+ * their own.  out and the workspace share no memory with each other or with an input (RT_ERR_UNSUPPORTED). */
 size_t rt_gqa_decode_paged_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim,
                                            int32_t page_size, int32_t table_pages);
 int rt_gqa_decode_paged_bf16(void *stream, const void *q, const void *k_pages, const void *v_pages, void *out,

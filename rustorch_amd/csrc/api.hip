@@ -1654,7 +1654,8 @@ RT_API int rt_flash_forward_packed_bf16_dev(void* stream, const rt_attention_sha
     if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15)
         return fail(err, RT_ERR_UNSUPPORTED, -1, 16, 0, "q, k, v and out must be 16-byte aligned");
     const size_t rows = (size_t)shape->seq * shape->dim * 2, q_bytes = rows * shape->heads, kv_bytes = rows * n_kv_heads;
-    if (rt::overlap(out, q_bytes, q, q_bytes) || rt::overlap(out, q_bytes, k, kv_bytes) || rt::overlap(out, q_bytes, v, kv_bytes))
+    if (rt::overlap(out, q_bytes, q, q_bytes) || rt::overlap(out, q_bytes, k, kv_bytes) || rt::overlap(out, q_bytes, v, kv_bytes) ||
+        rt::overlap(out, q_bytes, starts, (size_t)(shape->batch + 1) * 4))
         return fail(err, RT_ERR_UNSUPPORTED, -1, 0, 0, "out must share no memory with the inputs");
     rc = ensure_device(err);
     if (rc) return rc;

@@ -1063,12 +1063,13 @@ RT_API int rt_gqa_decode_paged_bf16(void* stream, const void* q, const void* k_p
     if (!workspace || workspace_bytes < need)
         return fail(err, RT_ERR_WORKSPACE_TOO_SMALL, -1, need, workspace ? workspace_bytes : 0, "workspace too small");
     if ((uintptr_t)workspace & 15) return fail(err, RT_ERR_WORKSPACE_TOO_SMALL, -1, 16, (uint64_t)((uintptr_t)workspace & 15), "workspace must be 16-byte aligned");
-    // (a workgroup writes its rows while others read theirs)
+    // (a workgroup writes its rows while others read theirs, and the lengths and the table, which have to be the same for all of them)
     const size_t q_bytes = (size_t)batch * n_heads * head_dim * 2, page_bytes = (size_t)n_pages * n_kv * page_size * head_dim * 2;
+    const size_t table_bytes = (size_t)batch * table_pages * 4, lens_bytes = (size_t)batch * 4;
     const struct {
         const void* at;
         size_t n;
-    } written[2] = {{out, q_bytes}, {workspace, need}}, read[3] = {{q, q_bytes}, {k_pages, page_bytes}, {v_pages, page_bytes}};
+    } written[2] = {{out, q_bytes}, {workspace, need}}, read[6] = {{q, q_bytes}, {k_pages, page_bytes}, {v_pages, page_bytes}, {page_table, table_bytes}, {kv_lens, lens_bytes}, {shared_lens, shared_lens ? 4u : 0u}};
     bool apart = !overlap(out, q_bytes, workspace, need);
     for (const auto& w : written)
         for (const auto& r : read) apart = apart && !overlap(w.at, w.n, r.at, r.n);

@@ -105,6 +105,20 @@ def test_decode_refuses_outputs_over_inputs(more):
     assert rc == L.RT_ERR_UNSUPPORTED and b"share no memory" in err.message
 
 
+@pytest.mark.parametrize("more", [dict(table=FAR), dict(table=FAR - 28), dict(lens=FAR + 4), dict(lens=FAR - 4), dict(lens=6 * FAR + 16), dict(table=6 * FAR + 64), dict(shared_lens=FAR + 8),
+                                  dict(shared_lens=6 * FAR)])
+def test_decode_refuses_outputs_over_its_table_and_lengths(more):
+    """What every workgroup reads, the second launch too: none may write there.  (Table of 2 x 4 entries, two lengths, one prefix.)"""
+    rc, err = decode(**more)
+    assert rc == L.RT_ERR_UNSUPPORTED and b"share no memory" in err.message
+
+
+def test_packed_prompts_refuse_an_output_over_their_starts():
+    for starts in (FAR, FAR + 64, FAR - 8):  # three of them
+        rc, err = prompt(starts=starts)
+        assert rc == L.RT_ERR_UNSUPPORTED and b"share no memory" in err.message
+
+
 def test_decode_refuses_with_the_reference_errors():
     assert decode(dim=0)[0] == L.RT_ERR_ZERO_DIM
     assert decode(heads=4, n_kv=3)[0] == decode(n_kv=0)[0] == L.RT_ERR_HEAD_COUNT_MISMATCH

@@ -4,6 +4,7 @@ calls enqueue and return."""
 from __future__ import annotations
 
 import functools
+import operator
 
 import numpy as np
 
@@ -46,9 +47,15 @@ class KVPages:
         return cls(HipStorage.zeros(n_bytes, stream), HipStorage.zeros(n_bytes, stream), n_pages, page_size)
 
 
+def _whole(x) -> int:
+    if isinstance(x, float) and x.is_integer():
+        return int(x)
+    return operator.index(x)
+
+
 @functools.lru_cache(maxsize=64)
 def _host_i32(values: tuple):
-    """(address, count, what keeps it alive) of host int32 values."""
+    """(address, count, what keeps it alive) of host int32 values: plain ints, so that equal ones are one entry and none of it changes."""
     a = np.array(values, dtype=np.int32)
     return a.ctypes.data, a.size, a
 
@@ -253,7 +260,7 @@ class LlmKernels:
         first token.  With `sections`, pairs of a head for each of up to four axes, a token's rotary positions are
         `axis_positions`, device int32[len(sections), tokens], and not its row."""
         ptr, pos = _host_or_dev(positions)
-        at, n_axes, _ = (None, 0, None) if sections is None else _host_i32(tuple(sections))
+        at, n_axes, _ = (None, 0, None) if sections is None else _host_i32(tuple(map(_whole, sections)))
         cos, sin = rope.device_tables()
         check(L.native.rt_qk_norm_rope_kv_append_paged_bf16(
             stream, q, q_out, k_in, k_out, v_in, pages.k, pages.v, page_table, starts, ptr, pos, axis_positions, at, n_axes, q_gamma, k_gamma, eps, cos, sin,

@@ -202,3 +202,62 @@ def test_pages_run_out():
         c.layer(0)
     with pytest.raises(KeyError):
         c.add(prefix_of=1, shared=16)
+
+
+class Calls:
+    """What reaches the append's native entry."""
+
+    def __init__(self, monkeypatch):
+        self.seen = []
+        monkeypatch.setattr(L, "native", self)
+
+    def rt_qk_norm_rope_kv_append_paged_bf16(self, *args):
+        at, n = args[13], args[14]
+        self.seen.append(None if at is None else list((C.c_int32 * n).from_address(at)))
+
+
+class Rope:
+    max_seq = 64
+
+    def device_tables(self):
+        return P, P
+
+
+def append_call(sections, rope=None, dim=64):
+    ra.LlmKernels.qk_norm_rope_kv_append_paged_bf16(None, P, FAR, 2 * FAR, 3 * FAR, ra.KVPages(4 * FAR, 5 * FAR, 8, 16), P, 4, P, rope or Rope(), 4, 2, 4, 2, dim,
+                                                    axis_positions=None if sections is None else P, sections=sections)
+
+
+def test_sections_are_the_numbers_that_a_call_is_given(monkeypatch):
+    """Whatever holds them, and whatever it held in the call before."""
+    calls = Calls(monkeypatch)
+    held = np.array([[8], [24]], dtype=np.int64)
+    for first in (8, 10):
+        held[:, 0] = first, 32 - first
+        append_call(held[:, 0])
+        append_call([int(x) for x in held[:, 0]])
+    assert calls.seen == [[8, 24], [8, 24], [10, 22], [10, 22]]
+
+    class Number:  # an integer by its protocol, as a tensor of one element is
+        def __init__(self, value):
+            self.value = value
+
+        def __index__(self):
+            return self.value
+
+        def __int__(self):
+            return self.value
+
+    calls.seen.clear()
+    mine = [Number(8), Number(24)]
+    append_call(mine)
+    mine[0].value, mine[1].value = 16, 16
+    append_call(mine)
+    assert calls.seen == [[8, 24], [16, 16]]
+    calls.seen.clear()
+    append_call([8.0, np.float64(24)])
+    append_call(held[:, 0].tolist() + [np.int32(0)])
+    assert calls.seen == [[8, 24], [10, 22, 0]]
+    for bad in ([16.5, 15.5], ["8", "24"], [float("nan"), 32]):
+        with pytest.raises(TypeError):
+            append_call(bad)

@@ -778,13 +778,17 @@ struct LlmKernels {
 
     // Norm, rotation and append of packed tokens [tokens, heads, head_dim] into pages; rotated k goes to k_out too, where it is not nullptr.
     // starts (device [batch + 1], nullptr: tokens / batch each) are the sequences' first tokens, positions (device, or pos) the rows of
-    // those; with sections, a head's pairs for each of up to four axes, the rotary positions are axis_positions [axes, tokens].
+    // those; with sections, a head's pairs for each of up to four axes, the rotary positions are axis_positions [axes, tokens].  rope is of
+    // heads of head_dim.
     static void qk_norm_rope_kv_append_paged_bf16(void* stream, const void* q, void* q_out, const void* k_in, void* k_out, const void* v_in,
                                                   const KVPages& pages, const int32_t* page_table, int32_t table_pages,
                                                   const int32_t* starts, const int32_t* positions, int32_t pos,
                                                   const int32_t* axis_positions, const std::vector<int32_t>& sections,
                                                   const float* q_gamma, const float* k_gamma, float eps, RoPE& rope, int32_t tokens,
                                                   int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim) {
+        const size_t have = rope.max_seq() * (rope.head_dim() / 2), want = rope.max_seq() * (size_t)(head_dim > 0 ? head_dim / 2 : rope.head_dim() / 2);
+        if (have != want)
+            throw RoPEError(RoPEError::Kind::WrongInputLen, want, have, "rope: expected buffer of " + std::to_string(want) + " f32, got " + std::to_string(have));
         if (sections.empty())
             check_rows(positions, pos, nullptr, rope, (int64_t)table_pages * pages.page_size, batch <= 0 || tokens <= 0 ? 0 : starts ? 1 : tokens / batch);
         rt_err_detail e;

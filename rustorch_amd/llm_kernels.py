@@ -10,7 +10,7 @@ import numpy as np
 
 from . import _lib as L
 from .device import HipStorage
-from .errors import Overflow, PositionOverflow, check
+from .errors import Overflow, PositionOverflow, RopeWrongInputLen, check
 
 
 class Q4Rows:
@@ -258,7 +258,10 @@ class LlmKernels:
         `q_out` and, where it is given, rotated k to `k_out`; each may be its input.  `starts`, device int32[batch + 1], are the
         sequences' first tokens (None: tokens / batch each); `positions`, an int or a device int32[batch] buffer, the row of a sequence's
         first token.  With `sections`, pairs of a head for each of up to four axes, a token's rotary positions are
-        `axis_positions`, device int32[len(sections), tokens], and not its row."""
+        `axis_positions`, device int32[len(sections), tokens], and not its row.  `rope` is of heads of head_dim."""
+        half = getattr(rope, "head_dim", head_dim) // 2
+        if head_dim > 0 and half != head_dim // 2:
+            raise RopeWrongInputLen(rope.max_seq * (head_dim // 2), rope.max_seq * half)
         ptr, pos = _host_or_dev(positions)
         at, n_axes, _ = (None, 0, None) if sections is None else _host_i32(tuple(map(_whole, sections)))
         cos, sin = rope.device_tables()

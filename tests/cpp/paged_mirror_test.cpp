@@ -55,6 +55,10 @@ static void rows() {
     CHECK(throws<KVCacheOverflow>([&] { call(some, 8, narrow, 1); }) && throws<KVCacheOverflow>([&] { call(nullptr, 7, narrow, 1); }));
     // (page tables of 2^31 and 2^32 rows, which the entry refuses as too large: no position is behind them)
     for (int32_t table_pages : {1 << 27, 1 << 28}) CHECK(throws<DeviceError>([&] { call(nullptr, 3, wide, table_pages); }));
+    // tables of another head dim than the heads'
+    RoPE half(32, 16);
+    for (int32_t dim : {64, 16})
+        CHECK(throws<RoPEError>([&] { LlmKernels::qk_norm_rope_kv_append_paged_bf16(nullptr, some, some, some, nullptr, some, wide, some, 4, some, some, 0, nullptr, {}, nullptr, nullptr, 1e-6f, half, 2, 1, 1, 1, dim); }));
 }
 
 template <typename T>

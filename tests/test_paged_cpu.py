@@ -261,3 +261,22 @@ def test_sections_are_the_numbers_that_a_call_is_given(monkeypatch):
     for bad in ([16.5, 15.5], ["8", "24"], [float("nan"), 32]):
         with pytest.raises(TypeError):
             append_call(bad)
+
+
+def test_tables_of_another_head_dim_are_refused(monkeypatch):
+    """The kernel takes half a head's angles a row: rows of fewer would be read past the tables' end, of more give others' angles."""
+    calls = Calls(monkeypatch)
+
+    class Of32(Rope):
+        head_dim = 32
+
+    for dim in (64, 16):
+        with pytest.raises(ra.RopeWrongInputLen) as e:
+            append_call(None, Of32(), dim)
+        assert (e.value.expected, e.value.got) == (64 * dim // 2, 64 * 16)
+    with pytest.raises(ra.RopeWrongInputLen):
+        append_call(None, ra.RoPE(128, 64), 64)
+    assert not calls.seen
+    append_call(None, Of32(), 32)
+    append_call(None)  # (tables that do not say what they are of)
+    assert calls.seen == [None, None]

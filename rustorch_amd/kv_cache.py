@@ -175,15 +175,21 @@ class PagedKVCache:
     def table(self, seqs, write_from=None) -> np.ndarray:
         """int32 [len(seqs), table_pages], the `page_table` of a call for these sequences.  write_from: for each of them the row from which
         the call may write; whole pages ahead of it are left out, so that an append keeps off what is shared."""
+        seqs = list(seqs)
         for seq in seqs:
             self._check(seq)
-        table = self._table[list(seqs)].copy()
-        for i, row in enumerate(write_from if write_from is not None else ()):
-            table[i, :row // self.page_size] = -1
+        table = self._table[seqs].copy()
+        if write_from is not None:
+            rows = list(write_from)
+            if len(rows) != len(seqs) or any(row < 0 for row in rows):
+                raise ValueError(f"write_from is a row for each of {len(seqs)} sequences, got {rows}")
+            for i, row in enumerate(rows):
+                table[i, :row // self.page_size] = -1
         return table
 
     def lengths(self, seqs) -> np.ndarray:
         """int32 [len(seqs)], the rows that each has."""
+        seqs = list(seqs)
         for seq in seqs:
             self._check(seq)
-        return self._lens[list(seqs)].copy()
+        return self._lens[seqs].copy()

@@ -280,3 +280,22 @@ def test_tables_of_another_head_dim_are_refused(monkeypatch):
     append_call(None, Of32(), 32)
     append_call(None)  # (tables that do not say what they are of)
     assert calls.seen == [None, None]
+
+
+def test_write_from_is_a_row_for_each_sequence():
+    """Fewer left the rest of the table's rows writable, a row below 0 cut the table from its end."""
+    c = NoPages(3, 8)
+    a = c.add()
+    c.reserve(a, 48)
+    c.advance(a, 40)
+    b = c.add(prefix_of=a, shared=32)
+    c.reserve(b, 1)
+    for bad in ([32], [], [40, 32, 0], [-1, 32], [40, -17]):
+        with pytest.raises(ValueError):
+            c.table([a, b], write_from=bad)
+    t = c.table([a, b])
+    got = c.table([a, b], write_from=np.array([0, 32], dtype=np.int32))
+    assert (got[0] == t[0]).all() and got[1].tolist()[:3] == [-1, -1, t[1, 2]]
+    assert (c.table([b, a], write_from=c.lengths([b, a]))[:, :2] == -1).all()  # a row past what it has: nothing ahead of it
+    assert c.table([], write_from=[]).shape == (0, 8)
+    assert (c.table(iter([a, b]), write_from=iter([0, 32])) == got).all() and c.lengths(iter([a, b])).tolist() == [40, 32]

@@ -485,8 +485,8 @@ int rt_flash_forward_packed_bf16_dev(void *stream, const rt_attention_shape *sha
  * device int32[batch] = keys of each sequence (counts above table_pages * page_size are that, below 0 are 0).  With P =
  * shared_lens[0] (device int32[1]) or, with shared_lens == NULL, `shared_len` (0: nothing in common), every sequence of at least P keys has
  * its first P in common with the others.  A row of the table holds all keys of its sequence; the common ones are read once for all,
- * through the row of the first sequence that has them, with a P on the device always, with a P that the host gives where that is shorter
- * than to read them for each.  P need not end with a page: there each sequence's page holds the rows ahead of P too.  A sequence that
+ * through the row of the first sequence that has them, with a P on the device always, with a P that the host gives where it saves so much
+ * reading that the call is expected to be shorter (by the call's sizes; the lengths are not known there).  P need not end with a page: there each sequence's page holds the rows ahead of P too.  A sequence that
  * sees no key (no keys, or none in pages) gives rows of +0.0.  kv head = h / (n_heads / n_kv), any number of heads a group.  f32 accumulation and
  * softmax, weights of one bf16 each, one rounding to bf16 at the end.  What is not seen does not count, whatever it holds; a dim in which a
  * V row that is seen is infinite or NaN comes out infinite or NaN.  The last bits of a sequence may depend on what else is in the batch

@@ -801,7 +801,7 @@ struct LlmKernels {
             e);
     }
     // A decode step over pages; the first shared_len keys (or shared_lens[0], on the device) of every sequence that has as many are the same
-    // for all of these, and are read once where that is shorter.
+    // for all of these, and are read once where the call's sizes say that it is shorter (shared_len), or always (shared_lens).
     static size_t gqa_decode_paged_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_kv, int32_t head_dim, int32_t page_size,
                                                    int32_t table_pages) {
         return rt_gqa_decode_paged_workspace_bytes(batch, n_heads, n_kv, head_dim, page_size, table_pages);

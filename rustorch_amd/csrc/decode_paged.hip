@@ -994,12 +994,6 @@ hipError_t launch_dim(hipStream_t stream, const PagedDecodeParams& p, bool share
 // Workgroups a CU, each with a wave on every SIMD (two of one: 16 heads of 64 without groups 24.9 us, one 32.9; 64 sequences behind 8192 keys 43.3,
 // 48.6; at dim 256 the registers are one's).
 constexpr int per_cu(int64_t dim) { return dim == 256 ? 1 : 2; }
-// A prefix that the host knows is read once where that saves 40 MB, of 64 keys or more; else each sequence reads it with its own keys, and there is
-// no second launch.  us, once / by each, heads, kv heads, dim, batch, keys (MB saved), some 200 keys of each's own: 32 8 128 16 256 (16) 13.3 / 11.4, 32 256
-// (33) 15.4 / 15.6, 16 1024 (63) 15.5 / 18.9, 64 256 (66) 17.8 / 22.9; 16 16 64 8 1024 (29) 13.5 / 12.9, 4 4096 (50) 15.5 / 17.3; 28 4 128 32 1024 (65) 18.8 /
-// 18.7, 16 4096 (126) 25.1 / 27.9; 40 1 128 64 1024 (33) 24.4 / 25.4; 16 16 256 8 256 (29) 16.8 / 16.8, 4 1024 (50) 18.3 / 18.5, 200 64 (209) 108 / 115, but 200 16
-// (52) 94 / 59; 16 2 256 16 4096 (126) 37 / 30, 64 1024 (132) 28.1 / 30.5, 200 256 (104) 33.9 / 33.9.
-bool shares(int64_t batch, int64_t kv_heads, int64_t dim, int64_t keys) { return keys >= 64 && (batch - 1) * keys * kv_heads * dim * 4 >= 40000000; }
 // Segments, steps and workgroups of a call at its longest, and what its workspace holds.
 struct Plan {
     int64_t chunks, rows, per_wave, per_tile, n_tiles, own_segments, pre_segments, places;
@@ -1025,6 +1019,19 @@ Plan plan_of(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dim, int64_
     a.part_bytes = round((size_t)(a.groups + a.pre_segments) * (size_t)(kWaves * kWaveRows) * (size_t)(a.dim + 2) * 4 + (size_t)(a.groups + a.own_segments) * (size_t)a.rows * (size_t)(a.dim + 2) * 4);
     a.word_bytes = (size_t)a.own_segments * kWordPitch + 256;
     return a;
+}
+
+// A prefix that the host knows is read once where that saves enough; else each sequence reads it with its own keys, and there is no second
+// launch.  What reading it once costs is that launch, a walk that is cut into pieces by the root of its steps, and partials of all rows for every
+// piece: it pays from 60 MB saved and as much more as the root of steps times rows, which at dim 256, with one workgroup a CU, weighs 4.5 times as
+// much.  Over 530 calls of 1 to 32 kv heads, 2 to 256 sequences, prefixes of 64 to 16000 keys and own keys of up to 1000 the way so
+// chosen takes 1 % more than the shorter one in the mean, 35 % at worst (from 40 MB saved, whatever the size: 9 %, twice as long).  us, once / by each, heads,
+// kv heads, dim, batch, keys (MB saved): 32 8 128 64 8192 (2114) 36 / 193; 16 16 64 24 1001 and up to 2000 own (94) 28.3 / 33.4; 28 4 128 16 4096 (126) 27.0 / 24.4, 32 1024 (65)
+// 18.4 / 16.5; 32 2 128 64 4096 (264) 39 / 32, 16 4096 (63) 33.7 / 20.3; 40 1 128 64 4096 (132) 37.7 / 44.2, 1024 (33) 25.9 / 20.1; 16 2 256 16 4096 (126) 38.0 / 27.2,
+// 64 4096 (528) 42.3 / 59.3, 128 1024 (266) 33.3 / 40.7; 16 16 256 16 1024 (252) 25.8 / 40.4, 4 1024 (50) 18.3 / 17.5, but 200 64 (209) 108 / 106.
+bool shares(const Plan& a, int64_t batch, int64_t kv_heads, int64_t dim, int64_t keys) {
+    const double saved = (double)(batch - 1) * (double)keys * (double)(kv_heads * dim * 4), steps = (double)((keys + kStep - 1) / kStep);
+    return keys >= 64 && saved >= 1e6 * (60.0 + (a.dim == 256 ? 4.5 : 1.0) * sqrt(steps * (double)a.rows));
 }
 
 }  // namespace
@@ -1108,7 +1115,7 @@ RT_API int rt_gqa_decode_paged_bf16(void* stream, const void* q, const void* k_p
     p.head = (unsigned char*)workspace + a.part_bytes;
     p.words = p.head + 256;
     p.launch_id = next_launch_id() << 8;  // (its low 16 bits zero)
-    const bool shared = shared_lens || shares(batch, n_kv, head_dim, shared_len);
+    const bool shared = shared_lens || shares(a, batch, n_kv, head_dim, shared_len);
     p.n_groups = std::min(a.groups, kCus * per_cu(a.dim));
     const hipStream_t s = (hipStream_t)stream;
     HIP_TRY(a.dim == 64 ? launch_dim<64>(s, p, shared) : a.dim == 128 ? launch_dim<128>(s, p, shared) : launch_dim<256>(s, p, shared), "paged_decode launch");

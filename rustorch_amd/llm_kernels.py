@@ -278,7 +278,7 @@ class LlmKernels:
                               workspace_bytes, shared_len=0):
         """`gqa_decode_batched_bf16` over a cache in pages: q/out [batch, n_heads, head_dim], kv_lens device int32[batch].  The
         first `shared_len` keys (an int or a device int32[1] buffer) of every sequence that has as many are the same for all of
-        these, and are read once where that is shorter (an int), or always (a buffer)."""
+        these, and are read once where the call's sizes say that it is shorter (an int), or always (a buffer)."""
         ptr, shared = _host_or_dev(shared_len)
         check(L.native.rt_gqa_decode_paged_bf16(stream, q, pages.k, pages.v, out, page_table, kv_lens, ptr, shared, batch, n_heads, n_kv,
                                                 head_dim, pages.n_pages, pages.page_size, table_pages, workspace, workspace_bytes))

@@ -26,8 +26,11 @@ uint64_t next_launch_id() { return 256; }
 }  // namespace rt
 
 static std::vector<rt::PagedAppendParams> g_append;
+static int g_decodes = 0, g_joins = 0;
 static void note_launch(const std::string& name, dim3, void** args, hipStream_t) {
     if (name.find("paged_append") != std::string::npos) g_append.push_back(*(rt::PagedAppendParams*)args[0]);
+    g_decodes += name.find("paged_decode_kernel") != std::string::npos;
+    g_joins += name.find("paged_join_kernel") != std::string::npos;  // (where a prefix is read once)
 }
 
 // an address of its own for every buffer; none is looked into
@@ -63,10 +66,34 @@ static void a_call_without_kv_heads_reads_no_table() {
     CHECK(a.call() == RT_ERR_NULL_POINTER);
 }
 
+// A prefix that the host gives is read once where that was measured to be shorter, on both sides of the rule; one on the device always.
+static void a_prefix_is_read_once_where_that_is_shorter() {
+    struct Case {
+        int32_t heads, kv, dim, batch, shared;
+        bool once;
+    };
+    for (const Case& c : {Case{16, 2, 256, 16, 4096, false}, Case{16, 2, 256, 8, 4096, false}, Case{8, 1, 256, 64, 1024, false}, Case{16, 16, 256, 4, 1024, false},
+                          Case{16, 16, 256, 16, 1024, true}, Case{32, 8, 256, 16, 1024, true}, Case{32, 8, 256, 64, 1024, true}, Case{16, 2, 256, 64, 4096, true}, Case{32, 2, 128, 16, 4096, false},
+                          Case{32, 2, 128, 32, 1024, false}, Case{28, 4, 128, 32, 1024, false}, Case{32, 8, 128, 64, 8192, true}, Case{16, 16, 64, 24, 1001, true}, Case{16, 16, 64, 8, 1024, false},
+                          Case{32, 8, 128, 200, 63, false}, Case{32, 8, 128, 1, 30000, false}, Case{40, 1, 128, 64, 4096, true}}) {
+        const int32_t columns = (c.shared + 512) / 16;
+        const size_t need = rt_gqa_decode_paged_workspace_bytes(c.batch, c.heads, c.kv, c.dim, 16, columns);
+        for (bool device : {false, true}) {
+            g_decodes = g_joins = 0;
+            CHECK(rt_gqa_decode_paged_bf16(nullptr, at(0), at(1), at(2), at(3), (const int32_t*)at(4), (const int32_t*)at(5), (const int32_t*)(device ? at(6) : nullptr), device ? 0 : c.shared,
+                                           c.batch, c.heads, c.kv, c.dim, 64, 16, columns, at(7), need, nullptr) == RT_OK);
+            const bool right = g_decodes == 1 && g_joins == (device || c.once ? 1 : 0);
+            if (!right) std::printf("%d heads on %d of %d, %d behind %d\n", c.heads, c.kv, c.dim, c.batch, c.shared);
+            CHECK(right);
+        }
+    }
+}
+
 int main(int argc, char** argv) {
     fake::on_launch() = note_launch;
     const std::map<std::string, std::function<void()>> tests = {
         {"a_call_without_kv_heads_reads_no_table", a_call_without_kv_heads_reads_no_table},
+        {"a_prefix_is_read_once_where_that_is_shorter", a_prefix_is_read_once_where_that_is_shorter},
     };
     if (argc == 2 && tests.count(argv[1])) tests.at(argv[1])();
     else {

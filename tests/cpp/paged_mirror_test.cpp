@@ -2,6 +2,7 @@
 //   paged_mirror_test errors   what they refuse, and as what: needs no GPU
 //   paged_mirror_test rows     what they say of a host position
 //   paged_mirror_test gpu      append, attention of the prompts, decode steps with a shared prefix
+//   paged_mirror_test prefix   which rows a prefix is read through
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -123,9 +124,35 @@ static void gpu() {
     }
 }
 
+// Two sequences of 32 keys, whose first 16 are said to be the same, in pages of their own that hold 1 and 5 (then 3 and 7) in every dim of V: which of
+// them a sequence's mean is made of is how the prefix was read.  On the device its length has it read once, through the first sequence; the host's
+// is too short for that, and 0 is no prefix.
+static void prefix() {
+    const int heads = 4, kv = 2, d = 64, page = 16;
+    std::vector<uint16_t> v(4 * kv * page * d);
+    for (int p = 0; p < 4; p++)
+        for (int i = 0; i < kv * page * d; i++) v[p * kv * page * d + i] = bits((float)(p == 0 ? 1 : p == 1 ? 3 : p == 2 ? 5 : 7));
+    HipStorage k_pages = up(std::vector<uint16_t>(v.size())), v_pages = up(v), q = up(std::vector<uint16_t>(2 * heads * d)), out(2 * heads * d * 2);
+    HipStorage table = up(std::vector<int32_t>{0, 1, 2, 3}), lens = up(std::vector<int32_t>{32, 32}), sixteen = up(std::vector<int32_t>{16}), none = up(std::vector<int32_t>{0});
+    const KVPages pages{k_pages.ptr(), v_pages.ptr(), 4, page};
+    const size_t bytes = LlmKernels::gqa_decode_paged_workspace_bytes(2, heads, kv, d, page, 2);
+    HipStorage space(bytes);
+    auto second = [&](const int32_t* shared_lens, int32_t shared) {  // the second sequence's mean; the first's is 2 whatever is read
+        LlmKernels::gqa_decode_paged_bf16(nullptr, q.ptr(), pages, out.ptr(), (int32_t*)table.ptr(), 2, (int32_t*)lens.ptr(), shared_lens, shared, 2, heads, kv, d, space.ptr(), bytes);
+        const std::vector<uint16_t> got = back(out, 2 * heads * d);
+        for (int i = 0; i < heads * d; i++) CHECK(value(got[i]) == 2.0f && got[heads * d + i] == got[heads * d]);
+        return value(got[heads * d]);
+    };
+    CHECK(second((int32_t*)sixteen.ptr(), 0) == 4.0f);
+    CHECK(second((int32_t*)sixteen.ptr(), -3) == 4.0f);  // (the host's is not looked at there)
+    CHECK(second((int32_t*)none.ptr(), 16) == 6.0f);
+    CHECK(second(nullptr, 16) == 6.0f && second(nullptr, 0) == 6.0f);
+}
+
 int main(int argc, char** argv) {
     if (argc > 1 && !std::strcmp(argv[1], "gpu")) gpu();
     else if (argc > 1 && !std::strcmp(argv[1], "rows")) rows();
+    else if (argc > 1 && !std::strcmp(argv[1], "prefix")) prefix();
     else errors();
     std::printf(g_failed ? "%d failed\n" : "ok\n", g_failed);
     return g_failed != 0;

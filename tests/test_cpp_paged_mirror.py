@@ -24,3 +24,8 @@ def test_cpp_host_positions_are_checked():
 @pytest.mark.gpu
 def test_cpp_prompts_and_steps():
     run("gpu")
+
+
+@pytest.mark.gpu
+def test_cpp_a_prefix_on_the_device_is_read_once():
+    run("prefix")

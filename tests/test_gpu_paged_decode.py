@@ -217,3 +217,33 @@ def test_a_prefix_that_is_read_once_or_by_each():
         lens = [shared + int(x) for x in rng.integers(0, 90, batch)]
         pages = Pages(rng, lens, 8, 128, 32, shared)
         check(normal_bits(rng, batch, 16, 128), pages, 8, shared)
+
+
+@pytest.mark.parametrize("batch,shared,once", [(48, 900, True), (6, 600, False)])
+def test_the_rows_that_a_prefix_is_read_through(batch, shared, once):
+    """Every sequence has pages of its own for the rows that are the same for all.  NaN in some of them shows whose are read: the first
+    sequence's, where the prefix is read once, or everybody's own."""
+    rng = np.random.default_rng(batch)
+    lens = [shared + 1 + int(x) for x in rng.integers(0, 90, batch)]
+    pages = Pages(rng, lens, 8, 128, 32)
+    full = shared // 32
+    for rows, pool in ((pages.rows_k, pages.k), (pages.rows_v, pages.v)):
+        for i in range(1, batch):
+            rows[i][:, :shared] = rows[0][:, :shared]
+            pool[pages.table[i, :full]] = pool[pages.table[0, :full]]
+            pool[pages.table[i, full], :, :shared % 32] = pool[pages.table[0, full], :, :shared % 32]
+    q = normal_bits(rng, batch, 16, 128)
+    want, sizes = expect_decode(q, pages)
+    assert_within_rounding(bf16_values(run_decode(q, pages, 8, 0)), want, sizes)
+    others, first = [pages.table[i, 3] for i in range(1, batch)], pages.table[0, 3]
+    for way, read_once in ((shared, once), (on_device(shared), True)):
+        assert_within_rounding(bf16_values(run_decode(q, pages, 8, way)), want, sizes)
+        for poisoned, seen in ((others, [] if read_once else range(1, batch)), (first, range(batch) if read_once else [0])):
+            was = pages.v[poisoned].copy()
+            pages.v[poisoned] = NAN_BITS
+            got = bf16_values(run_decode(q, pages, 8, way))
+            pages.v[poisoned] = was
+            ill = np.isin(np.arange(batch), list(seen))
+            assert np.isnan(got[ill]).all()
+            if not ill.all():
+                assert_within_rounding(got[~ill], want[~ill], sizes[~ill])

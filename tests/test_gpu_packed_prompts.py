@@ -203,3 +203,15 @@ def test_rows_behind_four_gigabytes(lens):
     copy("rt_memcpy_d2h", bufs[3], out)
     want, size = expect(q, k, v, starts - (t - n))
     assert_within_rounding(bf16_values(out), want, size)
+
+
+@pytest.mark.parametrize("dim,heads,n_kv,lens", [(64, 16, 16, [77, 300, 150]), (128, 16, 4, [1300, 20, 900]), (64, 32, 8, [5] * 40), (256, 8, 2, [100, 700, 33]), (128, 2, 1, [1700])])
+def test_the_same_call_gives_the_same_bits(dim, heads, n_kv, lens):
+    """A head's rows, a group's, walks in halves: nothing depends on the order in which workgroups end."""
+    rng = np.random.default_rng(15)
+    starts = np.concatenate([[0], np.cumsum(lens)])
+    t = int(starts[-1])
+    q, k, v = normal_bits(rng, t, heads, dim), normal_bits(rng, t, n_kv, dim), normal_bits(rng, t, n_kv, dim)
+    first = run(q, k, v, starts)
+    for _ in range(4):
+        assert np.array_equal(run(q, k, v, starts), first)

@@ -16,7 +16,8 @@
 // its few rows alone and is gone: us in a recorded loop, one pass a wave / all passes of a token by one wave, two at a time: 1 token
 // of 32 + 8 heads of 128 3.5 / 9.4, 256 5.0 / 10.9, 1000 9.8 / 13.6, 4 prompts up to 4096 66.8 / 69.3 (301 MB: 4.5 TB/s), 6 up to 2000
 // of 16 + 16 heads of 64 on three axes 27.9 / 27.1.  The angles of three axes 16 bytes a request where all sections are multiples of
-// four, or word by word: 27.9, 31.1 on the last.
+// four, or word by word: 27.9, 31.1 on the last.  (As it is, a call among others: the four prompts 64.9 to 65.9 on 2 to 8 sets of tensors in turn,
+// the six 25.2 to 26.1 on 4 or 8 and 20.4 to 21.6 on one or two, which the memory-side cache of 256 MB holds.)
 //
 // Rows go past the caches to the pages, which the attention of the same prompt does not read (call alone and with that attention behind
 // it, us, plainly / past: 8 prompts up to 300 of 32 + 8 heads of 128 12.6, 25.0 / 11.8, 24.2; 6 up to 2000 of 16 + 16 of 64 27.3, 63.9 / 26.8, 63.9;

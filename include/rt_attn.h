@@ -487,7 +487,7 @@ int rt_flash_forward_packed_bf16_dev(void *stream, const rt_attention_shape *sha
  * its first P in common with the others.  A row of the table holds all keys of its sequence; the common ones are read once for all,
  * through the row of the first sequence that has them, with a P on the device always, with a P that the host gives where it saves so much
  * reading that the call is expected to be shorter (by the call's sizes; the lengths are not known there).  P need not end with a page: there each sequence's page holds the rows ahead of P too.  A sequence that
- * sees no key (no keys, or none in pages) gives rows of +0.0.  kv head = h / (n_heads / n_kv), any number of heads a group.  f32 accumulation and
+ * sees no key (no keys, or none in pages) gives rows of +0.0; a row that sees keys whose scores are all -infinity gives NaN.  kv head = h / (n_heads / n_kv), any number of heads a group.  f32 accumulation and
  * softmax, weights of one bf16 each, one rounding to bf16 at the end.  What is not seen does not count, whatever it holds; a dim in which a
  * V row that is seen is infinite or NaN comes out infinite or NaN.  The last bits of a sequence may depend on what else is in the batch
  * (how its keys are cut into spans); the same call gives the same bits every time.  table_pages * page_size up to 2^28, a page of K below

@@ -39,7 +39,11 @@ constexpr int kStep = 32;   // keys a step
 constexpr int kWaves = 4;   // a workgroup
 constexpr int kCus = 256;
 constexpr int kMaxPieces = 256;  // partials of a sequence's kv head: half of the prefix, half of its own keys, or all of its own
+// The maximum of keys whose scores are all -infinity, which no score lies below; of no keys it is -infinity.  Where neither has a weight the one gives
+// NaN, as the exponentials of -infinity less itself do, the other zeros.
 constexpr float kNoMax = -3.0e38f;
+__device__ __forceinline__ float weight_of(float m, float top) { return __builtin_amdgcn_exp2f(m - (top == neg_inf() ? 0.0f : top)); }
+__device__ __forceinline__ float inverse(float l, float top) { return l != 0.0f ? 1.0f / l : top == neg_inf() ? 0.0f : quiet_nan(); }
 typedef float f32x2p __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2p __attribute__((ext_vector_type(2)));
 
@@ -342,16 +346,16 @@ __device__ __forceinline__ void join(const PagedDecodeParams& p, unsigned char* 
         __syncthreads();
         const int row = tid >> 4, col = tid & 15;  // sixteen lanes a row
         const bool on = row < rows;
-        float top = kNoMax, sum = 0.0f;
+        float top = neg_inf(), sum = 0.0f;
         for (int k = col; on && k < pieces; k += 16) top = fmaxf(top, wgt[k * p.rows + row]);
         top = sixteen_max(top);
         for (int k = col; on && k < pieces; k += 16) {
-            const float fk = __builtin_amdgcn_exp2f(wgt[k * p.rows + row] - top);
+            const float fk = weight_of(wgt[k * p.rows + row], top);
             wgt[k * p.rows + row] = fk;
             sum += wl[k * p.rows + row] * fk;
         }
         sum = sixteen_sum(sum);
-        if (on && col == 0) inv_l[row] = sum == 0.0f ? 0.0f : 1.0f / sum;
+        if (on && col == 0) inv_l[row] = inverse(sum, top);
     }
     __syncthreads();
     for (int i0 = 0; i0 < items; i0 += NT) {
@@ -589,8 +593,10 @@ __device__ __forceinline__ void step(State<D>& st, Keys<D>& x, const u32x4_t (&q
 template <int D, bool kWhole>
 __device__ __forceinline__ void walk(State<D>& st, Walk<D, kWhole>& at, Keys<D>& x, const Lanes<D, kWhole>& lanes, const u32x4_t (&q)[D / 32], int quad, float scale_log2e) {
     int i = 0;
+    uint32_t any = 0;
     for (int t = at.first; t < at.end; t += at.stride) {
         const uint32_t seen = at.seen;
+        any |= seen;
         const bool more = t + at.stride < at.end;
         step<D>(st, x, q, [&]() __attribute__((always_inline)) {
             if (more) {
@@ -600,6 +606,7 @@ __device__ __forceinline__ void walk(State<D>& st, Walk<D, kWhole>& at, Keys<D>&
         }, seen, quad, scale_log2e);
         if (more) at.load_v(x, lanes);
     }
+    if (!any) st.m = neg_inf();
 }
 
 // ---- the prefix: 32 query rows a wave, keys in LDS ------------------------------------------------------------------------------
@@ -713,6 +720,7 @@ __device__ __forceinline__ void prefix_walk(PrefixState<D>& st, Walk<D, kWhole>&
     constexpr int kAhead = R::kStages - 1;  // steps under way, beside the one that is read
     const int steps = at.end - at.first, hh = at.lane >> 5;
     int seen = 0;  // lane i % 64: of step i
+    uint32_t any = 0;
     auto request = [&](int i) __attribute__((always_inline)) {
         at.place_half(at.first + i, i, wave * R::kOwn / 16);
         if (at.lane == (i & 63)) seen = (int)at.seen;
@@ -738,8 +746,11 @@ __device__ __forceinline__ void prefix_walk(PrefixState<D>& st, Walk<D, kWhole>&
         else if (left >= 1) await(std::integral_constant<int, 1>{});
         else await(std::integral_constant<int, 0>{});
         if (i + kAhead < steps) request(i + kAhead);
-        if (rows) prefix_step<D, kWhole>(st, q, ring, space + (i & kAhead) * R::kStage, (uint32_t)__builtin_amdgcn_readlane(seen, i & 63), hh, scale_log2e);
+        const uint32_t now = (uint32_t)__builtin_amdgcn_readlane(seen, i & 63);
+        any |= now;
+        if (rows) prefix_step<D, kWhole>(st, q, ring, space + (i & kAhead) * R::kStage, now, hh, scale_log2e);
     }
+    if (!any) st.m = neg_inf();
     __syncthreads();
 }
 
@@ -778,9 +789,9 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void paged_decode_kerne
 #pragma unroll
         for (int w = 1; w < kWaves; w++) m_wg = fmaxf(m_wg, red_m[w][n]);
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) l_wg += red_l[w][n] * __builtin_amdgcn_exp2f(red_m[w][n] - m_wg);
+        for (int w = 0; w < kWaves; w++) l_wg += red_l[w][n] * weight_of(red_m[w][n], m_wg);
         if (n < rows) {
-            const float fw = __builtin_amdgcn_exp2f(st.m - m_wg);
+            const float fw = weight_of(st.m, m_wg);
             float* row = red + (wave * 16 + n) * kPitch;
 #pragma unroll
             for (int c = 0; c < D / 32; c++) {  // eight dims in a row
@@ -792,7 +803,7 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void paged_decode_kerne
                 *(f32x4_t*)(dst + 4) = f32x4_t{y[4], y[5], y[6], y[7]};
             }
             if (wave == 0 && quad == 0) {
-                inv_l[n] = l_wg == 0.0f ? 0.0f : 1.0f / l_wg;
+                inv_l[n] = inverse(l_wg, m_wg);
                 to_ml(n, m_wg, l_wg);
             }
         }

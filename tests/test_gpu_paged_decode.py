@@ -247,3 +247,40 @@ def test_the_rows_that_a_prefix_is_read_through(batch, shared, once):
             assert np.isnan(got[ill]).all()
             if not ill.all():
                 assert_within_rounding(got[~ill], want[~ill], sizes[~ill])
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("shared", [0, 70])
+def test_scores_of_minus_infinity(dim, shared):
+    """Keys that are seen and have no weight: beside others they count nothing, and of them alone the softmax is NaN, as in
+    gqa_decode_batched_bf16; zeros are what sequences have that see no key."""
+    rng = np.random.default_rng(dim + shared)
+    least = np.uint16(0xFF80)
+    # of each sequence the rows whose scores are -infinity (dim 3 of q is 1): with a prefix that is all of it, part of it, or none
+    for pre in (shared, shared // 2, 0):
+        lens = [shared + n for n in (1, 33, 100, 5000, 64)] + [0]
+        own = [slice(shared, None), slice(shared, None), slice(shared, shared + 90), slice(shared, shared + 4900), slice(0, 0), slice(0, 0)]
+        pages = Pages(rng, lens, 1, dim, 16, shared)
+        q = normal_bits(rng, len(lens), 6, dim)
+        q[..., 3] = 0x3F80
+        for i, n in enumerate(lens):
+            if n:
+                pages.rows_k[i][0, :pre, 3] = least
+                pages.rows_k[i][0, own[i], 3] = least
+                for r in range(n):
+                    pages.k[pages.table[i, r // 16], 0, r % 16, 3] = pages.rows_k[i][0, r, 3]
+        table = pages.table.copy()
+        table[4, shared // 16 + 1:] = -1  # (sees little beside the prefix, and nothing without: page shared / 16 is its own)
+        hidden = {4: range((shared // 16 + 1) * 16, lens[4])}
+        if not shared:
+            table[4] = -1
+            hidden = {4: range(lens[4])}
+        with np.errstate(invalid="ignore"):
+            want, sizes = expect_decode(q, pages, hidden=hidden)
+        ill = np.isnan(want)
+        assert ill[0].all() == (pre == shared) and not ill[4:].any()
+        for way in (shared, on_device(shared)) if shared else (0, on_device(0)):
+            got = bf16_values(run_decode(q, pages, 1, way, table=table))
+            assert np.array_equal(np.isnan(got), ill)
+            assert_within_rounding(got[~ill], want[~ill], sizes[~ill])
+            assert not got[5].any() and (shared or not got[4].any())

@@ -476,7 +476,7 @@ int rt_qk_norm_rope_kv_append_paged_bf16(void *stream, const void *q, void *q_ou
 /* Causal attention of whole prompts, packed: shape = {batch: sequences, heads, seq: tokens of all, dim}; q/out [seq, heads, dim], k/v [seq,
  * n_kv_heads, dim] (0 = heads), all bf16; token i of a sequence sees its tokens 0 .. i and no other sequence's.  Rows equal
  * rt_flash_forward_bnhd_bf16_dev of the sequence alone up to the last bits (which may depend on what else is in the launch, as with that
- * entry), and rt_set_strict_non_finite_v holds here too.  dim up to 256, a multiple of 8, tensors 16-byte aligned, k and v below
+ * entry), and rt_set_strict_non_finite_v holds here too.  (With both, scores of 2^30 and more, 64 and more apart in f32, may come out NaN.)  dim up to 256, a multiple of 8, tensors 16-byte aligned, k and v below
  * 4 GiB each, out apart from the inputs (RT_ERR_UNSUPPORTED). */
 int rt_flash_forward_packed_bf16_dev(void *stream, const rt_attention_shape *shape, uint64_t n_kv_heads, const void *q,
                                      const void *k, const void *v, const int32_t *starts, void *out, rt_err_detail *err);

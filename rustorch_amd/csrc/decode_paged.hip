@@ -39,10 +39,12 @@ constexpr int kStep = 32;   // keys a step
 constexpr int kWaves = 4;   // a workgroup
 constexpr int kCus = 256;
 constexpr int kMaxPieces = 256;  // partials of a sequence's kv head: half of the prefix, half of its own keys, or all of its own
-// The maximum of keys whose scores are all -infinity, which no score lies below; of no keys it is -infinity.  Where neither has a weight the one gives
+// Maxima are of scores as the products leave them, and a weight is 2^((score - maximum) log2(e) / sqrt(dim)): scaled first, two scores of 2^31 that
+// are the same would be a rounding of the scaled one apart, whose power of two is infinite or zero.
+// The maximum of keys whose scores are all -infinity, which no finite score lies below; of no keys it is -infinity.  Where neither has a weight the one gives
 // NaN, as the exponentials of -infinity less itself do, the other zeros.
-constexpr float kNoMax = -3.0e38f;
-__device__ __forceinline__ float weight_of(float m, float top) { return __builtin_amdgcn_exp2f(m - (top == neg_inf() ? 0.0f : top)); }
+constexpr float kNoMax = -__FLT_MAX__;
+__device__ __forceinline__ float weight_of(float m, float top, float scale_log2e) { return __builtin_amdgcn_exp2f((m - (top == neg_inf() ? 0.0f : top)) * scale_log2e); }
 __device__ __forceinline__ float inverse(float l, float top) { return l != 0.0f ? 1.0f / l : top == neg_inf() ? 0.0f : quiet_nan(); }
 typedef float f32x2p __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2p __attribute__((ext_vector_type(2)));
@@ -350,7 +352,7 @@ __device__ __forceinline__ void join(const PagedDecodeParams& p, unsigned char* 
         for (int k = col; on && k < pieces; k += 16) top = fmaxf(top, wgt[k * p.rows + row]);
         top = sixteen_max(top);
         for (int k = col; on && k < pieces; k += 16) {
-            const float fk = weight_of(wgt[k * p.rows + row], top);
+            const float fk = weight_of(wgt[k * p.rows + row], top, p.scale_log2e);
             wgt[k * p.rows + row] = fk;
             sum += wl[k * p.rows + row] * fk;
         }
@@ -558,14 +560,14 @@ __device__ __forceinline__ void step(State<D>& st, Keys<D>& x, const u32x4_t (&q
         }
     }
     k_done();
-    // The running maximum, common to the four lanes of a column, in the exponent of two.  It follows the scores only where they have risen
-    // by 8 in it: up to there sums of weights in f32 and weights of 8 bits are as exact, and sums are scaled once or twice a span.
+    // The running maximum, common to the four lanes of a column.  It follows the scores only where they have risen by 8 in the exponent of
+    // two: up to there sums of weights in f32 and weights of 8 bits are as exact, and sums are scaled once or twice a span.
     float top = y[0];
 #pragma unroll
     for (int e = 1; e < 8; e++) top = fmaxf(top, y[e]);
-    top = quad_max(top) * scale_log2e;
-    if (__any(top - st.m > 8.0f)) {
-        const float m_new = fmaxf(st.m, top), alpha = __builtin_amdgcn_exp2f(st.m - m_new);
+    top = quad_max(top);
+    if (__any((top - st.m) * scale_log2e > 8.0f)) {
+        const float m_new = fmaxf(st.m, top), alpha = __builtin_amdgcn_exp2f((st.m - m_new) * scale_log2e);
         st.m = m_new;
         st.l *= alpha;
 #pragma unroll
@@ -574,7 +576,7 @@ __device__ __forceinline__ void step(State<D>& st, Keys<D>& x, const u32x4_t (&q
     float f[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        f[e] = __builtin_amdgcn_exp2f(fmaf(y[e], scale_log2e, -st.m));
+        f[e] = __builtin_amdgcn_exp2f((y[e] - st.m) * scale_log2e);
         st.l += f[e];
     }
     u32x4_t w;  // the weights, as the operand's words
@@ -688,9 +690,9 @@ __device__ __forceinline__ void prefix_step(PrefixState<D>& st, const u32x4_t (&
 #pragma unroll
     for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
     const u32x2_t both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-    top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * scale_log2e;
-    if (__any(top - st.m > 8.0f)) {  // (as in step())
-        const float m_new = fmaxf(st.m, top), alpha = __builtin_amdgcn_exp2f(st.m - m_new);
+    top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+    if (__any((top - st.m) * scale_log2e > 8.0f)) {  // (as in step())
+        const float m_new = fmaxf(st.m, top), alpha = __builtin_amdgcn_exp2f((st.m - m_new) * scale_log2e);
         st.m = m_new;
         st.l *= alpha;
 #pragma unroll
@@ -703,7 +705,7 @@ __device__ __forceinline__ void prefix_step(PrefixState<D>& st, const u32x4_t (&
     for (int u = 0; u < 2; u++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float a = __builtin_amdgcn_exp2f(fmaf(s[8 * u + 2 * i], scale_log2e, -st.m)), b = __builtin_amdgcn_exp2f(fmaf(s[8 * u + 2 * i + 1], scale_log2e, -st.m));
+            const float a = __builtin_amdgcn_exp2f((s[8 * u + 2 * i] - st.m) * scale_log2e), b = __builtin_amdgcn_exp2f((s[8 * u + 2 * i + 1] - st.m) * scale_log2e);
             st.l += a + b;
             w[u][i] = two_bf16(a, b);
         }
@@ -789,9 +791,9 @@ __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void paged_decode_kerne
 #pragma unroll
         for (int w = 1; w < kWaves; w++) m_wg = fmaxf(m_wg, red_m[w][n]);
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) l_wg += red_l[w][n] * weight_of(red_m[w][n], m_wg);
+        for (int w = 0; w < kWaves; w++) l_wg += red_l[w][n] * weight_of(red_m[w][n], m_wg, p.scale_log2e);
         if (n < rows) {
-            const float fw = weight_of(st.m, m_wg);
+            const float fw = weight_of(st.m, m_wg, p.scale_log2e);
             float* row = red + (wave * 16 + n) * kPitch;
 #pragma unroll
             for (int c = 0; c < D / 32; c++) {  // eight dims in a row

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import rustorch_amd as ra
-from _cache import bf16_values
+from _cache import bf16_bits, bf16_values
 from _gpu import assert_within_rounding
 from _paged import NAN_BITS, Pages, dev, expect_decode, normal_bits, run_decode
 
@@ -284,3 +284,23 @@ def test_scores_of_minus_infinity(dim, shared):
             assert np.array_equal(np.isnan(got), ill)
             assert_within_rounding(got[~ill], want[~ill], sizes[~ill])
             assert not got[5].any() and (shared or not got[4].any())
+
+
+@pytest.mark.parametrize("shared", [0, 70])
+@pytest.mark.parametrize("power", [10, 31, 40, 77, 120])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_any_finite_size(shared, power, sign):
+    """q and k of one dim alone, so that scores are exact: of two values, a 64th apart, of which the smaller has no weight."""
+    rng = np.random.default_rng(power + shared)
+    lens = [shared + n for n in (1, 40, 900, 6000)]
+    pages = Pages(rng, lens, 1, 128, 16, shared)
+    q = np.zeros((4, 6, 128), dtype=np.uint16)
+    q[..., 5] = bf16_bits(np.float32(sign * 1.375 * 2.0 ** (power // 2)))
+    for i, n in enumerate(lens):
+        x = np.full(n, 1.5 * 2.0 ** (power - power // 2), dtype=np.float32)
+        x[1::3] *= np.float32(1 - 2.0 ** -6)
+        pages.rows_k[i][...] = 0
+        pages.rows_k[i][0, :, 5] = bf16_bits(x)
+        for r in range(n):
+            pages.k[pages.table[i, r // 16], :, r % 16] = pages.rows_k[i][:, r]
+    check(q, pages, 1, shared)

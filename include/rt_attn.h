@@ -476,8 +476,8 @@ int rt_qk_norm_rope_kv_append_paged_bf16(void *stream, const void *q, void *q_ou
 /* Causal attention of whole prompts, packed: shape = {batch: sequences, heads, seq: tokens of all, dim}; q/out [seq, heads, dim], k/v [seq,
  * n_kv_heads, dim] (0 = heads), all bf16; token i of a sequence sees its tokens 0 .. i and no other sequence's.  Rows equal
  * rt_flash_forward_bnhd_bf16_dev of the sequence alone up to the last bits (which may depend on what else is in the launch, as with that
- * entry), and rt_set_strict_non_finite_v holds here too.  (With both, scores of 2^30 and more, 64 and more apart in f32, may come out NaN.)  dim up to 256, a multiple of 8, tensors 16-byte aligned, k and v below
- * 4 GiB each, out apart from the inputs (RT_ERR_UNSUPPORTED). */
+ * entry), and rt_set_strict_non_finite_v holds here too.  (With both, scores of 2^30 and more, 64 and more apart in f32, may come out NaN.)
+ * dim up to 256, a multiple of 8, tensors 16-byte aligned, k and v below 4 GiB each, out apart from the inputs (RT_ERR_UNSUPPORTED). */
 int rt_flash_forward_packed_bf16_dev(void *stream, const rt_attention_shape *shape, uint64_t n_kv_heads, const void *q,
                                      const void *k, const void *v, const int32_t *starts, void *out, rt_err_detail *err);
 
@@ -486,10 +486,11 @@ int rt_flash_forward_packed_bf16_dev(void *stream, const rt_attention_shape *sha
  * shared_lens[0] (device int32[1]) or, with shared_lens == NULL, `shared_len` (0: nothing in common), every sequence of at least P keys has
  * its first P in common with the others.  A row of the table holds all keys of its sequence; the common ones are read once for all,
  * through the row of the first sequence that has them, with a P on the device always, with a P that the host gives where it saves so much
- * reading that the call is expected to be shorter (by the call's sizes; the lengths are not known there).  P need not end with a page: there each sequence's page holds the rows ahead of P too.  A sequence that
- * sees no key (no keys, or none in pages) gives rows of +0.0; a row that sees keys whose scores are all -infinity gives NaN.  kv head = h / (n_heads / n_kv), any number of heads a group.  f32 accumulation and
- * softmax, weights of one bf16 each, one rounding to bf16 at the end.  What is not seen does not count, whatever it holds; a dim in which a
- * V row that is seen is infinite or NaN comes out infinite or NaN.  The last bits of a sequence may depend on what else is in the batch
+ * reading that the call is expected to be shorter (by the call's sizes; the lengths are not known there).  P need not end with a page:
+ * there each sequence's page holds the rows ahead of P too.  A sequence that sees no key (no keys, or none in pages) gives rows of +0.0; a
+ * row that sees keys whose scores are all -infinity gives NaN.  kv head = h / (n_heads / n_kv), any number of heads a group.  f32
+ * accumulation and softmax, weights of one bf16 each, one rounding to bf16 at the end.  What is not seen does not count, whatever it holds;
+ * a dim in which a V row that is seen is infinite or NaN comes out infinite or NaN.  The last bits of a sequence may depend on what else is in the batch
  * (how its keys are cut into spans); the same call gives the same bits every time.  table_pages * page_size up to 2^28, a page of K below
  * 2 GiB.  `workspace`: rt_gqa_decode_paged_workspace_bytes(...) bytes of device memory, 16-byte aligned (RT_ERR_WORKSPACE_TOO_SMALL), which
  * the call works in alone and keeps nothing in: calls that may overlap (other streams, graphs replayed side by side) have workspaces of

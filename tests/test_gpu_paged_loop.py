@@ -191,3 +191,43 @@ def test_pages_behind_four_gigabytes():
             exp[:, at % page] = row
             copy("rt_memcpy_d2h", buf.ptr + p * size, got)
             assert np.array_equal(got, exp)
+
+
+def test_recorded_calls_that_share_a_workspace():
+    """One behind the other on one stream: without a prefix, with one on the device and with one that the host gives, recorded, replayed in
+    turn and mixed with calls that are not recorded.  What a call leaves in the workspace is nothing to the next, and lengths that change
+    between replays are those that a replay finds."""
+    rng = np.random.default_rng(16)
+    hip, stream, calls = Hip(), ra.Stream(), []
+    for batch, prefix, shared in ((20, 0, 0), (20, 500, dev(np.array([500], dtype=np.int32))), (48, 900, 900)):
+        lens = [max(prefix, 400) + 4 + int(x) for x in rng.integers(0, 300, batch)]
+        pages, q = Pages(rng, lens, 8, 128, 32, prefix), normal_bits(rng, batch, 16, 128)
+        at = [[n - 3 + i for n in lens] for i in range(3)]  # three steps' lengths; some of them at a unit's end
+        want = [run_decode(q, pages, 8, shared, lens=x) for x in at]
+        n = K.gqa_decode_paged_workspace_bytes(batch, 16, 8, 128, 32, pages.table_pages)
+        calls.append(dict(q=dev(q), pages=pages.dev(), out=ra.HipStorage(q.nbytes), table=dev(pages.table), columns=pages.table_pages, lens=ra.HipStorage(batch * 4), at=at, batch=batch,
+                          n=n, shared=shared, want=want))
+    ws = dev(np.full(max(c["n"] for c in calls), 0x5A, dtype=np.uint8))
+
+    def call(c, s):
+        K.gqa_decode_paged_bf16(s, c["q"], c["pages"], c["out"], c["table"], c["columns"], c["lens"], c["batch"], 16, 8, 128, ws, c["n"], shared_len=c["shared"])
+
+    graphs = [hip.capture(stream.handle, lambda c=c: call(c, stream.handle)) for c in calls]
+    assert [len(types) for _, _, types in graphs] == [1, 2, 2]
+    for i in range(12):
+        for j in rng.permutation(3):
+            c = calls[j]
+            c["lens"].upload(np.array(c["at"][i % 3], dtype=np.int32))
+            if (i + j) % 4 == 3:
+                call(c, stream.handle)
+            else:
+                hip.launch(graphs[j][1], stream.handle)
+            if i % 2:  # (every other time the next call is enqueued behind this one)
+                stream.synchronize()
+        stream.synchronize()
+        for c in calls:
+            got = c["out"].download(np.uint16).reshape(c["want"][0].shape)
+            assert np.array_equal(got, c["want"][i % 3])
+    for graph, exe, _ in graphs:
+        hip.destroy(graph, exe)
+    stream.destroy()

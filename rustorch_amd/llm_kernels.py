@@ -47,17 +47,16 @@ class KVPages:
         return cls(HipStorage.zeros(n_bytes, stream), HipStorage.zeros(n_bytes, stream), n_pages, page_size)
 
 
-def _whole(x) -> int:
-    if isinstance(x, float) and x.is_integer():
-        return int(x)
-    return operator.index(x)
-
-
-@functools.lru_cache(maxsize=64)
-def _host_i32(values: tuple):
-    """(address, count, what keeps it alive) of host int32 values: plain ints, so that equal ones are one entry and none of it changes."""
-    a = np.array(values, dtype=np.int32)
+def _host_i32(*values):
+    """(address, count, what keeps it alive) of host int32 values."""
+    a = np.array([int(x) if isinstance(x, float) and x.is_integer() else operator.index(x) for x in values], dtype=np.int32)
     return a.ctypes.data, a.size, a
+
+
+@functools.lru_cache(maxsize=64, typed=True)
+def _kept_i32(*values):
+    """The same, kept by the values; None where one of them is no plain int and may change (a tensor's element is kept by which it is)."""
+    return _host_i32(*values) if all(type(x) is int for x in values) else None
 
 
 def _host_or_dev(x):
@@ -259,11 +258,14 @@ class LlmKernels:
         sequences' first tokens (None: tokens / batch each); `positions`, an int or a device int32[batch] buffer, the row of a sequence's
         first token.  With `sections`, pairs of a head for each of up to four axes, a token's rotary positions are
         `axis_positions`, device int32[len(sections), tokens], and not its row.  `rope` is of heads of head_dim."""
-        half = getattr(rope, "head_dim", head_dim) // 2
-        if head_dim > 0 and half != head_dim // 2:
-            raise RopeWrongInputLen(rope.max_seq * (head_dim // 2), rope.max_seq * half)
+        of = getattr(rope, "head_dim", head_dim)
+        if of != head_dim and of // 2 != head_dim // 2 and head_dim > 0:
+            raise RopeWrongInputLen(rope.max_seq * (head_dim // 2), rope.max_seq * (of // 2))
         ptr, pos = _host_or_dev(positions)
-        at, n_axes, _ = (None, 0, None) if sections is None else _host_i32(tuple(map(_whole, sections)))
+        at, n_axes, _ = None, 0, None
+        if sections is not None:
+            sections = tuple(sections)
+            at, n_axes, _ = _kept_i32(*sections) or _host_i32(*sections)
         cos, sin = rope.device_tables()
         check(L.native.rt_qk_norm_rope_kv_append_paged_bf16(
             stream, q, q_out, k_in, k_out, v_in, pages.k, pages.v, page_table, starts, ptr, pos, axis_positions, at, n_axes, q_gamma, k_gamma, eps, cos, sin,

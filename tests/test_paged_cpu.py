@@ -257,7 +257,8 @@ def test_sections_are_the_numbers_that_a_call_is_given(monkeypatch):
     calls.seen.clear()
     append_call([8.0, np.float64(24)])
     append_call(held[:, 0].tolist() + [np.int32(0)])
-    assert calls.seen == [[8, 24], [10, 22, 0]]
+    append_call(x for x in (Number(8), 24))
+    assert calls.seen == [[8, 24], [10, 22, 0], [8, 24]]
     for bad in ([16.5, 15.5], ["8", "24"], [float("nan"), 32]):
         with pytest.raises(TypeError):
             append_call(bad)

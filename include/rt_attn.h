@@ -455,7 +455,7 @@ size_t rt_gqa_decode_workspace_bytes(int32_t batch, int32_t n_heads, int32_t n_k
  * rotated k to k_out too, which is NULL, k_in itself or shares no memory with it (what rt_flash_forward_packed_bf16_dev takes).
  * Token s of sequence b is row p_b + s of the sequence, p_b = positions[b] (device int32[batch]) or `pos` for all; with starts == NULL every
  * sequence has tokens / batch tokens (1 for a decode step).  Without kv heads (n_kv 0) nothing is stored, and k_in, v_in, the pages and the
- * table may be NULL.
+ * table may be NULL and of no width.
  * Its rotary position is its row, or, with n_axes of 1 to 4, axis_positions[a, token] (device int32[n_axes, tokens]) on axis a: the first
  * sections[0] pairs of a head (pair i: dims i and i + head_dim / 2) turn with axis 0, the next sections[1] with axis 1, and so on (host
  * int32[n_axes], their sum head_dim / 2, any of them 0; RT_ERR_ROPE_WRONG_INPUT_LEN otherwise).

@@ -790,7 +790,7 @@ struct LlmKernels {
         if (have != want)
             throw RoPEError(RoPEError::Kind::WrongInputLen, want, have, "rope: expected buffer of " + std::to_string(want) + " f32, got " + std::to_string(have));
         if (sections.empty())
-            check_rows(positions, pos, nullptr, rope, (int64_t)table_pages * pages.page_size, batch <= 0 || tokens <= 0 ? 0 : starts ? 1 : tokens / batch);
+            check_rows(positions, pos, nullptr, rope, n_kv > 0 ? (int64_t)table_pages * pages.page_size : INT64_MAX, batch <= 0 || tokens <= 0 ? 0 : starts ? 1 : tokens / batch);
         rt_err_detail e;
         detail::check_prepare(
             rt_qk_norm_rope_kv_append_paged_bf16(stream, q, q_out, k_in, k_out, v_in, pages.k, pages.v, page_table, starts, positions, pos,

@@ -238,7 +238,7 @@ RT_API int rt_qk_norm_rope_kv_append_paged_bf16(void* stream, const void* q, voi
         const int64_t last = (int64_t)pos + (batch == 0 || tokens == 0 ? 0 : starts ? 1 : tokens / batch);  // (of `starts` no more is known here)
         if (pos < 0 || (n_axes == 0 && last > table_rows))
             return fail(err, RT_ERR_ROPE_POSITION_OVERFLOW, -1, (uint64_t)table_rows, (uint64_t)last, "positions outside the RoPE tables");
-        if (last > (int64_t)table_pages * page_size)
+        if (n_kv > 0 && last > (int64_t)table_pages * page_size)
             return fail(err, RT_ERR_KV_OVERFLOW, -1, (uint64_t)((int64_t)table_pages * page_size), (uint64_t)last, "rows behind the page table");
     }
     if (batch == 0 || tokens == 0 || n_heads + n_kv == 0) return RT_OK;

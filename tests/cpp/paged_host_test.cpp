@@ -66,6 +66,24 @@ static void a_call_without_kv_heads_reads_no_table() {
     CHECK(a.call() == RT_ERR_NULL_POINTER);
 }
 
+// Nor is a host position behind a page table that there is no use for.
+static void a_call_without_kv_heads_has_no_last_row() {
+    Append a;
+    a.n_kv = a.table_pages = a.n_pages = 0;
+    a.table = a.positions = false;
+    for (bool starts : {true, false}) {
+        a.starts = starts;
+        a.pos = 0;
+        g_append.clear();
+        CHECK(a.call() == RT_OK && g_append.size() == 1);
+        a.pos = 64;
+        CHECK(a.call() == RT_ERR_ROPE_POSITION_OVERFLOW);
+    }
+    a.n_kv = 2;
+    a.pos = 0;
+    CHECK(a.call() == RT_ERR_KV_OVERFLOW);
+}
+
 // A prefix that the host gives is read once where that was measured to be shorter, on both sides of the rule; one on the device always.
 static void a_prefix_is_read_once_where_that_is_shorter() {
     struct Case {
@@ -93,6 +111,7 @@ int main(int argc, char** argv) {
     fake::on_launch() = note_launch;
     const std::map<std::string, std::function<void()>> tests = {
         {"a_call_without_kv_heads_reads_no_table", a_call_without_kv_heads_reads_no_table},
+        {"a_call_without_kv_heads_has_no_last_row", a_call_without_kv_heads_has_no_last_row},
         {"a_prefix_is_read_once_where_that_is_shorter", a_prefix_is_read_once_where_that_is_shorter},
     };
     if (argc == 2 && tests.count(argv[1])) tests.at(argv[1])();

@@ -9,6 +9,7 @@ CPP = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp")
 
 @pytest.mark.parametrize("name", [
     "a_call_without_kv_heads_reads_no_table",
+    "a_call_without_kv_heads_has_no_last_row",
     "a_prefix_is_read_once_where_that_is_shorter",
 ])
 def test_host_code(name):
